@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/dq_linear.h``.
+"""ctypes binding of the C ABI in ``include/``.
 
 The shared library must have been built (``diffuser_b200.build.build()``);
 there is no fallback: loading fails loudly when it is missing.
@@ -106,17 +106,46 @@ SIGNATURES = {
                                             ctypes.c_int, ctypes.c_void_p, _c_i64, ctypes.c_void_p,
                                             _c_sz, ctypes.c_void_p]),
     "dq_dequant_nf4_scaled": (ctypes.c_int, [_c_p, _c_p, ctypes.c_int, _c_i64, _c_p, _c_p]),
+    "dq_gated_norm": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _c_p, _c_i64,
+                                     _c_p, _c_p, _c_i64, _c_p, _c_p, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+                                     ctypes.c_float, ctypes.c_int, _c_p, _c_i64, _c_p, _c_i64, _c_p]),
+    "dq_gated_norm_backward_workspace": (_c_sz, [_c_i64, ctypes.c_int, ctypes.c_int]),
+    "dq_gated_norm_backward": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_i64,
+                                              ctypes.c_int, ctypes.c_int, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p,
+                                              ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, _c_p,
+                                              _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz,
+                                              _c_p]),
+    "dq_adapter_plan_bytes": (_c_sz, [_c_i64, _c_i64, ctypes.c_int]),
+    "dq_adapter_plan": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_sz, _c_p]),
+    "dq_adapter_add_workspace": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
+    "dq_adapter_add": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p,
+                                      ctypes.c_int, ctypes.c_int, _c_p, ctypes.c_int, _c_p, _c_i64, _c_p, _c_p,
+                                      _c_sz, _c_p]),
+    "dq_adapter_backward_workspace": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
+    "dq_adapter_backward": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
+                                           _c_p, _c_p, _c_p, ctypes.c_int, ctypes.c_int, _c_p, _c_p, _c_i64, _c_p,
+                                           _c_i64, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "dq_checkpoint_pack": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
+    "dq_checkpoint_unpack": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p]),
+    "dq_linear_dgrad_workspace": (_c_sz, [_c_i64, _c_i64]),
+    "dq_linear_nf4_dgrad": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p, ctypes.c_int, _c_i64, _c_p, _c_p,
+                                           _c_sz, _c_p]),
+    "dq_linear_fp8_dgrad": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_p, ctypes.c_float, _c_i64, _c_p, _c_p, _c_sz,
+                                           _c_p]),
     "dq_plan_info": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, ctypes.c_int] + [ctypes.POINTER(ctypes.c_int)] * 4),
 }
 
 DQ_OK = 0
 DQ_ERR_TIMEOUT = 5
 DQ_ERR_SCRATCH_LIMIT = 9
+DQ_ERR_INDEX = 10
 DQ_NOALLOC_SCRATCH_BYTES = 8 << 20
 DQ_IPC_HANDLE_BYTES = 64
 DQ_ACT_NONE, DQ_ACT_GELU_TANH, DQ_ACT_SWIGLU, DQ_ACT_GEGLU_TANH = 0, 1, 2, 3
 DQ_FMT_NF4, DQ_FMT_FP8 = 0, 1
 DQ_DTYPE_F32, DQ_DTYPE_BF16 = 0, 1
+DQ_NORM_NONE, DQ_NORM_RMS, DQ_NORM_LAYER = 0, 1, 2
+DQ_ROUND_ONCE, DQ_ROUND_OPS = 0, 1
 
 _LIB = None
 

@@ -1,0 +1,475 @@
+// dq_adapter.cu -- host side of include/dq_adapter.h: argument validation,
+// launch planning and launches of the adapter, activation-checkpoint and
+// input-gradient kernels.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "../../include/dq_adapter.h"
+#include "dq_adapter.cuh"
+#include "dq_checkpoint.cuh"
+#include "dq_internal.h"
+
+namespace dq {
+namespace {
+
+constexpr int64_t kMaxTokens = 1 << 30;
+constexpr int kMaxAdapters = 65536;
+constexpr int kMaxRank = 128;
+
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+int plan_shape(int64_t M, int64_t R, int A) {
+  return M < 0 || M > kMaxTokens || R < 0 || R > kMaxTokens || A < 1 || A > kMaxAdapters ? DQ_ERR_SHAPE : DQ_OK;
+}
+int bank_shape(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
+  if (plan_shape(M, R, A) != DQ_OK || K <= 0 || N <= 0 || K % 8 != 0 || N % 8 != 0 || r <= 0 || r % 8 != 0 ||
+      r > kMaxRank || K > INT32_MAX || N > INT32_MAX)
+    return DQ_ERR_SHAPE;
+  return DQ_OK;
+}
+bool row_stride_ok(int64_t ld, int64_t width) { return ld >= width && ld % 8 == 0; }
+
+// Rank the kernels are instantiated for: the next of 16, 32, 64, 128 (columns
+// past the rank are zeros).
+int rank_class(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+
+// 128-row tiles where the groups fill at least half of one on average, else
+// 16-row tiles.
+bool large_tiles(int64_t M, int64_t R, int A) {
+  return M >= 64 * std::max<int64_t>(1, std::min<int64_t>(A, R));
+}
+
+// k splits of the down kernel: enough CTAs for two per SM (one CTA streams a
+// 128-row tile; a split's sums cost 8 rank bytes of traffic per row, so large
+// tiles stop at four), each at least 256 features deep.
+struct DownPlan {
+  bool large;
+  int tiles, splits, k_per_split;
+};
+DownPlan down_plan(int64_t M, int64_t R, int A, int64_t F, int sms) {
+  DownPlan p;
+  const AdapterPlan lay = adapter_plan_layout(M, R, A);
+  p.large = large_tiles(M, R, A);
+  const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(A, R));
+  const int64_t likely = p.large ? ceil_div(M, kTileRows) + groups / 2
+                                 : std::max<int64_t>(ceil_div(M, 16), std::min<int64_t>(groups, M));
+  p.tiles = static_cast<int>(p.large ? lay.max_tiles : lay.cap / 16);
+  const int64_t want = std::max<int64_t>(1, 2 * sms / std::max<int64_t>(1, likely));
+  const int64_t most = std::min<int64_t>(p.large ? 4 : 16, std::max<int64_t>(1, F / 256));
+  const int64_t s = std::min(want, most);
+  p.k_per_split = static_cast<int>(ceil_div(ceil_div(F, s), 64) * 64);
+  p.splits = static_cast<int>(ceil_div(F, p.k_per_split));
+  return p;
+}
+
+size_t part_bytes(int64_t M, int64_t R, int A, int64_t F, int r, int sms) {
+  return up256(static_cast<size_t>(adapter_plan_layout(M, R, A).cap) * r * 4 * down_plan(M, R, A, F, sms).splits);
+}
+
+// Row splits of the weight-gradient kernel: the count (up to 16) that leaves
+// the smallest share of the resident CTA slots idle in its last wave, for
+// splits of at least 256 rows.
+struct WgradPlan {
+  int col_tiles, splits, rows_per_split;
+};
+WgradPlan wgrad_plan(int64_t M, int64_t R, int A, int64_t cols, int rc, bool i8, int sms) {
+  const AdapterPlan lay = adapter_plan_layout(M, R, A);
+  const int slots = sms * (rc <= 64 ? 2 : 1);
+  WgradPlan p;
+  p.col_tiles = static_cast<int>(ceil_div(cols, i8 ? 128 : 64));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, M / 256));
+  double best = 0;
+  int splits = 1;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t ctas = p.col_tiles * s;
+    const double fill = static_cast<double>(ctas) / static_cast<double>(ceil_div(ctas, slots) * slots);
+    if (fill > best + 0.02) {
+      best = fill;
+      splits = static_cast<int>(s);
+    }
+  }
+  p.rows_per_split = static_cast<int>(ceil_div(ceil_div(lay.cap, splits), 64) * 64);
+  p.splits = static_cast<int>(ceil_div(lay.cap, p.rows_per_split));
+  return p;
+}
+size_t wgrad_bytes(const WgradPlan& p, int64_t cols, int r) {
+  return up256(static_cast<size_t>(2) * p.splits * r * cols * 4);
+}
+
+// Launches with programmatic stream serialization: the kernel may start while
+// the one before it drains, and waits (griddepcontrol.wait) before it reads
+// that one's results.
+template <typename Args, typename... More>
+int launch_after(void (*kern)(Args, More...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args args,
+                 More... more) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args, more...) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+// Shared-memory opt-in of a kernel, once per device.
+constexpr int kMaxDevices = 64;
+template <typename K>
+int allow_smem(K kern, int bytes, std::atomic<int>* set) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
+  if (set[dev].load(std::memory_order_acquire)) return DQ_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return DQ_ERR_LAUNCH;
+  set[dev].store(1, std::memory_order_release);
+  return DQ_OK;
+}
+
+template <int R>
+int launch_down(const DownArgs& a, const DownPlan& p, cudaStream_t st) {
+  const dim3 grid(p.tiles, p.splits);
+  if (p.large) {
+    static std::atomic<int> set[kMaxDevices];
+    const int rc = allow_smem(adapter_down_kernel<R>, DownCfg<R>::kSmemBytes, set);
+    if (rc != DQ_OK) return rc;
+    adapter_down_kernel<R><<<grid, 256, DownCfg<R>::kSmemBytes, st>>>(a);
+  } else {
+    adapter_down_small_kernel<R><<<grid, 256, 0, st>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+template <int R, int WM>
+int launch_up_tiles(UpArgs a, int tiles, int64_t likely_tiles, int sms, cudaStream_t st) {
+  using C = UpCfg<R, WM>;
+  static std::atomic<int> set[kMaxDevices];
+  const int rc = allow_smem(adapter_up_kernel<R, WM>, C::kSmemBytes, set);
+  if (rc != DQ_OK) return rc;
+  // columns per CTA: up to 16 steps where that still leaves four CTAs per
+  // slot of two per SM (the tile's hidden rows are summed once per CTA)
+  int64_t steps = 16;
+  while (steps > 1 && likely_tiles * ceil_div(a.N, steps * C::kStepCols) < 8 * sms) steps /= 2;
+  a.cols_per_cta = static_cast<int>(steps * C::kStepCols);
+  const dim3 grid(tiles, static_cast<unsigned>(ceil_div(a.N, a.cols_per_cta)));
+  return launch_after(adapter_up_kernel<R, WM>, grid, 256, C::kSmemBytes, st, a);
+}
+
+template <int R>
+int launch_up(const UpArgs& a, const DownPlan& p, int64_t M, int sms, cudaStream_t st) {
+  const int64_t likely = std::max<int64_t>(1, ceil_div(M, p.large ? kTileRows : 16));
+  return p.large ? launch_up_tiles<R, 8>(a, p.tiles, likely, sms, st)
+                 : launch_up_tiles<R, 1>(a, p.tiles, likely, sms, st);
+}
+
+template <int R, bool I8>
+int launch_wgrad(const WgradArgs& a, const WgradPlan& p, cudaStream_t st) {
+  using C = WgradCfg<R, I8>;
+  static std::atomic<int> set[kMaxDevices];
+  int rc = allow_smem(adapter_wgrad_kernel<R, I8>, C::kSmemBytes, set);
+  if (rc != DQ_OK) return rc;
+  rc = launch_after(adapter_wgrad_kernel<R, I8>, dim3(p.col_tiles, p.splits), 256, C::kSmemBytes, st, a);
+  if (rc != DQ_OK) return rc;
+  const int64_t elems = static_cast<int64_t>(a.rank) * a.cols;
+  const unsigned bx = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 1024), 512));
+  return launch_after(adapter_wgrad_reduce_kernel, dim3(bx, a.A), 256, 0, st, a.words, a.lay, a.rows_per_split,
+                      static_cast<const float*>(a.part), a.dbank, elems);
+}
+
+// Calls f.template operator()<R>() for the rank class.
+template <typename F>
+int by_rank(int r, F&& f) {
+  switch (rank_class(r)) {
+    case 16: return f(std::integral_constant<int, 16>());
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+  }
+  return f(std::integral_constant<int, 128>());
+}
+
+int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, int64_t M, int64_t R, int64_t cols,
+          int r, int A, const int32_t* words, const AdapterPlan& lay, void* ws, void* dbank, int sms,
+          cudaStream_t st) {
+  const bool i8 = x_scales != nullptr;
+  const WgradPlan p = wgrad_plan(M, R, A, cols, rank_class(r), i8, sms);
+  WgradArgs a = {};
+  a.x = x;
+  a.x_scales = x_scales;
+  a.g = static_cast<const __nv_bfloat16*>(g);
+  a.words = words;
+  a.part = static_cast<float*>(ws);
+  a.dbank = static_cast<__nv_bfloat16*>(dbank);
+  a.lay = lay;
+  a.ldx = ldx;
+  a.cols = static_cast<int>(cols);
+  a.rank = r;
+  a.A = A;
+  a.rows_per_split = p.rows_per_split;
+  return by_rank(r, [&](auto rc) {
+    constexpr int R_ = decltype(rc)::value;
+    return i8 ? launch_wgrad<R_, true>(a, p, st) : launch_wgrad<R_, false>(a, p, st);
+  });
+}
+
+// Workspace of the backward pass: the down sums, g [M, r], and one region for
+// each weight gradient's partial sums.
+struct BackwardWs {
+  size_t part, g, up, down, total;
+};
+BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A, int sms) {
+  BackwardWs w;
+  const int rc = rank_class(r);
+  w.part = part_bytes(M, R, A, N, r, sms);
+  w.g = up256(static_cast<size_t>(M) * r * 2);
+  w.up = wgrad_bytes(wgrad_plan(M, R, A, N, rc, false, sms), N, r);
+  w.down = std::max(wgrad_bytes(wgrad_plan(M, R, A, K, rc, false, sms), K, r),
+                    wgrad_bytes(wgrad_plan(M, R, A, K, rc, true, sms), K, r));
+  w.total = w.part + w.g + w.up + w.down;
+  return w;
+}
+
+// v = x . P^T (down) then out = act(y + scale v . Q) (up), on one plan.
+int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void* y, int64_t ldy, int64_t F_out,
+            const void* Q, const float* scale, int64_t M, int64_t R, int r, int A, const int32_t* words, int act,
+            void* out, int64_t ldo, void* hidden, void* part, int sms, cudaStream_t st) {
+  const AdapterPlan lay = adapter_plan_layout(M, R, A);
+  const DownPlan p = down_plan(M, R, A, F_in, sms);
+  DownArgs d = {};
+  d.x = static_cast<const __nv_bfloat16*>(x);
+  d.bank = static_cast<const __nv_bfloat16*>(P);
+  d.words = words;
+  d.part = static_cast<float*>(part);
+  d.lay = lay;
+  d.ldx = ldx;
+  d.K = static_cast<int>(F_in);
+  d.rank = r;
+  d.A = A;
+  d.k_per_split = p.k_per_split;
+  UpArgs u = {};
+  u.y = static_cast<const __nv_bfloat16*>(y);
+  u.bank = static_cast<const __nv_bfloat16*>(Q);
+  u.scale = scale;
+  u.words = words;
+  u.part = d.part;
+  u.out = static_cast<__nv_bfloat16*>(out);
+  u.hidden = static_cast<__nv_bfloat16*>(hidden);
+  u.lay = lay;
+  u.ldy = ldy;
+  u.ldo = ldo;
+  u.N = static_cast<int>(F_out);
+  u.rank = r;
+  u.A = A;
+  u.splits = p.splits;
+  u.act = act;
+  u.with_none = act != kActNone || out != y || hidden != nullptr;
+  return by_rank(r, [&](auto rc) {
+    constexpr int R_ = decltype(rc)::value;
+    const int e = launch_down<R_>(d, p, st);
+    return e != DQ_OK ? e : launch_up<R_>(u, p, M, sms, st);
+  });
+}
+
+}  // namespace
+}  // namespace dq
+
+using namespace dq;
+
+extern "C" {
+
+size_t dq_adapter_plan_bytes(int64_t M, int64_t R, int A) {
+  if (plan_shape(M, R, A) != DQ_OK) return 0;
+  return static_cast<size_t>(adapter_plan_layout(M, R, A).words) * 4;
+}
+
+int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64_t M, int A, void* plan,
+                    size_t plan_bytes, dq_stream_t stream) {
+  int rc = plan_shape(M, R, A);
+  if (rc != DQ_OK) return rc;
+  if (offsets == nullptr || plan == nullptr || (R > 0 && ids == nullptr)) return DQ_ERR_ARG;
+  if (!aligned(ids, 4) || !aligned(offsets, 4) || !aligned(plan, 16)) return DQ_ERR_ALIGN;
+  if (plan_bytes < dq_adapter_plan_bytes(M, R, A)) return DQ_ERR_WORKSPACE;
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != DQ_OK) return rc;
+  unsigned int* error = nullptr;
+  if ((rc = error_word(&error)) != DQ_OK) return rc;
+  const AdapterPlan lay = adapter_plan_layout(M, R, A);
+  int32_t* words = static_cast<int32_t*>(plan);
+  const int grid = static_cast<int>(ceil_div(A + 1, 8));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  adapter_count_kernel<<<grid, 256, 0, st>>>(ids, offsets, static_cast<int>(R), static_cast<int>(M), A,
+                                             words + lay.off_counts, error);
+  adapter_place_kernel<<<grid, 256, 0, st>>>(ids, offsets, static_cast<int>(R), static_cast<int>(M), A, words,
+                                             lay, error);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+size_t dq_adapter_add_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
+  int sms = 0;
+  if (bank_shape(M, R, K, N, r, A) != DQ_OK || device_sms(&sms) != DQ_OK) return 0;
+  return part_bytes(M, R, A, K, r, sms);
+}
+
+int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t M, int64_t R, int64_t K,
+                   int64_t N, const void* down, const void* up, const float* scale, int r, int A,
+                   const void* plan, int act, void* out, int64_t ldo, void* hidden, void* workspace,
+                   size_t workspace_bytes, dq_stream_t stream) {
+  if (act < kActNone || act > kActGeGluTanh) return DQ_ERR_ARG;
+  int rc = bank_shape(M, R, K, N, r, A);
+  if (rc != DQ_OK) return rc;
+  const bool gated = act_is_gated(act);
+  if (gated && N % 32 != 0) return DQ_ERR_SHAPE;
+  if (!row_stride_ok(ldy, N) || !row_stride_ok(ldx, K) || !row_stride_ok(ldo, gated ? N / 2 : N)) return DQ_ERR_SHAPE;
+  if (M == 0) return DQ_OK;
+  if (y == nullptr || x == nullptr || down == nullptr || up == nullptr || scale == nullptr || plan == nullptr ||
+      out == nullptr)
+    return DQ_ERR_ARG;
+  if (gated && out == y) return DQ_ERR_ARG;  // rows change their width
+  if (out == y && ldo != ldy) return DQ_ERR_SHAPE;
+  if (!aligned(y, 16) || !aligned(x, 16) || !aligned(down, 16) || !aligned(up, 16) || !aligned(scale, 4) ||
+      !aligned(plan, 16) || !aligned(out, 16) || !aligned(hidden, 16))
+    return DQ_ERR_ALIGN;
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != DQ_OK) return rc;
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < part_bytes(M, R, A, K, r, sms))
+    return DQ_ERR_WORKSPACE;
+  return down_up(x, ldx, K, down, y, ldy, N, up, scale, M, R, r, A, static_cast<const int32_t*>(plan), act, out,
+                 ldo, hidden, workspace, sms, static_cast<cudaStream_t>(stream));
+}
+
+size_t dq_adapter_backward_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
+  int sms = 0;
+  if (bank_shape(M, R, K, N, r, A) != DQ_OK || device_sms(&sms) != DQ_OK) return 0;
+  return backward_ws(M, R, K, N, r, A, sms).total;
+}
+
+int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* x_scales,
+                        const void* hidden, int64_t M, int64_t R, int64_t K, int64_t N, const void* down,
+                        const void* up, const float* scale, int r, int A, const void* plan, const void* dx,
+                        int64_t lddx, void* dx_out, int64_t lddxo, void* ddown, void* dup, void* workspace,
+                        size_t workspace_bytes, dq_stream_t stream) {
+  int rc = bank_shape(M, R, K, N, r, A);
+  if (rc != DQ_OK) return rc;
+  const bool i8 = x_scales != nullptr;
+  const bool want_w = ddown != nullptr;
+  if (!row_stride_ok(lddy, N) || (i8 && (K % 16 != 0 || ldx < K || ldx % 16 != 0)) ||
+      (want_w && !i8 && !row_stride_ok(ldx, K)))
+    return DQ_ERR_SHAPE;
+  if (!row_stride_ok(lddx, K) || !row_stride_ok(lddxo, K)) return DQ_ERR_SHAPE;
+  if ((ddown == nullptr) != (dup == nullptr)) return DQ_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (want_w && (cudaMemsetAsync(ddown, 0, static_cast<size_t>(A) * r * K * 2, st) != cudaSuccess ||
+                   cudaMemsetAsync(dup, 0, static_cast<size_t>(A) * r * N * 2, st) != cudaSuccess))
+      return DQ_ERR_CUDA;
+    return DQ_OK;
+  }
+  if (dy == nullptr || down == nullptr || up == nullptr || scale == nullptr || plan == nullptr ||
+      dx == nullptr || dx_out == nullptr || (want_w && (x == nullptr || hidden == nullptr)))
+    return DQ_ERR_ARG;
+  if (dx == dx_out && lddx != lddxo) return DQ_ERR_SHAPE;
+  if (!aligned(dy, 16) || !aligned(x, 16) || !aligned(x_scales, 4) || !aligned(hidden, 16) || !aligned(down, 16) ||
+      !aligned(up, 16) || !aligned(scale, 4) || !aligned(plan, 16) || !aligned(dx, 16) || !aligned(dx_out, 16) ||
+      !aligned(ddown, 16) || !aligned(dup, 16))
+    return DQ_ERR_ALIGN;
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != DQ_OK) return rc;
+  const BackwardWs w = backward_ws(M, R, K, N, r, A, sms);
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < w.total) return DQ_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int32_t* words = static_cast<const int32_t*>(plan);
+  const AdapterPlan lay = adapter_plan_layout(M, R, A);
+  void* g = ws + w.part;
+  rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo,
+               want_w ? g : nullptr, ws, sms, st);
+  if (rc != DQ_OK || !want_w) return rc;
+  rc = wgrad(dy, lddy, nullptr, hidden, M, R, N, r, A, words, lay, ws + w.part + w.g, dup, sms, st);
+  if (rc != DQ_OK) return rc;
+  return wgrad(x, ldx, x_scales, g, M, R, K, r, A, words, lay, ws + w.part + w.g + w.up, ddown, sms, st);
+}
+
+int dq_checkpoint_pack(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* codes, float* scales,
+                       dq_stream_t stream) {
+  if (M < 0 || M > INT32_MAX || K <= 0 || K > INT32_MAX || K % 16 != 0 || !row_stride_ok(ldx, K)) return DQ_ERR_SHAPE;
+  if (M == 0) return DQ_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return DQ_ERR_ARG;
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4)) return DQ_ERR_ALIGN;
+  int sms = 0;
+  const int rc = device_sms(&sms);
+  if (rc != DQ_OK) return rc;
+  const int nrun = static_cast<int>(ceil_div(K, kCkptRun));
+  const int64_t runs = M * nrun;
+  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(runs, 16), static_cast<int64_t>(sms) * 8));
+  checkpoint_pack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const __nv_bfloat16*>(x), ldx, runs, nrun, static_cast<int>(K), codes, scales);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+int dq_checkpoint_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t K, void* out, int64_t ldo,
+                         dq_stream_t stream) {
+  if (M < 0 || M > INT32_MAX || K <= 0 || K > INT32_MAX || K % 16 != 0 || !row_stride_ok(ldo, K)) return DQ_ERR_SHAPE;
+  if (M == 0) return DQ_OK;
+  if (codes == nullptr || scales == nullptr || out == nullptr) return DQ_ERR_ARG;
+  if (!aligned(codes, 16) || !aligned(scales, 4) || !aligned(out, 16)) return DQ_ERR_ALIGN;
+  int sms = 0;
+  const int rc = device_sms(&sms);
+  if (rc != DQ_OK) return rc;
+  const int64_t total = M * (K / 8);
+  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(total, 256), static_cast<int64_t>(sms) * 8));
+  checkpoint_unpack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      codes, scales, M, static_cast<int>(K), static_cast<int>(ceil_div(K, kCkptRun)),
+      static_cast<__nv_bfloat16*>(out), ldo);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+size_t dq_linear_dgrad_workspace(int64_t N, int64_t K) {
+  return N <= 0 || K <= 0 ? 0 : up256(static_cast<size_t>(N) * K * 2);
+}
+
+static int dgrad_impl(int fmt, const void* dy, int64_t M, int64_t N, const uint8_t* w, const void* absmax, int sbf,
+                      float scale, int64_t K, void* dx, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  if (M < 0 || N <= 0 || K <= 0 || N % 8 != 0 || K % (fmt == kFmtNF4 ? 64 : 16) != 0 || M > INT32_MAX ||
+      N > INT32_MAX || K > INT32_MAX || ceil_div(N, 128) > 65535)
+    return DQ_ERR_SHAPE;
+  if (M == 0) return DQ_OK;
+  if (dy == nullptr || w == nullptr || dx == nullptr || (fmt == kFmtNF4 && absmax == nullptr)) return DQ_ERR_ARG;
+  if (!aligned(dy, 16) || !aligned(w, 16) || !aligned(dx, 16) || !aligned(absmax, sbf ? 2 : 4)) return DQ_ERR_ALIGN;
+  int sms = 0;
+  const int rc = device_sms(&sms);
+  if (rc != DQ_OK) return rc;
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_linear_dgrad_workspace(N, K))
+    return DQ_ERR_WORKSPACE;
+  const dim3 grid(static_cast<unsigned>(ceil_div(K, 64)), static_cast<unsigned>(ceil_div(N, 128)));
+  if (fmt == kFmtNF4)
+    decode_transposed_kernel<kFmtNF4><<<grid, 256, 0, st>>>(w, absmax, sbf, 0.f, static_cast<int>(N),
+                                                            static_cast<int>(K),
+                                                            static_cast<__nv_bfloat16*>(workspace));
+  else
+    decode_transposed_kernel<kFmtFP8><<<grid, 256, 0, st>>>(w, nullptr, 0, scale, static_cast<int>(N),
+                                                            static_cast<int>(K),
+                                                            static_cast<__nv_bfloat16*>(workspace));
+  if (cudaGetLastError() != cudaSuccess) return DQ_ERR_LAUNCH;
+  return bf16_gemm(dy, M, N, workspace, K, dx, K, st);
+}
+
+int dq_linear_nf4_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* packed, const void* absmax,
+                        int scale_dtype, int64_t K, void* dx, void* workspace, size_t workspace_bytes,
+                        dq_stream_t stream) {
+  if (scale_dtype != DQ_DTYPE_F32 && scale_dtype != DQ_DTYPE_BF16) return DQ_ERR_ARG;
+  return dgrad_impl(kFmtNF4, dy, M, N, packed, absmax, scale_dtype == DQ_DTYPE_BF16, 0.f, K, dx, workspace,
+                    workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int dq_linear_fp8_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* w8, float scale, int64_t K, void* dx,
+                        void* workspace, size_t workspace_bytes, dq_stream_t stream) {
+  return dgrad_impl(kFmtFP8, dy, M, N, w8, nullptr, 0, scale, K, dx, workspace, workspace_bytes,
+                    static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@
 
 #include "../../include/dq_linear.h"
 #include "../../include/dq_dit.h"
+#include "dq_internal.h"
 #include "dq_gemm.cuh"
 #include "dq_gemm2.cuh"
 #include "dq_bf16gemm2.cuh"
@@ -383,7 +384,8 @@ constexpr int kTwoPhaseGroupN = 16;
 // as far as their partial sums fit it; only a forced split count can exceed it.
 static Plan make_plan(int fmt, int64_t M, int64_t N, int64_t K, int sms, bool allow_split = true,
                       bool allow_twophase = true, bool allow_smallm = true,
-                      size_t max_split_ws = SIZE_MAX, bool gated = false) {
+                      size_t max_split_ws = SIZE_MAX, bool gated = false,
+                      bool force_pair_gemm = false) {
   Plan p;
   int long_k_split = 0;
   const int KB = static_cast<int>((K + 63) / 64);
@@ -426,8 +428,9 @@ static Plan make_plan(int fmt, int64_t M, int64_t N, int64_t K, int sms, bool al
   }
   auto units_of = [&](bool pair) { return pair ? sms / 2 : sms; };
   auto n_tiles_of = [&](bool pair) { return static_cast<int>((N + (pair ? 255 : 127)) / (pair ? 256 : 128)); };
-  const bool twophase = allow_twophase && M > 64 &&
-                        (opair == 3 || opair == 4 || (opair == 0 && M >= kTwoPhaseMinM));
+  const bool twophase = force_pair_gemm ||
+                        (allow_twophase && M > 64 &&
+                         (opair == 3 || opair == 4 || (opair == 0 && M >= kTwoPhaseMinM)));
   if (twophase) {
     p.pair = true;
     p.twophase = true;
@@ -1095,6 +1098,65 @@ static int linear_impl(int fmt, const void* x, int64_t M, int64_t K, const uint8
   return DQ_OK;
 }
 
+// The bf16 pair GEMM on operands that are already bf16 (dq_internal.h): the
+// two-phase plan's tile choice, no decode warps.
+int bf16_gemm(const void* x, int64_t M, int64_t K, const void* w, int64_t N, void* y, int64_t ldy,
+              cudaStream_t st) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 8 != 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX ||
+      ldy < N || ldy > INT32_MAX)
+    return DQ_ERR_SHAPE;
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 2)) return DQ_ERR_ALIGN;
+  DeviceInfo* d = nullptr;
+  const int rc = current_device(&d);
+  if (rc != DQ_OK) return rc;
+  const Plan p = make_plan(kFmtFP8, M, N, K, d->sms, false, true, false, SIZE_MAX, false, true);
+  CUtensorMap mx, ma;
+  if (!make_map_2d(&mx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, M, K * 2, 64, p.bm / 2,
+                   CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map_2d(&ma, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, N, K * 2, 64, 128,
+                   CU_TENSOR_MAP_SWIZZLE_128B))
+    return DQ_ERR_CUDA;
+  GemmArgs g = {};
+  g.M = static_cast<int>(M);
+  g.N = static_cast<int>(N);
+  g.K = static_cast<int>(K);
+  g.num_n_tiles = p.n_tiles;
+  g.tile_n = 256;
+  g.num_tiles = p.tiles;
+  g.splits = 1;
+  g.kb_per_split = p.kb_per_split;
+  g.group_n = kTwoPhaseGroupN;
+  g.act = kActNone;
+  g.outs[0] = y;
+  g.n_out = 1;
+  g.ldy = static_cast<int>(ldy);
+  g.vec_ok = (N % 8 == 0) && (ldy % 8 == 0) && aligned(y, 16);
+  return launch_bf16_gemm2_bm<-1>(d, p, mx, ma, g, st);
+}
+
+int device_sms(int* sms) {
+  DeviceInfo* d = nullptr;
+  const int rc = current_device(&d);
+  if (rc == DQ_OK) *sms = d->sms;
+  return rc;
+}
+
+static std::atomic<unsigned int*> g_error_addr[kMaxDevices];
+
+int error_word(unsigned int** word) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
+  unsigned int* p = g_error_addr[dev].load(std::memory_order_acquire);
+  if (p == nullptr) {
+    void* a = nullptr;
+    if (cudaGetSymbolAddress(&a, g_dq_error) != cudaSuccess || a == nullptr) return DQ_ERR_CUDA;
+    p = static_cast<unsigned int*>(a);
+    g_error_addr[dev].store(p, std::memory_order_release);
+  }
+  *word = p;
+  return DQ_OK;
+}
+
 static int tp_impl(int fmt, const void* x, int64_t M, int64_t K, const uint8_t* w,
                    const float* absmax, float scale, const void* bias, int64_t N, int rank,
                    int world, void* const* y_ranks, unsigned int* const* flag_ranks,
@@ -1145,6 +1207,7 @@ const char* dq_status_string(int s) {
     case DQ_ERR_WORKSPACE: return "workspace missing or too small";
     case DQ_ERR_ARG: return "null operand or unknown enum";
     case DQ_ERR_CUDA: return "CUDA runtime error";
+    case DQ_ERR_INDEX: return "an adapter index or a request offset was out of range";
     case DQ_ERR_SCRATCH_LIMIT:
       return "shape needs more split-K scratch than the allocation-free entry point holds (8 MiB)";
   }
@@ -1669,7 +1732,7 @@ int dq_device_error(int* code, dq_stream_t stream) {
   if (cudaStreamSynchronize(st) != cudaSuccess) return DQ_ERR_CUDA;
   const unsigned int zero = 0;
   if (v != 0 && cudaMemcpyToSymbol(g_dq_error, &zero, sizeof(zero)) != cudaSuccess) return DQ_ERR_CUDA;
-  *code = (v & (1u << kErrTimeout)) ? DQ_ERR_TIMEOUT : DQ_OK;
+  *code = (v & (1u << kErrTimeout)) ? DQ_ERR_TIMEOUT : (v & (1u << kErrIndex)) ? DQ_ERR_INDEX : DQ_OK;
   return DQ_OK;
 }
 

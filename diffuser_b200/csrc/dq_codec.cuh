@@ -19,6 +19,8 @@
 
 namespace dq {
 
+enum : int { kFmtNF4 = 0, kFmtFP8 = 1 };
+
 // bf16 bit patterns of the 16 NF4 levels of R/nf4_ltx23.R:15-21
 // (double literal -> float -> bf16, round to nearest even).
 constexpr uint16_t kNf4LevelBits[16] = {0xBF80, 0xBF32, 0xBF06, 0xBECA, 0xBE92, 0xBE3D,

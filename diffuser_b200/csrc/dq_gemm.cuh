@@ -39,11 +39,11 @@
 
 namespace dq {
 
-enum : int { kFmtNF4 = 0, kFmtFP8 = 1 };
 enum : unsigned int { kErrTimeout = 5u };
 
 // Per-device kernel error word (bit kErrTimeout: a bounded wait expired).
-// The library is a single translation unit, so it is defined here.
+// The GEMM kernels' translation unit defines it; others take its address
+// (error_word, dq_internal.h).
 __device__ unsigned int g_dq_error = 0;
 
 // Optional per-role timestamps (SM clock) of CTA 0, for pipeline analysis.

@@ -1,0 +1,26 @@
+// dq_internal.h -- what the translation units of the library share besides the
+// public headers (none of it is exported API).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace dq {
+
+// Facts of the current device; DQ_ERR_ARCH unless it is an sm_100.
+int device_sms(int* sms);
+
+// Device address of the current device's kernel error word (dq_device_error
+// reads and clears it): kernels of other translation units record bits there.
+// The first call on a device looks it up; it is cached from then on.
+int error_word(unsigned int** word);
+
+// Bits of the error word besides kErrTimeout (dq_gemm.cuh).
+enum : unsigned int { kErrIndex = 10u };
+
+// y[M, N] (row stride ldy) = x[M, K] . w[N, K]^T, all bf16, on the CTA-pair
+// GEMM without its decode.  K % 8 == 0, x / w 16-byte aligned.
+int bf16_gemm(const void* x, int64_t M, int64_t K, const void* w, int64_t N, void* y, int64_t ldy,
+              cudaStream_t st);
+
+}  // namespace dq

@@ -1,0 +1,156 @@
+// dq_norm.cu -- host side of dq_gated_norm and its backward pass
+// (include/dq_dit.h): argument validation and launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/dq_dit.h"
+#include "dq_internal.h"
+#include "dq_norm.cuh"
+
+namespace dq {
+namespace {
+
+inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
+inline const __nv_bfloat16* bf(const void* p) { return static_cast<const __nv_bfloat16*>(p); }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool stride_ok(int64_t ld, int D) { return ld >= D && ld % 4 == 0; }
+
+int shape_ok(int64_t T, int S, int D) {
+  return T < 0 || S <= 0 || D <= 0 || D % 4 != 0 || D > 8192 || T > INT32_MAX || T % S != 0 ? DQ_ERR_SHAPE : DQ_OK;
+}
+
+bool norms_ok(int post, int pre, const void* post_w) {
+  return post >= kNormNone && post <= kNormLayer && (pre == kNormRms || pre == kNormLayer) &&
+         (post_w == nullptr || post != kNormNone);
+}
+
+// Row runs of the backward pass: two CTAs per SM (one of the 512-thread form)
+// over all batch elements, at least four rows each.
+int chunks_of(int64_t B, int S, int D, int sms) {
+  const int64_t slots = static_cast<int64_t>(sms) * (D <= 4096 ? 2 : 1);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(1, B), ceil_div(S, 4))));
+}
+
+template <bool OPS>
+void launch_forward(const NormArgs& a, int sms, cudaStream_t st) {
+  const int runs = (a.D / 4 + 255) / 256;
+  auto go = [&](auto kern) {
+    int per_sm = 1;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, 256, 0);
+    const int grid = static_cast<int>(std::min<int64_t>(a.T, static_cast<int64_t>(sms) * std::max(per_sm, 1)));
+    kern<<<grid, 256, 0, st>>>(a);
+  };
+  switch (runs) {
+    case 1: return go(gated_norm_kernel<1, OPS>);
+    case 2: return go(gated_norm_kernel<2, OPS>);
+    case 3: return go(gated_norm_kernel<3, OPS>);
+    case 4: return go(gated_norm_kernel<4, OPS>);
+    case 5:
+    case 6: return go(gated_norm_kernel<6, OPS>);
+  }
+  go(gated_norm_kernel<8, OPS>);
+}
+
+}  // namespace
+}  // namespace dq
+
+using namespace dq;
+
+extern "C" {
+
+int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int64_t T, int S, int D,
+                  const void* gate, int64_t ld_gate, const void* scale, const void* shift, int64_t ld_mod,
+                  const void* post_weight, const void* pre_weight, int post, int pre, float residual_scale, float eps,
+                  int rounding, void* s, int64_t ld_s, void* h, int64_t ld_h, dq_stream_t stream) {
+  int rc = shape_ok(T, S, D);
+  if (rc != DQ_OK) return rc;
+  if (!norms_ok(post, pre, post_weight) || rounding < DQ_ROUND_ONCE || rounding > DQ_ROUND_OPS) return DQ_ERR_ARG;
+  if (T == 0) return DQ_OK;
+  if (x == nullptr || y == nullptr || s == nullptr || h == nullptr) return DQ_ERR_ARG;
+  if (!stride_ok(ld_x, D) || !stride_ok(ld_y, D) || !stride_ok(ld_s, D) || !stride_ok(ld_h, D) ||
+      (gate != nullptr && !stride_ok(ld_gate, D)) ||
+      ((scale != nullptr || shift != nullptr) && !stride_ok(ld_mod, D)))
+    return DQ_ERR_SHAPE;
+  for (const void* p : {x, y, gate, scale, shift, post_weight, pre_weight, static_cast<const void*>(s),
+                        static_cast<const void*>(h)})
+    if (!aligned8(p)) return DQ_ERR_ALIGN;
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != DQ_OK) return rc;
+  NormArgs a = {bf(x), bf(y), bf(gate), bf(scale), bf(shift), bf(post_weight), bf(pre_weight),
+                static_cast<__nv_bfloat16*>(s), static_cast<__nv_bfloat16*>(h), ld_x, ld_y, ld_gate, ld_mod, ld_s,
+                ld_h, T, S, D, post, pre, residual_scale, eps};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rounding == DQ_ROUND_OPS)
+    launch_forward<true>(a, sms, st);
+  else
+    launch_forward<false>(a, sms, st);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+size_t dq_gated_norm_backward_workspace(int64_t T, int S, int D) {
+  int sms = 0;
+  if (shape_ok(T, S, D) != DQ_OK || T == 0 || device_sms(&sms) != DQ_OK) return 0;
+  const int64_t B = T / S;
+  return static_cast<size_t>(B) * chunks_of(B, S, D, sms) * 3 * D * sizeof(float);
+}
+
+int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_t ld_dh, const void* s, int64_t ld_s,
+                           const void* y, int64_t ld_y, int64_t T, int S, int D, const void* gate, int64_t ld_gate,
+                           const void* scale, int64_t ld_mod, const void* post_weight, const void* pre_weight, int post,
+                           int pre, float residual_scale, float eps, void* dx, int64_t ld_dx, void* dy, int64_t ld_dy,
+                           float* dgate, float* dscale, float* dshift, float* dpost_weight, float* dpre_weight,
+                           void* workspace, size_t workspace_bytes, dq_stream_t stream) {
+  int rc = shape_ok(T, S, D);
+  if (rc != DQ_OK) return rc;
+  if (!norms_ok(post, pre, post_weight)) return DQ_ERR_ARG;
+  const int64_t B = T / S;
+  if (B > 65535) return DQ_ERR_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {  // no tokens: the weights' gradients are zeros
+    for (float* p : {dpost_weight, dpre_weight})
+      if (p != nullptr && cudaMemsetAsync(p, 0, static_cast<size_t>(D) * 4, st) != cudaSuccess) return DQ_ERR_CUDA;
+    return DQ_OK;
+  }
+  if (dh == nullptr || s == nullptr || y == nullptr || dx == nullptr || dy == nullptr) return DQ_ERR_ARG;
+  if ((ds != nullptr && !stride_ok(ld_ds, D)) || !stride_ok(ld_dh, D) || !stride_ok(ld_s, D) || !stride_ok(ld_y, D) ||
+      !stride_ok(ld_dx, D) || !stride_ok(ld_dy, D) || (gate != nullptr && !stride_ok(ld_gate, D)) ||
+      (scale != nullptr && !stride_ok(ld_mod, D)))
+    return DQ_ERR_SHAPE;
+  for (const void* p : {ds, dh, s, y, gate, scale, post_weight, pre_weight, static_cast<const void*>(dx),
+                        static_cast<const void*>(dy)})
+    if (!aligned8(p)) return DQ_ERR_ALIGN;
+  for (const float* p : {dgate, dscale, dshift, dpost_weight, dpre_weight})
+    if ((reinterpret_cast<uintptr_t>(p) & 3) != 0) return DQ_ERR_ALIGN;
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != DQ_OK) return rc;
+  const int chunks = chunks_of(B, S, D, sms);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+      workspace_bytes < static_cast<size_t>(B) * chunks * 3 * D * sizeof(float))
+    return DQ_ERR_WORKSPACE;
+  NormGradArgs a = {bf(ds), bf(dh), bf(s), bf(y), bf(gate), bf(scale), bf(post_weight), bf(pre_weight),
+                    static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dy), static_cast<float*>(workspace),
+                    ld_ds, ld_dh, ld_s, ld_y, ld_gate, ld_mod, ld_dx, ld_dy, S, D, post, pre,
+                    static_cast<int>(ceil_div(S, chunks)), residual_scale, eps};
+  const dim3 grid(chunks, static_cast<unsigned>(B));
+  const int runs = D / 4;
+  if (runs <= 256)
+    gated_norm_backward_kernel<256, 1><<<grid, 256, 0, st>>>(a);
+  else if (runs <= 512)
+    gated_norm_backward_kernel<256, 2><<<grid, 256, 0, st>>>(a);
+  else if (runs <= 768)
+    gated_norm_backward_kernel<256, 3><<<grid, 256, 0, st>>>(a);
+  else if (runs <= 1024)
+    gated_norm_backward_kernel<256, 4><<<grid, 256, 0, st>>>(a);
+  else
+    gated_norm_backward_kernel<512, 4><<<grid, 512, 0, st>>>(a);
+  NormReduceArgs q = {a.part, a.gate, a.scale, a.post_w, a.pre_w, dgate, dscale, dshift, dpost_weight, dpre_weight,
+                      ld_gate, ld_mod, static_cast<int>(B), chunks, D, residual_scale};
+  if (dgate != nullptr || dscale != nullptr || dshift != nullptr || dpost_weight != nullptr || dpre_weight != nullptr)
+    gated_norm_reduce_kernel<<<static_cast<unsigned>(ceil_div(D, 32)), 256, 0, st>>>(q);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _lib, modules
+from . import _lib, modules, ops
 
 
 # ------------------------------------------------------ fused attention glue
@@ -160,6 +160,132 @@ def gated_residual(x, gate, y):
     rc = _lib.lib().dq_gated_residual(_ptr(x), ldx, _ptr(gate), ldm, _ptr(y), ldy, b * s, s, d,
                                       _ptr(out), d, stream)
     _lib.check("dq_gated_residual", rc)
+    return out
+
+
+_NORMS = {None: _lib.DQ_NORM_NONE, "rms": _lib.DQ_NORM_RMS, "layer": _lib.DQ_NORM_LAYER}
+_ROUNDINGS = {"once": _lib.DQ_ROUND_ONCE, "ops": _lib.DQ_ROUND_OPS}
+
+
+def _token_rows(t, name, like):
+    """t [B, S, D] bf16 as evenly spaced rows whose starts are 8-byte aligned
+    (copied when they are not), and the row stride."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor: the engine has no CPU path")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.shape != like.shape or t.device != like.device:
+        raise ValueError(f"{name} is {tuple(t.shape)} on {t.device}, expected {tuple(like.shape)} on {like.device}")
+    b, s, d = t.shape
+    even = t.stride(2) == 1 and t.stride(1) >= d and t.stride(1) % 4 == 0 and t.data_ptr() % 8 == 0 and \
+        (b == 1 or t.stride(0) == s * t.stride(1))
+    if not even:
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t, t.stride(1)
+
+
+def _features(t, name, shape, like):
+    """A [B, D] modulation or a [D] weight in bf16 with aligned rows, or None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != like.device:
+        raise ValueError(f"{name} must be a tensor on {like.device}")
+    if t.dtype != torch.bfloat16 or t.shape != shape:
+        raise TypeError(f"{name} must be bfloat16 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.stride(-1) != 1 or t.data_ptr() % 8 != 0 or (t.dim() == 2 and (t.stride(0) % 4 != 0 or t.stride(0) < t.shape[1])):
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t
+
+
+def _norm_args(x, gate, scale, shift, post, pre, post_weight, pre_weight):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("the activations must be CUDA tensors: the engine has no CPU path")
+    if x.dim() != 3:
+        raise ValueError(f"activations must be [batch, tokens, features], got {tuple(x.shape)}")
+    if post not in _NORMS or pre not in ("rms", "layer"):
+        raise ValueError("post must be None, 'rms' or 'layer' and pre 'rms' or 'layer'")
+    if post is None and post_weight is not None:
+        raise ValueError("post_weight needs a post norm")
+    b, _, d = x.shape
+    if d % 4 != 0 or d > 8192 or d == 0:
+        raise ValueError("gated_norm needs a feature count that is a multiple of 4 up to 8192")
+    gate = _features(gate, "gate", (b, d), x)
+    scale = _features(scale, "scale", (b, d), x)
+    shift = _features(shift, "shift", (b, d), x)
+    if scale is not None and shift is not None and scale.stride(0) != shift.stride(0):
+        scale, shift = scale.contiguous(), shift.contiguous()
+    mod = scale if scale is not None else shift
+    return (gate, 0 if gate is None else max(gate.stride(0), d), scale, shift,
+            0 if mod is None else max(mod.stride(0), d), _features(post_weight, "post_weight", (d,), x),
+            _features(pre_weight, "pre_weight", (d,), x))
+
+
+def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_weight=None, scale=None,
+               shift=None, residual_scale: float = 1.0, eps: float = 1e-6, rounding: str = "once"):
+    """The boundary between two blocks in one kernel: the norm behind a block
+    with its gate and residual scale, the residual add, and the norm before the
+    next block with its modulation,
+
+        s = x + residual_scale * gate * N_post(y) * post_weight
+        h = N_pre(s) * pre_weight * (1 + scale) + shift
+
+    for x, y [B, S, D] bf16; gate, scale, shift [B, D]; weights [D]; any of the
+    latter may be None.  post: None, "rms" or "layer"; pre: "rms" or "layer".
+    rounding="once" computes in float32 and rounds s and h; "ops" rounds after
+    every op as the chain of tensor ops does (the bits of gated_residual
+    followed by adaln_modulate).  Returns (s, h)."""
+    gate, ldg, scale, shift, ldm, pw, qw = _norm_args(x, gate, scale, shift, post, pre, post_weight, pre_weight)
+    if rounding not in _ROUNDINGS:
+        raise ValueError("rounding must be 'once' or 'ops'")
+    b, n, d = x.shape
+    x2, ldx = _token_rows(x, "x", x)
+    y2, ldy = _token_rows(y, "y", x)
+    s = torch.empty((b, n, d), dtype=torch.bfloat16, device=x.device)
+    h = torch.empty((b, n, d), dtype=torch.bfloat16, device=x.device)
+    if x.numel() == 0:
+        return s, h
+    with ops._on(x):
+        _lib.check("dq_gated_norm", _lib.lib().dq_gated_norm(
+            _ptr(x2), ldx, _ptr(y2), ldy, b * n, n, d, _ptr(gate), ldg, _ptr(scale), _ptr(shift), ldm, _ptr(pw),
+            _ptr(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ROUNDINGS[rounding], _ptr(s), d, _ptr(h), d,
+            ops._stream(x.device)))
+    return s, h
+
+
+def gated_norm_backward(ds, dh, s, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_weight=None,
+                        scale=None, shift=None, residual_scale: float = 1.0, eps: float = 1e-6):
+    """Gradients of gated_norm: ds (or None) and dh [B, S, D] are the gradients
+    of its two results, s the one it returned, y and the rest its arguments.
+    Returns a dict: dx and dy bf16, dgate, dscale, dshift float32 [B, D] and
+    dpost_weight, dpre_weight float32 [D], None for those that were not given.
+    The same inputs give the same bits."""
+    gate, ldg, scale, shift, ldm, pw, qw = _norm_args(s, gate, scale, shift, post, pre, post_weight, pre_weight)
+    b, n, d = s.shape
+    s2, lds = _token_rows(s, "s", s)
+    y2, ldy = _token_rows(y, "y", s)
+    dh2, lddh = _token_rows(dh, "dh", s)
+    ds2, ldds = (None, 0) if ds is None else _token_rows(ds, "ds", s)
+    dx, dy = (torch.empty((b, n, d), dtype=torch.bfloat16, device=s.device) for _ in range(2))
+
+    def grad(of, *shape):
+        return None if of is None else torch.empty(shape, dtype=torch.float32, device=s.device)
+
+    out = dict(dx=dx, dy=dy, dgate=grad(gate, b, d), dscale=grad(scale, b, d), dshift=grad(shift, b, d),
+               dpost_weight=grad(pw, d), dpre_weight=grad(qw, d))
+    if s.numel() == 0:
+        for g in out.values():
+            if g is not None:
+                g.zero_()
+        return out
+    with ops._on(s):
+        lib = _lib.lib()
+        nbytes = lib.dq_gated_norm_backward_workspace(b * n, n, d)
+        ws = ops._scratch(nbytes, s)
+        _lib.check("dq_gated_norm_backward", lib.dq_gated_norm_backward(
+            _ptr(ds2), ldds, _ptr(dh2), lddh, _ptr(s2), lds, _ptr(y2), ldy, b * n, n, d, _ptr(gate), ldg,
+            _ptr(scale), ldm, _ptr(pw), _ptr(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ptr(dx), d,
+            _ptr(dy), d, _ptr(out["dgate"]), _ptr(out["dscale"]), _ptr(out["dshift"]), _ptr(out["dpost_weight"]),
+            _ptr(out["dpre_weight"]), _ptr(ws), nbytes, ops._stream(s.device)))
     return out
 
 

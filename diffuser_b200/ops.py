@@ -7,6 +7,7 @@ CPU tensor, a non-bf16 activation or a missing library raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 
@@ -331,8 +332,307 @@ def fp8_linear(x: torch.Tensor, w8: torch.Tensor, scale: float,
     return y.reshape(*x.shape[:-1], n_out)
 
 
+# ----------------------------------------------------------------- adapters
+def _on(t: torch.Tensor):
+    """Makes t's device the current one for the duration of a call."""
+    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    """Workspace of one call, from torch's allocator: calls on several streams
+    and captured graphs each hold their own."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=like.device)
+
+
+def _same_device(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    _require_cuda(t, name)
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+
+
+def _rows16(t: torch.Tensor, name: str, width: int, like: torch.Tensor) -> torch.Tensor:
+    """t as bf16 rows [-1, width] with unit stride along the features, 16-byte
+    aligned row starts and evenly spaced rows (copied when it is not)."""
+    _same_device(t, name, like)
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{name} must have {width} features, got shape {tuple(t.shape)}")
+    t2 = t if t.dim() == 2 else t.reshape(-1, width)
+    if t2.stride(1) != 1 or t2.stride(0) % 8 != 0 or t2.stride(0) < width or t2.data_ptr() % 16 != 0:
+        t2 = t2.new_empty(t2.shape).copy_(t2)
+    return t2
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _bank(down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, like: torch.Tensor):
+    """(adapters, rank, in_features, out_features) of a checked adapter bank."""
+    for t, name in ((down, "down"), (up, "up")):
+        _same_device(t, name, like)
+        if t.dtype != torch.bfloat16 or t.dim() != 3 or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous bfloat16 [adapters, rank, features] tensor")
+    a, r, k = down.shape
+    if up.shape[:2] != (a, r):
+        raise ValueError("down and up must hold the same adapters and rank")
+    _same_device(scale, "scale", like)
+    if scale.dtype != torch.float32 or scale.shape != (a,) or not scale.is_contiguous():
+        raise TypeError("scale must be a contiguous float32 [adapters] tensor")
+    if r % 8 != 0 or r > 128 or k % 8 != 0 or up.shape[2] % 8 != 0:
+        raise ValueError("rank (at most 128) and features must be multiples of 8")
+    return a, r, k, up.shape[2]
+
+
+class AdapterPlan:
+    """The tokens of a batch sorted by adapter (adapter_plan builds it)."""
+
+    def __init__(self, ids, offsets, n_adapters: int, tokens: int):
+        self.tokens, self.requests, self.n_adapters = int(tokens), ids.numel(), int(n_adapters)
+        nbytes = int(_lib.lib().dq_adapter_plan_bytes(self.tokens, self.requests, self.n_adapters))
+        if nbytes == 0:
+            raise ValueError("adapter_plan: tokens must be 0..2^30 and n_adapters 1..65536")
+        self.words = torch.empty(nbytes // 4, dtype=torch.int32, device=ids.device)
+        self.update_(ids, offsets)
+
+    def update_(self, ids: torch.Tensor, offsets: torch.Tensor) -> "AdapterPlan":
+        """Rebuild in place for new ids / offsets of the same counts (also
+        inside a graph capture: the plan's address does not change)."""
+        for t, name in ((ids, "ids"), (offsets, "offsets")):
+            _same_device(t, name, self.words)
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+                raise TypeError(f"{name} must be a contiguous 1-d int32 tensor")
+        if ids.numel() != self.requests or offsets.numel() != self.requests + 1:
+            raise ValueError("offsets must hold one more entry than ids, and both as many as before")
+        with _on(self.words):
+            _lib.check("dq_adapter_plan", _lib.lib().dq_adapter_plan(
+                _ptr(ids), _ptr(offsets), self.requests, self.tokens, self.n_adapters, _ptr(self.words),
+                self.words.numel() * 4, _stream(self.words.device)))
+        return self
+
+
+def adapter_plan(ids: torch.Tensor, offsets: torch.Tensor, tokens: int, n_adapters: int) -> AdapterPlan:
+    """Sort a batch's tokens by adapter, on the device, once for every layer
+    the batch passes.  ids int32 [R]: each request's adapter (-1: none);
+    offsets int32 [R + 1]: request i holds tokens offsets[i] .. offsets[i+1]-1
+    of the batch's `tokens`; tokens outside every request (padding) have no
+    adapter.  Neither is read by the host: ids out of range count as none,
+    offsets out of order leave every token without an adapter, and
+    device_error() then returns DQ_ERR_INDEX."""
+    _require_cuda(ids, "ids")
+    return AdapterPlan(ids, offsets, n_adapters, tokens)
+
+
+def _check_plan(plan: AdapterPlan, m: int, a: int, like: torch.Tensor) -> None:
+    if not isinstance(plan, AdapterPlan):
+        raise TypeError("plan must come from adapter_plan")
+    if plan.tokens != m or plan.n_adapters != a:
+        raise ValueError(f"the plan is for {plan.tokens} tokens and {plan.n_adapters} adapters, "
+                         f"the operands hold {m} and {a}")
+    _same_device(plan.words, "plan", like)
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
+                scale: torch.Tensor, plan: AdapterPlan, act: str | None = None,
+                out: torch.Tensor | None = None, return_hidden: bool = False):
+    """act(y + scale_a * (x . down_a^T) . up_a) for every token with its own
+    adapter a (act(y) where it has none): the low-rank adapters of many
+    requests beside a shared projection's output y [..., N], x [..., K] its
+    input.  down bf16 [A, r, K], up bf16 [A, r, N] (the transposed second
+    factor), scale float32 [A].  act as nf4_linear's; the gated ones take y and
+    up in the gated row order and return N / 2 columns.  out may be y itself
+    (in place, not with a gated act).  With return_hidden also the bf16
+    [tokens, r] scale_a * x . down_a^T that adapter_backward takes."""
+    _require_cuda(y, "y")
+    a, r, k, n = _bank(down, up, scale, y)
+    code, n_out = _act_code(act, n)
+    x2, y2 = _rows16(x, "x", k, y), _rows16(y, "y", n, y)
+    m = y2.shape[0]
+    if x2.shape[0] != m:
+        raise ValueError(f"x holds {x2.shape[0]} tokens, y {m}")
+    _check_plan(plan, m, a, y)
+    if out is None:
+        o2 = torch.empty((m, n_out), dtype=torch.bfloat16, device=y.device)
+    else:
+        o2 = _rows16(out, "out", n_out, y)
+        if o2.data_ptr() != out.data_ptr():
+            raise ValueError("out must have evenly spaced, 16-byte aligned rows with unit feature stride")
+        if o2.shape[0] != m:
+            raise ValueError(f"out holds {o2.shape[0]} tokens, y {m}")
+    hidden = torch.empty((m, r), dtype=torch.bfloat16, device=y.device) if return_hidden else None
+    with _on(y):
+        lib = _lib.lib()
+        nbytes = lib.dq_adapter_add_workspace(m, plan.requests, k, n, r, a)
+        ws = _scratch(nbytes, y)
+        _lib.check("dq_adapter_add", lib.dq_adapter_add(
+            _ptr(y2), _row_stride(y2), _ptr(x2), _row_stride(x2), m, plan.requests, k, n, _ptr(down), _ptr(up),
+            _ptr(scale), r, a, _ptr(plan.words), code, _ptr(o2), _row_stride(o2), _ptr(hidden), _ptr(ws), nbytes,
+            _stream(y.device)))
+    res = out if out is not None else o2.reshape(*y.shape[:-1], n_out)
+    return (res, hidden) if return_hidden else res
+
+
+def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
+                     scale: torch.Tensor, plan: AdapterPlan, dx: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None):
+    """Gradients of adapter_add (without act): returns (dx, ddown, dup).
+
+    dy [..., N] is the output's gradient; x the forward's input, as bf16
+    [..., K] or as checkpoint_pack packed it; hidden what adapter_add returned.
+    dx [..., K], if given, is the shared projection's input gradient
+    (nf4_linear_dgrad / fp8_linear_dgrad): the adapters' part is added to it, in
+    `out` (which may be dx) or a new tensor.  ddown / dup have the layouts of
+    down / up, zeros for adapters without tokens.  The same inputs give the
+    same bits."""
+    _require_cuda(dy, "dy")
+    a, r, k, n = _bank(down, up, scale, dy)
+    dy2 = _rows16(dy, "dy", n, dy)
+    m = dy2.shape[0]
+    _check_plan(plan, m, a, dy)
+    if isinstance(x, PackedActivation):
+        if x.codes.shape[-1] != k or x.codes.numel() != m * k:
+            raise ValueError(f"the packed activation holds {tuple(x.codes.shape)}, expected [{m}, {k}]")
+        _same_device(x.codes, "x", dy)
+        x2, scales, ldx = x.codes, x.scales, k
+    else:
+        x2, scales = _rows16(x, "x", k, dy), None
+        ldx = _row_stride(x2)
+        if x2.shape[0] != m:
+            raise ValueError(f"x holds {x2.shape[0]} tokens, dy {m}")
+    _same_device(hidden, "hidden", dy)
+    if hidden.dtype != torch.bfloat16 or hidden.shape != (m, r) or not hidden.is_contiguous():
+        raise TypeError(f"hidden must be a contiguous bfloat16 [{m}, {r}] tensor")
+    dx2 = torch.zeros((m, k), dtype=torch.bfloat16, device=dy.device) if dx is None else _rows16(dx, "dx", k, dy)
+    if dx2.shape[0] != m:
+        raise ValueError(f"dx holds {dx2.shape[0]} tokens, dy {m}")
+    if out is None:
+        o2 = dx2 if dx is None else torch.empty((m, k), dtype=torch.bfloat16, device=dy.device)
+    else:
+        o2 = _rows16(out, "out", k, dy)
+        if o2.data_ptr() != out.data_ptr() or o2.shape[0] != m:
+            raise ValueError("out must hold dy's tokens in evenly spaced, 16-byte aligned rows")
+    ddown, dup = torch.empty_like(down), torch.empty_like(up)
+    with _on(dy):
+        lib = _lib.lib()
+        nbytes = lib.dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
+        ws = _scratch(nbytes, dy)
+        _lib.check("dq_adapter_backward", lib.dq_adapter_backward(
+            _ptr(dy2), _row_stride(dy2), _ptr(x2), ldx, _ptr(scales), _ptr(hidden), m, plan.requests, k, n,
+            _ptr(down), _ptr(up), _ptr(scale), r, a, _ptr(plan.words), _ptr(dx2), _row_stride(dx2), _ptr(o2),
+            _row_stride(o2), _ptr(ddown), _ptr(dup), _ptr(ws), nbytes, _stream(dy.device)))
+    if out is not None:
+        return out, ddown, dup
+    return o2.reshape(*dy.shape[:-1], k), ddown, dup
+
+
+# ---------------------------------------------------- activation checkpoints
+CHECKPOINT_RUN = 128
+
+
+class PackedActivation:
+    """An activation in 8 bits: int8 codes [..., K] and float32 scales
+    [rows, ceil(K / 128)], one per row and run of 128 features."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _require_cuda(codes, "codes")
+        _same_device(scales, "scales", codes)
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.dim() < 1:
+            raise TypeError("codes must be int8 and scales float32")
+        k = codes.shape[-1]
+        if k == 0 or k % 16 != 0:
+            raise ValueError("an 8-bit activation needs a feature count that is a multiple of 16")
+        if scales.shape != (codes.numel() // k, -(-k // CHECKPOINT_RUN)):
+            raise ValueError("scales must hold one value per row and run of 128 features")
+        self.codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.contiguous().clone()
+        self.scales = scales.contiguous()
+
+
+def checkpoint_pack(x: torch.Tensor) -> PackedActivation:
+    """Pack a bf16 activation [..., K] (K % 16 == 0) to 8 bits for the backward
+    pass: per row and run of 128 features scale = max(max|x|, 1e-12) / 127,
+    codes = x / scale rounded to the nearest (ties to even).  A run that is not
+    finite comes back as NaN."""
+    _require_cuda(x, "x")
+    k = x.shape[-1]
+    if k == 0 or k % 16 != 0:
+        raise ValueError("an 8-bit activation needs a feature count that is a multiple of 16")
+    x2 = _rows16(x, "x", k, x)
+    m = x2.shape[0]
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((m, -(-k // CHECKPOINT_RUN)), dtype=torch.float32, device=x.device)
+    with _on(x):
+        _lib.check("dq_checkpoint_pack", _lib.lib().dq_checkpoint_pack(
+            _ptr(x2), _row_stride(x2), m, k, _ptr(codes), _ptr(scales), _stream(x.device)))
+    return PackedActivation(codes, scales)
+
+
+def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The bf16 activation that a packed one stands for."""
+    if not isinstance(packed, PackedActivation):
+        raise TypeError("packed must come from checkpoint_pack")
+    codes = packed.codes
+    k = codes.shape[-1]
+    o2 = torch.empty(codes.shape, dtype=torch.bfloat16, device=codes.device) if out is None else out
+    rows = _rows16(o2, "out", k, codes)
+    m = codes.numel() // k
+    if rows.data_ptr() != o2.data_ptr() or rows.shape[0] != m:
+        raise ValueError("out must hold the packed rows, evenly spaced and 16-byte aligned")
+    with _on(codes):
+        _lib.check("dq_checkpoint_unpack", _lib.lib().dq_checkpoint_unpack(
+            _ptr(codes), _ptr(packed.scales), m, k, _ptr(rows), _row_stride(rows), _stream(codes.device)))
+    return o2
+
+
+# -------------------------------------------------------- input gradients
+def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor):
+    _same_device(weight, "weight", dy)
+    if n % 8 != 0:
+        raise ValueError("the input gradient needs out_features % 8 == 0")
+    dy2 = _prep_x(dy, n)
+    dx = torch.empty((dy2.shape[0], k), dtype=torch.bfloat16, device=dy.device)
+    return dy2, dx, _lib.lib().dq_linear_dgrad_workspace(n, k)
+
+
+def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
+                     in_features: int) -> torch.Tensor:
+    """dx = dy . dequant_nf4(W), the input gradient of nf4_linear: dy bf16
+    [..., N] -> [..., K].  absmax float32 or bf16 as for the forward."""
+    _require_cuda(dy, "dy")
+    k = int(in_features)
+    n = packed.numel() * 2 // k
+    if n * k != packed.numel() * 2 or absmax.numel() * NF4_BLOCK != n * k:
+        raise ValueError("packed / absmax sizes do not match in_features")
+    dy2, dx, nbytes = _prep_dgrad(dy, n, k, packed)
+    am = absmax if absmax.dtype in (torch.float32, torch.bfloat16) else absmax.float()
+    with _on(dy):
+        ws = _scratch(nbytes, dy)
+        _lib.check("dq_linear_nf4_dgrad", _lib.lib().dq_linear_nf4_dgrad(
+            _ptr(dy2), dy2.shape[0], n, _ptr(packed), _ptr(am), _dtype_code(am), k, _ptr(dx), _ptr(ws), nbytes,
+            _stream(dy.device)))
+    return dx.reshape(*dy.shape[:-1], k)
+
+
+def fp8_linear_dgrad(dy: torch.Tensor, w8: torch.Tensor, scale: float) -> torch.Tensor:
+    """dx = dy . (e4m3(W) * bf16(scale)), the input gradient of fp8_linear."""
+    _require_cuda(dy, "dy")
+    n, k = int(w8.shape[0]), int(w8.shape[1])
+    raw = w8.view(torch.uint8)
+    dy2, dx, nbytes = _prep_dgrad(dy, n, k, raw)
+    with _on(dy):
+        ws = _scratch(nbytes, dy)
+        _lib.check("dq_linear_fp8_dgrad", _lib.lib().dq_linear_fp8_dgrad(
+            _ptr(dy2), dy2.shape[0], n, _ptr(raw), float(scale), k, _ptr(dx), _ptr(ws), nbytes,
+            _stream(dy.device)))
+    return dx.reshape(*dy.shape[:-1], k)
+
+
 def device_error(device=None) -> int:
-    """Read and clear the device's kernel error word (DQ_OK or DQ_ERR_TIMEOUT)."""
+    """Read and clear the device's kernel error word (DQ_OK, DQ_ERR_TIMEOUT or
+    DQ_ERR_INDEX)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     code = ctypes.c_int(0)
     with torch.cuda.device(dev):

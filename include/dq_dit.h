@@ -67,6 +67,49 @@ int dq_gated_residual(const void* x, int64_t ld_x, const void* gate, int64_t ld_
                       int64_t ld_y, int64_t T, int S, int D, void* out, int64_t ld_out,
                       dq_stream_t stream);
 
+/* The boundary between two blocks in one pass: the norm behind a block with
+ * its gate and residual scale, the residual add, and the norm before the next
+ * block with its modulation.  Per token (T = B * S tokens, batch element
+ * t / S) with D features:
+ *   s = x + residual_scale * gate * N_post(y) * post_weight
+ *   h = N_pre(s) * pre_weight * (1 + scale) + shift
+ * N is a LayerNorm without affine, an RMS norm, or (post only) nothing, with
+ * eps; statistics in float32; N_pre sees s as stored (bf16).  gate [B, D]
+ * (row stride ld_gate), scale / shift [B, D] (row stride ld_mod),
+ * post_weight / pre_weight [D]: each may be NULL (a factor of one, no shift);
+ * post_weight needs a post norm.  rounding: DQ_ROUND_ONCE computes in float32
+ * and rounds s and h once; DQ_ROUND_OPS rounds to bf16 after every tensor op
+ * (norm, weight, gate, residual scale when it is not 1; norm, weight, 1 +
+ * scale, product), the bits of dq_gated_residual followed by
+ * dq_adaln_modulate.  s may be x or y.  D a multiple of 4 up to 8192; every
+ * row start 8-byte aligned. */
+enum { DQ_NORM_NONE = 0, DQ_NORM_RMS = 1, DQ_NORM_LAYER = 2 };
+enum { DQ_ROUND_ONCE = 0, DQ_ROUND_OPS = 1 };
+int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int64_t T, int S, int D,
+                  const void* gate, int64_t ld_gate, const void* scale, const void* shift,
+                  int64_t ld_mod, const void* post_weight, const void* pre_weight, int post, int pre,
+                  float residual_scale, float eps, int rounding, void* s, int64_t ld_s, void* h,
+                  int64_t ld_h, dq_stream_t stream);
+
+/* Its gradients, of the formulas above without intermediate roundings.  ds
+ * (NULL: zero) and dh are the gradients of s and h; s as dq_gated_norm stored
+ * it, y as it was given.  dx (bf16, row stride ld_dx) is the whole gradient
+ * of s, dy (bf16) that of y; dgate, dscale, dshift f32 [B, D] and dpost_weight,
+ * dpre_weight f32 [D], contiguous, each may be NULL (dgate without gate is the
+ * gradient of a gate of ones, and so on).  The statistics are recomputed from
+ * s and y.  Sums over tokens are float32 in a fixed order.  dx may be ds, dy
+ * may be y.  The workspace (dq_gated_norm_backward_workspace bytes, 16-byte
+ * aligned) holds the partial sums.  B = T / S. */
+size_t dq_gated_norm_backward_workspace(int64_t T, int S, int D);
+int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_t ld_dh, const void* s,
+                           int64_t ld_s, const void* y, int64_t ld_y, int64_t T, int S, int D,
+                           const void* gate, int64_t ld_gate, const void* scale, int64_t ld_mod,
+                           const void* post_weight, const void* pre_weight, int post, int pre,
+                           float residual_scale, float eps, void* dx, int64_t ld_dx, void* dy,
+                           int64_t ld_dy, float* dgate, float* dscale, float* dshift,
+                           float* dpost_weight, float* dpre_weight, void* workspace,
+                           size_t workspace_bytes, dq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,7 +41,8 @@ typedef enum dq_status {
   DQ_ERR_WORKSPACE = 6, /* workspace NULL or smaller than dq_workspace_size() */
   DQ_ERR_ARG = 7,       /* NULL operand pointer or unknown enum value */
   DQ_ERR_CUDA = 8,      /* another CUDA runtime error */
-  DQ_ERR_SCRATCH_LIMIT = 9 /* dq_linear_nf4_noalloc: shape needs more scratch than it has */
+  DQ_ERR_SCRATCH_LIMIT = 9, /* dq_linear_nf4_noalloc: shape needs more scratch than it has */
+  DQ_ERR_INDEX = 10 /* dq_adapter_plan: an id or offset on the device was out of range (dq_device_error) */
 } dq_status;
 
 typedef enum dq_format { DQ_FMT_NF4 = 0, DQ_FMT_FP8 = 1 } dq_format;
@@ -129,7 +130,7 @@ int dq_linear_nf4_noalloc(const void* x, int64_t M, int64_t K,
 
 /* ---------------------------------------------------------------- errors
  * Reads and clears the current device's kernel error word (synchronizes
- * `stream`).  *code receives DQ_OK or DQ_ERR_TIMEOUT. */
+ * `stream`).  *code receives DQ_OK, DQ_ERR_TIMEOUT or DQ_ERR_INDEX. */
 int dq_device_error(int* code, dq_stream_t stream);
 
 /* Kernel-configuration override for benchmarking sweeps: x-tile rows
