@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/dq_adapter.h"
 #include "dq_adapter.cuh"
@@ -16,8 +17,9 @@ namespace dq {
 namespace {
 
 constexpr int64_t kMaxTokens = 1 << 30;
-constexpr int kMaxAdapters = 65536;
+constexpr int kMaxAdapters = 65535;
 constexpr int kMaxRank = 128;
+constexpr int kMaxCluster = 8;
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -44,31 +46,32 @@ bool large_tiles(int64_t M, int64_t R, int A) {
   return M >= 64 * std::max<int64_t>(1, std::min<int64_t>(A, R));
 }
 
-// k splits of the down kernel: enough CTAs for two per SM (one CTA streams a
-// 128-row tile; a split's sums cost 8 rank bytes of traffic per row, so large
-// tiles stop at four), each at least 256 features deep.
+// Feature splits of the large-tile down kernel, the CTAs of a cluster: the size
+// with the least waves x (stages of 64 features per CTA + a fixed cost of
+// eight), each split at least 256 features deep.  How many clusters are
+// resident at once decides, because a cluster stays within a graphics
+// processing cluster of the device: at 4608 tokens 36 clusters of eight run in
+// two waves, of six in one.  clusters[c]: how many of c CTAs fit.
 struct DownPlan {
-  bool large;
   int tiles, splits, k_per_split;
 };
-DownPlan down_plan(int64_t M, int64_t R, int A, int64_t F, int sms) {
+DownPlan down_plan(int64_t M, int64_t R, int A, int64_t F, const int* clusters) {
   DownPlan p;
-  const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  p.large = large_tiles(M, R, A);
   const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(A, R));
-  const int64_t likely = p.large ? ceil_div(M, kTileRows) + groups / 2
-                                 : std::max<int64_t>(ceil_div(M, 16), std::min<int64_t>(groups, M));
-  p.tiles = static_cast<int>(p.large ? lay.max_tiles : lay.cap / 16);
-  const int64_t want = std::max<int64_t>(1, 2 * sms / std::max<int64_t>(1, likely));
-  const int64_t most = std::min<int64_t>(p.large ? 4 : 16, std::max<int64_t>(1, F / 256));
-  const int64_t s = std::min(want, most);
+  const int64_t likely = ceil_div(M, kTileRows) + groups / 2;
+  p.tiles = static_cast<int>(adapter_plan_layout(M, R, A).max_tiles);
+  int64_t best = INT64_MAX, s = 1;
+  for (int64_t c : {1, 2, 4, 6, 8}) {
+    if (c > std::max<int64_t>(1, F / 256)) break;
+    const int64_t cost = ceil_div(likely, std::max(1, clusters[c])) * (ceil_div(ceil_div(F, c), 64) + 8);
+    if (cost < best) {
+      best = cost;
+      s = c;
+    }
+  }
   p.k_per_split = static_cast<int>(ceil_div(ceil_div(F, s), 64) * 64);
   p.splits = static_cast<int>(ceil_div(F, p.k_per_split));
   return p;
-}
-
-size_t part_bytes(int64_t M, int64_t R, int A, int64_t F, int r, int sms) {
-  return up256(static_cast<size_t>(adapter_plan_layout(M, R, A).cap) * r * 4 * down_plan(M, R, A, F, sms).splits);
 }
 
 // Row splits of the weight-gradient kernel: the count (up to 16) that leaves
@@ -79,9 +82,9 @@ struct WgradPlan {
 };
 WgradPlan wgrad_plan(int64_t M, int64_t R, int A, int64_t cols, int rc, bool i8, int sms) {
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  const int slots = sms * (rc <= 64 ? 2 : 1);
+  const int slots = sms * (rc <= 64 || !i8 ? 2 : 1);  // WgradCfg::kMinCtas
   WgradPlan p;
-  p.col_tiles = static_cast<int>(ceil_div(cols, i8 ? 128 : 64));
+  p.col_tiles = static_cast<int>(ceil_div(cols, 128));
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, M / 256));
   double best = 0;
   int splits = 1;
@@ -101,22 +104,31 @@ size_t wgrad_bytes(const WgradPlan& p, int64_t cols, int r) {
   return up256(static_cast<size_t>(2) * p.splits * r * cols * 4);
 }
 
-// Launches with programmatic stream serialization: the kernel may start while
-// the one before it drains, and waits (griddepcontrol.wait) before it reads
-// that one's results.
+// after: programmatic stream serialization -- the kernel may start while the
+// one before it drains, and waits (griddepcontrol.wait) before it reads that
+// one's results.  cluster: CTAs of a cluster along (x, y).
 template <typename Args, typename... More>
-int launch_after(void (*kern)(Args, More...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args args,
-                 More... more) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+int launch(void (*kern)(Args, More...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool after,
+           dim3 cluster, Args args, More... more) {
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (after) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster.x * cluster.y > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster.x;
+    attr[n].val.clusterDim.y = cluster.y;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, args, more...) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
@@ -133,40 +145,89 @@ int allow_smem(K kern, int bytes, std::atomic<int>* set) {
   return DQ_OK;
 }
 
+// Resident clusters of the down kernel by their (even) size, once per device.
+// The runtime's occupancy query counts one CTA per SM for a kernel that
+// allocates tensor memory, though two fit by its shared memory and run, so the
+// count for c CTAs is the one it gives for c / 2.
 template <int R>
-int launch_down(const DownArgs& a, const DownPlan& p, cudaStream_t st) {
-  const dim3 grid(p.tiles, p.splits);
-  if (p.large) {
-    static std::atomic<int> set[kMaxDevices];
-    const int rc = allow_smem(adapter_down_kernel<R>, DownCfg<R>::kSmemBytes, set);
-    if (rc != DQ_OK) return rc;
-    adapter_down_kernel<R><<<grid, 256, DownCfg<R>::kSmemBytes, st>>>(a);
-  } else {
-    adapter_down_small_kernel<R><<<grid, 256, 0, st>>>(a);
-  }
-  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
-}
-
-template <int R, int WM>
-int launch_up_tiles(UpArgs a, int tiles, int64_t likely_tiles, int sms, cudaStream_t st) {
-  using C = UpCfg<R, WM>;
-  static std::atomic<int> set[kMaxDevices];
-  const int rc = allow_smem(adapter_up_kernel<R, WM>, C::kSmemBytes, set);
+int down_clusters(const int** out) {
+  using C = DownCfg<R>;
+  static std::atomic<int> set[kMaxDevices], probed[kMaxDevices];
+  static int table[kMaxDevices][kMaxCluster + 1];
+  static std::mutex mu;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
+  const int rc = allow_smem(adapter_down_kernel<R>, C::kSmemBytes, set);
   if (rc != DQ_OK) return rc;
-  // columns per CTA: up to 16 steps where that still leaves four CTAs per
-  // slot of two per SM (the tile's hidden rows are summed once per CTA)
-  int64_t steps = 16;
-  while (steps > 1 && likely_tiles * ceil_div(a.N, steps * C::kStepCols) < 8 * sms) steps /= 2;
-  a.cols_per_cta = static_cast<int>(steps * C::kStepCols);
-  const dim3 grid(tiles, static_cast<unsigned>(ceil_div(a.N, a.cols_per_cta)));
-  return launch_after(adapter_up_kernel<R, WM>, grid, 256, C::kSmemBytes, st, a);
+  if (!probed[dev].load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lk(mu);
+    for (int half = 1; half <= kMaxCluster / 2; ++half) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1;
+      attr[0].val.clusterDim.y = half;
+      attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1024, half);
+      cfg.blockDim = dim3(C::kThreads);
+      cfg.dynamicSmemBytes = C::kSmemBytes;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, adapter_down_kernel<R>, &cfg) != cudaSuccess) return DQ_ERR_LAUNCH;
+      table[dev][2 * half] = n;
+      if (half == 1) table[dev][1] = 2 * n;
+    }
+    probed[dev].store(1, std::memory_order_release);
+  }
+  *out = table[dev];
+  return DQ_OK;
 }
 
 template <int R>
-int launch_up(const UpArgs& a, const DownPlan& p, int64_t M, int sms, cudaStream_t st) {
-  const int64_t likely = std::max<int64_t>(1, ceil_div(M, p.large ? kTileRows : 16));
-  return p.large ? launch_up_tiles<R, 8>(a, p.tiles, likely, sms, st)
-                 : launch_up_tiles<R, 1>(a, p.tiles, likely, sms, st);
+int launch_down(DownArgs a, int64_t M, int64_t requests, cudaStream_t st) {
+  using C = DownCfg<R>;
+  const int* clusters = nullptr;
+  const int rc = down_clusters<R>(&clusters);
+  if (rc != DQ_OK) return rc;
+  const DownPlan p = down_plan(M, requests, a.A, a.K, clusters);
+  a.k_per_split = p.k_per_split;
+  return launch(adapter_down_kernel<R>, dim3(p.tiles, p.splits), C::kThreads, C::kSmemBytes, st, false,
+                dim3(1, p.splits), a);
+}
+
+template <int R>
+int launch_up(UpArgs a, int tiles, int64_t M, int sms, cudaStream_t st) {
+  using C = UpCfg<R>;
+  static std::atomic<int> set[kMaxDevices];
+  const int rc = allow_smem(adapter_up_kernel<R>, C::kSmemBytes, set);
+  if (rc != DQ_OK) return rc;
+  // columns per CTA: 256 where that leaves four CTAs per SM, else 128 (wider
+  // ones spread a CTA's fixed cost, its rows of hidden and its first loads'
+  // latency, over more steps but leave the last wave emptier)
+  const int cols = ceil_div(M, kTileRows) * ceil_div(a.N, 256) < 4 * sms ? 128 : 256;
+  a.cols_per_cta = cols;
+  return launch(adapter_up_kernel<R>, dim3(tiles, static_cast<unsigned>(ceil_div(a.N, cols))), 256, C::kSmemBytes, st,
+                true, dim3(1), a);
+}
+
+template <int R>
+int launch_small(SmallArgs a, int64_t M, int64_t R_, int sms, cudaStream_t st) {
+  using C = SmallCfg<R>;
+  static std::atomic<int> set[kMaxDevices];
+  const int rc = allow_smem(adapter_small_kernel<R>, C::kSmemBytes, set);
+  if (rc != DQ_OK) return rc;
+  a.k_per_rank = static_cast<int>(ceil_div(ceil_div(a.K, kSmallCluster), 32) * 32);
+  // clusters per tile: more than one (each repeats the down projection) only
+  // while the CTAs have more than one step of columns and the SMs have room
+  const int64_t tiles = std::max<int64_t>(ceil_div(M, kBlockRows), std::min<int64_t>(std::min<int64_t>(a.A, R_), M));
+  int clusters = 1;
+  while (clusters < 8 && a.N > clusters * kSmallCluster * C::kStepCols && 2 * clusters * kSmallCluster * tiles <= 3 * sms)
+    clusters *= 2;
+  a.cols_per_cta = static_cast<int>(ceil_div(ceil_div(a.N, clusters * kSmallCluster), 64) * 64);
+  a.ctas_per_tile = clusters * kSmallCluster;
+  const dim3 grid(static_cast<unsigned>(a.lay.cap / kBlockRows) * a.ctas_per_tile);
+  return launch(adapter_small_kernel<R>, grid, 256, C::kSmemBytes, st, false, dim3(kSmallCluster), a);
 }
 
 template <int R, bool I8>
@@ -175,12 +236,12 @@ int launch_wgrad(const WgradArgs& a, const WgradPlan& p, cudaStream_t st) {
   static std::atomic<int> set[kMaxDevices];
   int rc = allow_smem(adapter_wgrad_kernel<R, I8>, C::kSmemBytes, set);
   if (rc != DQ_OK) return rc;
-  rc = launch_after(adapter_wgrad_kernel<R, I8>, dim3(p.col_tiles, p.splits), 256, C::kSmemBytes, st, a);
+  rc = launch(adapter_wgrad_kernel<R, I8>, dim3(p.col_tiles, p.splits), C::kThreads, C::kSmemBytes, st, true, dim3(1), a);
   if (rc != DQ_OK) return rc;
   const int64_t elems = static_cast<int64_t>(a.rank) * a.cols;
   const unsigned bx = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 1024), 512));
-  return launch_after(adapter_wgrad_reduce_kernel, dim3(bx, a.A), 256, 0, st, a.words, a.lay, a.rows_per_split,
-                      static_cast<const float*>(a.part), a.dbank, elems);
+  return launch(adapter_wgrad_reduce_kernel, dim3(bx, a.A), 256, 0, st, true, dim3(1), a.words, a.lay,
+                a.rows_per_split, static_cast<const float*>(a.part), a.dbank, elems);
 }
 
 // Calls f.template operator()<R>() for the rank class.
@@ -194,7 +255,7 @@ int by_rank(int r, F&& f) {
   return f(std::integral_constant<int, 128>());
 }
 
-int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, int64_t M, int64_t R, int64_t cols,
+int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, const float* g32, int64_t M, int64_t R, int64_t cols,
           int r, int A, const int32_t* words, const AdapterPlan& lay, void* ws, void* dbank, int sms,
           cudaStream_t st) {
   const bool i8 = x_scales != nullptr;
@@ -203,6 +264,9 @@ int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, int6
   a.x = x;
   a.x_scales = x_scales;
   a.g = static_cast<const __nv_bfloat16*>(g);
+  a.g32 = g32;
+  int e = error_word(&a.error);
+  if (e != DQ_OK) return e;
   a.words = words;
   a.part = static_cast<float*>(ws);
   a.dbank = static_cast<__nv_bfloat16*>(dbank);
@@ -218,61 +282,87 @@ int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, int6
   });
 }
 
-// Workspace of the backward pass: the down sums, g [M, r], and one region for
-// each weight gradient's partial sums.
+// Workspace of the backward pass: g [M, r] in bf16 and in f32, and one region
+// for each weight gradient's partial sums.
 struct BackwardWs {
-  size_t part, g, up, down, total;
+  size_t g, g32, up, down, total;
 };
 BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A, int sms) {
   BackwardWs w;
   const int rc = rank_class(r);
-  w.part = part_bytes(M, R, A, N, r, sms);
   w.g = up256(static_cast<size_t>(M) * r * 2);
   w.up = wgrad_bytes(wgrad_plan(M, R, A, N, rc, false, sms), N, r);
   w.down = std::max(wgrad_bytes(wgrad_plan(M, R, A, K, rc, false, sms), K, r),
                     wgrad_bytes(wgrad_plan(M, R, A, K, rc, true, sms), K, r));
-  w.total = w.part + w.g + w.up + w.down;
+  w.g32 = up256(static_cast<size_t>(M) * r * 4);
+  w.total = w.g + w.g32 + w.up + w.down;
   return w;
 }
 
-// v = x . P^T (down) then out = act(y + scale v . Q) (up), on one plan.
+// hidden = scale x . P^T (down), out = act(y + hidden . Q) (up), on one plan.
+// hidden: where the low-rank intermediate goes, complete (zero rows without an
+// adapter) if want_hidden; the small-batch kernel takes NULL.
 int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void* y, int64_t ldy, int64_t F_out,
             const void* Q, const float* scale, int64_t M, int64_t R, int r, int A, const int32_t* words, int act,
-            void* out, int64_t ldo, void* hidden, void* part, int sms, cudaStream_t st) {
+            void* out, int64_t ldo, void* hidden, bool want_hidden, float* hidden32, int sms, cudaStream_t st) {
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  const DownPlan p = down_plan(M, R, A, F_in, sms);
+  const int with_none = act != kActNone || out != y || want_hidden;
+  if (!large_tiles(M, R, A)) {
+    SmallArgs a = {};
+    a.x = static_cast<const __nv_bfloat16*>(x);
+    a.y = static_cast<const __nv_bfloat16*>(y);
+    a.down = static_cast<const __nv_bfloat16*>(P);
+    a.up = static_cast<const __nv_bfloat16*>(Q);
+    a.scale = scale;
+    a.words = words;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.hidden = want_hidden ? static_cast<__nv_bfloat16*>(hidden) : nullptr;
+    a.hidden32 = hidden32;
+    a.lay = lay;
+    a.ldx = ldx;
+    a.ldy = ldy;
+    a.ldo = ldo;
+    a.K = static_cast<int>(F_in);
+    a.N = static_cast<int>(F_out);
+    a.rank = r;
+    a.A = A;
+    a.act = act;
+    a.with_none = with_none;
+    return by_rank(r, [&](auto rc) { return launch_small<decltype(rc)::value>(a, M, R, sms, st); });
+  }
   DownArgs d = {};
+  int e = error_word(&d.error);
+  if (e != DQ_OK) return e;
   d.x = static_cast<const __nv_bfloat16*>(x);
   d.bank = static_cast<const __nv_bfloat16*>(P);
+  d.scale = scale;
   d.words = words;
-  d.part = static_cast<float*>(part);
+  d.hidden = static_cast<__nv_bfloat16*>(hidden);
+  d.hidden32 = hidden32;
   d.lay = lay;
   d.ldx = ldx;
   d.K = static_cast<int>(F_in);
   d.rank = r;
   d.A = A;
-  d.k_per_split = p.k_per_split;
   UpArgs u = {};
   u.y = static_cast<const __nv_bfloat16*>(y);
   u.bank = static_cast<const __nv_bfloat16*>(Q);
-  u.scale = scale;
+  u.hidden = d.hidden;
   u.words = words;
-  u.part = d.part;
   u.out = static_cast<__nv_bfloat16*>(out);
-  u.hidden = static_cast<__nv_bfloat16*>(hidden);
+  u.zero_hidden = want_hidden ? d.hidden : nullptr;
   u.lay = lay;
   u.ldy = ldy;
   u.ldo = ldo;
   u.N = static_cast<int>(F_out);
   u.rank = r;
   u.A = A;
-  u.splits = p.splits;
   u.act = act;
-  u.with_none = act != kActNone || out != y || hidden != nullptr;
+  u.with_none = with_none;
   return by_rank(r, [&](auto rc) {
     constexpr int R_ = decltype(rc)::value;
-    const int e = launch_down<R_>(d, p, st);
-    return e != DQ_OK ? e : launch_up<R_>(u, p, M, sms, st);
+    const int e2 = launch_down<R_>(d, M, R, st);
+    return e2 != DQ_OK ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, sms, st);
   });
 }
 
@@ -310,10 +400,8 @@ int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
-size_t dq_adapter_add_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
-  int sms = 0;
-  if (bank_shape(M, R, K, N, r, A) != DQ_OK || device_sms(&sms) != DQ_OK) return 0;
-  return part_bytes(M, R, A, K, r, sms);
+size_t dq_adapter_add_workspace(int64_t M, int r) {
+  return M <= 0 || r <= 0 ? 0 : static_cast<size_t>(M) * r * 2;
 }
 
 int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t M, int64_t R, int64_t K,
@@ -337,10 +425,12 @@ int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64
     return DQ_ERR_ALIGN;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
-  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < part_bytes(M, R, A, K, r, sms))
+  if (hidden == nullptr &&
+      (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_adapter_add_workspace(M, r)))
     return DQ_ERR_WORKSPACE;
   return down_up(x, ldx, K, down, y, ldy, N, up, scale, M, R, r, A, static_cast<const int32_t*>(plan), act, out,
-                 ldo, hidden, workspace, sms, static_cast<cudaStream_t>(stream));
+                 ldo, hidden != nullptr ? hidden : workspace, hidden != nullptr, nullptr, sms,
+                 static_cast<cudaStream_t>(stream));
 }
 
 size_t dq_adapter_backward_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
@@ -385,13 +475,14 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int32_t* words = static_cast<const int32_t*>(plan);
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  void* g = ws + w.part;
-  rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo,
-               want_w ? g : nullptr, ws, sms, st);
+  float* g32 = reinterpret_cast<float*>(ws + w.g);
+  uint8_t* parts = ws + w.g + w.g32;
+  rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo, ws, want_w,
+               want_w && i8 ? g32 : nullptr, sms, st);
   if (rc != DQ_OK || !want_w) return rc;
-  rc = wgrad(dy, lddy, nullptr, hidden, M, R, N, r, A, words, lay, ws + w.part + w.g, dup, sms, st);
+  rc = wgrad(dy, lddy, nullptr, hidden, nullptr, M, R, N, r, A, words, lay, parts, dup, sms, st);
   if (rc != DQ_OK) return rc;
-  return wgrad(x, ldx, x_scales, g, M, R, K, r, A, words, lay, ws + w.part + w.g + w.up, ddown, sms, st);
+  return wgrad(x, ldx, x_scales, ws, g32, M, R, K, r, A, words, lay, parts + w.up, ddown, sms, st);
 }
 
 int dq_checkpoint_pack(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* codes, float* scales,

@@ -56,9 +56,9 @@ __host__ __device__ inline AdapterPlan adapter_plan_layout(int64_t M, int64_t R,
   p.off_start = AdapterPlan::kHeader;
   p.off_counts = p.off_start + up4(A + 2);
   p.off_perm = p.off_counts + up4(A + 1);
-  p.off_blk = p.off_perm + p.cap;
+  p.off_blk = p.off_perm + p.cap;  // cap is a multiple of 16
   p.off_tiles = p.off_blk + up4(p.cap / 16);
-  p.words = p.off_tiles + up4(p.max_tiles);
+  p.words = p.off_tiles + 4 * p.max_tiles;
   return p;
 }
 
@@ -177,7 +177,17 @@ __global__ void __launch_bounds__(256)
   for (int i = mine + lane; i < rows; i += 32) perm[row0 + i] = -1;
   for (int i = lane; i < rows / 16; i += 32) words[lay.off_blk + row0 / 16 + i] = a;
   const int tiles = (mine + kTileRows - 1) / kTileRows;
-  for (int i = lane; i < tiles; i += 32) words[lay.off_tiles + tile0 + i] = row0 + i * kTileRows;
+  // large tiles: first row, rows with a token, bucket, and the first token if
+  // the tile's tokens follow one another (their readers then skip perm), else -1
+  __syncwarp();
+  for (int i = 0; i < tiles; ++i) {
+    const int r0 = row0 + i * kTileRows, n = min(kTileRows, mine - i * kTileRows);
+    const int first = perm[r0];
+    bool run = true;
+    for (int j = lane; j < n; j += 32) run = run && perm[r0 + j] == first + j;
+    run = __all_sync(0xffffffffu, run);
+    if (lane == 0) reinterpret_cast<int4*>(words + lay.off_tiles)[tile0 + i] = make_int4(r0, n, a, run ? first : -1);
+  }
   if (lane == 0) {
     words[lay.off_start + a] = row0;
     if (a == A) {
@@ -193,20 +203,30 @@ __global__ void __launch_bounds__(256)
 // One tile of up to T rows of one bucket; rows == 0: none for this CTA.
 struct PlanTile {
   int row, rows, adapter;
+  int first;  // large tiles: the first token if they follow one another, else -1
+  // token of row i, or -1
+  __device__ __forceinline__ int token(const int32_t* perm, int i) const {
+    return i >= rows ? -1 : first >= 0 ? first + i : perm[row + i];
+  }
 };
 template <int T>
 __device__ __forceinline__ PlanTile plan_tile(const int32_t* words, const AdapterPlan& lay, int A,
                                               int tile, bool with_none) {
-  PlanTile t{0, 0, A};
+  PlanTile t{0, 0, A, -1};
   if constexpr (T == kTileRows) {
-    if (tile >= words[with_none ? AdapterPlan::kAllTiles : AdapterPlan::kTiles]) return t;
-    t.row = words[lay.off_tiles + tile];
-    t.adapter = words[lay.off_blk + t.row / 16];
-    t.rows = min(T, words[lay.off_start + t.adapter + 1] - t.row);
+    const int count = words[with_none ? AdapterPlan::kAllTiles : AdapterPlan::kTiles];
+    const int4 e = __ldg(reinterpret_cast<const int4*>(words + lay.off_tiles) + tile);  // grid <= max_tiles
+    if (tile >= count) return t;
+    t.row = e.x;
+    t.rows = e.y;
+    t.adapter = e.z;
+    t.first = e.w;
   } else {
     t.row = tile * T;
-    if (t.row >= words[with_none ? AdapterPlan::kRows : AdapterPlan::kNoneStart]) return t;
-    t.adapter = words[lay.off_blk + tile];
+    const int count = words[with_none ? AdapterPlan::kRows : AdapterPlan::kNoneStart];
+    const int adapter = words[lay.off_blk + tile];  // grid <= cap / 16
+    if (t.row >= count) return t;
+    t.adapter = adapter;
     t.rows = T;
   }
   return t;
@@ -219,9 +239,19 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_4z(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0)
+// The same for a stream whose neighbouring bytes are read next: the rest of the
+// 256 bytes is brought to L2 with it.
+__device__ __forceinline__ void cp_async_16_l2(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
+}
+__device__ __forceinline__ uint4 ld_global_l2(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -238,70 +268,176 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
+// mma_16816_bf16 onto zeros (no accumulator registers to clear).
+__device__ __forceinline__ void mma_16816_bf16_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                    uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 2^x by the special-function unit (relative error 2^-22, subnormals to zero).
+__device__ __forceinline__ float exp2f_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t lo, uint32_t hi) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(lo), "r"(hi) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+// 1 / x by the special-function unit (relative error 2^-23, 1 / inf = 0).
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Loads from the shared memory of a CTA of the cluster (address from mapa).
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[smem] * B[smem], one CTA, kind::f16, elected-lane issue.
+__device__ __forceinline__ void tc_mma_ss_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ------------------------------------------------------------------- down
-// part[split][row][r] = sum over the split's k of X[perm[row]][k] P_a[r][k],
-// f32; the reader adds the splits in order.
+// hidden[token, :] = bf16(s_a X[token, :] . P_a^T), and f32 unrounded for the
+// caller that multiplies it further.
 //
-// Large tiles (128 rows, one warp per 16): X and P move through a cp.async
-// ring of 64-feature stages (128-byte rows, 16-byte chunk c of row i at
-// c ^ (i % 8): conflict-free for the copies and for ldmatrix).
+// Large tiles: 128 rows, D = X P^T on tcgen05 (M = 128, N = R, f32 in tensor
+// memory).  The stream of X needs 2 r FLOP per 2 bytes, 412 TFLOP/s at r = 64
+// and the copy bandwidth; warp-level MMAs stop at about 320 here (measured:
+// r = 64, 4608 x 12288, 55 us, 2.0 TB/s, with their pipe 41% busy and the
+// rest of the time in fragment loads), the tensor-memory ones are free next
+// to the stream.  Eight warps copy 64-feature stages with cp.async (the rows
+// are gathered through the plan; 128-byte rows, 16-byte chunk c of row i at
+// c ^ (i % 8), the 128-byte swizzle the MMA descriptors name), each thread
+// several stages ahead: its copies of a stage are waited for, fenced towards
+// the async proxy and reported to the stage's barrier when it issues the one
+// kAhead later (two less than the ring, so that the MMAs of the stage to be
+// refilled are not waited for).  A ninth warp issues the MMAs.
+//
+// The features are split over the CTAs of a cluster (enough of them to give
+// every SM a CTA); their partial sums meet through distributed shared memory,
+// in rank order, so nothing but the bf16 result reaches global memory.
 template <int R>
 struct DownCfg {
   static constexpr int kStageX = kTileRows * 128;
-  static constexpr int kStageP = R * 128;
-  static constexpr int kStages = R <= 64 ? 4 : 3;
-  static constexpr int kSmemBytes = kStages * (kStageX + kStageP);
+  static constexpr int kStage = kStageX + R * 128;
+  static constexpr int kStages = 110 * 1024 / kStage;  // two CTAs per SM
+  static constexpr int kAhead = kStages - 2;           // stages a thread's copies run ahead
+  static constexpr int kProducers = 8;
+  static constexpr int kThreads = (kProducers + 1) * 32;
+  static constexpr int kRedStride = R + 4;  // floats; conflict-free 16-byte rows
+  static constexpr int kOffBar = kStages * kStage;
+  static constexpr int kSmemBytes = kOffBar + 16 * kStages + 32 + 1024;
+  static constexpr int kTmemCols = R < 32 ? 32 : R;
+  static_assert(kTileRows * kRedStride * 4 <= kStages * kStage, "the sums fit the drained ring");
 };
 
 struct DownArgs {
   const __nv_bfloat16* x;
   const __nv_bfloat16* bank;
+  const float* scale;
   const int32_t* words;
-  float* part;
+  __nv_bfloat16* hidden;  // [M, rank]
+  float* hidden32;        // [M, rank] or NULL
+  unsigned int* error;
   AdapterPlan lay;
   int64_t ldx;
   int K, rank, A, k_per_split;
 };
 
 template <int R>
-__global__ void __launch_bounds__(256, 2) adapter_down_kernel(const DownArgs a) {
+__global__ void __launch_bounds__(DownCfg<R>::kThreads, 2) adapter_down_kernel(const DownArgs a) {
   using C = DownCfg<R>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const uint32_t sbase = smem_u32(smem_raw);
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sbase - raw);
   const PlanTile t = plan_tile<kTileRows>(a.words, a.lay, a.A, blockIdx.x, false);
-  grid_launch_dependents();
-  if (t.rows == 0) return;
+  if (t.rows == 0) return;  // the whole cluster: it shares the tile
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto full_bar = [&](int s) { return sbase + C::kOffBar + 8u * s; };
+  auto empty_bar = [&](int s) { return sbase + C::kOffBar + 8u * (C::kStages + s); };
+  const uint32_t done_bar = sbase + C::kOffBar + 16u * C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffBar + 16 * C::kStages + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + 16 * C::kStages + 16);
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full_bar(s), C::kProducers);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == C::kProducers) {
+    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_launch_dependents();
   const int k_lo = blockIdx.y * a.k_per_split;
   const int k_hi = min(a.K, k_lo + a.k_per_split);
   const int steps = (k_hi - k_lo + 63) / 64;
-  const __nv_bfloat16* P = a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.K;
 
-  // this thread copies chunk tid % 8 of rows tid / 8 + 32 i
-  const int chunk = tid & 7;
-  const __nv_bfloat16* src[4];
+  if (warp < C::kProducers) {
+    const __nv_bfloat16* P = a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.K;
+    const int chunk = tid & 7;  // this thread copies chunk tid % 8 of rows tid / 8 + 32 i
+    const __nv_bfloat16* src[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (tid >> 3) + 32 * i;
-    const int token = row < t.rows ? a.words[a.lay.off_perm + t.row + row] : -1;
-    src[i] = token >= 0 ? a.x + static_cast<int64_t>(token) * a.ldx : nullptr;
-  }
-  auto load = [&](int step) {
-    if (step < steps) {
-      const uint32_t sx = sbase + (step % C::kStages) * (C::kStageX + C::kStageP);
-      const uint32_t sp = sx + C::kStageX;
-      const int k = k_lo + step * 64 + chunk * 8;
+    for (int i = 0; i < 4; ++i) {
+      const int row = (tid >> 3) + 32 * i;
+      const int token = t.token(a.words + a.lay.off_perm, row);
+      src[i] = token >= 0 ? a.x + static_cast<int64_t>(token) * a.ldx : nullptr;
+    }
+    int it = 0;
+    for (; it < steps; ++it) {
+      const int slot = it % C::kStages;
+      if (!mbar_wait(empty_bar(slot), static_cast<uint32_t>(((it / C::kStages) & 1) ^ 1), abort_flag)) break;
+      const uint32_t sx = sbase + slot * C::kStage, sp = sx + C::kStageX;
+      const int k = k_lo + it * 64 + chunk * 8;
       const bool in = k < k_hi;
+      // rows without a token keep whatever the stage holds: row i of X only
+      // reaches row i of D, which is not stored then
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = (tid >> 3) + 32 * i;
-        const bool ok = in && src[i] != nullptr;
-        cp_async_16(sx + row * 128 + ((chunk ^ (row & 7)) << 4), ok ? src[i] + k : a.x, ok);
+        if (src[i] != nullptr) cp_async_16_l2(sx + row * 128 + ((chunk ^ (row & 7)) << 4), in ? src[i] + k : a.x, in);
       }
 #pragma unroll
       for (int i = 0; i < (R * 8 + 255) / 256; ++i) {
@@ -311,149 +447,95 @@ __global__ void __launch_bounds__(256, 2) adapter_down_kernel(const DownArgs a) 
           cp_async_16(sp + row * 128 + ((chunk ^ (row & 7)) << 4),
                       ok ? P + static_cast<int64_t>(row) * a.K + k : a.bank, ok);
       }
-    }
-    cp_async_commit();
-  };
-
-  float acc[R / 8][4] = {};
-#pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) load(s);
-  const bool active = warp * 16 < t.rows;
-  for (int step = 0; step < steps; ++step) {
-    cp_async_wait<C::kStages - 2>();
-    __syncthreads();
-    load(step + C::kStages - 1);
-    if (!active) continue;
-    const uint32_t sx = sbase + (step % C::kStages) * (C::kStageX + C::kStageP);
-    const uint32_t sp = sx + C::kStageX;
-    const int arow = warp * 16 + (lane & 15);
-    const int brow = (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t af[4];
-      ldmatrix_x4(sx + arow * 128 + (((2 * ks + (lane >> 4)) ^ (arow & 7)) << 4), af);
-#pragma unroll
-      for (int nt = 0; nt < R / 16; ++nt) {
-        uint32_t bf[4];
-        const int row = nt * 16 + brow;
-        ldmatrix_x4(sp + row * 128 + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4), bf);
-        mma_16816_bf16(acc[2 * nt], af[0], af[1], af[2], af[3], bf[0], bf[1]);
-        mma_16816_bf16(acc[2 * nt + 1], af[0], af[1], af[2], af[3], bf[2], bf[3]);
+      cp_async_commit();
+      if (it >= C::kAhead) {
+        cp_async_wait<C::kAhead>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar((it - C::kAhead) % C::kStages));
       }
     }
-  }
-  if (!active) return;
-  float* out = a.part + (static_cast<int64_t>(blockIdx.y) * a.lay.cap + t.row + warp * 16) * a.rank;
-  const int g4 = lane >> 2, tig = lane & 3;
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (it == steps && lane == 0)
+      for (int s = max(0, steps - C::kAhead); s < steps; ++s) mbar_arrive(full_bar(s % C::kStages));
+  } else {
+    constexpr uint32_t idesc = make_idesc_bf16(128, R);
+    int it = 0;
+    for (; it < steps; ++it) {
+      const int slot = it % C::kStages;
+      if (!mbar_wait(full_bar(slot), static_cast<uint32_t>((it / C::kStages) & 1), abort_flag)) break;
+      tc_fence_after();
+      const uint64_t ad = make_sw128_kmajor_desc(sbase + slot * C::kStage);
+      const uint64_t bd = make_sw128_kmajor_desc(sbase + slot * C::kStage + C::kStageX);
 #pragma unroll
-  for (int nt = 0; nt < R / 8; ++nt)
-    if (nt * 8 < a.rank) {
-      const int c = nt * 8 + 2 * tig;
-      *reinterpret_cast<float2*>(out + static_cast<int64_t>(g4) * a.rank + c) = make_float2(acc[nt][0], acc[nt][1]);
-      *reinterpret_cast<float2*>(out + static_cast<int64_t>(g4 + 8) * a.rank + c) =
-          make_float2(acc[nt][2], acc[nt][3]);
+      for (int ks = 0; ks < 4; ++ks) tc_mma_ss_elect(tmem, ad + 2 * ks, bd + 2 * ks, idesc, (it | ks) != 0);
+      tc_commit_elect(empty_bar(slot));
     }
-}
-
-// Small tiles (16 rows): the latency of the chain launch -> plan -> operands
-// -> sum is what counts, so the warps of a CTA share the split's k between
-// them and load straight into MMA fragments.  A sum over k may visit k in any
-// order as long as both operands use the same one: thread tig of a quad takes
-// the eight consecutive features 8 tig .. of every group of 32 (one 16-byte
-// load per row), as k slots 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9 of two MMAs.
-template <int R>
-__global__ void __launch_bounds__(256) adapter_down_small_kernel(const DownArgs a) {
-  __shared__ float red[4][16 * R];
-  const PlanTile t = plan_tile<kBlockRows>(a.words, a.lay, a.A, blockIdx.x, false);
-  grid_launch_dependents();
-  if (t.rows == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g4 = lane >> 2, tig = lane & 3;
-  const int t0 = a.words[a.lay.off_perm + t.row + g4];
-  const int t1 = a.words[a.lay.off_perm + t.row + g4 + 8];
-  const __nv_bfloat16* x0 = a.x + static_cast<int64_t>(t0) * a.ldx;
-  const __nv_bfloat16* x1 = a.x + static_cast<int64_t>(t1) * a.ldx;
-  const __nv_bfloat16* P = a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.K;
-  const int k_hi = min(a.K, static_cast<int>(blockIdx.y + 1) * a.k_per_split);
-  float acc[R / 8][4] = {};
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll (R <= 32 ? 2 : 1)
-  for (int k = blockIdx.y * a.k_per_split + warp * 32 + tig * 8; k < k_hi + tig * 8; k += 256) {
-    const bool in = k < k_hi;
-    const uint4 u0 = in && t0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-    const uint4 u1 = in && t1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
-    uint4 p[R / 8];
+    tc_commit_elect(done_bar);
+    __syncwarp();
+  }
+  // partial sums [128][R] f32 in this CTA's (drained) ring
+  float* red = reinterpret_cast<float*>(smem);
+  const bool ok = mbar_wait(done_bar, 0, abort_flag);
+  tc_fence_after();
+  constexpr int kHalves = R >= 32 ? 2 : 1;
+  constexpr int kCols = R / kHalves;
+  if (ok && warp < 4 * kHalves) {
+    const int q = warp & 3, c0 = (warp >> 2) * kCols;
+    float* dst = red + (32 * q + lane) * C::kRedStride + c0;
 #pragma unroll
-    for (int nt = 0; nt < R / 8; ++nt)
-      p[nt] = in && nt * 8 < a.rank
-                  ? ld_stream16(P + static_cast<int64_t>(nt * 8 + g4) * a.K + k)
-                  : zero;
+    for (int c = 0; c < kCols; c += 16) {
+      uint32_t v[16];
+      tmem_ld_x16(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0 + c, v);
+      tmem_wait_ld();
 #pragma unroll
-    for (int nt = 0; nt < R / 8; ++nt) {
-      mma_16816_bf16(acc[nt], u0.x, u1.x, u0.y, u1.y, p[nt].x, p[nt].y);
-      mma_16816_bf16(acc[nt], u0.z, u1.z, u0.w, u1.w, p[nt].z, p[nt].w);
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
   }
-  // the eight warps' sums, in a fixed order: w + (w + 4), then over w
-  auto at = [&](int nt, int i) { return (g4 + 8 * (i >> 1)) * R + nt * 8 + 2 * tig + (i & 1); };
-  if (warp >= 4) {
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();
+  const int ranks = gridDim.y, me = blockIdx.y;  // the cluster spans grid.y
+  const int per = (t.rows + ranks - 1) / ranks;
+  const int row_hi = min(t.rows, (me + 1) * per);
+  const float s = a.scale[t.adapter];
+  if (!*abort_flag) {
+    for (int i = me * per * (R / 4) + tid; i < row_hi * (R / 4); i += C::kThreads) {
+      const int row = i / (R / 4), c = (i % (R / 4)) * 4;
+      const int token = t.token(a.words + a.lay.off_perm, row);
+      if (c >= a.rank) continue;
+      const uint32_t at = sbase + static_cast<uint32_t>(row * C::kRedStride + c) * 4u;
+      float4 u[8];  // every rank's loads before the first sum
 #pragma unroll
-    for (int nt = 0; nt < R / 8; ++nt)
+      for (int q = 0; q < 8; ++q)
+        if (q < ranks) u[q] = ld_cluster_f4(mapa_shared(at, q));
+      float v[4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp - 4][at(nt, i)] = acc[nt][i];
+      for (int q = 0; q < 8; ++q)
+        if (q < ranks) {
+          v[0] += u[q].x;
+          v[1] += u[q].y;
+          v[2] += u[q].z;
+          v[3] += u[q].w;
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= s;
+      const int64_t o = static_cast<int64_t>(token) * a.rank + c;
+      *reinterpret_cast<uint2*>(a.hidden + o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      if (a.hidden32 != nullptr) *reinterpret_cast<float4*>(a.hidden32 + o) = make_float4(v[0], v[1], v[2], v[3]);
+    }
   }
-  __syncthreads();
-  if (warp < 4) {
-#pragma unroll
-    for (int nt = 0; nt < R / 8; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp][at(nt, i)] += acc[nt][i];
-  }
-  __syncthreads();
-  float* out = a.part + (static_cast<int64_t>(blockIdx.y) * a.lay.cap + t.row) * a.rank;
-  for (int i = threadIdx.x; i < 16 * R; i += 256) {
-    const int row = i / R, c = i - row * R;
-    if (c < a.rank) out[row * a.rank + c] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+  __syncwarp();
+  cluster_sync();  // the other ranks have read this one's sums
+  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << 5);
+  if (warp == C::kProducers) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
   }
 }
-
-// --------------------------------------------------------------------- up
-// O[m, :] = act(Y[m, :] + s_a v[m, :] . P_a), v the sum of the down kernel's
-// splits, rounded to bf16 here, once, for the MMA (its 2^-9 is on the added
-// term alone; O is rounded to bf16 after the add).
-//
-// A warp owns 16 rows and CW columns at a time.  P's 64-column pieces are
-// staged in shared memory with their columns permuted: 4-byte pair j of the
-// 16-byte chunk t of a 32-column group is stored as pair t of chunk j, so that
-// MMA column 2 tig + e of n-tile j is column 8 tig + 2 j + e of the group and
-// each thread's accumulators are 16 consecutive bytes of a row of O: Y is read
-// and O written in 16-byte pieces without another trip through shared memory.
-template <int R, int WM>
-struct UpCfg {
-  static constexpr int kRows = 16 * WM;
-  static constexpr int WN = 8 / WM;
-  static constexpr int kWarpCols = WM == 8 ? 64 : 32;
-  static constexpr int kStepCols = WN * kWarpCols;  // 64 or 256
-  static constexpr int kGroups = kWarpCols / 32;
-  static constexpr int kChunks = R * kStepCols / 8;          // 16-byte pieces of P per step
-  static constexpr int kPerThread = (kChunks + 255) / 256;
-  static constexpr int kBuf = R * kStepCols * 2;
-  static constexpr int kBufs = WM == 8 ? 2 : 1;
-  static constexpr int kSmemBytes = kBufs * kBuf;
-};
-
-struct UpArgs {
-  const __nv_bfloat16* y;
-  const __nv_bfloat16* bank;
-  const float* scale;
-  const int32_t* words;
-  const float* part;
-  __nv_bfloat16* out;
-  __nv_bfloat16* hidden;
-  AdapterPlan lay;
-  int64_t ldy, ldo;
-  int N, rank, A, splits, act, with_none, cols_per_cta;
-};
 
 __device__ __forceinline__ void unpack8(uint4 u, float* v) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -468,34 +550,93 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
                     pack_bf16x2(v[6], v[7]));
 }
 
-template <int R, int WM>
-__global__ void __launch_bounds__(256, 2) adapter_up_kernel(const UpArgs a) {
-  using C = UpCfg<R, WM>;
+// Activations of the sum y + delta, float32 in and out (rounded once, with the
+// result): gelu_tanh(x) = x sigmoid(2 u), u = sqrt(2/pi) (x + 0.044715 x^3), and
+// silu(x) = x sigmoid(x), sigmoid(z) = 1 / (1 + 2^(-z log2 e)): an exponential
+// and a reciprocal of the special-function unit, whose 16 results a cycle and
+// SM stay below the stream's time (2^inf gives 1 / inf = 0: no clamp).
+__device__ __forceinline__ float sigmoid_of_neg_log2(float z) { return rcp_approx(1.0f + exp2f_approx(z)); }
+__device__ __forceinline__ void gelu_tanh4(float* x) {
+  constexpr float k = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] *= sigmoid_of_neg_log2(x[i] * fmaf(x[i] * x[i], 0.044715f * k, k));
+}
+__device__ __forceinline__ void silu4(float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] *= sigmoid_of_neg_log2(x[i] * -1.4426950408889634f);
+}
+__device__ __forceinline__ void gate4(float* x, int act) {
+  if (act == kActSwiGlu)
+    silu4(x);
+  else
+    gelu_tanh4(x);
+}
+
+// --------------------------------------------------------------------- up
+// O[m, :] = act(Y[m, :] + hidden[m, :] . P_a): 128-row tiles, one warp per 16.
+//
+// Bound: the stream of Y and O (P and hidden are small and reread from L2).
+// The products take a sixteenth of the warp MMA rate at the copy bandwidth,
+// so they stay warp-level with their sums in registers, and the layout is
+// arranged for the stream: P's 64-column pieces are staged in shared memory
+// with their columns permuted -- 4-byte pair j of the 16-byte chunk t of a
+// 32-column group is stored as pair t of chunk j -- so that MMA column
+// 2 tig + e of n-tile j is column 8 tig + 2 j + e of the group and each
+// thread's sums are 16 consecutive bytes of a row of O: Y is read and O
+// written in 16-byte pieces, the next step's Y and P while this one computes.
+template <int R>
+struct UpCfg {
+  static constexpr int kStepCols = 64;
+  static constexpr int kChunks = R * kStepCols / 8;  // 16-byte pieces of P per step
+  static constexpr int kPerThread = (kChunks + 255) / 256;
+  static constexpr int kBuf = R * kStepCols * 2;
+  static constexpr int kSmemBytes = 2 * kBuf;
+};
+
+struct UpArgs {
+  const __nv_bfloat16* y;
+  const __nv_bfloat16* bank;
+  const __nv_bfloat16* hidden;
+  const int32_t* words;
+  __nv_bfloat16* out;
+  __nv_bfloat16* zero_hidden;  // rows without an adapter are zeroed here (or NULL)
+  AdapterPlan lay;
+  int64_t ldy, ldo;
+  int N, rank, A, act, with_none, cols_per_cta;
+};
+
+template <int R>
+__global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const UpArgs a) {
+  using C = UpCfg<R>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
-  const PlanTile t = plan_tile<C::kRows>(a.words, a.lay, a.A, blockIdx.x, a.with_none != 0);
+  const PlanTile t = plan_tile<kTileRows>(a.words, a.lay, a.A, blockIdx.x, a.with_none != 0);
   if (t.rows == 0) {
     grid_wait();  // no CTA ends before the grid it depends on
     return;
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, tig = lane & 3;
-  const int wm = warp % WM, wn = warp / WM;
   const int n_lo = blockIdx.y * a.cols_per_cta;
   const int n_hi = min(a.N, n_lo + a.cols_per_cta);
   const bool none = t.adapter >= a.A;
-  const bool active = wm * 16 < t.rows;
-  const int tok0 = active ? a.words[a.lay.off_perm + t.row + wm * 16 + g4] : -1;
-  const int tok1 = active ? a.words[a.lay.off_perm + t.row + wm * 16 + g4 + 8] : -1;
+  const int tok0 = t.token(a.words + a.lay.off_perm, warp * 16 + g4);
+  const int tok1 = t.token(a.words + a.lay.off_perm, warp * 16 + g4 + 8);
   const __nv_bfloat16* P = none ? a.bank : a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.N;
+  const __nv_bfloat16* y0 = a.y + static_cast<int64_t>(tok0) * a.ldy + 8 * tig;
+  const __nv_bfloat16* y1 = a.y + static_cast<int64_t>(tok1) * a.ldy + 8 * tig;
   const bool gated = act_is_gated(a.act);
+  // gated: lanes 0, 1 of a quad write its 16 output columns of a 32-column group
+  __nv_bfloat16* o0 = a.out + static_cast<int64_t>(tok0) * a.ldo + 8 * tig;
+  __nv_bfloat16* o1 = a.out + static_cast<int64_t>(tok1) * a.ldo + 8 * tig;
+  const bool st0 = tok0 >= 0 && (!gated || tig < 2), st1 = tok1 >= 0 && (!gated || tig < 2);
 
   uint4 preg[C::kPerThread];
   auto load_p = [&](int n0) {
 #pragma unroll
     for (int i = 0; i < C::kPerThread; ++i) {
       const int c = tid + 256 * i;
-      const int row = c / (C::kStepCols / 8), col = n0 + (c % (C::kStepCols / 8)) * 8;
+      const int row = c >> 3, col = n0 + (c & 7) * 8;
       const bool ok = !none && row < a.rank && col < n_hi && c < C::kChunks;
       preg[i] = ok ? __ldg(reinterpret_cast<const uint4*>(P + static_cast<int64_t>(row) * a.N + col))
                    : make_uint4(0u, 0u, 0u, 0u);
@@ -506,70 +647,51 @@ __global__ void __launch_bounds__(256, 2) adapter_up_kernel(const UpArgs a) {
     for (int i = 0; i < C::kPerThread; ++i) {
       const int c = tid + 256 * i;
       if (C::kChunks % 256 != 0 && c >= C::kChunks) break;
-      const int row = c / (C::kStepCols / 8), cc = c % (C::kStepCols / 8);
-      // 64-column piece cc / 8, 32-column group (cc / 4) % 2, chunk cc % 4
-      const uint32_t base = sbase + buf * C::kBuf + (cc >> 3) * (R * 128) + row * 128 + 4 * (cc & 3);
+      const int row = c >> 3, cc = c & 7;  // 32-column group cc / 4, chunk cc % 4 of it
+      const uint32_t base = sbase + buf * C::kBuf + row * 128 + 4 * (cc & 3);
       const uint32_t w[4] = {preg[i].x, preg[i].y, preg[i].z, preg[i].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sts32(base + (((((cc >> 2) & 1) * 4 + j) ^ (row & 7)) << 4), w[j]);
+      for (int j = 0; j < 4; ++j) sts32(base + ((((cc >> 2) * 4 + j) ^ (row & 7)) << 4), w[j]);
     }
   };
-  // this thread's 8 columns of each 32-column group of its two rows
-  uint4 yreg[C::kGroups][2];
+  // this thread's 8 columns of both 32-column groups of its two rows
+  uint4 yreg[2][2] = {};
   auto load_y = [&](int n0) {
 #pragma unroll
-    for (int g = 0; g < C::kGroups; ++g) {
-      const int col = n0 + wn * C::kWarpCols + g * 32 + 8 * tig;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int tok = h ? tok1 : tok0;
-        if (tok >= 0 && col < n_hi)
-          yreg[g][h] = *reinterpret_cast<const uint4*>(a.y + static_cast<int64_t>(tok) * a.ldy + col);
+    for (int g = 0; g < 2; ++g) {
+      const int col = n0 + g * 32;
+      if (col + 8 * tig < n_hi) {
+        if (tok0 >= 0) yreg[g][0] = ld_global_l2(y0 + col);
+        if (tok1 >= 0) yreg[g][1] = ld_global_l2(y1 + col);
       }
     }
   };
   load_p(n_lo);
   load_y(n_lo);
-
-  // the down kernel's sums
-  grid_wait();
-  uint32_t vf[R / 16][4];
-  {
-    const float s = none ? 0.f : a.scale[t.adapter];
-    const int64_t split_stride = a.lay.cap * a.rank;
-    const float* base = a.part + static_cast<int64_t>(t.row + wm * 16 + g4) * a.rank + 2 * tig;
-#pragma unroll
-    for (int ks = 0; ks < R / 16; ++ks)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = ks * 16 + 8 * (q >> 1);
-        float2 v = make_float2(0.f, 0.f);
-        if (!none && active && c < a.rank) {
-          const float* p = base + static_cast<int64_t>(8 * (q & 1)) * a.rank + c;
-          for (int i = 0; i < a.splits; ++i) {
-            const float2 u = __ldcg(reinterpret_cast<const float2*>(p + i * split_stride));
-            v.x += u.x;
-            v.y += u.y;
-          }
-        }
-        vf[ks][q] = pack_bf16x2(v.x * s, v.y * s);
-        if (a.hidden != nullptr && blockIdx.y == 0 && wn == 0 && c < a.rank) {
-          const int tok = (q & 1) ? tok1 : tok0;
-          if (tok >= 0)
-            *reinterpret_cast<uint32_t*>(a.hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig) = vf[ks][q];
-        }
-      }
-  }
-  grid_launch_dependents();
   store_p(0);
+
+  grid_wait();  // hidden is the down kernel's
+  uint32_t vf[R / 16][4];
+#pragma unroll
+  for (int ks = 0; ks < R / 16; ++ks)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = ks * 16 + 8 * (q >> 1);
+      const int tok = (q & 1) ? tok1 : tok0;
+      const bool ok = !none && tok >= 0 && c < a.rank;
+      vf[ks][q] = ok ? __ldcg(reinterpret_cast<const unsigned int*>(a.hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig))
+                     : 0u;
+      if (none && a.zero_hidden != nullptr && blockIdx.y == 0 && tok >= 0 && c < a.rank)
+        *reinterpret_cast<uint32_t*>(a.zero_hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig) = 0u;
+    }
+  grid_launch_dependents();
   __syncthreads();
 
   int buf = 0;
   for (int n0 = n_lo; n0 < n_hi; n0 += C::kStepCols) {
-    uint4 ycur[C::kGroups][2];
+    uint4 ycur[2][2];
 #pragma unroll
-    for (int g = 0; g < C::kGroups; ++g) {
+    for (int g = 0; g < 2; ++g) {
       ycur[g][0] = yreg[g][0];
       ycur[g][1] = yreg[g][1];
     }
@@ -578,316 +700,656 @@ __global__ void __launch_bounds__(256, 2) adapter_up_kernel(const UpArgs a) {
       load_p(n0 + C::kStepCols);
       load_y(n0 + C::kStepCols);
     }
-    float acc[C::kGroups][4][4] = {};
-    if (!none && active) {
-      const int wcol = wn * C::kWarpCols;
-      const uint32_t piece = sbase + buf * C::kBuf + (wcol / 64) * (R * 128);
-      const int g0 = (wcol % 64) / 32;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float acc[4][4];
+      // (a tile without an adapter multiplies zeros: P's pieces were loaded as such)
       const int krow = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
       for (int ks = 0; ks < R / 16; ++ks)
 #pragma unroll
-        for (int g = 0; g < C::kGroups; ++g)
-#pragma unroll
-          for (int jp = 0; jp < 2; ++jp) {
-            uint32_t bf[4];
-            const int row = ks * 16 + krow;
-            const int ch = (g0 + g) * 4 + 2 * jp + (lane >> 4);
-            ldmatrix_x4_trans(piece + row * 128 + ((ch ^ (row & 7)) << 4), bf);
-            mma_16816_bf16(acc[g][2 * jp], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[0], bf[1]);
-            mma_16816_bf16(acc[g][2 * jp + 1], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[2], bf[3]);
+        for (int jp = 0; jp < 2; ++jp) {
+          uint32_t bf[4];
+          const int row = ks * 16 + krow;
+          const int ch = g * 4 + 2 * jp + (lane >> 4);
+          ldmatrix_x4_trans(sbase + buf * C::kBuf + row * 128 + ((ch ^ (row & 7)) << 4), bf);
+          if (ks == 0) {
+            mma_16816_bf16_zero(acc[2 * jp], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[0], bf[1]);
+            mma_16816_bf16_zero(acc[2 * jp + 1], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[2], bf[3]);
+          } else {
+            mma_16816_bf16(acc[2 * jp], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[0], bf[1]);
+            mma_16816_bf16(acc[2 * jp + 1], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[2], bf[3]);
           }
-    }
-#pragma unroll
-    for (int g = 0; g < C::kGroups; ++g) {
-      const int col = n0 + wn * C::kWarpCols + g * 32 + 8 * tig;
+        }
+      const int col = n0 + g * 32;
+      const bool in = col + 8 * tig < n_hi;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int tok = h ? tok1 : tok0;
-        float v[8] = {};
-        if (tok >= 0 && col < n_hi) unpack8(ycur[g][h], v);
+        float v[8];
+        unpack8(ycur[g][h], v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[2 * j] += acc[g][j][2 * h];
-          v[2 * j + 1] += acc[g][j][2 * h + 1];
+          v[2 * j] += acc[j][2 * h];
+          v[2 * j + 1] += acc[j][2 * h + 1];
         }
-        if (gated) {
+        int oc = col;
+        if (a.act == kActGeluTanh) {
+          gelu_tanh4(v);
+          gelu_tanh4(v + 4);
+        } else if (gated) {
           // lanes 0, 1 of the quad hold 16 gate columns, lanes 2, 3 their up columns
+          float u[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float up = __shfl_down_sync(0xffffffffu, v[e], 2, 4);
-            v[e] = gated_value(v[e], up, a.act);
-          }
-          if (tok >= 0 && col < n_hi && tig < 2)
-            *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(tok) * a.ldo + (col - 8 * tig) / 2 + 8 * tig) =
-                pack8(v);
-        } else if (tok >= 0 && col < n_hi) {
-          if (a.act != kActNone) {
+          for (int e = 0; e < 8; ++e) u[e] = __shfl_down_sync(0xffffffffu, v[e], 2, 4);
+          gate4(v, a.act);
+          gate4(v + 4, a.act);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = apply_act(v[e], a.act);
-          }
-          *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(tok) * a.ldo + col) = pack8(v);
+          for (int e = 0; e < 8; ++e) v[e] *= u[e];
+          oc = col / 2;
         }
+        if (in && (h ? st1 : st0)) *reinterpret_cast<uint4*>((h ? o1 : o0) + oc) = pack8(v);
       }
     }
     if (more) {
-      if constexpr (C::kBufs == 2) {
-        buf ^= 1;
-      } else {
-        __syncthreads();
-      }
+      buf ^= 1;
       store_p(buf);
       __syncthreads();
     }
   }
 }
 
+// ------------------------------------------------------------------ small
+// Small batches: down and up of one 16-row tile in one launch.  What counts is
+// the chain launch -> plan -> operands -> sum -> operands -> store, so it is
+// made short: a cluster of eight CTAs shares the tile, each summing an eighth
+// of the features (its warps straight from global memory into MMA fragments),
+// the sums meet through distributed shared memory in rank order, and each CTA
+// then writes its share of the columns, whose piece of P and Y it asked for
+// before the first sum.  A sum over k may visit k in any order as long as both
+// operands use the same one: thread tig of a quad takes the eight consecutive
+// features 8 tig .. of every group of 32 (one 16-byte load per row), as k slots
+// 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9 of two MMAs.
+constexpr int kSmallCluster = 8;
+template <int R>
+struct SmallCfg {
+  static constexpr int kStepCols = 256;  // 32 per warp
+  static constexpr int kYStride = kStepCols * 2 + 16;  // bytes of a staged row of Y (conflict-free 4-byte reads)
+  static constexpr int kOffY = R * kStepCols * 2;      // in a buffer: P's four pieces, then Y's 16 rows
+  static constexpr int kBuf = kOffY + 16 * kYStride + 256;
+  static constexpr int kBufs = R <= 16 ? 4 : R <= 64 ? 3 : 2;  // steps of P and Y, all but one asked for at the start
+  static_assert(kBuf % 128 == 0, "P's pieces are 128-byte rows");
+  static constexpr int kOffRed = kBufs * kBuf;              // 4 x [16][R] f32
+  static constexpr int kOffSum = kOffRed + 4 * 16 * R * 4;  // [16][R] f32, read by the cluster
+  static constexpr int kVStride = R * 2 + 16;              // bytes of a row of the bf16 hidden tile
+  static constexpr int kOffV = kOffSum + 16 * R * 4;
+  static constexpr int kSmemBytes = kOffV + 16 * kVStride;
+};
+
+struct SmallArgs {
+  const __nv_bfloat16 *x, *y, *down, *up;
+  const float* scale;
+  const int32_t* words;
+  __nv_bfloat16* out;
+  __nv_bfloat16* hidden;  // [M, rank] or NULL
+  float* hidden32;        // [M, rank] or NULL
+  AdapterPlan lay;
+  int64_t ldx, ldy, ldo;
+  int K, N, rank, A, act, with_none, k_per_rank, cols_per_cta, ctas_per_tile;
+};
+
+template <int R>
+__global__ void __launch_bounds__(256, R <= 32 ? 3 : 1) adapter_small_kernel(const SmallArgs a) {
+  using C = SmallCfg<R>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t sbase = smem_u32(smem_raw);
+  float* red = reinterpret_cast<float*>(smem_raw + C::kOffRed);
+  const PlanTile t = plan_tile<kBlockRows>(a.words, a.lay, a.A, blockIdx.x / a.ctas_per_tile, a.with_none != 0);
+  if (t.rows == 0) return;  // the whole cluster: it shares the tile
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g4 = lane >> 2, tig = lane & 3;
+  const int part = blockIdx.x % a.ctas_per_tile;  // of the columns
+  const int rank = part % kSmallCluster;          // in the cluster
+  const bool none = t.adapter >= a.A;
+  const int tok0 = a.words[a.lay.off_perm + t.row + g4];
+  const int tok1 = a.words[a.lay.off_perm + t.row + g4 + 8];
+  const int ytok0 = a.words[a.lay.off_perm + t.row + warp];
+  const int ytok1 = a.words[a.lay.off_perm + t.row + warp + 8];
+  const int n_lo = part * a.cols_per_cta;
+  const int n_hi = min(a.N, n_lo + a.cols_per_cta);
+  const __nv_bfloat16* U = none ? a.up : a.up + static_cast<int64_t>(t.adapter) * a.rank * a.N;
+
+  // columns n0 .. n0 + 255 of P (four 64-column pieces of [R][128 bytes]) and of
+  // the tile's rows of Y
+  auto load_step = [&](int n0, int buf) {
+    if (n0 < n_hi) {
+      if (!none) {
+#pragma unroll 4
+        for (int c = tid; c < R * 32; c += 256) {
+          const int row = c >> 5, cc = c & 31, col = n0 + cc * 8;
+          const bool ok = row < a.rank && col < n_hi;
+          cp_async_16(sbase + buf * C::kBuf + (cc >> 3) * (R * 128) + row * 128 + (((cc & 7) ^ (row & 7)) << 4),
+                      ok ? U + static_cast<int64_t>(row) * a.N + col : a.up, ok);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // rows warp and warp + 8
+        const int col = n0 + lane * 8;
+        const int tok = i ? ytok1 : ytok0;
+        if (tok >= 0 && col < n_hi)
+          cp_async_16(sbase + buf * C::kBuf + C::kOffY + (warp + 8 * i) * C::kYStride + lane * 16,
+                      a.y + static_cast<int64_t>(tok) * a.ldy + col, true);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < C::kBufs - 1; ++i) load_step(n_lo + i * C::kStepCols, i);
+
+  if (!none) {
+    const __nv_bfloat16* x0 = a.x + static_cast<int64_t>(tok0) * a.ldx;
+    const __nv_bfloat16* x1 = a.x + static_cast<int64_t>(tok1) * a.ldx;
+    const __nv_bfloat16* P = a.down + static_cast<int64_t>(t.adapter) * a.rank * a.K;
+    const int k_hi = min(a.K, (rank + 1) * a.k_per_rank);
+    float acc[R / 8][4] = {};
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll (R <= 32 ? 2 : 1)
+    for (int k = rank * a.k_per_rank + warp * 32 + tig * 8; k < k_hi + tig * 8; k += 256) {
+      const bool in = k < k_hi;
+      const uint4 u0 = in && tok0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+      const uint4 u1 = in && tok1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+      uint4 p[R / 8];
+#pragma unroll
+      for (int nt = 0; nt < R / 8; ++nt)
+        p[nt] = in && nt * 8 < a.rank ? ld_stream16(P + static_cast<int64_t>(nt * 8 + g4) * a.K + k) : zero;
+#pragma unroll
+      for (int nt = 0; nt < R / 8; ++nt) {
+        mma_16816_bf16(acc[nt], u0.x, u1.x, u0.y, u1.y, p[nt].x, p[nt].y);
+        mma_16816_bf16(acc[nt], u0.z, u1.z, u0.w, u1.w, p[nt].z, p[nt].w);
+      }
+    }
+    // the eight warps' sums, in a fixed order: w + (w + 4), then over w
+    auto at = [&](int w, int nt, int i) {
+      return (w * 16 + g4 + 8 * (i >> 1)) * R + nt * 8 + 2 * tig + (i & 1);
+    };
+    if (warp >= 4) {
+#pragma unroll
+      for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[at(warp - 4, nt, i)] = acc[nt][i];
+    }
+    __syncthreads();
+    if (warp < 4) {
+#pragma unroll
+      for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[at(warp, nt, i)] += acc[nt][i];
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * R; i += 256)
+      *reinterpret_cast<float*>(smem_raw + C::kOffSum + 4 * i) =
+          (red[i] + red[16 * R + i]) + (red[32 * R + i] + red[48 * R + i]);
+  }
+  __syncwarp();
+  cluster_sync();
+  {
+    const float s = none ? 0.f : a.scale[t.adapter];
+    for (int i = tid; i < 16 * (R / 2); i += 256) {
+      const int row = i / (R / 2), c = (i % (R / 2)) * 2;
+      float2 v = make_float2(0.f, 0.f);
+      if (!none) {
+        float2 u[kSmallCluster];
+#pragma unroll
+        for (int q = 0; q < kSmallCluster; ++q)
+          u[q] = ld_cluster_f2(mapa_shared(sbase + C::kOffSum + 4u * (row * R + c), q));
+#pragma unroll
+        for (int q = 0; q < kSmallCluster; ++q) {
+          v.x += u[q].x;
+          v.y += u[q].y;
+        }
+      }
+      v.x *= s;
+      v.y *= s;
+      const uint32_t b = pack_bf16x2(v.x, v.y);
+      sts32(sbase + C::kOffV + row * C::kVStride + 2 * c, b);
+      if (part == 0 && a.hidden != nullptr && c < a.rank) {
+        const int tok = a.words[a.lay.off_perm + t.row + row];
+        if (tok >= 0) {
+          const int64_t o = static_cast<int64_t>(tok) * a.rank + c;
+          *reinterpret_cast<uint32_t*>(a.hidden + o) = b;
+          if (a.hidden32 != nullptr) *reinterpret_cast<float2*>(a.hidden32 + o) = v;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  cluster_arrive();  // this CTA has read the others' sums
+
+  int buf = 0;
+  for (int n0 = n_lo; n0 < n_hi; n0 += C::kStepCols, buf = buf + 1 == C::kBufs ? 0 : buf + 1) {
+    cp_async_wait<C::kBufs - 2>();
+    __syncthreads();  // P of this step and the hidden tile are there; the last step's buffer is free
+    load_step(n0 + (C::kBufs - 1) * C::kStepCols, buf == 0 ? C::kBufs - 1 : buf - 1);
+    float acc[4][4] = {};
+    if (!none) {
+      const int wcol = warp * 32;
+      const uint32_t piece = sbase + buf * C::kBuf + (wcol / 64) * (R * 128);
+      const int krow = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+      for (int ks = 0; ks < R / 16; ++ks) {
+        uint32_t af[4];
+        ldmatrix_x4(sbase + C::kOffV + (lane & 15) * C::kVStride + (2 * ks + (lane >> 4)) * 16, af);
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+          uint32_t bf[4];
+          const int row = ks * 16 + krow;
+          const int ch = (wcol % 64) / 8 + 2 * jp + (lane >> 4);
+          ldmatrix_x4_trans(piece + row * 128 + ((ch ^ (row & 7)) << 4), bf);
+          mma_16816_bf16(acc[2 * jp], af[0], af[1], af[2], af[3], bf[0], bf[1]);
+          mma_16816_bf16(acc[2 * jp + 1], af[0], af[1], af[2], af[3], bf[2], bf[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int tok = h ? tok1 : tok0;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = lds32(sbase + buf * C::kBuf + C::kOffY + (g4 + 8 * h) * C::kYStride + (warp * 32 + 8 * j + 2 * tig) * 2);
+        v[2 * j] = __uint_as_float(u << 16) + acc[j][2 * h];
+        v[2 * j + 1] = __uint_as_float(u & 0xFFFF0000u) + acc[j][2 * h + 1];
+      }
+      const int col = n0 + warp * 32 + 2 * tig;
+      if (a.act == kActGeluTanh) {
+        gelu_tanh4(v);
+        gelu_tanh4(v + 4);
+      } else if (a.act != kActNone) {  // n-tiles 0, 1 hold 16 gate columns, 2, 3 their up columns
+        gate4(v, a.act);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= v[4 + e];
+      }
+      if (tok < 0) continue;
+      if (a.act == kActNone || a.act == kActGeluTanh) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + 8 * j < n_hi)
+            *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + col + 8 * j) =
+                pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      } else if (col < n_hi) {
+        const int oc = (n0 + warp * 32) / 2 + 2 * tig;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + oc + 8 * j) =
+              pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+  cluster_wait();  // the others have read this CTA's sums
+}
+
 // ------------------------------------------------------------------ wgrad
-// dP_a[r, c] = sum over a's rows of G[m, r] X[m, c].  CTA = (column tile, row
-// split): the plan's rows are cut into splits of L rows whatever the adapters;
-// a CTA walks its rows in stages of 64 (cp.async ring), and at each adapter's
-// end adds its warps' sums in shared memory in a fixed order and writes them:
-// straight to the bf16 result if the split holds all of the adapter's rows,
-// else to one of the split's two f32 slots: 0 for the adapter that began in an
-// earlier split, 1 for the one that goes on in a later one (there is at most
-// one of each).  A reduce kernel adds an adapter's slots in order.  No atomics.
+// dP_a[r, c] = sum over a's rows of G[m, r] X[m, c], as D = X^T G on tcgen05:
+// M = 128 columns of X, N = R, k = tokens, both operands MN-major (a token's
+// features are contiguous) in 128-byte-swizzled [64 tokens][64 features]
+// blocks.  D's lanes are columns of dP, so its rows leave tensor memory
+// coalesced, without a transpose.  (Warp-level MMAs with ldmatrix.trans
+// fragments ran the same sums at 1.7 TB/s of X.)
 //
-// Both operands have the tokens as the MMA's k: G^T and X come through
-// ldmatrix.trans.  An 8-bit X (int8 codes) is read the same way as 16-bit
-// pairs; each loaded word then holds the codes of two columns at two tokens,
-// which byte permutes turn into the fragments of an even and an odd column
-// tile: the code as a bf16 is exact ((128 + low seven bits) - (128 or 256)),
-// and the row's scale of this 128-column tile multiplies G instead, in f32,
-// rounded once to bf16 as the MMA's operand.
+// CTA = (column tile, row split): the plan's rows are cut into splits of L rows
+// whatever the adapters; a CTA walks its rows in stages of 64 and changes to
+// its other accumulator at each adapter's end, while four warps write the
+// finished one: straight to the bf16 result if the split holds all of the
+// adapter's rows, else to one of the split's two f32 slots: 0 for the adapter
+// that began in an earlier split, 1 for the one that goes on in a later one
+// (there is at most one of each).  A reduce kernel adds an adapter's slots in
+// order.  No atomics.
+//
+// An 8-bit X: the codes go through a ring of their own (each thread converts
+// the 16 bytes it copied itself), become bf16 exactly ((128 + low seven bits)
+// - (128 or 256)), and the row's scale of this 128-column tile multiplies G
+// instead, in f32, rounded once to bf16 as the MMA's operand.
 template <int R, bool I8>
 struct WgradCfg {
-  static constexpr int kCols = I8 ? 128 : 64;              // 128 bytes of X per row
-  static constexpr int WC = (I8 && R >= 64) ? 4 : 2;       // warps along the columns
-  static constexpr int WK = 8 / WC;                        // warps along the tokens
-  static constexpr int kWarpCols = kCols / WC;
-  static constexpr int kNT = kWarpCols / 8;
+  static constexpr int kCols = 128;
   static constexpr int kRows = 64;
-  static constexpr int kStageX = kRows * 128;
-  static constexpr int kStageG = kRows * R * 2;
-  static constexpr int kStageS = I8 ? kRows * 4 : 0;
-  static constexpr int kStage = kStageX + kStageG + kStageS;
-  static constexpr int kStages = R <= 32 ? 6 : R <= 64 ? (I8 ? 4 : 5) : 3;
-  static constexpr int kRedBytes = R * kCols * 4;
-  static constexpr int kSmemBytes = kStages * kStage + kRedBytes;
+  static constexpr int kBlock = kRows * 128;            // [64 tokens][64 features] bf16
+  static constexpr int kGBlocks = (R + 63) / 64;
+  static constexpr int kStage = (2 + kGBlocks) * kBlock;
+  static constexpr int kStages = I8 ? 3 : (R <= 64 ? 4 : 3);
+  static constexpr int kAhead = I8 ? 0 : kStages - 2;   // stages a thread's copies run ahead
+  static constexpr int kRaw = I8 ? 4 : 0;               // stages of raw codes
+  static constexpr int kRawStage = kRows * 128;
+  static constexpr int kThreads = (4 + 1 + 8) * 32;     // epilogue, MMA, producer warps
+  static constexpr int kOffRaw = kStages * kStage;
+  static constexpr int kOffBar = kOffRaw + kRaw * kRawStage;
+  static constexpr int kSmemBytes = kOffBar + 16 * kStages + 64 + 1024;
+  static constexpr int kMinCtas = 2 * (kSmemBytes + 1024) <= 228 * 1024 ? 2 : 1;
+  static constexpr int kTmemCols = 2 * R;
 };
 
 struct WgradArgs {
   const void* x;
   const float* x_scales;
   const __nv_bfloat16* g;
+  const float* g32;  // with an 8-bit X
   const int32_t* words;
   float* part;
   __nv_bfloat16* dbank;
+  unsigned int* error;
   AdapterPlan lay;
   int64_t ldx;
   int cols, rank, A, rows_per_split;
 };
 
-template <int R>
-__device__ __forceinline__ uint32_t g_swizzle(int row, int chunk) {
-  constexpr int kCh = R / 8;  // 16-byte chunks per row of G
-  const int f = kCh >= 8 ? (row & 7) : kCh == 4 ? ((row >> 1) & 3) : ((row >> 2) & 1);
-  return static_cast<uint32_t>(row * (R * 2) + ((chunk ^ f) << 4));
+// Descriptor of an MN-major operand in 128-byte-swizzled blocks of 64 MN
+// elements x 8 k rows (1024 bytes): consecutive 8-row groups 1024 bytes apart
+// (stride offset), the next 64 MN elements `block` bytes on (leading offset).
+__device__ __forceinline__ uint64_t make_sw128_mnmajor_desc(uint32_t smem_addr, uint32_t block) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
 }
 
-// Four int8 codes (bytes: token 0 columns 0, 1; token 1 columns 0, 1) -> the
-// bf16 pairs (token 0, token 1) of column 0 and of column 1, exact.
-__device__ __forceinline__ void i8_pairs(uint32_t u, uint32_t& even, uint32_t& odd) {
+// Four int8 codes -> two bf16 pairs, exact.
+__device__ __forceinline__ void i8_to_bf16(uint32_t u, uint32_t& p01, uint32_t& p23) {
   const uint32_t low = u & 0x7F7F7F7Fu, sign = u & 0x80808080u;
-  const uint32_t e1 = prmt(low, 0x43u, 0x4240u), e2 = prmt(sign, 0x43u, 0x4240u);
-  const uint32_t o1 = prmt(low, 0x43u, 0x4341u), o2 = prmt(sign, 0x43u, 0x4341u);
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(even) : "r"(e1), "r"(e2));
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(odd) : "r"(o1), "r"(o2));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p01) : "r"(prmt(low, 0x43u, 0x4140u)), "r"(prmt(sign, 0x43u, 0x4140u)));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p23) : "r"(prmt(low, 0x43u, 0x4342u)), "r"(prmt(sign, 0x43u, 0x4342u)));
 }
 
-__device__ __forceinline__ uint32_t scale_pair(uint32_t g, float s0, float s1) {
-  return pack_bf16x2(__uint_as_float(g << 16) * s0, __uint_as_float(g & 0xFFFF0000u) * s1);
-}
+// Rows of a split in stages of 64 that never cross an adapter's end.
+struct RowCursor {
+  const int32_t* blk;
+  const int32_t* starts;
+  int pos, end, hi, adapter;
+  __device__ __forceinline__ RowCursor(const int32_t* words, const AdapterPlan& lay, int lo, int hi_)
+      : blk(words + lay.off_blk), starts(words + lay.off_start), pos(lo), end(lo), hi(hi_), adapter(0) {
+    open();
+  }
+  __device__ __forceinline__ bool live() const { return pos < hi; }
+  __device__ __forceinline__ void open() {
+    if (pos < hi) {
+      adapter = blk[pos / 16];
+      end = min(hi, starts[adapter + 1]);
+    }
+  }
+  // to the next stage; true if the adapter's rows of this split are done
+  __device__ __forceinline__ bool next() {
+    pos += 64;
+    if (pos < end) return false;
+    pos = end;
+    open();
+    return true;
+  }
+};
 
 template <int R, bool I8>
-__global__ void __launch_bounds__(256, R <= 64 ? 2 : 1) adapter_wgrad_kernel(const WgradArgs a) {
+__global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kMinCtas)
+    adapter_wgrad_kernel(const WgradArgs a) {
   using C = WgradCfg<R, I8>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const uint32_t sbase = smem_u32(smem_raw);
-  float* red = reinterpret_cast<float*>(smem_raw + C::kStages * C::kStage);
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sbase - raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g4 = lane >> 2, tig = lane & 3;
-  const int wc = warp % C::WC, wk = warp / C::WC;
+  auto full_bar = [&](int s) { return sbase + C::kOffBar + 8u * s; };
+  auto empty_bar = [&](int s) { return sbase + C::kOffBar + 8u * (C::kStages + s); };
+  auto acc_full = [&](int b) { return sbase + C::kOffBar + 16u * C::kStages + 8u * b; };
+  auto acc_empty = [&](int b) { return sbase + C::kOffBar + 16u * C::kStages + 16u + 8u * b; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffBar + 16 * C::kStages + 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + 16 * C::kStages + 40);
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full_bar(s), 8);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 4);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   const int col0 = blockIdx.x * C::kCols;
-  const int32_t* perm = a.words + a.lay.off_perm;
-  const int32_t* blk = a.words + a.lay.off_blk;
-  const int32_t* starts = a.words + a.lay.off_start;
   const int row_lo = blockIdx.y * a.rows_per_split;
   const int row_hi = min(row_lo + a.rows_per_split, a.words[AdapterPlan::kNoneStart]);
   grid_wait();  // G may be the output of the kernel before this one
-  if (row_lo >= row_hi) return;
+  RowCursor cur(a.words, a.lay, row_lo, row_hi);
 
-  // stages: 64 rows from `pos`, not past the adapter's end `end`
-  struct Cursor {
-    int pos, end, adapter;
-  };
-  auto open = [&](Cursor& c) {
-    if (c.pos < row_hi) {
-      c.adapter = blk[c.pos / 16];
-      c.end = min(row_hi, starts[c.adapter + 1]);
+  if (warp >= 5) {
+    // -------------------------------------------------------------- producers
+    const int32_t* perm = a.words + a.lay.off_perm;
+    const int pt = tid - 160;
+    if constexpr (!I8) {
+      const int ch = pt & 15;  // 16-byte chunk of a row's 128 columns
+      const bool col_ok = col0 + ch * 8 < a.cols;
+      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x) + col0 + ch * 8;
+      // the tokens of a stage's rows, looked up one stage ahead
+      constexpr int kG = (64 * (R / 8) + 255) / 256;
+      int tx[4], tg[kG];
+      auto look_up = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (pt >> 4) + 16 * i;
+          tx[i] = cur.live() && cur.pos + row < cur.end ? perm[cur.pos + row] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+          const int row = (pt + 256 * i) / (R / 8);
+          tg[i] = cur.live() && row < 64 && cur.pos + row < cur.end ? perm[cur.pos + row] : -1;
+        }
+      };
+      look_up();
+      int it = 0;
+      for (; cur.live(); ++it) {
+        const int slot = it % C::kStages;
+        if (!mbar_wait(empty_bar(slot), static_cast<uint32_t>(((it / C::kStages) & 1) ^ 1), abort_flag)) break;
+        const uint32_t sx = sbase + slot * C::kStage, sg = sx + 2 * C::kBlock;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (pt >> 4) + 16 * i;
+          const bool ok = tx[i] >= 0 && col_ok;
+          cp_async_16_l2(sx + (ch >> 3) * C::kBlock + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
+                         ok ? x + static_cast<int64_t>(tx[i]) * a.ldx : static_cast<const __nv_bfloat16*>(a.x), ok);
+        }
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+          const int e = pt + 256 * i;
+          const int row = e / (R / 8), gc = e % (R / 8);
+          if (64 * (R / 8) % 256 != 0 && row >= 64) break;
+          const bool ok = tg[i] >= 0 && gc * 8 < a.rank;
+          cp_async_16(sg + (gc >> 3) * C::kBlock + row * 128 + (((gc & 7) ^ (row & 7)) << 4),
+                      ok ? a.g + static_cast<int64_t>(tg[i]) * a.rank + gc * 8 : a.g, ok);
+        }
+        cp_async_commit();
+        cur.next();
+        look_up();
+        if (it >= C::kAhead) {
+          cp_async_wait<C::kAhead>();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full_bar((it - C::kAhead) % C::kStages));
+        }
+      }
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (!cur.live() && lane == 0)
+        for (int s = max(0, it - C::kAhead); s < it; ++s) mbar_arrive(full_bar(s % C::kStages));
+    } else {
+      const int8_t* x = static_cast<const int8_t*>(a.x);
+      const int ncb = (a.cols + 127) / 128;
+      const int ch = pt & 7;  // 16 codes
+      const bool col_ok = col0 + ch * 16 < a.cols;
+      RowCursor rc(a.words, a.lay, row_lo, row_hi);  // raw codes, kRaw stages ahead
+      int rit = 0;
+      int tx[2];  // tokens of the next stage's rows, looked up one stage ahead
+      auto look_raw = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = (pt >> 3) + 32 * i;
+          tx[i] = rc.live() && rc.pos + row < rc.end ? perm[rc.pos + row] : -1;
+        }
+      };
+      look_raw();
+      auto load_raw = [&]() {
+        if (rc.live()) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int token = tx[i];
+            const bool ok = token >= 0 && col_ok;
+            cp_async_16(sbase + C::kOffRaw + (rit % C::kRaw) * C::kRawStage + (pt + 256 * i) * 16,
+                        ok ? x + static_cast<int64_t>(token) * a.ldx + col0 + ch * 16 : x, ok);
+          }
+          rc.next();
+          ++rit;
+          look_raw();
+        }
+        cp_async_commit();
+      };
+      // G: four threads per row, R / 4 values each, one stage ahead
+      RowCursor gc(a.words, a.lay, row_lo, row_hi);
+      const int grow = pt >> 2, g0 = (pt & 3) * (R / 4);
+      float4 gv[R / 16];
+      float gs = 0.f;
+      int tg = gc.live() && gc.pos + grow < gc.end ? perm[gc.pos + grow] : -1;
+      auto load_g = [&]() {
+        gs = 0.f;
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i) gv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (gc.live()) {
+          const int token = tg;
+          if (token >= 0) {
+            gs = __ldg(a.x_scales + static_cast<int64_t>(token) * ncb + blockIdx.x);
+#pragma unroll
+            for (int i = 0; i < R / 16; ++i)
+              if (g0 + 4 * i < a.rank)
+                gv[i] = __ldg(reinterpret_cast<const float4*>(a.g32 + static_cast<int64_t>(token) * a.rank + g0 + 4 * i));
+          }
+          gc.next();
+          tg = gc.live() && gc.pos + grow < gc.end ? perm[gc.pos + grow] : -1;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < C::kRaw - 1; ++i) load_raw();
+      load_g();
+      int it = 0;
+      for (; cur.live(); ++it) {
+        const int slot = it % C::kStages;
+        load_raw();
+        cp_async_wait<C::kRaw - 1>();
+        uint4 codes[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          codes[i] = lds128(sbase + C::kOffRaw + (it % C::kRaw) * C::kRawStage + (pt + 256 * i) * 16);
+        if (!mbar_wait(empty_bar(slot), static_cast<uint32_t>(((it / C::kStages) & 1) ^ 1), abort_flag)) break;
+        const uint32_t sx = sbase + slot * C::kStage, sg = sx + 2 * C::kBlock;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = (pt >> 3) + 32 * i;
+          const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) i8_to_bf16(w[q], o[2 * q], o[2 * q + 1]);
+          const uint32_t base = sx + (ch >> 2) * C::kBlock + row * 128;
+          const int c0 = (ch & 3) * 2;
+          sts128(base + ((c0 ^ (row & 7)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
+          sts128(base + (((c0 + 1) ^ (row & 7)) << 4), make_uint4(o[4], o[5], o[6], o[7]));
+        }
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i) {
+          const int c = g0 + 4 * i;  // 8 bytes: half a chunk
+          const uint32_t at = sg + (c >> 6) * C::kBlock + grow * 128 + ((((c & 63) >> 3) ^ (grow & 7)) << 4) + (c & 4) * 2;
+          sts64(at, pack_bf16x2(gv[i].x * gs, gv[i].y * gs), pack_bf16x2(gv[i].z * gs, gv[i].w * gs));
+        }
+        load_g();
+        cur.next();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(slot));
+      }
+      cp_async_wait<0>();
     }
-  };
-  const int chunk = tid & 7;
-  const int elem = I8 ? 1 : 2;  // bytes per element of X
-  const int ncb = (a.cols + 127) / 128;
-  auto load = [&](Cursor& c, int slot) {
-    if (c.pos < row_hi) {
-      const uint32_t sx = sbase + slot * C::kStage, sg = sx + C::kStageX, ss = sg + C::kStageG;
-      const int col = col0 + chunk * (16 / elem);
+  } else if (warp == 4) {
+    // ------------------------------------------------------------------- MMA
+    constexpr uint32_t idesc = make_idesc_bf16(128, R) | (1u << 15) | (1u << 16);  // both operands MN-major
+    int it = 0, seg = 0;
+    bool fresh = true;
+    while (cur.live()) {
+      const int slot = it % C::kStages, b = seg & 1;
+      if (fresh && !mbar_wait(acc_empty(b), static_cast<uint32_t>(((seg >> 1) & 1) ^ 1), abort_flag)) break;
+      if (!mbar_wait(full_bar(slot), static_cast<uint32_t>((it / C::kStages) & 1), abort_flag)) break;
+      tc_fence_after();
+      const uint64_t ad = make_sw128_mnmajor_desc(sbase + slot * C::kStage, C::kBlock);
+      const uint64_t bd = make_sw128_mnmajor_desc(sbase + slot * C::kStage + 2 * C::kBlock, C::kBlock);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = (tid >> 3) + 32 * i;
-        const int token = c.pos + row < c.end ? perm[c.pos + row] : -1;
-        const bool ok = token >= 0 && col < a.cols;
-        const uint8_t* src = static_cast<const uint8_t*>(a.x);
-        if (ok) src += (static_cast<int64_t>(token) * a.ldx + col) * elem;
-        cp_async_16(sx + row * 128 + ((chunk ^ (row & 7)) << 4), src, ok);
-        if constexpr (I8) {
-          if (chunk == 0)
-            cp_async_4z(ss + row * 4,
-                        token >= 0 ? a.x_scales + static_cast<int64_t>(token) * ncb + col0 / 128 : a.x_scales,
-                        token >= 0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < (64 * (R / 8) + 255) / 256; ++i) {
-        const int e = tid + 256 * i;
-        const int row = e / (R / 8), ch = e % (R / 8);
-        if (64 * (R / 8) % 256 != 0 && row >= 64) break;
-        const int token = c.pos + row < c.end ? perm[c.pos + row] : -1;
-        const bool ok = token >= 0 && ch * 8 < a.rank;
-        cp_async_16(sg + g_swizzle<R>(row, ch), ok ? a.g + static_cast<int64_t>(token) * a.rank + ch * 8 : a.g, ok);
-      }
-      c.pos += C::kRows;
-      if (c.pos >= c.end) {
-        c.pos = c.end;
-        open(c);
+      for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two 8-row groups, 2048 bytes
+        tc_mma_ss_elect(tmem + b * R, ad + 128 * ks, bd + 128 * ks, idesc, !(fresh && ks == 0));
+      tc_commit_elect(empty_bar(slot));
+      ++it;
+      fresh = cur.next();
+      if (fresh) {
+        tc_commit_elect(acc_full(b));
+        ++seg;
       }
     }
-    cp_async_commit();
-  };
-
-  Cursor in{row_lo, 0, 0}, at{row_lo, 0, 0};
-  open(in);
-  open(at);
-#pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) load(in, s);
-
-  float acc[R / 16][C::kNT][4] = {};
-  int step = 0;
-  while (at.pos < row_hi) {
-    cp_async_wait<C::kStages - 2>();
-    __syncthreads();
-    load(in, (step + C::kStages - 1) % C::kStages);
-    const uint32_t sx = sbase + (step % C::kStages) * C::kStage, sg = sx + C::kStageX;
-    const float* ss = reinterpret_cast<const float*>(smem_raw + (step % C::kStages) * C::kStage + C::kStageX + C::kStageG);
-    ++step;
-#pragma unroll
-    for (int kb = 0; kb < C::kRows / 16 / C::WK; ++kb) {
-      const int m0 = (kb * C::WK + wk) * 16;
-      if (at.pos + m0 >= at.end) continue;  // warp-uniform
-      uint32_t bf[C::kNT][2];
-      if constexpr (!I8) {
-#pragma unroll
-        for (int np = 0; np < C::kNT / 2; ++np) {
-          uint32_t r4[4];
-          const int row = m0 + (lane & 7) + ((lane >> 3) & 1) * 8;
-          const int ch = wc * (C::kWarpCols / 8) + 2 * np + (lane >> 4);
-          ldmatrix_x4_trans(sx + row * 128 + ((ch ^ (row & 7)) << 4), r4);
-          bf[2 * np][0] = r4[0];
-          bf[2 * np][1] = r4[1];
-          bf[2 * np + 1][0] = r4[2];
-          bf[2 * np + 1][1] = r4[3];
-        }
-      } else {
-        // 16-byte chunk = 16 columns = an even and an odd tile
-#pragma unroll
-        for (int np = 0; np < C::kNT / 4; ++np) {
-          uint32_t r4[4];
-          const int row = m0 + (lane & 7) + ((lane >> 3) & 1) * 8;
-          const int ch = wc * (C::kWarpCols / 16) + 2 * np + (lane >> 4);
-          ldmatrix_x4_trans(sx + row * 128 + ((ch ^ (row & 7)) << 4), r4);
-          i8_pairs(r4[0], bf[4 * np][0], bf[4 * np + 1][0]);
-          i8_pairs(r4[1], bf[4 * np][1], bf[4 * np + 1][1]);
-          i8_pairs(r4[2], bf[4 * np + 2][0], bf[4 * np + 3][0]);
-          i8_pairs(r4[3], bf[4 * np + 2][1], bf[4 * np + 3][1]);
-        }
-      }
-#pragma unroll
-      for (int rt = 0; rt < R / 16; ++rt) {
-        // G^T: matrices (r 0-7, m 0-7), (r 8-15, m 0-7), (r 0-7, m 8-15), (r 8-15, m 8-15)
-        uint32_t af[4];
-        const int row = m0 + (lane & 7) + (lane >> 4) * 8;
-        ldmatrix_x4_trans(sg + g_swizzle<R>(row, 2 * rt + ((lane >> 3) & 1)), af);
-        if constexpr (I8) {
-          const float2 s0 = *reinterpret_cast<const float2*>(ss + m0 + 2 * tig);
-          const float2 s1 = *reinterpret_cast<const float2*>(ss + m0 + 8 + 2 * tig);
-          af[0] = scale_pair(af[0], s0.x, s0.y);
-          af[1] = scale_pair(af[1], s0.x, s0.y);
-          af[2] = scale_pair(af[2], s1.x, s1.y);
-          af[3] = scale_pair(af[3], s1.x, s1.y);
-        }
-#pragma unroll
-        for (int nt = 0; nt < C::kNT; ++nt)
-          mma_16816_bf16(acc[rt][nt], af[0], af[1], af[2], af[3], bf[nt][0], bf[nt][1]);
-      }
-    }
-    at.pos += C::kRows;
-    if (at.pos < at.end) continue;
-    // the adapter's rows of this split are done: add the warps' sums
-    const int ad = at.adapter;
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- epilogue
+    const int32_t* starts = a.words + a.lay.off_start;
+    const int col = col0 + 32 * warp + lane;
+    for (int seg = 0; cur.live(); ++seg) {
+      const int b = seg & 1, ad = cur.adapter;
+      if (!mbar_wait(acc_full(b), static_cast<uint32_t>((seg >> 1) & 1), abort_flag)) break;
+      tc_fence_after();
+      const bool whole = starts[ad] >= row_lo && starts[ad + 1] <= row_lo + a.rows_per_split;
+      const int64_t slot = whole ? ad : 2 * static_cast<int>(blockIdx.y) + (starts[ad] < row_lo ? 0 : 1);
+      const int64_t base = slot * a.rank * a.cols + col;
 #pragma unroll 1
-    for (int w = 0; w < C::WK; ++w) {
-      if (wk == w) {
+      for (int c = 0; c < R; c += 16) {
+        uint32_t v[16];
+        tmem_ld_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + b * R + c, v);
+        tmem_wait_ld();
+        if (col < a.cols) {
 #pragma unroll
-        for (int rt = 0; rt < R / 16; ++rt)
-#pragma unroll
-          for (int nt = 0; nt < C::kNT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = rt * 16 + g4 + 8 * (i >> 1);
-              int c;
-              if constexpr (I8)  // tile pairs: even columns, odd columns of 16
-                c = wc * C::kWarpCols + (nt >> 1) * 16 + 2 * (2 * tig + (i & 1)) + (nt & 1);
-              else
-                c = wc * C::kWarpCols + nt * 8 + 2 * tig + (i & 1);
-              float* p = red + r * C::kCols + c;
-              *p = (w == 0 ? 0.f : *p) + acc[rt][nt][i];
-              acc[rt][nt][i] = 0.f;
-            }
+          for (int e = 0; e < 16; ++e) {
+            if (c + (e & 8) >= a.rank) break;
+            const int64_t o = base + static_cast<int64_t>(c + e) * a.cols;
+            if (whole)
+              a.dbank[o] = __float2bfloat16_rn(__uint_as_float(v[e]));
+            else
+              a.part[o] = __uint_as_float(v[e]);
+          }
+        }
       }
-      __syncthreads();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(b));
+      cur.pos = cur.end;
+      cur.open();
     }
-    const bool whole = starts[ad] >= row_lo && starts[ad + 1] <= row_lo + a.rows_per_split;
-    const int64_t slot = whole ? ad : 2 * static_cast<int>(blockIdx.y) + (starts[ad] < row_lo ? 0 : 1);
-    const int64_t base = slot * a.rank * a.cols;
-    for (int e = tid; e < R * (C::kCols / 4); e += 256) {
-      const int r = e / (C::kCols / 4), c = (e % (C::kCols / 4)) * 4;
-      if (r < a.rank && col0 + c < a.cols) {
-        const float4 v = *reinterpret_cast<const float4*>(red + r * C::kCols + c);
-        const int64_t o = base + static_cast<int64_t>(r) * a.cols + col0 + c;
-        if (whole)
-          *reinterpret_cast<uint2*>(a.dbank + o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-        else
-          *reinterpret_cast<float4*>(a.part + o) = v;
-      }
-    }
-    // (the next adapter's end writes `red` again only after the barrier at the
-    // top of the loop, which every thread reaches after its reads here)
-    at.pos = at.end;
-    open(at);
   }
-  cp_async_wait<0>();
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << 5);
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
 }
 
 // Adds the slots of adapters that several splits share, in split order; zeros

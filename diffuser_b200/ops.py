@@ -395,7 +395,7 @@ class AdapterPlan:
         self.tokens, self.requests, self.n_adapters = int(tokens), ids.numel(), int(n_adapters)
         nbytes = int(_lib.lib().dq_adapter_plan_bytes(self.tokens, self.requests, self.n_adapters))
         if nbytes == 0:
-            raise ValueError("adapter_plan: tokens must be 0..2^30 and n_adapters 1..65536")
+            raise ValueError("adapter_plan: tokens must be 0..2^30 and n_adapters 1..65535")
         self.words = torch.empty(nbytes // 4, dtype=torch.int32, device=ids.device)
         self.update_(ids, offsets)
 
@@ -466,8 +466,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
     hidden = torch.empty((m, r), dtype=torch.bfloat16, device=y.device) if return_hidden else None
     with _on(y):
         lib = _lib.lib()
-        nbytes = lib.dq_adapter_add_workspace(m, plan.requests, k, n, r, a)
-        ws = _scratch(nbytes, y)
+        nbytes = 0 if return_hidden else m * r * 2
+        ws = None if return_hidden else _scratch(nbytes, y)
         _lib.check("dq_adapter_add", lib.dq_adapter_add(
             _ptr(y2), _row_stride(y2), _ptr(x2), _row_stride(x2), m, plan.requests, k, n, _ptr(down), _ptr(up),
             _ptr(scale), r, a, _ptr(plan.words), code, _ptr(o2), _row_stride(o2), _ptr(hidden), _ptr(ws), nbytes,

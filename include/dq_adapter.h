@@ -30,7 +30,7 @@ extern "C" {
  * request have no adapter.  Both arrays are device memory and are not read by
  * the host.  An id outside -1..A-1 counts as none, and offsets that decrease
  * or leave 0..M leave every token without an adapter; either is recorded as
- * DQ_ERR_INDEX for dq_device_error.  M <= 2^30, 1 <= A <= 65536, R >= 0.
+ * DQ_ERR_INDEX for dq_device_error.  M <= 2^30, 1 <= A <= 65535, R >= 0.
  * The plan buffer (dq_adapter_plan_bytes) is 16-byte aligned and needs no
  * initialization; it may be rebuilt in place, also inside a captured graph,
  * as long as M, R and A stay the same. */
@@ -46,8 +46,10 @@ int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64
  * hidden (or NULL): bf16 [M, r], receives scale_a * x . down_a^T (zero rows
  * where there is none), which the backward pass takes.
  * The sums of the down projection are kept in float32 over K, rounded once
- * to bf16 for the up projection, which accumulates in float32 onto y. */
-size_t dq_adapter_add_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A);
+ * to bf16 for the up projection, which accumulates in float32 onto y; out is
+ * rounded once.  The workspace (M * r * 2 bytes, 16-byte aligned) is needed
+ * only where hidden is NULL. */
+size_t dq_adapter_add_workspace(int64_t M, int r);
 int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t M, int64_t R,
                    int64_t K, int64_t N, const void* down, const void* up, const float* scale, int r,
                    int A, const void* plan, int act, void* out, int64_t ldo, void* hidden,

@@ -30,7 +30,7 @@ def _add(lib, *, M=4, R=1, K=64, N=64, r=16, A=2, act=0, y=P, ldy=None, x=P, ldx
 
 @pytest.mark.parametrize("kw,status", [
     (dict(K=60), SHAPE), (dict(N=60), SHAPE), (dict(r=12), SHAPE), (dict(r=136), SHAPE), (dict(r=0), SHAPE),
-    (dict(A=0), SHAPE), (dict(A=65537), SHAPE), (dict(M=-1), SHAPE), (dict(M=(1 << 30) + 1), SHAPE),
+    (dict(A=0), SHAPE), (dict(A=65536), SHAPE), (dict(M=-1), SHAPE), (dict(M=(1 << 30) + 1), SHAPE),
     (dict(R=-1), SHAPE), (dict(ldy=56), SHAPE), (dict(ldy=68), SHAPE), (dict(ldx=60), SHAPE), (dict(ldo=8), SHAPE),
     (dict(act=2, N=48), SHAPE), (dict(act=4), ARG), (dict(act=-1), ARG), (dict(y=None), ARG), (dict(x=None), ARG),
     (dict(down=None), ARG), (dict(up=None), ARG), (dict(scale=None), ARG), (dict(plan=None), ARG),
@@ -76,7 +76,7 @@ def test_plan_capacity_holds_every_split_into_groups(lib):
         words = lib.dq_adapter_plan_bytes(m, r, a) // 4
         groups = min(a, r) + 1
         need = m + 15 * groups
-        assert words >= 16 + (a + 2) + (a + 1) + need + need // 16 + (m // 128 + groups)
+        assert words >= 16 + (a + 2) + (a + 1) + need + need // 16 + 4 * (m // 128 + groups)
 
 
 @pytest.mark.parametrize("args,status", [
