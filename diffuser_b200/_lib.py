@@ -117,7 +117,7 @@ SIGNATURES = {
                                               _c_p]),
     "dq_adapter_plan_bytes": (_c_sz, [_c_i64, _c_i64, ctypes.c_int]),
     "dq_adapter_plan": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_sz, _c_p]),
-    "dq_adapter_add_workspace": (_c_sz, [_c_i64, ctypes.c_int]),
+    "dq_adapter_add_workspace": (_c_sz, [_c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
     "dq_adapter_add": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p,
                                       ctypes.c_int, ctypes.c_int, _c_p, ctypes.c_int, _c_p, _c_i64, _c_p, _c_p,
                                       _c_sz, _c_p]),

@@ -400,8 +400,9 @@ int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
-size_t dq_adapter_add_workspace(int64_t M, int r) {
-  return M <= 0 || r <= 0 ? 0 : static_cast<size_t>(M) * r * 2;
+size_t dq_adapter_add_workspace(int64_t M, int64_t R, int r, int A) {
+  if (plan_shape(M, R, A) != DQ_OK || r <= 0 || r > kMaxRank || !large_tiles(M, R, A)) return 0;
+  return static_cast<size_t>(M) * r * 2;
 }
 
 int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t M, int64_t R, int64_t K,
@@ -425,9 +426,8 @@ int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64
     return DQ_ERR_ALIGN;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
-  if (hidden == nullptr &&
-      (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_adapter_add_workspace(M, r)))
-    return DQ_ERR_WORKSPACE;
+  const size_t need = hidden == nullptr ? dq_adapter_add_workspace(M, R, r, A) : 0;
+  if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)) return DQ_ERR_WORKSPACE;
   return down_up(x, ldx, K, down, y, ldy, N, up, scale, M, R, r, A, static_cast<const int32_t*>(plan), act, out,
                  ldo, hidden != nullptr ? hidden : workspace, hidden != nullptr, nullptr, sms,
                  static_cast<cudaStream_t>(stream));

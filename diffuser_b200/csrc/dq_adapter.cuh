@@ -590,7 +590,11 @@ struct UpCfg {
   static constexpr int kChunks = R * kStepCols / 8;  // 16-byte pieces of P per step
   static constexpr int kPerThread = (kChunks + 255) / 256;
   static constexpr int kBuf = R * kStepCols * 2;
-  static constexpr int kSmemBytes = 2 * kBuf;
+  static constexpr int kYStages = R <= 32 ? 2 : 3;
+  static constexpr int kYStage = kTileRows * kStepCols * 2;
+  static constexpr int kOffY = 2 * kBuf;
+  static constexpr int kSmemBytes = kOffY + kYStages * kYStage;
+  static constexpr int kMinCtas = R <= 32 ? 4 : R <= 64 ? 3 : 2;
 };
 
 struct UpArgs {
@@ -606,7 +610,7 @@ struct UpArgs {
 };
 
 template <int R>
-__global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const UpArgs a) {
+__global__ void __launch_bounds__(256, UpCfg<R>::kMinCtas) adapter_up_kernel(const UpArgs a) {
   using C = UpCfg<R>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
@@ -623,8 +627,13 @@ __global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const 
   const int tok0 = t.token(a.words + a.lay.off_perm, warp * 16 + g4);
   const int tok1 = t.token(a.words + a.lay.off_perm, warp * 16 + g4 + 8);
   const __nv_bfloat16* P = none ? a.bank : a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.N;
-  const __nv_bfloat16* y0 = a.y + static_cast<int64_t>(tok0) * a.ldy + 8 * tig;
-  const __nv_bfloat16* y1 = a.y + static_cast<int64_t>(tok1) * a.ldy + 8 * tig;
+  // this lane copies chunk lane % 8 of its warp's rows lane / 8 + 4 i
+  const __nv_bfloat16* ysrc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = t.token(a.words + a.lay.off_perm, warp * 16 + (lane >> 3) + 4 * i);
+    ysrc[i] = tok >= 0 ? a.y + static_cast<int64_t>(tok) * a.ldy + (lane & 7) * 8 : nullptr;
+  }
   const bool gated = act_is_gated(a.act);
   // gated: lanes 0, 1 of a quad write its 16 output columns of a 32-column group
   __nv_bfloat16* o0 = a.out + static_cast<int64_t>(tok0) * a.ldo + 8 * tig;
@@ -654,20 +663,19 @@ __global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const 
       for (int j = 0; j < 4; ++j) sts32(base + ((((cc >> 2) * 4 + j) ^ (row & 7)) << 4), w[j]);
     }
   };
-  // this thread's 8 columns of both 32-column groups of its two rows
-  uint4 yreg[2][2] = {};
-  auto load_y = [&](int n0) {
+  auto load_y = [&](int n0, int stage) {
+    if (n0 + (lane & 7) * 8 < n_hi) {
+      const uint32_t dst = sbase + C::kOffY + stage * C::kYStage + (warp * 16 + (lane >> 3)) * 128;
+      const uint32_t c = static_cast<uint32_t>(((lane & 7) ^ ((lane >> 1) & 4)) << 4);  // row % 2 = (lane / 8) % 2
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int col = n0 + g * 32;
-      if (col + 8 * tig < n_hi) {
-        if (tok0 >= 0) yreg[g][0] = ld_global_l2(y0 + col);
-        if (tok1 >= 0) yreg[g][1] = ld_global_l2(y1 + col);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (ysrc[i] != nullptr) cp_async_16_l2(dst + i * 512 + c, ysrc[i] + n0, true);
     }
+    cp_async_commit();
   };
+#pragma unroll
+  for (int i = 0; i < C::kYStages - 1; ++i) load_y(n_lo + i * C::kStepCols, i);
   load_p(n_lo);
-  load_y(n_lo);
   store_p(0);
 
   grid_wait();  // hidden is the down kernel's
@@ -685,21 +693,15 @@ __global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const 
         *reinterpret_cast<uint32_t*>(a.zero_hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig) = 0u;
     }
   grid_launch_dependents();
-  __syncthreads();
 
-  int buf = 0;
+  int buf = 0, ys = 0;
   for (int n0 = n_lo; n0 < n_hi; n0 += C::kStepCols) {
-    uint4 ycur[2][2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      ycur[g][0] = yreg[g][0];
-      ycur[g][1] = yreg[g][1];
-    }
+    cp_async_wait<C::kYStages - 2>();
+    __syncthreads();  // this step's P and Y; every warp is done with the last step's
+    load_y(n0 + (C::kYStages - 1) * C::kStepCols, ys == 0 ? C::kYStages - 1 : ys - 1);
     const bool more = n0 + C::kStepCols < n_hi;
-    if (more) {
-      load_p(n0 + C::kStepCols);
-      load_y(n0 + C::kStepCols);
-    }
+    if (more) load_p(n0 + C::kStepCols);
+    const uint32_t yrow = sbase + C::kOffY + ys * C::kYStage + (warp * 16 + g4) * 128;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       float acc[4][4];
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
-        unpack8(ycur[g][h], v);
+        unpack8(lds128(yrow + h * 1024 + (((4 * g + tig) ^ ((g4 & 1) * 4)) << 4)), v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[2 * j] += acc[j][2 * h];
@@ -750,12 +752,11 @@ __global__ void __launch_bounds__(256, R <= 64 ? 3 : 2) adapter_up_kernel(const 
         if (in && (h ? st1 : st0)) *reinterpret_cast<uint4*>((h ? o1 : o0) + oc) = pack8(v);
       }
     }
-    if (more) {
-      buf ^= 1;
-      store_p(buf);
-      __syncthreads();
-    }
+    buf ^= 1;
+    if (more) store_p(buf);
+    ys = ys + 1 == C::kYStages ? 0 : ys + 1;
   }
+  cp_async_wait<0>();
 }
 
 // ------------------------------------------------------------------ small

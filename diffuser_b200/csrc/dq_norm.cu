@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/dq_dit.h"
@@ -37,21 +38,25 @@ int chunks_of(int64_t B, int S, int D, int sms) {
 template <bool OPS>
 void launch_forward(const NormArgs& a, int sms, cudaStream_t st) {
   const int runs = (a.D / 4 + 255) / 256;
-  auto go = [&](auto kern) {
-    int per_sm = 1;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, 256, 0);
+  auto go = [&](auto kern, std::atomic<int>& cached) {
+    int per_sm = cached.load(std::memory_order_relaxed);  // the same on every sm_100
+    if (per_sm == 0) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, 256, 0) != cudaSuccess) per_sm = 1;
+      cached.store(per_sm, std::memory_order_relaxed);
+    }
     const int grid = static_cast<int>(std::min<int64_t>(a.T, static_cast<int64_t>(sms) * std::max(per_sm, 1)));
     kern<<<grid, 256, 0, st>>>(a);
   };
+  static std::atomic<int> resident[9];
   switch (runs) {
-    case 1: return go(gated_norm_kernel<1, OPS>);
-    case 2: return go(gated_norm_kernel<2, OPS>);
-    case 3: return go(gated_norm_kernel<3, OPS>);
-    case 4: return go(gated_norm_kernel<4, OPS>);
+    case 1: return go(gated_norm_kernel<1, OPS>, resident[1]);
+    case 2: return go(gated_norm_kernel<2, OPS>, resident[2]);
+    case 3: return go(gated_norm_kernel<3, OPS>, resident[3]);
+    case 4: return go(gated_norm_kernel<4, OPS>, resident[4]);
     case 5:
-    case 6: return go(gated_norm_kernel<6, OPS>);
+    case 6: return go(gated_norm_kernel<6, OPS>, resident[6]);
   }
-  go(gated_norm_kernel<8, OPS>);
+  go(gated_norm_kernel<8, OPS>, resident[8]);
 }
 
 }  // namespace

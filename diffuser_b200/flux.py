@@ -167,9 +167,16 @@ _NORMS = {None: _lib.DQ_NORM_NONE, "rms": _lib.DQ_NORM_RMS, "layer": _lib.DQ_NOR
 _ROUNDINGS = {"once": _lib.DQ_ROUND_ONCE, "ops": _lib.DQ_ROUND_OPS}
 
 
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 def _token_rows(t, name, like):
     """t [B, S, D] bf16 as evenly spaced rows whose starts are 8-byte aligned
     (copied when they are not), and the row stride."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.shape == like.shape and \
+            t.is_contiguous() and t.get_device() == like.get_device() and t.data_ptr() % 8 == 0:
+        return t, like.shape[2]
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor: the engine has no CPU path")
     if t.dtype != torch.bfloat16:
@@ -188,6 +195,9 @@ def _features(t, name, shape, like):
     """A [B, D] modulation or a [D] weight in bf16 with aligned rows, or None."""
     if t is None:
         return None
+    if isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.shape == shape and t.is_contiguous() and \
+            t.get_device() == like.get_device() and t.data_ptr() % 8 == 0:
+        return t
     if not isinstance(t, torch.Tensor) or t.device != like.device:
         raise ValueError(f"{name} must be a tensor on {like.device}")
     if t.dtype != torch.bfloat16 or t.shape != shape:
@@ -215,8 +225,8 @@ def _norm_args(x, gate, scale, shift, post, pre, post_weight, pre_weight):
     if scale is not None and shift is not None and scale.stride(0) != shift.stride(0):
         scale, shift = scale.contiguous(), shift.contiguous()
     mod = scale if scale is not None else shift
-    return (gate, 0 if gate is None else max(gate.stride(0), d), scale, shift,
-            0 if mod is None else max(mod.stride(0), d), _features(post_weight, "post_weight", (d,), x),
+    row = lambda t: 0 if t is None else d if b == 1 else t.stride(0)  # noqa: E731
+    return (gate, row(gate), scale, shift, row(mod), _features(post_weight, "post_weight", (d,), x),
             _features(pre_weight, "pre_weight", (d,), x))
 
 
@@ -241,14 +251,14 @@ def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_w
     x2, ldx = _token_rows(x, "x", x)
     y2, ldy = _token_rows(y, "y", x)
     s = torch.empty((b, n, d), dtype=torch.bfloat16, device=x.device)
-    h = torch.empty((b, n, d), dtype=torch.bfloat16, device=x.device)
+    h = torch.empty_like(s)
     if x.numel() == 0:
         return s, h
     with ops._on(x):
         _lib.check("dq_gated_norm", _lib.lib().dq_gated_norm(
-            _ptr(x2), ldx, _ptr(y2), ldy, b * n, n, d, _ptr(gate), ldg, _ptr(scale), _ptr(shift), ldm, _ptr(pw),
-            _ptr(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ROUNDINGS[rounding], _ptr(s), d, _ptr(h), d,
-            ops._stream(x.device)))
+            x2.data_ptr(), ldx, y2.data_ptr(), ldy, b * n, n, d, _address(gate), ldg, _address(scale), _address(shift),
+            ldm, _address(pw), _address(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ROUNDINGS[rounding],
+            s.data_ptr(), d, h.data_ptr(), d, ops._raw_stream(x)))
     return s, h
 
 
@@ -282,10 +292,11 @@ def gated_norm_backward(ds, dh, s, y, gate=None, *, post=None, pre="rms", post_w
         nbytes = lib.dq_gated_norm_backward_workspace(b * n, n, d)
         ws = ops._scratch(nbytes, s)
         _lib.check("dq_gated_norm_backward", lib.dq_gated_norm_backward(
-            _ptr(ds2), ldds, _ptr(dh2), lddh, _ptr(s2), lds, _ptr(y2), ldy, b * n, n, d, _ptr(gate), ldg,
-            _ptr(scale), ldm, _ptr(pw), _ptr(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ptr(dx), d,
-            _ptr(dy), d, _ptr(out["dgate"]), _ptr(out["dscale"]), _ptr(out["dshift"]), _ptr(out["dpost_weight"]),
-            _ptr(out["dpre_weight"]), _ptr(ws), nbytes, ops._stream(s.device)))
+            _address(ds2), ldds, dh2.data_ptr(), lddh, s2.data_ptr(), lds, y2.data_ptr(), ldy, b * n, n, d,
+            _address(gate), ldg, _address(scale), ldm, _address(pw), _address(qw), _NORMS[post], _NORMS[pre],
+            residual_scale, eps, dx.data_ptr(), d, dy.data_ptr(), d, _address(out["dgate"]), _address(out["dscale"]),
+            _address(out["dshift"]), _address(out["dpost_weight"]), _address(out["dpre_weight"]), ws.data_ptr(), nbytes,
+            ops._raw_stream(s)))
     return out
 
 

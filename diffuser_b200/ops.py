@@ -333,12 +333,21 @@ def fp8_linear(x: torch.Tensor, w8: torch.Tensor, scale: float,
 
 
 # ----------------------------------------------------------------- adapters
+# The calls below are small next to a Python call, so their checks come in two
+# parts: a short one that accepts the usual operands (contiguous, aligned), and
+# the full one that names what is wrong or copies what is only laid out badly.
+_NO_SWITCH = contextlib.nullcontext()
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
 def _on(t: torch.Tensor):
     """Makes t's device the current one for the duration of a call."""
-    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_SWITCH if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-_NO_SWITCH = contextlib.nullcontext()
+def _raw_stream(t: torch.Tensor) -> int:
+    """Handle of the current stream on t's device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
@@ -357,7 +366,7 @@ def _rows16(t: torch.Tensor, name: str, width: int, like: torch.Tensor) -> torch
     """t as bf16 rows [-1, width] with unit stride along the features, 16-byte
     aligned row starts and evenly spaced rows (copied when it is not)."""
     _same_device(t, name, like)
-    if t.dtype != torch.bfloat16:
+    if t.dtype != _BF16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError(f"{name} must have {width} features, got shape {tuple(t.shape)}")
@@ -367,21 +376,43 @@ def _rows16(t: torch.Tensor, name: str, width: int, like: torch.Tensor) -> torch
     return t2
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _row_operand(t: torch.Tensor, name: str, width: int, like: torch.Tensor, must_alias: bool = False):
+    """(tensor that holds the rows, address, row stride, rows) of a bf16
+    [..., width] operand; with must_alias it may not be a copy of t."""
+    if isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.is_contiguous() and \
+            t.get_device() == like.get_device() and t.is_cuda and t.dim() and t.shape[-1] == width:
+        p = t.data_ptr()
+        if p % 16 == 0 and width % 8 == 0:
+            return t, p, width, t.numel() // width
+    t2 = _rows16(t, name, width, like)
+    if must_alias and t2.data_ptr() != t.data_ptr():
+        raise ValueError(f"{name} must have evenly spaced, 16-byte aligned rows with unit feature stride")
+    m = t2.shape[0]
+    return t2, t2.data_ptr(), (t2.stride(0) if m > 1 else max(t2.stride(0), width)), m
 
 
 def _bank(down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, like: torch.Tensor):
     """(adapters, rank, in_features, out_features) of a checked adapter bank."""
+    try:
+        a, r, k = down.shape
+        a2, r2, n = up.shape
+        d = like.get_device()
+        if down.dtype is up.dtype is _BF16 and scale.dtype is _F32 and a == a2 == scale.numel() and r == r2 and \
+                scale.dim() == 1 and r % 8 == 0 and 0 < r <= 128 and k % 8 == 0 and n % 8 == 0 and \
+                down.is_contiguous() and up.is_contiguous() and scale.is_contiguous() and \
+                down.get_device() == up.get_device() == scale.get_device() == d:
+            return a, r, k, n
+    except (AttributeError, ValueError):
+        pass
     for t, name in ((down, "down"), (up, "up")):
         _same_device(t, name, like)
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or not t.is_contiguous():
+        if t.dtype != _BF16 or t.dim() != 3 or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous bfloat16 [adapters, rank, features] tensor")
     a, r, k = down.shape
     if up.shape[:2] != (a, r):
         raise ValueError("down and up must hold the same adapters and rank")
     _same_device(scale, "scale", like)
-    if scale.dtype != torch.float32 or scale.shape != (a,) or not scale.is_contiguous():
+    if scale.dtype != _F32 or scale.shape != (a,) or not scale.is_contiguous():
         raise TypeError("scale must be a contiguous float32 [adapters] tensor")
     if r % 8 != 0 or r > 128 or k % 8 != 0 or up.shape[2] % 8 != 0:
         raise ValueError("rank (at most 128) and features must be multiples of 8")
@@ -393,10 +424,14 @@ class AdapterPlan:
 
     def __init__(self, ids, offsets, n_adapters: int, tokens: int):
         self.tokens, self.requests, self.n_adapters = int(tokens), ids.numel(), int(n_adapters)
-        nbytes = int(_lib.lib().dq_adapter_plan_bytes(self.tokens, self.requests, self.n_adapters))
+        lib = _lib.lib()
+        nbytes = int(lib.dq_adapter_plan_bytes(self.tokens, self.requests, self.n_adapters))
         if nbytes == 0:
             raise ValueError("adapter_plan: tokens must be 0..2^30 and n_adapters 1..65535")
+        # bytes of adapter_add's workspace per unit of rank
+        self.add_workspace = int(lib.dq_adapter_add_workspace(self.tokens, self.requests, 1, self.n_adapters))
         self.words = torch.empty(nbytes // 4, dtype=torch.int32, device=ids.device)
+        self.address = self.words.data_ptr()
         self.update_(ids, offsets)
 
     def update_(self, ids: torch.Tensor, offsets: torch.Tensor) -> "AdapterPlan":
@@ -410,8 +445,8 @@ class AdapterPlan:
             raise ValueError("offsets must hold one more entry than ids, and both as many as before")
         with _on(self.words):
             _lib.check("dq_adapter_plan", _lib.lib().dq_adapter_plan(
-                _ptr(ids), _ptr(offsets), self.requests, self.tokens, self.n_adapters, _ptr(self.words),
-                self.words.numel() * 4, _stream(self.words.device)))
+                _ptr(ids), _ptr(offsets), self.requests, self.tokens, self.n_adapters, self.address,
+                self.words.numel() * 4, _raw_stream(self.words)))
         return self
 
 
@@ -433,7 +468,8 @@ def _check_plan(plan: AdapterPlan, m: int, a: int, like: torch.Tensor) -> None:
     if plan.tokens != m or plan.n_adapters != a:
         raise ValueError(f"the plan is for {plan.tokens} tokens and {plan.n_adapters} adapters, "
                          f"the operands hold {m} and {a}")
-    _same_device(plan.words, "plan", like)
+    if plan.words.get_device() != like.get_device():
+        _same_device(plan.words, "plan", like)
 
 
 def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
@@ -449,30 +485,29 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
     [tokens, r] scale_a * x . down_a^T that adapter_backward takes."""
     _require_cuda(y, "y")
     a, r, k, n = _bank(down, up, scale, y)
-    code, n_out = _act_code(act, n)
-    x2, y2 = _rows16(x, "x", k, y), _rows16(y, "y", n, y)
-    m = y2.shape[0]
-    if x2.shape[0] != m:
-        raise ValueError(f"x holds {x2.shape[0]} tokens, y {m}")
+    code, n_out = (_lib.DQ_ACT_NONE, n) if act is None else _act_code(act, n)
+    x2, xp, ldx, mx = _row_operand(x, "x", k, y)
+    y2, yp, ldy, m = _row_operand(y, "y", n, y)
+    if mx != m:
+        raise ValueError(f"x holds {mx} tokens, y {m}")
     _check_plan(plan, m, a, y)
     if out is None:
-        o2 = torch.empty((m, n_out), dtype=torch.bfloat16, device=y.device)
+        res = torch.empty_like(y) if n_out == n and y2 is y else \
+            torch.empty((*y.shape[:-1], n_out), dtype=_BF16, device=y.device)
+        op, ldo = res.data_ptr(), n_out
     else:
-        o2 = _rows16(out, "out", n_out, y)
-        if o2.data_ptr() != out.data_ptr():
-            raise ValueError("out must have evenly spaced, 16-byte aligned rows with unit feature stride")
-        if o2.shape[0] != m:
-            raise ValueError(f"out holds {o2.shape[0]} tokens, y {m}")
-    hidden = torch.empty((m, r), dtype=torch.bfloat16, device=y.device) if return_hidden else None
+        res = out
+        _, op, ldo, mo = _row_operand(out, "out", n_out, y, must_alias=True)
+        if mo != m:
+            raise ValueError(f"out holds {mo} tokens, y {m}")
+    hidden = torch.empty((m, r), dtype=_BF16, device=y.device) if return_hidden else None
+    nbytes = 0 if return_hidden else plan.add_workspace * r
+    ws = _scratch(nbytes, y) if nbytes else None
     with _on(y):
-        lib = _lib.lib()
-        nbytes = 0 if return_hidden else m * r * 2
-        ws = None if return_hidden else _scratch(nbytes, y)
-        _lib.check("dq_adapter_add", lib.dq_adapter_add(
-            _ptr(y2), _row_stride(y2), _ptr(x2), _row_stride(x2), m, plan.requests, k, n, _ptr(down), _ptr(up),
-            _ptr(scale), r, a, _ptr(plan.words), code, _ptr(o2), _row_stride(o2), _ptr(hidden), _ptr(ws), nbytes,
-            _stream(y.device)))
-    res = out if out is not None else o2.reshape(*y.shape[:-1], n_out)
+        _lib.check("dq_adapter_add", _lib.lib().dq_adapter_add(
+            yp, ldy, xp, ldx, m, plan.requests, k, n, down.data_ptr(), up.data_ptr(), scale.data_ptr(), r, a,
+            plan.address, code, op, ldo, None if hidden is None else hidden.data_ptr(),
+            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(y)))
     return (res, hidden) if return_hidden else res
 
 
@@ -490,43 +525,46 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
     same bits."""
     _require_cuda(dy, "dy")
     a, r, k, n = _bank(down, up, scale, dy)
-    dy2 = _rows16(dy, "dy", n, dy)
-    m = dy2.shape[0]
+    dy2, dyp, lddy, m = _row_operand(dy, "dy", n, dy)
     _check_plan(plan, m, a, dy)
     if isinstance(x, PackedActivation):
         if x.codes.shape[-1] != k or x.codes.numel() != m * k:
             raise ValueError(f"the packed activation holds {tuple(x.codes.shape)}, expected [{m}, {k}]")
         _same_device(x.codes, "x", dy)
-        x2, scales, ldx = x.codes, x.scales, k
+        x2, xp, ldx, scales = x.codes, x.codes.data_ptr(), k, x.scales.data_ptr()
     else:
-        x2, scales = _rows16(x, "x", k, dy), None
-        ldx = _row_stride(x2)
-        if x2.shape[0] != m:
-            raise ValueError(f"x holds {x2.shape[0]} tokens, dy {m}")
+        x2, xp, ldx, mx = _row_operand(x, "x", k, dy)
+        scales = None
+        if mx != m:
+            raise ValueError(f"x holds {mx} tokens, dy {m}")
     _same_device(hidden, "hidden", dy)
-    if hidden.dtype != torch.bfloat16 or hidden.shape != (m, r) or not hidden.is_contiguous():
+    if hidden.dtype != _BF16 or hidden.shape != (m, r) or not hidden.is_contiguous() or hidden.data_ptr() % 16 != 0:
         raise TypeError(f"hidden must be a contiguous bfloat16 [{m}, {r}] tensor")
-    dx2 = torch.zeros((m, k), dtype=torch.bfloat16, device=dy.device) if dx is None else _rows16(dx, "dx", k, dy)
-    if dx2.shape[0] != m:
-        raise ValueError(f"dx holds {dx2.shape[0]} tokens, dy {m}")
-    if out is None:
-        o2 = dx2 if dx is None else torch.empty((m, k), dtype=torch.bfloat16, device=dy.device)
+    shape = (*dy.shape[:-1], k)
+    if dx is None:
+        base = torch.zeros(shape, dtype=_BF16, device=dy.device)
     else:
-        o2 = _rows16(out, "out", k, dy)
-        if o2.data_ptr() != out.data_ptr() or o2.shape[0] != m:
-            raise ValueError("out must hold dy's tokens in evenly spaced, 16-byte aligned rows")
+        base = dx
+    dx2, dxp, lddx, md = _row_operand(base, "dx", k, dy)
+    if md != m:
+        raise ValueError(f"dx holds {md} tokens, dy {m}")
+    if out is None:
+        res = base if dx is None else torch.empty(shape, dtype=_BF16, device=dy.device)
+    else:
+        res = out
+    _, op, ldo, mo = _row_operand(res, "out", k, dy, must_alias=True)
+    if mo != m:
+        raise ValueError(f"out holds {mo} tokens, dy {m}")
     ddown, dup = torch.empty_like(down), torch.empty_like(up)
     with _on(dy):
         lib = _lib.lib()
         nbytes = lib.dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
         ws = _scratch(nbytes, dy)
         _lib.check("dq_adapter_backward", lib.dq_adapter_backward(
-            _ptr(dy2), _row_stride(dy2), _ptr(x2), ldx, _ptr(scales), _ptr(hidden), m, plan.requests, k, n,
-            _ptr(down), _ptr(up), _ptr(scale), r, a, _ptr(plan.words), _ptr(dx2), _row_stride(dx2), _ptr(o2),
-            _row_stride(o2), _ptr(ddown), _ptr(dup), _ptr(ws), nbytes, _stream(dy.device)))
-    if out is not None:
-        return out, ddown, dup
-    return o2.reshape(*dy.shape[:-1], k), ddown, dup
+            dyp, lddy, xp, ldx, scales, hidden.data_ptr(), m, plan.requests, k, n, down.data_ptr(), up.data_ptr(),
+            scale.data_ptr(), r, a, plan.address, dxp, lddx, op, ldo, ddown.data_ptr(), dup.data_ptr(),
+            ws.data_ptr(), nbytes, _raw_stream(dy)))
+    return res, ddown, dup
 
 
 # ---------------------------------------------------- activation checkpoints
@@ -540,7 +578,7 @@ class PackedActivation:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         _require_cuda(codes, "codes")
         _same_device(scales, "scales", codes)
-        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.dim() < 1:
+        if codes.dtype != torch.int8 or scales.dtype != _F32 or codes.dim() < 1:
             raise TypeError("codes must be int8 and scales float32")
         k = codes.shape[-1]
         if k == 0 or k % 16 != 0:
@@ -557,17 +595,17 @@ def checkpoint_pack(x: torch.Tensor) -> PackedActivation:
     codes = x / scale rounded to the nearest (ties to even).  A run that is not
     finite comes back as NaN."""
     _require_cuda(x, "x")
-    k = x.shape[-1]
+    k = x.shape[-1] if x.dim() else 0
     if k == 0 or k % 16 != 0:
         raise ValueError("an 8-bit activation needs a feature count that is a multiple of 16")
-    x2 = _rows16(x, "x", k, x)
-    m = x2.shape[0]
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty((m, -(-k // CHECKPOINT_RUN)), dtype=torch.float32, device=x.device)
+    x2, xp, ldx, m = _row_operand(x, "x", k, x)
+    packed = object.__new__(PackedActivation)
+    packed.codes = codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    packed.scales = scales = torch.empty((m, -(-k // CHECKPOINT_RUN)), dtype=_F32, device=x.device)
     with _on(x):
         _lib.check("dq_checkpoint_pack", _lib.lib().dq_checkpoint_pack(
-            _ptr(x2), _row_stride(x2), m, k, _ptr(codes), _ptr(scales), _stream(x.device)))
-    return PackedActivation(codes, scales)
+            xp, ldx, m, k, codes.data_ptr(), scales.data_ptr(), _raw_stream(x)))
+    return packed
 
 
 def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -576,15 +614,18 @@ def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None)
         raise TypeError("packed must come from checkpoint_pack")
     codes = packed.codes
     k = codes.shape[-1]
-    o2 = torch.empty(codes.shape, dtype=torch.bfloat16, device=codes.device) if out is None else out
-    rows = _rows16(o2, "out", k, codes)
-    m = codes.numel() // k
-    if rows.data_ptr() != o2.data_ptr() or rows.shape[0] != m:
-        raise ValueError("out must hold the packed rows, evenly spaced and 16-byte aligned")
+    if out is None:
+        res = torch.empty(codes.shape, dtype=_BF16, device=codes.device)
+        op, ldo, m = res.data_ptr(), k, codes.numel() // k
+    else:
+        res = out
+        _, op, ldo, m = _row_operand(out, "out", k, codes, must_alias=True)
+        if m != codes.numel() // k:
+            raise ValueError("out must hold the packed rows")
     with _on(codes):
         _lib.check("dq_checkpoint_unpack", _lib.lib().dq_checkpoint_unpack(
-            _ptr(codes), _ptr(packed.scales), m, k, _ptr(rows), _row_stride(rows), _stream(codes.device)))
-    return o2
+            codes.data_ptr(), packed.scales.data_ptr(), m, k, op, ldo, _raw_stream(codes)))
+    return res
 
 
 # -------------------------------------------------------- input gradients
@@ -592,9 +633,13 @@ def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor):
     _same_device(weight, "weight", dy)
     if n % 8 != 0:
         raise ValueError("the input gradient needs out_features % 8 == 0")
-    dy2 = _prep_x(dy, n)
-    dx = torch.empty((dy2.shape[0], k), dtype=torch.bfloat16, device=dy.device)
-    return dy2, dx, _lib.lib().dq_linear_dgrad_workspace(n, k)
+    if dy.dtype != _BF16:
+        raise TypeError(f"gradients must be bfloat16 on the GPU path, got {dy.dtype}")
+    if dy.dim() < 1 or dy.shape[-1] != n:
+        raise ValueError(f"last dim of dy is {tuple(dy.shape)[-1:]}, expected out_features={n}")
+    dy2 = dy if dy.is_contiguous() and dy.data_ptr() % 16 == 0 else dy.new_empty(dy.shape).copy_(dy)
+    dx = torch.empty((*dy.shape[:-1], k), dtype=_BF16, device=dy.device)
+    return dy2, dx, 2 * n * k + 255 & ~255  # dq_linear_dgrad_workspace
 
 
 def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
@@ -607,27 +652,27 @@ def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tenso
     if n * k != packed.numel() * 2 or absmax.numel() * NF4_BLOCK != n * k:
         raise ValueError("packed / absmax sizes do not match in_features")
     dy2, dx, nbytes = _prep_dgrad(dy, n, k, packed)
-    am = absmax if absmax.dtype in (torch.float32, torch.bfloat16) else absmax.float()
+    _same_device(absmax, "absmax", dy)
+    am = absmax if absmax.dtype in (_F32, _BF16) else absmax.float()
     with _on(dy):
         ws = _scratch(nbytes, dy)
         _lib.check("dq_linear_nf4_dgrad", _lib.lib().dq_linear_nf4_dgrad(
-            _ptr(dy2), dy2.shape[0], n, _ptr(packed), _ptr(am), _dtype_code(am), k, _ptr(dx), _ptr(ws), nbytes,
-            _stream(dy.device)))
-    return dx.reshape(*dy.shape[:-1], k)
+            dy2.data_ptr(), dy2.numel() // n, n, packed.data_ptr(), am.data_ptr(), _dtype_code(am), k,
+            dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy)))
+    return dx
 
 
 def fp8_linear_dgrad(dy: torch.Tensor, w8: torch.Tensor, scale: float) -> torch.Tensor:
     """dx = dy . (e4m3(W) * bf16(scale)), the input gradient of fp8_linear."""
     _require_cuda(dy, "dy")
     n, k = int(w8.shape[0]), int(w8.shape[1])
-    raw = w8.view(torch.uint8)
-    dy2, dx, nbytes = _prep_dgrad(dy, n, k, raw)
+    dy2, dx, nbytes = _prep_dgrad(dy, n, k, w8)
     with _on(dy):
         ws = _scratch(nbytes, dy)
         _lib.check("dq_linear_fp8_dgrad", _lib.lib().dq_linear_fp8_dgrad(
-            _ptr(dy2), dy2.shape[0], n, _ptr(raw), float(scale), k, _ptr(dx), _ptr(ws), nbytes,
-            _stream(dy.device)))
-    return dx.reshape(*dy.shape[:-1], k)
+            dy2.data_ptr(), dy2.numel() // n, n, w8.data_ptr(), float(scale), k, dx.data_ptr(), ws.data_ptr(),
+            nbytes, _raw_stream(dy)))
+    return dx
 
 
 def device_error(device=None) -> int:

@@ -47,9 +47,9 @@ int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64
  * where there is none), which the backward pass takes.
  * The sums of the down projection are kept in float32 over K, rounded once
  * to bf16 for the up projection, which accumulates in float32 onto y; out is
- * rounded once.  The workspace (M * r * 2 bytes, 16-byte aligned) is needed
- * only where hidden is NULL. */
-size_t dq_adapter_add_workspace(int64_t M, int r);
+ * rounded once.  The workspace (16-byte aligned, at most M * r * 2 bytes; none
+ * for small batches) is needed only where hidden is NULL. */
+size_t dq_adapter_add_workspace(int64_t M, int64_t R, int r, int A);
 int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t M, int64_t R,
                    int64_t K, int64_t N, const void* down, const void* up, const float* scale, int r,
                    int A, const void* plan, int act, void* out, int64_t ldo, void* hidden,
