@@ -11,44 +11,60 @@ namespace dq {
 constexpr int kCkptRun = 128;  // features per scale
 
 // Pack: 16 lanes per run of 128 features, 8 features (16 bytes) per lane, two
-// runs per warp.  The maximum is taken over the bit patterns of |x| (bf16
-// magnitudes order like integers, infinities and NaN above every number), so
-// a run that is not finite is seen whatever the order.  The quotient is the
-// IEEE one, as the definition has it: a product with 1 / scale would round
-// values next to a half the other way.  HBM-bound: 3 bytes per feature.
+// runs per warp and two warps' worth of loads in flight.  The maximum is taken
+// over the bit patterns of |x| (bf16 magnitudes order like integers, infinities
+// and NaN above every number), so a run that is not finite is seen whatever the
+// order.  HBM-bound: 3 bytes per feature; an IEEE division per feature made it
+// 127 us at 6144 x 16384 (floor 47), so the quotient is taken as x (1 / scale),
+// off by at most 127 (2^-24 + 2^-24) = 1.6e-5 from the exact one, and divided
+// only where that could round to another integer: within 1e-4 of a half.
+__device__ __forceinline__ uint32_t pack_code(float v, float scale, float inv) {
+  const float t = v * inv;
+  float q = rintf(t);
+  if (fabsf(t - q) > 0.4999f) q = rintf(__fdiv_rn(v, scale));
+  return static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu;
+}
+
 __global__ void __launch_bounds__(256)
     checkpoint_pack_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int64_t runs, int nrun,
                            int K, int8_t* __restrict__ codes, float* __restrict__ scales) {
   const int half = (threadIdx.x & 31) >> 4, sub = threadIdx.x & 15;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 16;
-  for (int64_t base = blockIdx.x * 16ll + (threadIdx.x >> 5) * 2; base < runs; base += stride) {
-    const int64_t run = base + half;
-    const int64_t row = run / nrun;
-    const int k = static_cast<int>(run - row * nrun) * kCkptRun + sub * 8;
-    const bool in = run < runs && k < K;
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (in) u = *reinterpret_cast<const uint4*>(x + row * ldx + k);
-    uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
-                          __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+  for (int64_t base = blockIdx.x * 16ll + (threadIdx.x >> 5) * 2; base < runs; base += 2 * stride) {
+    uint4 u[2];
+    int64_t row[2];
+    int k[2];
+    bool in[2];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t top = max(m & 0xFFFFu, m >> 16);
-    const bool finite = top < 0x7F80u;
-    const float amax = fmaxf(__uint_as_float(top << 16), 1e-12f);
-    const float scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7FC00000u);
-    if (!in) continue;
-    float v[8];
-    unpack8(u, v);
-    uint32_t w[2] = {0u, 0u};
-    if (finite) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int q = __float2int_rn(__fdiv_rn(v[e], scale));
-        w[e >> 2] |= static_cast<uint32_t>(q & 0xFF) << (8 * (e & 3));
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int64_t run = base + i * stride + half;
+      row[i] = run / nrun;
+      k[i] = static_cast<int>(run - row[i] * nrun) * kCkptRun + sub * 8;
+      in[i] = run < runs && k[i] < K;
+      u[i] = in[i] ? ld_stream16(x + row[i] * ldx + k[i]) : make_uint4(0u, 0u, 0u, 0u);
     }
-    *reinterpret_cast<uint2*>(codes + row * K + k) = make_uint2(w[0], w[1]);
-    if (sub == 0) scales[run] = scale;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t m = __vmaxu2(__vmaxu2(u[i].x & 0x7FFF7FFFu, u[i].y & 0x7FFF7FFFu),
+                            __vmaxu2(u[i].z & 0x7FFF7FFFu, u[i].w & 0x7FFF7FFFu));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const uint32_t top = max(m & 0xFFFFu, m >> 16);
+      const bool finite = top < 0x7F80u;
+      const float amax = fmaxf(__uint_as_float(top << 16), 1e-12f);
+      const float scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7FC00000u);
+      if (!in[i]) continue;
+      uint32_t w[2] = {0u, 0u};
+      if (finite) {
+        const float inv = __frcp_rn(scale);
+        float v[8];
+        unpack8(u[i], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= pack_code(v[e], scale, inv) << (8 * (e & 3));
+      }
+      *reinterpret_cast<uint2*>(codes + row[i] * K + k[i]) = make_uint2(w[0], w[1]);
+      if (sub == 0) scales[base + i * stride + half] = scale;
+    }
   }
 }
 

@@ -13,6 +13,7 @@
 namespace dq {
 namespace {
 
+constexpr int kMaxDevices = 64;
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 inline const __nv_bfloat16* bf(const void* p) { return static_cast<const __nv_bfloat16*>(p); }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -28,35 +29,70 @@ bool norms_ok(int post, int pre, const void* post_w) {
          (post_w == nullptr || post != kNormNone);
 }
 
-// Row runs of the backward pass: two CTAs per SM (one of the 512-thread form)
-// over all batch elements, at least four rows each.
-int chunks_of(int64_t B, int S, int D, int sms) {
-  const int64_t slots = static_cast<int64_t>(sms) * (D <= 4096 ? 2 : 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(1, B), ceil_div(S, 4))));
+// CTAs per batch element: what fills `slots` over all elements, at least `least`
+// rows each (a CTA's factors and, backward, its column sums are a fixed cost).
+int chunks_of(int64_t B, int S, int64_t slots, int least) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(1, B), ceil_div(S, least))));
+}
+int64_t backward_slots(int D, int sms) { return static_cast<int64_t>(sms) * (D <= 4096 ? 2 : 1); }
+
+// Shared-memory opt-in of a kernel and its resident CTAs per SM, once per
+// kernel and device.
+struct KernelInfo {
+  std::atomic<int> per_sm[kMaxDevices];  // 0: not set up
+};
+template <typename K>
+int set_up(K kern, int threads, size_t most, size_t smem, KernelInfo& info, int* per_sm) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
+  int n = info.per_sm[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, most) != cudaSuccess || n < 1)
+      return DQ_ERR_LAUNCH;
+    info.per_sm[dev].store(n, std::memory_order_release);
+  }
+  *per_sm = n;
+  return DQ_OK;
+}
+
+template <int NPT, bool OPS>
+int launch_forward_npt(NormArgs a, int64_t B, int sms, cudaStream_t st) {
+  static KernelInfo info;
+  const size_t per_feature = kNormAhead * 4 + (OPS ? 0 : 12);
+  int per_sm = 1;
+  const int rc = set_up(gated_norm_kernel<NPT, OPS>, kNormThreads, per_feature * NPT * kNormThreads * 4,
+                        per_feature * a.D, info, &per_sm);
+  if (rc != DQ_OK) return rc;
+  a.chunks = chunks_of(B, a.S, static_cast<int64_t>(sms) * per_sm, 1);
+  gated_norm_kernel<NPT, OPS><<<static_cast<unsigned>(B * a.chunks), kNormThreads, per_feature * a.D, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 template <bool OPS>
-void launch_forward(const NormArgs& a, int sms, cudaStream_t st) {
-  const int runs = (a.D / 4 + 255) / 256;
-  auto go = [&](auto kern, std::atomic<int>& cached) {
-    int per_sm = cached.load(std::memory_order_relaxed);  // the same on every sm_100
-    if (per_sm == 0) {
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, 256, 0) != cudaSuccess) per_sm = 1;
-      cached.store(per_sm, std::memory_order_relaxed);
-    }
-    const int grid = static_cast<int>(std::min<int64_t>(a.T, static_cast<int64_t>(sms) * std::max(per_sm, 1)));
-    kern<<<grid, 256, 0, st>>>(a);
-  };
-  static std::atomic<int> resident[9];
-  switch (runs) {
-    case 1: return go(gated_norm_kernel<1, OPS>, resident[1]);
-    case 2: return go(gated_norm_kernel<2, OPS>, resident[2]);
-    case 3: return go(gated_norm_kernel<3, OPS>, resident[3]);
-    case 4: return go(gated_norm_kernel<4, OPS>, resident[4]);
+int launch_forward(const NormArgs& a, int64_t B, int sms, cudaStream_t st) {
+  switch ((a.D / 4 + kNormThreads - 1) / kNormThreads) {
+    case 1: return launch_forward_npt<1, OPS>(a, B, sms, st);
+    case 2: return launch_forward_npt<2, OPS>(a, B, sms, st);
+    case 3: return launch_forward_npt<3, OPS>(a, B, sms, st);
+    case 4: return launch_forward_npt<4, OPS>(a, B, sms, st);
     case 5:
-    case 6: return go(gated_norm_kernel<6, OPS>, resident[6]);
+    case 6: return launch_forward_npt<6, OPS>(a, B, sms, st);
   }
-  go(gated_norm_kernel<8, OPS>, resident[8]);
+  return launch_forward_npt<8, OPS>(a, B, sms, st);
+}
+
+template <int THREADS, int NPT>
+int launch_backward(const NormGradArgs& a, int64_t B, cudaStream_t st) {
+  static KernelInfo info;
+  constexpr size_t kPerFeature = kNormGradAhead * 8 + 8;
+  int per_sm = 1;
+  const int rc = set_up(gated_norm_backward_kernel<THREADS, NPT>, THREADS, kPerFeature * THREADS * NPT * 4,
+                        kPerFeature * a.D, info, &per_sm);
+  if (rc != DQ_OK) return rc;
+  gated_norm_backward_kernel<THREADS, NPT>
+      <<<static_cast<unsigned>(B * a.chunks), THREADS, kPerFeature * a.D, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -84,22 +120,18 @@ int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int6
     if (!aligned8(p)) return DQ_ERR_ALIGN;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
-  NormArgs a = {bf(x), bf(y), bf(gate), bf(scale), bf(shift), bf(post_weight), bf(pre_weight),
-                static_cast<__nv_bfloat16*>(s), static_cast<__nv_bfloat16*>(h), ld_x, ld_y, ld_gate, ld_mod, ld_s,
-                ld_h, T, S, D, post, pre, residual_scale, eps};
+  const NormArgs a = {bf(x), bf(y), bf(gate), bf(scale), bf(shift), bf(post_weight), bf(pre_weight),
+                      static_cast<__nv_bfloat16*>(s), static_cast<__nv_bfloat16*>(h), ld_x, ld_y, ld_gate, ld_mod,
+                      ld_s, ld_h, S, D, post, pre, 0, residual_scale, eps};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rounding == DQ_ROUND_OPS)
-    launch_forward<true>(a, sms, st);
-  else
-    launch_forward<false>(a, sms, st);
-  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+  return rounding == DQ_ROUND_OPS ? launch_forward<true>(a, T / S, sms, st) : launch_forward<false>(a, T / S, sms, st);
 }
 
 size_t dq_gated_norm_backward_workspace(int64_t T, int S, int D) {
   int sms = 0;
   if (shape_ok(T, S, D) != DQ_OK || T == 0 || device_sms(&sms) != DQ_OK) return 0;
   const int64_t B = T / S;
-  return static_cast<size_t>(B) * chunks_of(B, S, D, sms) * 3 * D * sizeof(float);
+  return static_cast<size_t>(B) * chunks_of(B, S, backward_slots(D, sms), 4) * 3 * D * sizeof(float);
 }
 
 int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_t ld_dh, const void* s, int64_t ld_s,
@@ -112,7 +144,6 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
   if (rc != DQ_OK) return rc;
   if (!norms_ok(post, pre, post_weight)) return DQ_ERR_ARG;
   const int64_t B = T / S;
-  if (B > 65535) return DQ_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {  // no tokens: the weights' gradients are zeros
     for (float* p : {dpost_weight, dpre_weight})
@@ -131,30 +162,25 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
     if ((reinterpret_cast<uintptr_t>(p) & 3) != 0) return DQ_ERR_ALIGN;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
-  const int chunks = chunks_of(B, S, D, sms);
+  const int chunks = chunks_of(B, S, backward_slots(D, sms), 4);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
       workspace_bytes < static_cast<size_t>(B) * chunks * 3 * D * sizeof(float))
     return DQ_ERR_WORKSPACE;
   NormGradArgs a = {bf(ds), bf(dh), bf(s), bf(y), bf(gate), bf(scale), bf(post_weight), bf(pre_weight),
                     static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dy), static_cast<float*>(workspace),
                     ld_ds, ld_dh, ld_s, ld_y, ld_gate, ld_mod, ld_dx, ld_dy, S, D, post, pre,
-                    static_cast<int>(ceil_div(S, chunks)), residual_scale, eps};
-  const dim3 grid(chunks, static_cast<unsigned>(B));
+                    chunks, residual_scale, eps};
   const int runs = D / 4;
-  if (runs <= 256)
-    gated_norm_backward_kernel<256, 1><<<grid, 256, 0, st>>>(a);
-  else if (runs <= 512)
-    gated_norm_backward_kernel<256, 2><<<grid, 256, 0, st>>>(a);
-  else if (runs <= 768)
-    gated_norm_backward_kernel<256, 3><<<grid, 256, 0, st>>>(a);
-  else if (runs <= 1024)
-    gated_norm_backward_kernel<256, 4><<<grid, 256, 0, st>>>(a);
-  else
-    gated_norm_backward_kernel<512, 4><<<grid, 512, 0, st>>>(a);
+  rc = runs <= 256    ? launch_backward<256, 1>(a, B, st)
+       : runs <= 512  ? launch_backward<256, 2>(a, B, st)
+       : runs <= 768  ? launch_backward<256, 3>(a, B, st)
+       : runs <= 1024 ? launch_backward<256, 4>(a, B, st)
+                      : launch_backward<512, 4>(a, B, st);
+  if (rc != DQ_OK) return rc;
   NormReduceArgs q = {a.part, a.gate, a.scale, a.post_w, a.pre_w, dgate, dscale, dshift, dpost_weight, dpre_weight,
                       ld_gate, ld_mod, static_cast<int>(B), chunks, D, residual_scale};
   if (dgate != nullptr || dscale != nullptr || dshift != nullptr || dpost_weight != nullptr || dpre_weight != nullptr)
-    gated_norm_reduce_kernel<<<static_cast<unsigned>(ceil_div(D, 32)), 256, 0, st>>>(q);
+    gated_norm_reduce_kernel<<<static_cast<unsigned>(ceil_div(D, 32)), 32 * kReduceWarps, 0, st>>>(q);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 

@@ -4,13 +4,17 @@
 //   s = x + rs * gate * Npost(y) * wpost      h = Npre(s) * wpre * (1 + scale) + shift
 //
 // Bound: HBM.  Forward 8 bytes per element (x, y in; s, h out), backward 12
-// (ds, dh, s, y in; dx, dy out), against a few tens of instructions.  A CTA
-// takes one token row at a time, every feature in registers (thread i owns
-// 4-feature runs i, i + threads, ...), and walks rows with the next row's
-// operands already loading while the sums of this one go around: the block
-// reductions' latency then costs nothing as long as two or more CTAs share an
-// SM.  Each reduction has its own shared words, doubled by row parity, so it
-// takes one barrier.
+// (ds, dh, s, y in; dx, dy out).  At those rates an SM has about 20 and 30
+// issue slots per element, so the arithmetic runs on packed float32 pairs
+// (fma.rn.f32x2 and its kin) and everything that does not change along a CTA's
+// rows is prepared once: a CTA walks rows of one batch element, its factors
+// (rs gate wpost; wpre (1 + scale); shift) in shared memory as float32.  One
+// row at a time, thread i owning the 4-feature runs i, i + threads, ...; the
+// next rows' operands arrive by cp.async in slots that only their own thread
+// reads (no barrier).  Each block reduction has shared words of its own,
+// doubled by row parity, so it takes one barrier.  (With scalar arithmetic,
+// bf16 factors from L1 and the next row prefetched in registers: 42 instructions
+// per element and 35 us forward, 68 and 98 us backward at 4608 x 4096.)
 //
 // Backward.  With t = Npre(s), m = wpre (1 + scale), dt = dh m, and yh = Npost(y):
 //   dx = ds + rstd_s (dt - [mean dt] - t mean(dt t))            (mean dt: LayerNorm only)
@@ -19,27 +23,74 @@
 //   q0 = sum dh,  q1 = sum dh t,  q2 = sum dx yh,
 // because dshift = q0, dscale = wpre q1, dgate = rs wpost q2 per batch element
 // and dwpre = sum_b (1 + scale_b) q1_b, dwpost = rs sum_b gate_b q2_b.  A CTA
-// keeps them in registers over its run of rows of one batch element and writes
-// them once; a second kernel adds the runs in order (no atomics).
+// keeps them in registers over its rows and writes them once; a second kernel
+// adds the CTAs' in order (no atomics).
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cstdint>
 
+#include "dq_ptx.cuh"
+
 namespace dq {
 
 enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 
-__device__ __forceinline__ void unpack4(uint2 u, float* v) {
-  v[0] = __uint_as_float(u.x << 16);
-  v[1] = __uint_as_float(u.x & 0xFFFF0000u);
-  v[2] = __uint_as_float(u.y << 16);
-  v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+// ------------------------------------------------------- packed float32 pairs
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
 }
-__device__ __forceinline__ uint2 pack4(const float* v) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]);
-  const __nv_bfloat162 b = __floats2bfloat162_rn(v[2], v[3]);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ float2 unpair(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum_pair(F2 a) {
+  const float2 u = unpair(a);
+  return u.x + u.y;
+}
+// bf16 pair -> float32 pair (exact), and back (RNE)
+__device__ __forceinline__ F2 widen(uint32_t w) { return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ uint32_t narrow(F2 a) {
+  const float2 u = unpair(a);
+  const __nv_bfloat162 b = __floats2bfloat162_rn(u.x, u.y);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Thread-private 8-byte copy into shared memory.
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 // Sum over the CTA's W warps, in the order of block_sum_256 (dq_dit.cuh); red:
@@ -76,151 +127,241 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* red) {
 struct NormArgs {
   const __nv_bfloat16 *x, *y, *gate, *scale, *shift, *post_w, *pre_w;
   __nv_bfloat16 *s, *h;
-  int64_t ld_x, ld_y, ld_gate, ld_mod, ld_s, ld_h, T;
-  int S, D, post, pre;
+  int64_t ld_x, ld_y, ld_gate, ld_mod, ld_s, ld_h;
+  int S, D, post, pre, chunks;
   float rs, eps;
 };
 
-template <bool OPS>
-__device__ __forceinline__ float op_round(float v) {
-  return OPS ? __bfloat162float(__float2bfloat16_rn(v)) : v;
-}
+// This thread's run r of the three factor rows of batch element b, float32:
+// rs gate wpost, wpre (1 + scale), shift.
+struct NormFactors {
+  const uint2 *gate, *scale, *shift, *post_w, *pre_w;
+  float rs;
+  __device__ __forceinline__ static void times(float* m, const uint2* p, int r, float plus) {
+    if (p == nullptr) return;
+    const uint2 u = __ldg(p + r);
+    m[0] *= __uint_as_float(u.x << 16) + plus;
+    m[1] *= __uint_as_float(u.x & 0xFFFF0000u) + plus;
+    m[2] *= __uint_as_float(u.y << 16) + plus;
+    m[3] *= __uint_as_float(u.y & 0xFFFF0000u) + plus;
+  }
+  __device__ __forceinline__ float4 behind(int r) const {
+    float m[4] = {rs, rs, rs, rs};
+    times(m, post_w, r, 0.f);
+    times(m, gate, r, 0.f);
+    return make_float4(m[0], m[1], m[2], m[3]);
+  }
+  __device__ __forceinline__ float4 before(int r) const {
+    float m[4] = {1.f, 1.f, 1.f, 1.f};
+    times(m, pre_w, r, 0.f);
+    times(m, scale, r, 1.f);
+    return make_float4(m[0], m[1], m[2], m[3]);
+  }
+  __device__ __forceinline__ float4 shifts(int r) const {
+    float m[4] = {1.f, 1.f, 1.f, 1.f};
+    if (shift == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);
+    times(m, shift, r, 0.f);
+    return make_float4(m[0], m[1], m[2], m[3]);
+  }
+};
 
+__device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ F2 bf16_round2(F2 a) { return widen(narrow(a)); }
+
+// CTA (batch element, chunk): rows chunk, chunk + chunks, ... of the element.
+// OPS rounds after every op of the tensor chain, from the bf16 factors, with
+// the sums in the order of adaln_modulate_kernel: the same bits.
+constexpr int kNormThreads = 256;
+constexpr int kNormAhead = 2;  // rows whose operands are on their way
 template <int NPT, bool OPS>
-__global__ void __launch_bounds__(256) gated_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_kernel(const NormArgs a) {
   __shared__ float red[2][4][8];
+  extern __shared__ __align__(16) uint8_t smem[];
   const int nrun = a.D / 4;
   const float dim = static_cast<float>(a.D);
-  uint2 nx[NPT], ny[NPT];
-  auto fetch = [&](int64_t t) {
-    const uint2* xr = reinterpret_cast<const uint2*>(a.x + t * a.ld_x);
-    const uint2* yr = reinterpret_cast<const uint2*>(a.y + t * a.ld_y);
+  const int64_t b = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x - static_cast<int>(b) * a.chunks;
+  const NormFactors f = {reinterpret_cast<const uint2*>(a.gate == nullptr ? nullptr : a.gate + b * a.ld_gate),
+                         reinterpret_cast<const uint2*>(a.scale == nullptr ? nullptr : a.scale + b * a.ld_mod),
+                         reinterpret_cast<const uint2*>(a.shift == nullptr ? nullptr : a.shift + b * a.ld_mod),
+                         reinterpret_cast<const uint2*>(a.post_w), reinterpret_cast<const uint2*>(a.pre_w), a.rs};
+  // slots [row][x, y][run], then (not OPS) the factor rows
+  const uint32_t slot0 = smem_u32(smem) + 8u * threadIdx.x;
+  const uint32_t row_bytes = 8u * static_cast<uint32_t>(nrun);
+  float4* fac = reinterpret_cast<float4*>(smem + kNormAhead * 2 * row_bytes);
+  auto fetch = [&](int row, int slot) {
+    if (row < a.S) {
+      const int64_t t = b * a.S + row;
+      const uint2* xr = reinterpret_cast<const uint2*>(a.x + t * a.ld_x);
+      const uint2* yr = reinterpret_cast<const uint2*>(a.y + t * a.ld_y);
+      const uint32_t dst = slot0 + static_cast<uint32_t>(slot) * 2u * row_bytes;
 #pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      const int r = threadIdx.x + 256 * j;
-      nx[j] = ny[j] = make_uint2(0u, 0u);
-      if (r < nrun) {
-        nx[j] = xr[r];
-        ny[j] = yr[r];
+      for (int j = 0; j < NPT; ++j) {
+        const int r = threadIdx.x + kNormThreads * j;
+        if (r < nrun) {
+          cp_async_8(dst + 8u * kNormThreads * j, xr + r);
+          cp_async_8(dst + row_bytes + 8u * kNormThreads * j, yr + r);
+        }
       }
     }
+    copies_commit();
   };
-  fetch(blockIdx.x);
-  int par = 0;
-  for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, par ^= 1) {
-    float v[NPT][4];
-    uint2 cx[NPT];
 #pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      cx[j] = nx[j];
-      unpack4(ny[j], v[j]);
-    }
-    if (t + gridDim.x < a.T) fetch(t + gridDim.x);
-    const int64_t b = t / a.S;
-
-    // the norm behind the block
-    if (a.post != kNormNone) {
-      float mean = 0.f;
-      if (a.post == kNormLayer) {
-        float sum = 0.f;
+  for (int i = 0; i < kNormAhead; ++i) fetch(chunk + i * a.chunks, i);
+  if constexpr (!OPS) {
 #pragma unroll
-        for (int j = 0; j < NPT; ++j)
-          if (threadIdx.x + 256 * j < nrun) sum += (v[j][0] + v[j][1]) + (v[j][2] + v[j][3]);
-        mean = row_sum<8>(sum, red[par][0]) / dim;
-      }
-      float sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < NPT; ++j)
-        if (threadIdx.x + 256 * j < nrun) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float d = v[j][e] - mean;
-            sq += d * d;
-          }
-        }
-      const float rstd = rsqrtf(row_sum<8>(sq, red[par][1]) / dim + a.eps);
-#pragma unroll
-      for (int j = 0; j < NPT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>((v[j][e] - mean) * rstd);
-    }
-    // weight, gate, residual scale, residual
-    const uint2* pw = reinterpret_cast<const uint2*>(a.post_w);
-    const uint2* gt = reinterpret_cast<const uint2*>(a.gate + b * a.ld_gate);
-    uint2* so = reinterpret_cast<uint2*>(a.s + t * a.ld_s);
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      const int r = threadIdx.x + 256 * j;
+    for (int j = 0; j < NPT; ++j) {  // each thread reads back what it wrote
+      const int r = threadIdx.x + kNormThreads * j;
       if (r < nrun) {
-        float c[4];
-        if (a.post_w != nullptr) {
-          unpack4(__ldg(pw + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>(v[j][e] * c[e]);
-        }
-        if (a.gate != nullptr) {
-          unpack4(__ldg(gt + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>(c[e] * v[j][e]);
-        }
-        if (a.rs != 1.0f) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>(a.rs * v[j][e]);
-        }
-        unpack4(cx[j], c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = c[e] + v[j][e];
-        const uint2 u = pack4(v[j]);
-        so[r] = u;
-        unpack4(u, v[j]);  // the next norm sees s as stored
-        sum += (v[j][0] + v[j][1]) + (v[j][2] + v[j][3]);
-      }
-    }
-    // the norm before the next block
-    float mean = 0.f;
-    if (a.pre == kNormLayer) mean = row_sum<8>(sum, red[par][2]) / dim;
-    float sq = 0.f;
-#pragma unroll
-    for (int j = 0; j < NPT; ++j)
-      if (threadIdx.x + 256 * j < nrun) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float d = v[j][e] - mean;
-          sq += d * d;
-        }
-      }
-    const float rstd = rsqrtf(row_sum<8>(sq, red[par][3]) / dim + a.eps);
-    const uint2* qw = reinterpret_cast<const uint2*>(a.pre_w);
-    const uint2* sc = reinterpret_cast<const uint2*>(a.scale + b * a.ld_mod);
-    const uint2* sh = reinterpret_cast<const uint2*>(a.shift + b * a.ld_mod);
-    uint2* ho = reinterpret_cast<uint2*>(a.h + t * a.ld_h);
-#pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      const int r = threadIdx.x + 256 * j;
-      if (r < nrun) {
-        float c[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>((v[j][e] - mean) * rstd);
-        if (a.pre_w != nullptr) {
-          unpack4(__ldg(qw + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>(v[j][e] * c[e]);
-        }
-        if (a.scale != nullptr) {
-          unpack4(__ldg(sc + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = op_round<OPS>(v[j][e] * op_round<OPS>(c[e] + 1.0f));
-        }
-        if (a.shift != nullptr) {
-          unpack4(__ldg(sh + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] + c[e];
-        }
-        ho[r] = pack4(v[j]);
+        fac[r] = f.behind(r);
+        fac[nrun + r] = f.before(r);
+        fac[2 * nrun + r] = f.shifts(r);
       }
     }
   }
+  int par = 0, slot = 0;
+  for (int row = chunk; row < a.S; row += a.chunks, par ^= 1, slot = slot + 1 == kNormAhead ? 0 : slot + 1) {
+    const int64_t t = b * a.S + row;
+    copies_wait<kNormAhead - 1>();
+    const uint32_t src = slot0 + static_cast<uint32_t>(slot) * 2u * row_bytes;
+    F2 v[NPT][2];
+    uint2 cx[NPT];
+#pragma unroll
+    for (int j = 0; j < NPT; ++j) {
+      const int r = threadIdx.x + kNormThreads * j;
+      cx[j] = make_uint2(0u, 0u);
+      uint2 y = make_uint2(0u, 0u);
+      if (r < nrun) {
+        cx[j] = lds64(src + 8u * kNormThreads * j);
+        y = lds64(src + row_bytes + 8u * kNormThreads * j);
+      }
+      v[j][0] = widen(y.x);
+      v[j][1] = widen(y.y);
+    }
+    fetch(row + kNormAhead * a.chunks, slot);
+
+    // (v - mean) squared, summed: in adaln_modulate_kernel's order with OPS
+    auto squares = [&](float mean) {
+      if constexpr (OPS) {
+        float sq = 0.f;
+#pragma unroll
+        for (int j = 0; j < NPT; ++j)
+          if (threadIdx.x + kNormThreads * j < nrun) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const float2 u = unpair(v[j][p]);
+              const float d0 = u.x - mean, d1 = u.y - mean;
+              sq += d0 * d0;
+              sq += d1 * d1;
+            }
+          }
+        return sq;
+      } else {
+        F2 sq = f2(0.f);
+        const F2 m = f2(-mean);
+#pragma unroll
+        for (int j = 0; j < NPT; ++j)
+          if (threadIdx.x + kNormThreads * j < nrun) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const F2 d = add2(v[j][p], m);
+              sq = fma2(d, d, sq);
+            }
+          }
+        return sum_pair(sq);
+      }
+    };
+    auto sums = [&]() {  // idle runs hold zeros
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NPT; ++j) sum += sum_pair(v[j][0]) + sum_pair(v[j][1]);
+      return sum;
+    };
+
+    // the norm behind the block
+    if (a.post != kNormNone) {
+      const float mean = a.post == kNormLayer ? row_sum<8>(sums(), red[par][0]) / dim : 0.f;
+      const float rstd = rsqrtf(row_sum<8>(squares(mean), red[par][1]) / dim + a.eps);
+#pragma unroll
+      for (int j = 0; j < NPT; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          v[j][p] = mul2(add2(v[j][p], f2(-mean)), f2(rstd));
+          if constexpr (OPS) v[j][p] = bf16_round2(v[j][p]);
+        }
+    }
+    // weight, gate, residual scale, residual
+    uint2* so = reinterpret_cast<uint2*>(a.s + t * a.ld_s);
+#pragma unroll
+    for (int j = 0; j < NPT; ++j) {
+      const int r = threadIdx.x + kNormThreads * j;
+      if (r < nrun) {
+        uint2 u;
+        if constexpr (OPS) {
+          if (a.post_w != nullptr) {
+            const uint2 c = __ldg(f.post_w + r);
+            v[j][0] = bf16_round2(mul2(v[j][0], widen(c.x)));
+            v[j][1] = bf16_round2(mul2(v[j][1], widen(c.y)));
+          }
+          if (a.gate != nullptr) {
+            const uint2 c = __ldg(f.gate + r);
+            v[j][0] = bf16_round2(mul2(widen(c.x), v[j][0]));
+            v[j][1] = bf16_round2(mul2(widen(c.y), v[j][1]));
+          }
+          if (a.rs != 1.0f) {
+            v[j][0] = bf16_round2(mul2(f2(a.rs), v[j][0]));
+            v[j][1] = bf16_round2(mul2(f2(a.rs), v[j][1]));
+          }
+          u = make_uint2(narrow(add2(widen(cx[j].x), v[j][0])), narrow(add2(widen(cx[j].y), v[j][1])));
+        } else {
+          const float4 g = fac[r];
+          u = make_uint2(narrow(fma2(v[j][0], f2(g.x, g.y), widen(cx[j].x))),
+                         narrow(fma2(v[j][1], f2(g.z, g.w), widen(cx[j].y))));
+        }
+        so[r] = u;
+        v[j][0] = widen(u.x);  // the next norm sees s as stored
+        v[j][1] = widen(u.y);
+      } else {
+        v[j][0] = v[j][1] = f2(0.f);
+      }
+    }
+    // the norm before the next block
+    const float mean = a.pre == kNormLayer ? row_sum<8>(sums(), red[par][2]) / dim : 0.f;
+    const float rstd = rsqrtf(row_sum<8>(squares(mean), red[par][3]) / dim + a.eps);
+    uint2* ho = reinterpret_cast<uint2*>(a.h + t * a.ld_h);
+#pragma unroll
+    for (int j = 0; j < NPT; ++j) {
+      const int r = threadIdx.x + kNormThreads * j;
+      if (r < nrun) {
+        F2 n0 = mul2(add2(v[j][0], f2(-mean)), f2(rstd)), n1 = mul2(add2(v[j][1], f2(-mean)), f2(rstd));
+        if constexpr (OPS) {
+          n0 = bf16_round2(n0);
+          n1 = bf16_round2(n1);
+          if (a.pre_w != nullptr) {
+            const uint2 c = __ldg(f.pre_w + r);
+            n0 = bf16_round2(mul2(n0, widen(c.x)));
+            n1 = bf16_round2(mul2(n1, widen(c.y)));
+          }
+          if (a.scale != nullptr) {
+            const uint2 c = __ldg(f.scale + r);
+            n0 = bf16_round2(mul2(n0, bf16_round2(add2(widen(c.x), f2(1.0f)))));
+            n1 = bf16_round2(mul2(n1, bf16_round2(add2(widen(c.y), f2(1.0f)))));
+          }
+          if (a.shift != nullptr) {
+            const uint2 c = __ldg(f.shift + r);
+            n0 = add2(n0, widen(c.x));
+            n1 = add2(n1, widen(c.y));
+          }
+        } else {
+          const float4 m = fac[nrun + r], h = fac[2 * nrun + r];
+          n0 = fma2(n0, f2(m.x, m.y), f2(h.x, h.y));
+          n1 = fma2(n1, f2(m.z, m.w), f2(h.z, h.w));
+        }
+        ho[r] = make_uint2(narrow(n0), narrow(n1));
+      }
+    }
+  }
+  copies_wait<0>();
 }
 
 struct NormGradArgs {
@@ -228,190 +369,204 @@ struct NormGradArgs {
   __nv_bfloat16 *dx, *dy;
   float* part;  // [B, chunks, 3, D]
   int64_t ld_ds, ld_dh, ld_s, ld_y, ld_gate, ld_mod, ld_dx, ld_dy;
-  int S, D, post, pre, rows_per_chunk;
+  int S, D, post, pre, chunks;
   float rs, eps;
 };
 
-// CTA (chunk, batch element): rows chunk * rows_per_chunk .. of one element.
+// CTA (batch element, chunk): rows chunk, chunk + chunks, ... of the element.
+constexpr int kNormGradAhead = 2;
 template <int THREADS, int NPT>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     gated_norm_backward_kernel(const NormGradArgs a) {
   constexpr int W = THREADS / 32;
   __shared__ float2 red[2][4][W];
+  extern __shared__ __align__(16) uint8_t smem[];
   const int nrun = a.D / 4;
   const float inv = 1.0f / static_cast<float>(a.D);
-  const int64_t b = blockIdx.y;
-  const int r_lo = blockIdx.x * a.rows_per_chunk, r_hi = min(a.S, r_lo + a.rows_per_chunk);
-  const uint2* gt = reinterpret_cast<const uint2*>(a.gate + b * a.ld_gate);
-  const uint2* sc = reinterpret_cast<const uint2*>(a.scale + b * a.ld_mod);
-  const uint2* pw = reinterpret_cast<const uint2*>(a.post_w);
-  const uint2* qw = reinterpret_cast<const uint2*>(a.pre_w);
-  float q0[NPT][4] = {}, q1[NPT][4] = {}, q2[NPT][4] = {};
-  uint2 n_ds[NPT], n_dh[NPT], n_s[NPT], n_y[NPT];
-  auto fetch = [&](int row) {
+  const int64_t b = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x - static_cast<int>(b) * a.chunks;
+  const uint32_t slot0 = smem_u32(smem) + 8u * threadIdx.x;
+  const uint32_t row_bytes = 8u * static_cast<uint32_t>(nrun);
+  // slots [row][s, y, dh, ds][run], then the factor rows
+  float4* fac = reinterpret_cast<float4*>(smem + kNormGradAhead * 4 * row_bytes);
+  auto fetch = [&](int row, int slot) {
+    if (row < a.S) {
+      const int64_t t = b * a.S + row;
+      const uint32_t dst = slot0 + static_cast<uint32_t>(slot) * 4u * row_bytes;
+#pragma unroll
+      for (int j = 0; j < NPT; ++j) {
+        const int r = threadIdx.x + THREADS * j;
+        if (r < nrun) {
+          const uint32_t d = dst + 8u * THREADS * j;
+          cp_async_8(d, reinterpret_cast<const uint2*>(a.s + t * a.ld_s) + r);
+          cp_async_8(d + row_bytes, reinterpret_cast<const uint2*>(a.y + t * a.ld_y) + r);
+          cp_async_8(d + 2 * row_bytes, reinterpret_cast<const uint2*>(a.dh + t * a.ld_dh) + r);
+          if (a.ds != nullptr) cp_async_8(d + 3 * row_bytes, reinterpret_cast<const uint2*>(a.ds + t * a.ld_ds) + r);
+        }
+      }
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kNormGradAhead; ++i) fetch(chunk + i * a.chunks, i);
+  const NormFactors f = {reinterpret_cast<const uint2*>(a.gate == nullptr ? nullptr : a.gate + b * a.ld_gate),
+                         reinterpret_cast<const uint2*>(a.scale == nullptr ? nullptr : a.scale + b * a.ld_mod),
+                         nullptr, reinterpret_cast<const uint2*>(a.post_w), reinterpret_cast<const uint2*>(a.pre_w),
+                         a.rs};
+#pragma unroll
+  for (int j = 0; j < NPT; ++j) {  // each thread reads back what it wrote
+    const int r = threadIdx.x + THREADS * j;
+    if (r < nrun) {
+      fac[r] = f.behind(r);
+      fac[nrun + r] = f.before(r);
+    }
+  }
+  F2 q0[NPT][2], q1[NPT][2], q2[NPT][2];
+#pragma unroll
+  for (int j = 0; j < NPT; ++j)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) q0[j][p] = q1[j][p] = q2[j][p] = f2(0.f);
+  const bool means = a.pre == kNormLayer || a.post == kNormLayer;
+  int par = 0, slot = 0;
+  for (int row = chunk; row < a.S; row += a.chunks, par ^= 1, slot = slot + 1 == kNormGradAhead ? 0 : slot + 1) {
     const int64_t t = b * a.S + row;
+    copies_wait<kNormGradAhead - 1>();
+    const uint32_t src = slot0 + static_cast<uint32_t>(slot) * 4u * row_bytes;
+    uint2 us[NPT], uy[NPT];
+    F2 dt[NPT][2];  // dh
+    uint2 ud[NPT];  // ds
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {
       const int r = threadIdx.x + THREADS * j;
-      n_ds[j] = n_dh[j] = n_s[j] = n_y[j] = make_uint2(0u, 0u);
+      const uint32_t d = src + 8u * THREADS * j;
+      us[j] = uy[j] = ud[j] = make_uint2(0u, 0u);
+      uint2 u = make_uint2(0u, 0u);
       if (r < nrun) {
-        n_s[j] = reinterpret_cast<const uint2*>(a.s + t * a.ld_s)[r];
-        n_y[j] = reinterpret_cast<const uint2*>(a.y + t * a.ld_y)[r];
-        n_dh[j] = reinterpret_cast<const uint2*>(a.dh + t * a.ld_dh)[r];
-        if (a.ds != nullptr) n_ds[j] = reinterpret_cast<const uint2*>(a.ds + t * a.ld_ds)[r];
+        us[j] = lds64(d);
+        uy[j] = lds64(d + row_bytes);
+        u = lds64(d + 2 * row_bytes);
+        if (a.ds != nullptr) ud[j] = lds64(d + 3 * row_bytes);
       }
+      dt[j][0] = widen(u.x);
+      dt[j][1] = widen(u.y);
     }
-  };
-  if (r_lo < r_hi) fetch(r_lo);
-  int par = 0;
-  for (int row = r_lo; row < r_hi; ++row, par ^= 1) {
-    const int64_t t = b * a.S + row;
-    uint2 u_ds[NPT], u_dh[NPT], u_s[NPT], u_y[NPT];
-#pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      u_ds[j] = n_ds[j];
-      u_dh[j] = n_dh[j];
-      u_s[j] = n_s[j];
-      u_y[j] = n_y[j];
-    }
-    if (row + 1 < r_hi) fetch(row + 1);
-    // statistics of s (x) and y (y); idle threads hold zeros
+    fetch(row + kNormGradAhead * a.chunks, slot);
+    // statistics of s (x) and y (y); idle runs hold zeros
     float2 mean = make_float2(0.f, 0.f);
-    if (a.pre == kNormLayer || a.post == kNormLayer) {
-      float2 sum = make_float2(0.f, 0.f);
+    if (means) {
+      F2 ms = f2(0.f), my = f2(0.f);
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
-        float p[4], q[4];
-        unpack4(u_s[j], p);
-        unpack4(u_y[j], q);
-        sum.x += (p[0] + p[1]) + (p[2] + p[3]);
-        sum.y += (q[0] + q[1]) + (q[2] + q[3]);
+        ms = add2(ms, add2(widen(us[j].x), widen(us[j].y)));
+        my = add2(my, add2(widen(uy[j].x), widen(uy[j].y)));
       }
-      sum = row_sum2<W>(sum, red[par][0]);
+      const float2 sum = row_sum2<W>(make_float2(sum_pair(ms), sum_pair(my)), red[par][0]);
       if (a.pre == kNormLayer) mean.x = sum.x * inv;
       if (a.post == kNormLayer) mean.y = sum.y * inv;
     }
-    float2 sq = make_float2(0.f, 0.f);
+    float rstd_s, rstd_y = 1.0f;
+    {
+      F2 ss = f2(0.f), sy = f2(0.f);
 #pragma unroll
-    for (int j = 0; j < NPT; ++j)
-      if (threadIdx.x + THREADS * j < nrun) {
-        float p[4], q[4];
-        unpack4(u_s[j], p);
-        unpack4(u_y[j], q);
+      for (int j = 0; j < NPT; ++j)
+        if (threadIdx.x + THREADS * j < nrun) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sq.x += (p[e] - mean.x) * (p[e] - mean.x);
-          sq.y += (q[e] - mean.y) * (q[e] - mean.y);
+          for (int p = 0; p < 2; ++p) {
+            const F2 ds = add2(widen(p ? us[j].y : us[j].x), f2(-mean.x));
+            const F2 dy = add2(widen(p ? uy[j].y : uy[j].x), f2(-mean.y));
+            ss = fma2(ds, ds, ss);
+            sy = fma2(dy, dy, sy);
+          }
         }
-      }
-    sq = row_sum2<W>(sq, red[par][1]);
-    const float rstd_s = rsqrtf(sq.x * inv + a.eps);
-    const float rstd_y = a.post == kNormNone ? 1.0f : rsqrtf(sq.y * inv + a.eps);
-
-    // dt = dh wpre (1 + scale); q0, q1
-    float dt[NPT][4];
-    float2 d = make_float2(0.f, 0.f);  // sum dt, sum dt t
-#pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      const int r = threadIdx.x + THREADS * j;
-      if (r < nrun) {
-        float s4[4], c[4];
-        unpack4(u_s[j], s4);
-        unpack4(u_dh[j], dt[j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s4[e] = (s4[e] - mean.x) * rstd_s;
-          q0[j][e] += dt[j][e];
-          q1[j][e] += dt[j][e] * s4[e];
-        }
-        if (a.pre_w != nullptr) {
-          unpack4(__ldg(qw + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dt[j][e] *= c[e];
-        }
-        if (a.scale != nullptr) {
-          unpack4(__ldg(sc + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dt[j][e] *= 1.0f + c[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d.x += dt[j][e];
-          d.y += dt[j][e] * s4[e];
-        }
-      }
+      const float2 sq = row_sum2<W>(make_float2(sum_pair(ss), sum_pair(sy)), red[par][1]);
+      rstd_s = rsqrtf(sq.x * inv + a.eps);
+      if (a.post != kNormNone) rstd_y = rsqrtf(sq.y * inv + a.eps);
     }
-    d = row_sum2<W>(d, red[par][2]);
-    d.x = a.pre == kNormLayer ? d.x * inv : 0.f;
-    d.y *= inv;
-
-    // dx, then dq = rs gate wpost dx; q2
+    // dt = dh wpre (1 + scale); q0, q1; sums of dt and dt t
+    float2 d;
+    {
+      F2 d0 = f2(0.f), d1 = f2(0.f);
+#pragma unroll
+      for (int j = 0; j < NPT; ++j) {
+        const int r = threadIdx.x + THREADS * j;
+        if (r < nrun) {
+          const float4 m = fac[nrun + r];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const F2 tt = mul2(add2(widen(p ? us[j].y : us[j].x), f2(-mean.x)), f2(rstd_s));
+            q0[j][p] = add2(q0[j][p], dt[j][p]);
+            q1[j][p] = fma2(dt[j][p], tt, q1[j][p]);
+            dt[j][p] = mul2(dt[j][p], p ? f2(m.z, m.w) : f2(m.x, m.y));
+            d0 = add2(d0, dt[j][p]);
+            d1 = fma2(dt[j][p], tt, d1);
+          }
+        }
+      }
+      d = row_sum2<W>(make_float2(sum_pair(d0), sum_pair(d1)), red[par][2]);
+      d.x = a.pre == kNormLayer ? d.x * inv : 0.f;
+      d.y *= inv;
+    }
+    // dx = ds + rstd (dt - mean dt - t mean(dt t)); q2; dq = rs gate wpost dx
     uint2* dxo = reinterpret_cast<uint2*>(a.dx + t * a.ld_dx);
-    float2 g = make_float2(0.f, 0.f);  // sum dq, sum dq yh
+    float2 g;
+    {
+      F2 g0 = f2(0.f), g1 = f2(0.f);
 #pragma unroll
-    for (int j = 0; j < NPT; ++j) {
-      const int r = threadIdx.x + THREADS * j;
-      if (r < nrun) {
-        float p[4], c[4];
-        unpack4(u_s[j], p);
-        unpack4(u_ds[j], c);
+      for (int j = 0; j < NPT; ++j) {
+        const int r = threadIdx.x + THREADS * j;
+        if (r < nrun) {
+          const float4 n = fac[r];
+          uint32_t o[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          dt[j][e] = c[e] + rstd_s * (dt[j][e] - d.x - (p[e] - mean.x) * rstd_s * d.y);
-        dxo[r] = pack4(dt[j]);
-        unpack4(u_y[j], p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = (p[e] - mean.y) * rstd_y;
-          q2[j][e] += dt[j][e] * p[e];
-        }
-        if (a.post_w != nullptr) {
-          unpack4(__ldg(pw + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dt[j][e] *= c[e];
-        }
-        if (a.gate != nullptr) {
-          unpack4(__ldg(gt + r), c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dt[j][e] *= c[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dt[j][e] *= a.rs;
-          g.x += dt[j][e];
-          g.y += dt[j][e] * p[e];
+          for (int p = 0; p < 2; ++p) {
+            const F2 tt = mul2(add2(widen(p ? us[j].y : us[j].x), f2(-mean.x)), f2(rstd_s));
+            const F2 in = fma2(tt, f2(-d.y), add2(dt[j][p], f2(-d.x)));
+            const F2 dx = fma2(in, f2(rstd_s), widen(p ? ud[j].y : ud[j].x));
+            o[p] = narrow(dx);
+            const F2 yh = mul2(add2(widen(p ? uy[j].y : uy[j].x), f2(-mean.y)), f2(rstd_y));
+            q2[j][p] = fma2(dx, yh, q2[j][p]);
+            dt[j][p] = mul2(dx, p ? f2(n.z, n.w) : f2(n.x, n.y));
+            g0 = add2(g0, dt[j][p]);
+            g1 = fma2(dt[j][p], yh, g1);
+          }
+          dxo[r] = make_uint2(o[0], o[1]);
         }
       }
-    }
-    if (a.post != kNormNone) {
-      g = row_sum2<W>(g, red[par][3]);
-      g.x = a.post == kNormLayer ? g.x * inv : 0.f;
-      g.y *= inv;
-    } else {
       g = make_float2(0.f, 0.f);
+      if (a.post != kNormNone) {
+        g = row_sum2<W>(make_float2(sum_pair(g0), sum_pair(g1)), red[par][3]);
+        g.x = a.post == kNormLayer ? g.x * inv : 0.f;
+        g.y *= inv;
+      }
     }
     uint2* dyo = reinterpret_cast<uint2*>(a.dy + t * a.ld_dy);
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {
       const int r = threadIdx.x + THREADS * j;
       if (r < nrun) {
-        float p[4];
-        unpack4(u_y[j], p);
+        uint32_t o[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          dt[j][e] = rstd_y * (dt[j][e] - g.x - (p[e] - mean.y) * rstd_y * g.y);
-        dyo[r] = pack4(dt[j]);
+        for (int p = 0; p < 2; ++p) {
+          const F2 yh = mul2(add2(widen(p ? uy[j].y : uy[j].x), f2(-mean.y)), f2(rstd_y));
+          o[p] = narrow(mul2(fma2(yh, f2(-g.y), add2(dt[j][p], f2(-g.x))), f2(rstd_y)));
+        }
+        dyo[r] = make_uint2(o[0], o[1]);
       }
     }
   }
-  float4* part = reinterpret_cast<float4*>(a.part + (b * gridDim.x + blockIdx.x) * 3 * a.D);
+  copies_wait<0>();
+  float4* part = reinterpret_cast<float4*>(a.part + static_cast<int64_t>(blockIdx.x) * 3 * a.D);
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
     const int r = threadIdx.x + THREADS * j;
     if (r < nrun) {
-      part[r] = make_float4(q0[j][0], q0[j][1], q0[j][2], q0[j][3]);
-      part[nrun + r] = make_float4(q1[j][0], q1[j][1], q1[j][2], q1[j][3]);
-      part[2 * nrun + r] = make_float4(q2[j][0], q2[j][1], q2[j][2], q2[j][3]);
+      auto put = [&](int i, F2 (&q)[2]) {
+        const float2 u = unpair(q[0]), w = unpair(q[1]);
+        part[i * nrun + r] = make_float4(u.x, u.y, w.x, w.y);
+      };
+      put(0, q0[j]);
+      put(1, q1[j]);
+      put(2, q2[j]);
     }
   }
 }
@@ -425,11 +580,15 @@ struct NormReduceArgs {
   float rs;
 };
 
-// CTA: 32 columns.  With eight or more runs per batch element warp w adds every
-// 8th of them and the warps' sums meet in order; with fewer, warp w takes every
-// 8th batch element whole (a gate per token has as many elements as tokens).
-__global__ void __launch_bounds__(256) gated_norm_reduce_kernel(const NormReduceArgs a) {
-  __shared__ float red[8][3][32];
+// CTA: 32 columns and 32 warps.  With 32 or more chunks per batch element warp w
+// adds every 32nd of them (all its loads in flight at once: the sums are latency
+// bound, eight warps took 16 us at 2 x 148 chunks x 4096) and the warps' sums
+// meet in order; with fewer, warp w takes every 32nd batch element whole (a gate
+// per token has as many elements as tokens).
+constexpr int kReduceWarps = 32;
+__global__ void __launch_bounds__(32 * kReduceWarps) gated_norm_reduce_kernel(const NormReduceArgs a) {
+  constexpr int W = kReduceWarps;
+  __shared__ float red[W][3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
   const bool in = col < a.D;
@@ -438,7 +597,7 @@ __global__ void __launch_bounds__(256) gated_norm_reduce_kernel(const NormReduce
   float dpre = 0.f, dpost = 0.f;
   auto add = [&](int b, int first, int step, float* q) {
     if (!in) return;
-#pragma unroll 4
+#pragma unroll 8
     for (int c = first; c < a.chunks; c += step) {
       const float* p = a.part + (static_cast<int64_t>(b) * a.chunks + c) * 3 * a.D + col;
 #pragma unroll
@@ -454,8 +613,8 @@ __global__ void __launch_bounds__(256) gated_norm_reduce_kernel(const NormReduce
     dpre += (a.scale != nullptr ? 1.0f + __bfloat162float(a.scale[b * a.ld_mod + col]) : 1.0f) * s[1];
     dpost += (a.gate != nullptr ? __bfloat162float(a.gate[b * a.ld_gate + col]) : 1.0f) * s[2];
   };
-  if (a.chunks < 8) {
-    for (int b = warp; b < a.B; b += 8) {
+  if (a.chunks < W) {
+    for (int b = warp; b < a.B; b += W) {
       float q[3] = {};
       add(b, 0, 1, q);
       finish(b, q);
@@ -465,14 +624,14 @@ __global__ void __launch_bounds__(256) gated_norm_reduce_kernel(const NormReduce
     __syncthreads();
     dpre = dpost = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < W; ++w) {
       dpre += red[w][0][lane];
       dpost += red[w][1][lane];
     }
   } else {
     for (int b = 0; b < a.B; ++b) {
       float q[3] = {};
-      add(b, warp, 8, q);
+      add(b, warp, W, q);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 3; ++i) red[warp][i][lane] = q[i];
@@ -480,7 +639,7 @@ __global__ void __launch_bounds__(256) gated_norm_reduce_kernel(const NormReduce
       if (warp == 0) {
         float s[3] = {};
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
+        for (int w = 0; w < W; ++w)
 #pragma unroll
           for (int i = 0; i < 3; ++i) s[i] += red[w][i][lane];
         finish(b, s);

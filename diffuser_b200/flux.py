@@ -250,7 +250,7 @@ def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_w
     b, n, d = x.shape
     x2, ldx = _token_rows(x, "x", x)
     y2, ldy = _token_rows(y, "y", x)
-    s = torch.empty((b, n, d), dtype=torch.bfloat16, device=x.device)
+    s = torch.empty_like(x, memory_format=torch.contiguous_format)
     h = torch.empty_like(s)
     if x.numel() == 0:
         return s, h

@@ -600,8 +600,8 @@ def checkpoint_pack(x: torch.Tensor) -> PackedActivation:
         raise ValueError("an 8-bit activation needs a feature count that is a multiple of 16")
     x2, xp, ldx, m = _row_operand(x, "x", k, x)
     packed = object.__new__(PackedActivation)
-    packed.codes = codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    packed.scales = scales = torch.empty((m, -(-k // CHECKPOINT_RUN)), dtype=_F32, device=x.device)
+    packed.codes = codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    packed.scales = scales = x.new_empty((m, -(-k // CHECKPOINT_RUN)), dtype=_F32)
     with _on(x):
         _lib.check("dq_checkpoint_pack", _lib.lib().dq_checkpoint_pack(
             xp, ldx, m, k, codes.data_ptr(), scales.data_ptr(), _raw_stream(x)))
@@ -615,7 +615,7 @@ def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None)
     codes = packed.codes
     k = codes.shape[-1]
     if out is None:
-        res = torch.empty(codes.shape, dtype=_BF16, device=codes.device)
+        res = torch.empty_like(codes, dtype=_BF16)
         op, ldo, m = res.data_ptr(), k, codes.numel() // k
     else:
         res = out

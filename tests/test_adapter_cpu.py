@@ -126,7 +126,7 @@ def test_gated_norm_backward_checks_its_arguments(lib):
     def call(T=4, S=2, D=64, dh=P, s=P, post=0, pw=None, lddx=64, dx=P, dgate=P):
         return lib.dq_gated_norm_backward(None, 0, dh, 64, s, 64, P, 64, T, S, D, P, 64, P, 64, pw, None, post, 1,
                                           F(1.0), F(1e-6), dx, lddx, P, 64, dgate, P, P, None, None, P, 1 << 30, None)
-    assert call(D=66) == SHAPE and call(T=3) == SHAPE and call(T=1 << 17, S=1) == SHAPE and call(lddx=60) == SHAPE
+    assert call(D=66) == SHAPE and call(T=3) == SHAPE and call(T=1 << 31, S=1) == SHAPE and call(lddx=60) == SHAPE
     assert call(dh=None) == ARG and call(s=None) == ARG and call(dx=None) == ARG and call(pw=P) == ARG
     assert call(dx=P + 4) == ALIGN and call(dgate=P + 2) == ALIGN
     assert lib.dq_gated_norm_backward_workspace(5, 2, 64) == 0
