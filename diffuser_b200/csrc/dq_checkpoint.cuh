@@ -5,88 +5,156 @@
 
 #include "dq_adapter.cuh"
 #include "dq_codec.cuh"
+#include "dq_f32x2.cuh"
 
 namespace dq {
 
 constexpr int kCkptRun = 128;  // features per scale
 
+// Row and column of a flat index that advances by a constant stride: one
+// division at the start instead of one per step (a 64-bit division per 8
+// features was a quarter of the pack kernel's instructions).
+struct RowWalk {
+  int64_t row, step_rows;
+  int col, step_cols, width;
+  __device__ __forceinline__ RowWalk(int64_t start, int64_t stride, int width_) : width(width_) {
+    row = start / width;
+    col = static_cast<int>(start - row * width);
+    step_rows = stride / width;
+    step_cols = static_cast<int>(stride - step_rows * width);
+  }
+  __device__ __forceinline__ void next() {
+    row += step_rows;
+    col += step_cols;
+    if (col >= width) {
+      col -= width;
+      ++row;
+    }
+  }
+};
+
 // Pack: 16 lanes per run of 128 features, 8 features (16 bytes) per lane, two
 // runs per warp and two warps' worth of loads in flight.  The maximum is taken
-// over the bit patterns of |x| (bf16 magnitudes order like integers, infinities
-// and NaN above every number), so a run that is not finite is seen whatever the
-// order.  HBM-bound: 3 bytes per feature; an IEEE division per feature made it
-// 127 us at 6144 x 16384 (floor 47), so the quotient is taken as x (1 / scale),
-// off by at most 127 (2^-24 + 2^-24) = 1.6e-5 from the exact one, and divided
-// only where that could round to another integer: within 1e-4 of a half.
-__device__ __forceinline__ uint32_t pack_code(float v, float scale, float inv) {
-  const float t = v * inv;
-  float q = rintf(t);
-  if (fabsf(t - q) > 0.4999f) q = rintf(__fdiv_rn(v, scale));
-  return static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu;
+// over bf16 pairs and keeps NaN, so a run that is not finite is seen.  HBM-bound: 3 bytes per feature, 47 us at 6144 x 16384.  An IEEE
+// division per feature made it 127 us, so the quotient is taken as
+// x (1 / scale), off by at most 127 (2^-23 + 2^-24) = 2.3e-5 from the exact one,
+// and divided only where that could round to another integer: within 1e-4 of a
+// half.  Adding 1.5 2^23 rounds to an integer (ties to even) and leaves it in
+// the low bits, without the special-function unit's conversions.
+constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
+__device__ __forceinline__ void pack_pair(uint32_t w, float scale, F2 inv, uint32_t& c0, uint32_t& c1) {
+  const F2 v = widen(w), t = mul2(v, inv);
+  F2 u = add2(t, f2(kRoundMagic));
+  const float2 d = unpair(add2(t, f2_neg(add2(u, f2(-kRoundMagic)))));
+  float2 r = unpair(u);
+  if (fmaxf(fabsf(d.x), fabsf(d.y)) > 0.4999f) {
+    const float2 x = unpair(v);
+    r.x = __fadd_rn(__fdiv_rn(x.x, scale), kRoundMagic);
+    r.y = __fadd_rn(__fdiv_rn(x.y, scale), kRoundMagic);
+  }
+  c0 = __float_as_uint(r.x);
+  c1 = __float_as_uint(r.y);
+}
+
+// amax / 127, correctly rounded: the product with the rounded 1 / 127, then one
+// residual step in fused arithmetic (Markstein's division); the same as the
+// IEEE quotient for every bf16 magnitude of at least 1e-12.
+__device__ __forceinline__ float over_127(float amax) {
+  constexpr float c = 1.0f / 127.0f;
+  const float q = amax * c;
+  return fmaf(fmaf(-127.0f, q, amax), c, q);
+}
+
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 __global__ void __launch_bounds__(256)
-    checkpoint_pack_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int64_t runs, int nrun,
-                           int K, int8_t* __restrict__ codes, float* __restrict__ scales) {
+    checkpoint_pack_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int64_t M, int nrun, int K,
+                           int8_t* __restrict__ codes, float* __restrict__ scales) {
   const int half = (threadIdx.x & 31) >> 4, sub = threadIdx.x & 15;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 16;
-  for (int64_t base = blockIdx.x * 16ll + (threadIdx.x >> 5) * 2; base < runs; base += 2 * stride) {
+  RowWalk at(blockIdx.x * 16ll + (threadIdx.x >> 5) * 2 + half, stride, nrun);
+  while (__any_sync(0xffffffffu, at.row < M)) {
     uint4 u[2];
     int64_t row[2];
-    int k[2];
+    int run[2];
     bool in[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t run = base + i * stride + half;
-      row[i] = run / nrun;
-      k[i] = static_cast<int>(run - row[i] * nrun) * kCkptRun + sub * 8;
-      in[i] = run < runs && k[i] < K;
-      u[i] = in[i] ? ld_stream16(x + row[i] * ldx + k[i]) : make_uint4(0u, 0u, 0u, 0u);
+      row[i] = at.row;
+      run[i] = at.col;
+      const int k = run[i] * kCkptRun + sub * 8;
+      in[i] = row[i] < M && k < K;
+      u[i] = in[i] ? ld_stream16(x + row[i] * ldx + k) : make_uint4(0u, 0u, 0u, 0u);
+      at.next();
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint32_t m = __vmaxu2(__vmaxu2(u[i].x & 0x7FFF7FFFu, u[i].y & 0x7FFF7FFFu),
-                            __vmaxu2(u[i].z & 0x7FFF7FFFu, u[i].w & 0x7FFF7FFFu));
+      constexpr uint32_t kAbs = 0x7FFF7FFFu;
+      uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u[i].x & kAbs, u[i].y & kAbs),
+                                  max_nan_bf16x2(u[i].z & kAbs, u[i].w & kAbs));
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const uint32_t top = max(m & 0xFFFFu, m >> 16);
+      for (int o = 8; o > 0; o >>= 1) m = max_nan_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const uint32_t top = max(m & 0x7FFFu, (m >> 16) & 0x7FFFu);
       const bool finite = top < 0x7F80u;
-      const float amax = fmaxf(__uint_as_float(top << 16), 1e-12f);
-      const float scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7FC00000u);
+      const float scale =
+          finite ? over_127(fmaxf(__uint_as_float(top << 16), 1e-12f)) : __uint_as_float(0x7FC00000u);
       if (!in[i]) continue;
       uint32_t w[2] = {0u, 0u};
       if (finite) {
-        const float inv = __frcp_rn(scale);
-        float v[8];
-        unpack8(u[i], v);
+        const F2 inv = f2(rcp_approx(scale));
+        uint32_t c[8];
+        pack_pair(u[i].x, scale, inv, c[0], c[1]);
+        pack_pair(u[i].y, scale, inv, c[2], c[3]);
+        pack_pair(u[i].z, scale, inv, c[4], c[5]);
+        pack_pair(u[i].w, scale, inv, c[6], c[7]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= pack_code(v[e], scale, inv) << (8 * (e & 3));
+        for (int q = 0; q < 2; ++q)
+          w[q] = prmt(prmt(c[4 * q], c[4 * q + 1], 0x0040u), prmt(c[4 * q + 2], c[4 * q + 3], 0x0040u), 0x5410u);
       }
-      *reinterpret_cast<uint2*>(codes + row[i] * K + k[i]) = make_uint2(w[0], w[1]);
-      if (sub == 0) scales[base + i * stride + half] = scale;
+      *reinterpret_cast<uint2*>(codes + row[i] * K + run[i] * kCkptRun + sub * 8) = make_uint2(w[0], w[1]);
+      if (sub == 0) scales[row[i] * nrun + run[i]] = scale;
     }
   }
 }
 
-// Unpack: 8 codes per thread.
+// Unpack: 8 codes per thread, two pieces in flight.  The codes become bf16
+// exactly, so float32 by a shift, without integer conversions.
 __global__ void __launch_bounds__(256)
     checkpoint_unpack_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
                              int64_t M, int K, int nrun, __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  const int per_row = K / 8;
-  const int64_t total = M * per_row;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total; i += stride) {
-    const int64_t row = i / per_row;
-    const int k = static_cast<int>(i - row * per_row) * 8;
-    const uint2 u = *reinterpret_cast<const uint2*>(codes + row * K + k);
-    const float s = __ldg(scales + row * nrun + k / kCkptRun);
-    float v[8];
+  RowWalk at(blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x, stride, K / 8);
+  while (at.row < M) {
+    uint2 u[2];
+    float s[2];
+    int64_t row[2];
+    int k[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t w = e < 4 ? u.x : u.y;
-      v[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * (e & 3)))) * s;
+    for (int i = 0; i < 2; ++i) {
+      row[i] = at.row;
+      k[i] = at.col * 8;
+      if (row[i] < M) {
+        u[i] = __ldg(reinterpret_cast<const uint2*>(codes + row[i] * K + k[i]));
+        s[i] = __ldg(scales + row[i] * nrun + k[i] / kCkptRun);
+      }
+      at.next();
     }
-    *reinterpret_cast<uint4*>(out + row * ldo + k) = pack8(v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (row[i] >= M) break;
+      uint4 p;
+      i8_to_bf16(u[i].x, p.x, p.y);
+      i8_to_bf16(u[i].y, p.z, p.w);
+      float v[8];
+      unpack8(p, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= s[i];
+      *reinterpret_cast<uint4*>(out + row[i] * ldo + k[i]) = pack8(v);
+    }
   }
 }
 

@@ -56,43 +56,55 @@ int set_up(K kern, int threads, size_t most, size_t smem, KernelInfo& info, int*
   return DQ_OK;
 }
 
-template <int NPT, bool OPS>
+template <int NPT, bool OPS, bool FULL>
 int launch_forward_npt(NormArgs a, int64_t B, int sms, cudaStream_t st) {
   static KernelInfo info;
   const size_t per_feature = kNormAhead * 4 + (OPS ? 0 : 12);
   int per_sm = 1;
-  const int rc = set_up(gated_norm_kernel<NPT, OPS>, kNormThreads, per_feature * NPT * kNormThreads * 4,
+  const int rc = set_up(gated_norm_kernel<NPT, OPS, FULL>, kNormThreads, per_feature * NPT * kNormThreads * 4,
                         per_feature * a.D, info, &per_sm);
   if (rc != DQ_OK) return rc;
   a.chunks = chunks_of(B, a.S, static_cast<int64_t>(sms) * per_sm, 1);
-  gated_norm_kernel<NPT, OPS><<<static_cast<unsigned>(B * a.chunks), kNormThreads, per_feature * a.D, st>>>(a);
+  gated_norm_kernel<NPT, OPS, FULL><<<static_cast<unsigned>(B * a.chunks), kNormThreads, per_feature * a.D, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+}
+
+template <int NPT, bool OPS>
+int launch_forward_runs(const NormArgs& a, int64_t B, int sms, cudaStream_t st) {
+  return a.D == 4 * NPT * kNormThreads ? launch_forward_npt<NPT, OPS, true>(a, B, sms, st)
+                                       : launch_forward_npt<NPT, OPS, false>(a, B, sms, st);
 }
 
 template <bool OPS>
 int launch_forward(const NormArgs& a, int64_t B, int sms, cudaStream_t st) {
   switch ((a.D / 4 + kNormThreads - 1) / kNormThreads) {
-    case 1: return launch_forward_npt<1, OPS>(a, B, sms, st);
-    case 2: return launch_forward_npt<2, OPS>(a, B, sms, st);
-    case 3: return launch_forward_npt<3, OPS>(a, B, sms, st);
-    case 4: return launch_forward_npt<4, OPS>(a, B, sms, st);
+    case 1: return launch_forward_runs<1, OPS>(a, B, sms, st);
+    case 2: return launch_forward_runs<2, OPS>(a, B, sms, st);
+    case 3: return launch_forward_runs<3, OPS>(a, B, sms, st);
+    case 4: return launch_forward_runs<4, OPS>(a, B, sms, st);
     case 5:
-    case 6: return launch_forward_npt<6, OPS>(a, B, sms, st);
+    case 6: return launch_forward_runs<6, OPS>(a, B, sms, st);
   }
-  return launch_forward_npt<8, OPS>(a, B, sms, st);
+  return launch_forward_runs<8, OPS>(a, B, sms, st);
+}
+
+template <int THREADS, int NPT, bool FULL>
+int launch_backward_npt(const NormGradArgs& a, int64_t B, cudaStream_t st) {
+  static KernelInfo info;
+  constexpr size_t kPerFeature = kNormGradAhead * 8 + 8;
+  int per_sm = 1;
+  const int rc = set_up(gated_norm_backward_kernel<THREADS, NPT, FULL>, THREADS, kPerFeature * THREADS * NPT * 4,
+                        kPerFeature * a.D, info, &per_sm);
+  if (rc != DQ_OK) return rc;
+  gated_norm_backward_kernel<THREADS, NPT, FULL>
+      <<<static_cast<unsigned>(B * a.chunks), THREADS, kPerFeature * a.D, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 template <int THREADS, int NPT>
 int launch_backward(const NormGradArgs& a, int64_t B, cudaStream_t st) {
-  static KernelInfo info;
-  constexpr size_t kPerFeature = kNormGradAhead * 8 + 8;
-  int per_sm = 1;
-  const int rc = set_up(gated_norm_backward_kernel<THREADS, NPT>, THREADS, kPerFeature * THREADS * NPT * 4,
-                        kPerFeature * a.D, info, &per_sm);
-  if (rc != DQ_OK) return rc;
-  gated_norm_backward_kernel<THREADS, NPT>
-      <<<static_cast<unsigned>(B * a.chunks), THREADS, kPerFeature * a.D, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+  return a.D == 4 * NPT * THREADS ? launch_backward_npt<THREADS, NPT, true>(a, B, st)
+                                  : launch_backward_npt<THREADS, NPT, false>(a, B, st);
 }
 
 }  // namespace

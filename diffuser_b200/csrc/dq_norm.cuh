@@ -30,53 +30,12 @@
 #include <cuda_bf16.h>
 #include <cstdint>
 
+#include "dq_f32x2.cuh"
 #include "dq_ptx.cuh"
 
 namespace dq {
 
 enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
-
-// ------------------------------------------------------- packed float32 pairs
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
-__device__ __forceinline__ float2 unpair(F2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ float sum_pair(F2 a) {
-  const float2 u = unpair(a);
-  return u.x + u.y;
-}
-// bf16 pair -> float32 pair (exact), and back (RNE)
-__device__ __forceinline__ F2 widen(uint32_t w) { return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
-__device__ __forceinline__ uint32_t narrow(F2 a) {
-  const float2 u = unpair(a);
-  const __nv_bfloat162 b = __floats2bfloat162_rn(u.x, u.y);
-  return *reinterpret_cast<const uint32_t*>(&b);
-}
 
 // Thread-private 8-byte copy into shared memory.
 __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
@@ -93,35 +52,42 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   return v;
 }
 
-// Sum over the CTA's W warps, in the order of block_sum_256 (dq_dit.cuh); red:
-// W floats that no other reduction of this row or the next uses.
-template <int W>
+// Sum over the CTA's 8 warps, in the order of block_sum_256 (dq_dit.cuh); red:
+// 8 floats (16-byte aligned) that no other reduction of this row or the next uses.
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
+  const float4 a = *reinterpret_cast<const float4*>(red), b = *reinterpret_cast<const float4*>(red + 4);
   float t = 0.f;
-#pragma unroll
-  for (int i = 0; i < W; ++i) t += red[i];
+  t += a.x;
+  t += a.y;
+  t += a.z;
+  t += a.w;
+  t += b.x;
+  t += b.y;
+  t += b.z;
+  t += b.w;
   return t;
 }
+// Two sums at once over W warps; red: W pairs (16-byte aligned).
 template <int W>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* red) {
+__device__ __forceinline__ float2 row_sum2(F2 v, float2* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    const float2 u = unpair(v);
+    v = add2(v, f2(__shfl_xor_sync(0xffffffffu, u.x, o), __shfl_xor_sync(0xffffffffu, u.y, o)));
   }
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = unpair(v);
   __syncthreads();
-  float2 t = make_float2(0.f, 0.f);
+  F2 t = f2(0.f);
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    t.x += red[i].x;
-    t.y += red[i].y;
+  for (int i = 0; i < W / 2; ++i) {
+    const float4 u = *reinterpret_cast<const float4*>(red + 2 * i);
+    t = add2(t, add2(f2(u.x, u.y), f2(u.z, u.w)));
   }
-  return t;
+  return unpair(t);
 }
 
 struct NormArgs {
@@ -173,12 +139,14 @@ __device__ __forceinline__ F2 bf16_round2(F2 a) { return widen(narrow(a)); }
 // the sums in the order of adaln_modulate_kernel: the same bits.
 constexpr int kNormThreads = 256;
 constexpr int kNormAhead = 2;  // rows whose operands are on their way
-template <int NPT, bool OPS>
+// FULL: D is NPT runs for every thread.
+template <int NPT, bool OPS, bool FULL>
 __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_kernel(const NormArgs a) {
-  __shared__ float red[2][4][8];
+  __shared__ __align__(16) float red[2][4][8];
   extern __shared__ __align__(16) uint8_t smem[];
   const int nrun = a.D / 4;
-  const float dim = static_cast<float>(a.D);
+  const float dim = static_cast<float>(a.D), inv = 1.0f / dim;
+  auto mean_of = [&](float sum) { return OPS ? sum / dim : sum * inv; };
   const int64_t b = blockIdx.x / a.chunks;
   const int chunk = blockIdx.x - static_cast<int>(b) * a.chunks;
   const NormFactors f = {reinterpret_cast<const uint2*>(a.gate == nullptr ? nullptr : a.gate + b * a.ld_gate),
@@ -198,7 +166,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
         const int r = threadIdx.x + kNormThreads * j;
-        if (r < nrun) {
+        if (FULL || r < nrun) {
           cp_async_8(dst + 8u * kNormThreads * j, xr + r);
           cp_async_8(dst + row_bytes + 8u * kNormThreads * j, yr + r);
         }
@@ -212,7 +180,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {  // each thread reads back what it wrote
       const int r = threadIdx.x + kNormThreads * j;
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         fac[r] = f.behind(r);
         fac[nrun + r] = f.before(r);
         fac[2 * nrun + r] = f.shifts(r);
@@ -231,7 +199,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
       const int r = threadIdx.x + kNormThreads * j;
       cx[j] = make_uint2(0u, 0u);
       uint2 y = make_uint2(0u, 0u);
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         cx[j] = lds64(src + 8u * kNormThreads * j);
         y = lds64(src + row_bytes + 8u * kNormThreads * j);
       }
@@ -246,7 +214,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
         float sq = 0.f;
 #pragma unroll
         for (int j = 0; j < NPT; ++j)
-          if (threadIdx.x + kNormThreads * j < nrun) {
+          if (FULL || threadIdx.x + kNormThreads * j < nrun) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
               const float2 u = unpair(v[j][p]);
@@ -261,7 +229,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
         const F2 m = f2(-mean);
 #pragma unroll
         for (int j = 0; j < NPT; ++j)
-          if (threadIdx.x + kNormThreads * j < nrun) {
+          if (FULL || threadIdx.x + kNormThreads * j < nrun) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
               const F2 d = add2(v[j][p], m);
@@ -280,8 +248,8 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
 
     // the norm behind the block
     if (a.post != kNormNone) {
-      const float mean = a.post == kNormLayer ? row_sum<8>(sums(), red[par][0]) / dim : 0.f;
-      const float rstd = rsqrtf(row_sum<8>(squares(mean), red[par][1]) / dim + a.eps);
+      const float mean = a.post == kNormLayer ? mean_of(row_sum(sums(), red[par][0])) : 0.f;
+      const float rstd = rsqrtf(mean_of(row_sum(squares(mean), red[par][1])) + a.eps);
 #pragma unroll
       for (int j = 0; j < NPT; ++j)
 #pragma unroll
@@ -295,7 +263,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {
       const int r = threadIdx.x + kNormThreads * j;
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         uint2 u;
         if constexpr (OPS) {
           if (a.post_w != nullptr) {
@@ -326,13 +294,13 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
       }
     }
     // the norm before the next block
-    const float mean = a.pre == kNormLayer ? row_sum<8>(sums(), red[par][2]) / dim : 0.f;
-    const float rstd = rsqrtf(row_sum<8>(squares(mean), red[par][3]) / dim + a.eps);
+    const float mean = a.pre == kNormLayer ? mean_of(row_sum(sums(), red[par][2])) : 0.f;
+    const float rstd = rsqrtf(mean_of(row_sum(squares(mean), red[par][3])) + a.eps);
     uint2* ho = reinterpret_cast<uint2*>(a.h + t * a.ld_h);
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {
       const int r = threadIdx.x + kNormThreads * j;
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         F2 n0 = mul2(add2(v[j][0], f2(-mean)), f2(rstd)), n1 = mul2(add2(v[j][1], f2(-mean)), f2(rstd));
         if constexpr (OPS) {
           n0 = bf16_round2(n0);
@@ -375,11 +343,11 @@ struct NormGradArgs {
 
 // CTA (batch element, chunk): rows chunk, chunk + chunks, ... of the element.
 constexpr int kNormGradAhead = 2;
-template <int THREADS, int NPT>
+template <int THREADS, int NPT, bool FULL>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     gated_norm_backward_kernel(const NormGradArgs a) {
   constexpr int W = THREADS / 32;
-  __shared__ float2 red[2][4][W];
+  __shared__ __align__(16) float2 red[2][4][W];
   extern __shared__ __align__(16) uint8_t smem[];
   const int nrun = a.D / 4;
   const float inv = 1.0f / static_cast<float>(a.D);
@@ -396,12 +364,19 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
         const int r = threadIdx.x + THREADS * j;
-        if (r < nrun) {
+        if (FULL || r < nrun) {
           const uint32_t d = dst + 8u * THREADS * j;
           cp_async_8(d, reinterpret_cast<const uint2*>(a.s + t * a.ld_s) + r);
           cp_async_8(d + row_bytes, reinterpret_cast<const uint2*>(a.y + t * a.ld_y) + r);
           cp_async_8(d + 2 * row_bytes, reinterpret_cast<const uint2*>(a.dh + t * a.ld_dh) + r);
-          if (a.ds != nullptr) cp_async_8(d + 3 * row_bytes, reinterpret_cast<const uint2*>(a.ds + t * a.ld_ds) + r);
+        }
+      }
+      if (a.ds != nullptr) {
+#pragma unroll
+        for (int j = 0; j < NPT; ++j) {
+          const int r = threadIdx.x + THREADS * j;
+          if (FULL || r < nrun)
+            cp_async_8(dst + 3 * row_bytes + 8u * THREADS * j, reinterpret_cast<const uint2*>(a.ds + t * a.ld_ds) + r);
         }
       }
     }
@@ -416,9 +391,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {  // each thread reads back what it wrote
     const int r = threadIdx.x + THREADS * j;
-    if (r < nrun) {
+    if (FULL || r < nrun) {
       fac[r] = f.behind(r);
       fac[nrun + r] = f.before(r);
+      if (a.ds == nullptr)  // its slots stay zero
+        for (int i = 0; i < kNormGradAhead; ++i)
+          *reinterpret_cast<uint2*>(smem + (4 * i + 3) * row_bytes + 8 * r) = make_uint2(0u, 0u);
     }
   }
   F2 q0[NPT][2], q1[NPT][2], q2[NPT][2];
@@ -441,11 +419,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
       const uint32_t d = src + 8u * THREADS * j;
       us[j] = uy[j] = ud[j] = make_uint2(0u, 0u);
       uint2 u = make_uint2(0u, 0u);
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         us[j] = lds64(d);
         uy[j] = lds64(d + row_bytes);
         u = lds64(d + 2 * row_bytes);
-        if (a.ds != nullptr) ud[j] = lds64(d + 3 * row_bytes);
+        ud[j] = lds64(d + 3 * row_bytes);
       }
       dt[j][0] = widen(u.x);
       dt[j][1] = widen(u.y);
@@ -460,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
         ms = add2(ms, add2(widen(us[j].x), widen(us[j].y)));
         my = add2(my, add2(widen(uy[j].x), widen(uy[j].y)));
       }
-      const float2 sum = row_sum2<W>(make_float2(sum_pair(ms), sum_pair(my)), red[par][0]);
+      const float2 sum = row_sum2<W>(f2(sum_pair(ms), sum_pair(my)), red[par][0]);
       if (a.pre == kNormLayer) mean.x = sum.x * inv;
       if (a.post == kNormLayer) mean.y = sum.y * inv;
     }
@@ -469,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
       F2 ss = f2(0.f), sy = f2(0.f);
 #pragma unroll
       for (int j = 0; j < NPT; ++j)
-        if (threadIdx.x + THREADS * j < nrun) {
+        if (FULL || threadIdx.x + THREADS * j < nrun) {
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const F2 ds = add2(widen(p ? us[j].y : us[j].x), f2(-mean.x));
@@ -478,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
             sy = fma2(dy, dy, sy);
           }
         }
-      const float2 sq = row_sum2<W>(make_float2(sum_pair(ss), sum_pair(sy)), red[par][1]);
+      const float2 sq = row_sum2<W>(f2(sum_pair(ss), sum_pair(sy)), red[par][1]);
       rstd_s = rsqrtf(sq.x * inv + a.eps);
       if (a.post != kNormNone) rstd_y = rsqrtf(sq.y * inv + a.eps);
     }
@@ -489,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
         const int r = threadIdx.x + THREADS * j;
-        if (r < nrun) {
+        if (FULL || r < nrun) {
           const float4 m = fac[nrun + r];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
@@ -502,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
           }
         }
       }
-      d = row_sum2<W>(make_float2(sum_pair(d0), sum_pair(d1)), red[par][2]);
+      d = row_sum2<W>(f2(sum_pair(d0), sum_pair(d1)), red[par][2]);
       d.x = a.pre == kNormLayer ? d.x * inv : 0.f;
       d.y *= inv;
     }
@@ -514,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
         const int r = threadIdx.x + THREADS * j;
-        if (r < nrun) {
+        if (FULL || r < nrun) {
           const float4 n = fac[r];
           uint32_t o[2];
 #pragma unroll
@@ -534,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
       }
       g = make_float2(0.f, 0.f);
       if (a.post != kNormNone) {
-        g = row_sum2<W>(make_float2(sum_pair(g0), sum_pair(g1)), red[par][3]);
+        g = row_sum2<W>(f2(sum_pair(g0), sum_pair(g1)), red[par][3]);
         g.x = a.post == kNormLayer ? g.x * inv : 0.f;
         g.y *= inv;
       }
@@ -543,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
     for (int j = 0; j < NPT; ++j) {
       const int r = threadIdx.x + THREADS * j;
-      if (r < nrun) {
+      if (FULL || r < nrun) {
         uint32_t o[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -559,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
     const int r = threadIdx.x + THREADS * j;
-    if (r < nrun) {
+    if (FULL || r < nrun) {
       auto put = [&](int i, F2 (&q)[2]) {
         const float2 u = unpair(q[0]), w = unpair(q[1]);
         part[i * nrun + r] = make_float4(u.x, u.y, w.x, w.y);
@@ -597,11 +575,19 @@ __global__ void __launch_bounds__(32 * kReduceWarps) gated_norm_reduce_kernel(co
   float dpre = 0.f, dpost = 0.f;
   auto add = [&](int b, int first, int step, float* q) {
     if (!in) return;
-#pragma unroll 8
-    for (int c = first; c < a.chunks; c += step) {
-      const float* p = a.part + (static_cast<int64_t>(b) * a.chunks + c) * 3 * a.D + col;
+    for (int c0 = first; c0 < a.chunks; c0 += 8 * step) {
+      float u[8][3];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) q[i] += p[static_cast<int64_t>(i) * a.D];
+      for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k * step;
+        const float* p = a.part + (static_cast<int64_t>(b) * a.chunks + c) * 3 * a.D + col;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) u[k][i] = c < a.chunks ? __ldcg(p + static_cast<int64_t>(i) * a.D) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) q[i] += u[k][i];
     }
   };
   auto finish = [&](int b, const float* s) {
