@@ -496,7 +496,7 @@ int dq_checkpoint_pack(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t*
   if (rc != DQ_OK) return rc;
   const int nrun = static_cast<int>(ceil_div(K, kCkptRun));
   const int64_t runs = M * nrun;
-  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(runs, 16), static_cast<int64_t>(sms) * 5));  // resident CTAs
+  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(runs, 32), static_cast<int64_t>(sms) * 6));  // resident CTAs
   checkpoint_pack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const __nv_bfloat16*>(x), ldx, M, nrun, static_cast<int>(K), codes, scales);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
