@@ -113,6 +113,9 @@ def heads_to_tokens(x, s_txt: int, img_out=None):
 # AdaLN modulation and gated residuals as one kernel each (False: the
 # reference's chain of tensor ops).
 FUSED_ADALN = True
+# The residual behind a block and the norm before the next one as one kernel,
+# with the roundings (and so the bits) of the two (False: the two).
+FUSED_BOUNDARY = True
 # q/k/v projections through one concatenated NF4 linear where fuse_qkv_projections
 # built it (False: three linears, as the reference calls them).
 FUSED_QKV = True
@@ -243,7 +246,13 @@ def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_w
     latter may be None.  post: None, "rms" or "layer"; pre: "rms" or "layer".
     rounding="once" computes in float32 and rounds s and h; "ops" rounds after
     every op as the chain of tensor ops does (the bits of gated_residual
-    followed by adaln_modulate).  Returns (s, h)."""
+    followed by adaln_modulate).  Returns (s, h), differentiable in every
+    tensor where gradients are enabled (with the gradients of the formula,
+    whatever the rounding)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, y, gate, scale, shift, post_weight, pre_weight)):
+        return _GatedNorm.apply(x, y, gate, scale, shift, post_weight, pre_weight, post, pre, residual_scale, eps,
+                                rounding)
     gate, ldg, scale, shift, ldm, pw, qw = _norm_args(x, gate, scale, shift, post, pre, post_weight, pre_weight)
     if rounding not in _ROUNDINGS:
         raise ValueError("rounding must be 'once' or 'ops'")
@@ -300,6 +309,30 @@ def gated_norm_backward(ds, dh, s, y, gate=None, *, post=None, pre="rms", post_w
     return out
 
 
+class _GatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, shift, post_weight, pre_weight, post, pre, residual_scale, eps, rounding):
+        with torch.no_grad():
+            s, h = gated_norm(x, y, gate, post=post, pre=pre, post_weight=post_weight, pre_weight=pre_weight,
+                              scale=scale, shift=shift, residual_scale=residual_scale, eps=eps, rounding=rounding)
+        ctx.save_for_backward(s, y, gate, scale, shift, post_weight, pre_weight)
+        ctx.args = dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps)
+        ctx.set_materialize_grads(False)
+        return s, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, ds, dh):
+        s, y, gate, scale, shift, pw, qw = ctx.saved_tensors
+        if dh is None:  # only s was used
+            dh = torch.zeros_like(s)
+        g = gated_norm_backward(ds, dh, s, y, gate, post_weight=pw, pre_weight=qw, scale=scale, shift=shift,
+                                **ctx.args)
+        low = lambda t: None if t is None else t.to(torch.bfloat16)  # noqa: E731
+        return (g["dx"], g["dy"], low(g["dgate"]), low(g["dscale"]), low(g["dshift"]), low(g["dpost_weight"]),
+                low(g["dpre_weight"]), None, None, None, None, None)
+
+
 def _adaln_ok(x):
     return FUSED_ADALN and x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.shape[-1] % 4 == 0
 
@@ -316,6 +349,26 @@ def _gated_add(x, gate, y):
     return x + gate[:, None] * y
 
 
+def _add_and_modulate(x, gate, y, norm, scale, shift):
+    """(x + gate * y, norm(that) * (1 + scale) + shift)."""
+    if FUSED_BOUNDARY and _adaln_ok(x) and y.shape == x.shape and norm.weight is None and norm.bias is None and \
+            x.shape[-1] <= 8192:
+        return gated_norm(x, y, gate, pre="layer", scale=scale, shift=shift, eps=norm.eps, rounding="ops")
+    s = _gated_add(x, gate, y)
+    return s, _modulate(norm, s, scale, shift)
+
+
+# The linears that take an activation and an output view.
+_ENGINE_LINEARS = (modules.Ltx23Nf4Linear, modules.Ltx23Fp8Linear, modules.AdapterLinear)
+
+
+def _differentiable(x, proj):
+    """Whether an adapted linear's call is recorded for a backward pass (it
+    then writes no caller-given output)."""
+    return isinstance(proj, modules.AdapterLinear) and torch.is_grad_enabled() and \
+        (x.requires_grad or proj.down.requires_grad)
+
+
 # GELU-tanh after the up-projections runs in the quantized linear's epilogue
 # (False: a separate activation pass, as the reference does).
 FUSED_GELU = True
@@ -325,7 +378,7 @@ def _proj_gelu_tanh(proj, x, out=None):
     """GELU-tanh of a projection; fused into the quantized linear's epilogue on
     the engine (the projection is still rounded to bf16 before the activation).
     With `out` the result is written there."""
-    if FUSED_GELU and isinstance(proj, (modules.Ltx23Nf4Linear, modules.Ltx23Fp8Linear)) and x.is_cuda:
+    if FUSED_GELU and isinstance(proj, _ENGINE_LINEARS) and x.is_cuda:
         if out is None:  # forwards that predate `out` keep working
             return proj(x, act="gelu_tanh")
         return proj(x, act="gelu_tanh", out=out)
@@ -601,11 +654,10 @@ class DoubleBlock(nn.Module):
         nx, g_msa, sh_mlp, sc_mlp, g_mlp = self.norm1(x, temb)
         nc, cg_msa, csh_mlp, csc_mlp, cg_mlp = self.norm1_context(ctx, temb)
         a_img, a_txt = self.attn(nx, nc, rope)
-        x = _gated_add(x, g_msa, a_img)
-        x = _gated_add(x, g_mlp, self.ff(_modulate(self.norm2, x, sc_mlp, sh_mlp)))
-        ctx = _gated_add(ctx, cg_msa, a_txt)
-        ctx = _gated_add(ctx, cg_mlp, self.ff_context(
-            _modulate(self.norm2_context, ctx, csc_mlp, csh_mlp)))
+        x, h = _add_and_modulate(x, g_msa, a_img, self.norm2, sc_mlp, sh_mlp)
+        x = _gated_add(x, g_mlp, self.ff(h))
+        ctx, h = _add_and_modulate(ctx, cg_msa, a_txt, self.norm2_context, csc_mlp, csh_mlp)
+        ctx = _gated_add(ctx, cg_mlp, self.ff_context(h))
         if ctx.dtype == torch.float16:
             ctx = ctx.clamp(-65504, 65504)
         return ctx, x
@@ -625,7 +677,7 @@ class SingleBlock(nn.Module):
     def forward(self, x, temb, rope):
         n, gate = self.norm(x, temb)
         if FUSED_CONCAT and _fused_ok(n, self.attn.norm_q.weight.shape[0]) and \
-                isinstance(self.proj_mlp, (modules.Ltx23Nf4Linear, modules.Ltx23Fp8Linear)):
+                isinstance(self.proj_mlp, _ENGINE_LINEARS) and not _differentiable(n, self.proj_mlp):
             # attention and MLP outputs land in the two column ranges of the
             # proj_out input, which is then read whole (no concatenation pass)
             d_attn = self.attn.to_q.out_features

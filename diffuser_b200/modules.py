@@ -142,13 +142,16 @@ class Ltx23Fp8Linear(nn.Module):
     def forward(self, x: torch.Tensor, act: str | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
         act = act or self.gated_act
+        return ops.fp8_linear(x, self._weight_on(x.device), self._scale_f, self.bias, act=act, out=out)
+
+    def _weight_on(self, device: torch.device) -> torch.Tensor:
         if self.weight_fp8 is None:
             raise RuntimeError("set_fp8_weight() has not been called")
         w8 = self._resident
-        if w8 is None or w8.device != x.device:
-            w8 = self.weight_fp8.to(device=x.device, non_blocking=True)
+        if w8 is None or w8.device != device:
+            w8 = self.weight_fp8.to(device=device, non_blocking=True)
             self._resident = w8
-        return ops.fp8_linear(x, w8, self._scale_f, self.bias, act=act, out=out)
+        return w8
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, format=fp8"
@@ -214,6 +217,206 @@ class Flux2FeedForward(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.linear_out(self.linear_in(x))
+
+
+# ------------------------------------------------------------------ adapters
+class AdapterSelection:
+    """Which adapter each batch element uses: ids, int32 on the GPU, one per
+    element (-1: none).  Every adapted linear of a model shares it; the plan for
+    a token count is built at its first use (an element's tokens follow one
+    another, equally many for each)."""
+
+    def __init__(self, ids: torch.Tensor, n_adapters: int):
+        if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or \
+                ids.numel() == 0:
+            raise ValueError("ids must be a 1-d int32 CUDA tensor, one entry per batch element")
+        self.ids = ids.contiguous()
+        self.n_adapters = int(n_adapters)
+        self._plans: dict = {}
+
+    def plan(self, tokens: int) -> ops.AdapterPlan:
+        plan = self._plans.get(tokens)
+        if plan is None:
+            batch = self.ids.numel()
+            if tokens % batch != 0:
+                raise ValueError(f"{tokens} tokens are not a whole number per element of a batch of {batch}")
+            offsets = torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
+            plan = self._plans[tokens] = ops.adapter_plan(self.ids, offsets, tokens, self.n_adapters)
+        return plan
+
+    def update_(self, ids: torch.Tensor) -> "AdapterSelection":
+        """Other adapters for the same batch size: the plans built so far are
+        rebuilt in place (captured graphs that read them see the new ones)."""
+        self.ids.copy_(ids)
+        batch = self.ids.numel()
+        for tokens, plan in self._plans.items():
+            offsets = torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
+            plan.update_(self.ids, offsets)
+        return self
+
+
+class _AdaptedProjection(torch.autograd.Function):
+    """base(x) + adapters, with the base frozen: gradients of x, down and up."""
+
+    @staticmethod
+    def forward(ctx, x, down, up, scale, plan, base, pack):
+        y = base.project(x)
+        y, hidden = ops.adapter_add(y, x, down, up, scale, plan, out=y, return_hidden=True)
+        if pack:
+            packed = ops.checkpoint_pack(x)
+            ctx.save_for_backward(hidden, down, up, scale, packed.codes, packed.scales)
+        else:
+            ctx.save_for_backward(hidden, down, up, scale, x)
+        ctx.plan, ctx.base, ctx.pack = plan, base, pack
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        hidden, down, up, scale, *x = ctx.saved_tensors
+        x = ops.PackedActivation(*x) if ctx.pack else x[0]
+        dx = ctx.base.input_grad(dy) if ctx.needs_input_grad[0] else None
+        dx, ddown, dup = ops.adapter_backward(dy, x, hidden, down, up, scale, ctx.plan, dx=dx, out=dx)
+        return dx if ctx.needs_input_grad[0] else None, ddown, dup, None, None, None, None
+
+
+class AdapterLinear(nn.Module):
+    """A quantized linear with a bank of low-rank adapters beside it: every
+    batch element's tokens pass the shared weight and its own adapter,
+    y + scale_a * (x . down_a^T) . up_a.
+
+    The bank's factors are parameters (bf16, ``down`` [A, r, K], ``up``
+    [A, r, N]); the base is frozen.  Set ``selection`` (AdapterSelection), or
+    pass a plan, before calling; without either the base runs alone.  With
+    gradients enabled the call is differentiable in x and the factors, and
+    keeps its input for the backward pass as it is or, with
+    ``pack_activations``, in 8 bits."""
+
+    def __init__(self, base: nn.Module, n_adapters: int, rank: int, pack_activations: bool = False):
+        super().__init__()
+        if not isinstance(base, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
+            raise TypeError("AdapterLinear wraps a quantized linear")
+        rank = -(-int(rank) // 8) * 8  # the kernels take multiples of 8; the rest stays zero
+        if not 8 <= rank <= 128 or base.out_features % 8 != 0 or base.in_features % 8 != 0:
+            raise ValueError("adapters need a rank of 1..128 and features that are multiples of 8")
+        if pack_activations and base.in_features % 16 != 0:
+            raise ValueError("8-bit activations need in_features % 16 == 0")
+        self.base = base
+        self.in_features, self.out_features = base.in_features, base.out_features
+        self.pack_activations = bool(pack_activations)
+        dev = base.weight_nf4.device if isinstance(base, Ltx23Nf4Linear) else \
+            (base.weight_fp8.device if base.weight_fp8 is not None else None)
+        zeros = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=dev)  # noqa: E731
+        self.down = nn.Parameter(zeros(n_adapters, rank, base.in_features))
+        self.up = nn.Parameter(zeros(n_adapters, rank, base.out_features))
+        self.register_buffer("scale", torch.ones(n_adapters, dtype=torch.float32, device=dev))
+        self.selection: AdapterSelection | None = None
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.scale.dtype != torch.float32:
+            self.scale = self.scale.float()
+        return self
+
+    def set_adapter(self, index: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0):
+        """Install adapter `index` from its two factors as checkpoints store
+        them, a [r, in_features] and b [out_features, r] (r up to the bank's
+        rank), with the factor scale (alpha / r).  For a gated base b is in the
+        [gate; up] row order."""
+        r = a.shape[0]
+        if a.shape != (r, self.in_features) or b.shape != (self.out_features, r) or r > self.down.shape[1]:
+            raise ValueError(f"expected [r, {self.in_features}] and [{self.out_features}, r] with r <= "
+                             f"{self.down.shape[1]}, got {tuple(a.shape)} and {tuple(b.shape)}")
+        if not 0 <= index < self.down.shape[0]:
+            raise IndexError(f"adapter {index} of {self.down.shape[0]}")
+        with torch.no_grad():
+            u = b.t()
+            if self.base.gated_act is not None:
+                u = u.index_select(1, ops.gated_row_order(self.out_features, b.device))
+            self.down[index].zero_()[:r].copy_(a)
+            self.up[index].zero_()[:r].copy_(u)
+            self.scale[index] = float(scale)
+        return self
+
+    @property
+    def bias(self):
+        return self.base.bias
+
+    def project(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The base's projection alone, without an activation."""
+        b = self.base
+        if isinstance(b, Ltx23Nf4Linear):
+            return ops.nf4_linear(x, b.weight_nf4, b.weight_absmax, b.out_features, b.bias, out=out)
+        return ops.fp8_linear(x, b._weight_on(x.device), b._scale_f, b.bias, out=out)
+
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        b = self.base
+        if isinstance(b, Ltx23Nf4Linear):
+            return ops.nf4_linear_dgrad(dy, b.weight_nf4, b.weight_absmax, b.in_features)
+        return ops.fp8_linear_dgrad(dy, b._weight_on(dy.device), b._scale_f)
+
+    def forward(self, x: torch.Tensor, act: str | None = None, out: torch.Tensor | None = None,
+                plan: ops.AdapterPlan | None = None) -> torch.Tensor:
+        if plan is None:
+            if self.selection is None:
+                return self.base(x, act=act, out=out)
+            plan = self.selection.plan(x.numel() // self.in_features)
+        act = act or self.base.gated_act
+        if torch.is_grad_enabled() and (x.requires_grad or self.down.requires_grad or self.up.requires_grad):
+            if out is not None or act in ops.GATED_ACTS:
+                raise RuntimeError("a differentiable call takes neither out nor a gated activation")
+            y = _AdaptedProjection.apply(x, self.down, self.up, self.scale, plan, self, self.pack_activations)
+            return y if act is None else nn.functional.gelu(y, approximate="tanh")
+        down, up = self.down.detach(), self.up.detach()
+        if act is None:
+            y = self.project(x, out=out)
+            return ops.adapter_add(y, x, down, up, self.scale, plan, out=y)
+        return ops.adapter_add(self.project(x), x, down, up, self.scale, plan, act=act, out=out)
+
+    def extra_repr(self) -> str:
+        return f"adapters={self.down.shape[0]}, rank={self.down.shape[1]}"
+
+
+def attach_adapters(model: nn.Module, n_adapters: int, rank: int, is_adapted_key=None,
+                    pack_activations: bool = False) -> list[str]:
+    """Wrap the model's quantized linears (those whose ``<name>.weight`` key
+    is_adapted_key accepts; all of them without it) in AdapterLinear.  Linears
+    that flux.fuse_qkv_projections concatenated are dropped where one of their
+    parts is wrapped.  Returns the wrapped names."""
+    wrapped = []
+    for name, mod in list(model.named_modules()):
+        if not isinstance(mod, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
+            continue
+        segs = name.split(".")
+        if segs[-1] in ("to_qkv", "add_qkv") or (is_adapted_key is not None and not is_adapted_key(name + ".weight")):
+            continue
+        parent = _walk(model, segs[:-1]) if len(segs) > 1 else model
+        wrap = AdapterLinear(mod, n_adapters, rank, pack_activations)
+        if segs[-1].isdigit():
+            parent[int(segs[-1])] = wrap
+        else:
+            setattr(parent, segs[-1], wrap)
+        for fused, parts in (("to_qkv", ("to_q", "to_k", "to_v")),
+                             ("add_qkv", ("add_q_proj", "add_k_proj", "add_v_proj"))):
+            if segs[-1] in parts and getattr(parent, fused, None) is not None:
+                delattr(parent, fused)
+        wrapped.append(name)
+    return wrapped
+
+
+def select_adapters(model: nn.Module, ids: torch.Tensor | None) -> AdapterSelection | None:
+    """Give every adapted linear of `model` the adapters of the next batch: ids
+    int32 on the GPU, one per batch element (-1: none); None takes them off."""
+    layers = [m for m in model.modules() if isinstance(m, AdapterLinear)]
+    if not layers:
+        raise ValueError("the model has no adapted linears")
+    counts = {m.down.shape[0] for m in layers}
+    if len(counts) != 1:
+        raise ValueError(f"the model's banks hold different numbers of adapters: {sorted(counts)}")
+    selection = None if ids is None else AdapterSelection(ids, counts.pop())
+    for m in layers:
+        m.selection = selection
+    return selection
 
 
 # Reference-spelled aliases, so callers read like the R API.
