@@ -34,7 +34,9 @@ bool norms_ok(int post, int pre, const void* post_w) {
 int chunks_of(int64_t B, int S, int64_t slots, int least) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(1, B), ceil_div(S, least))));
 }
-int64_t backward_slots(int D, int sms) { return static_cast<int64_t>(sms) * (D <= 4096 ? 2 : 1); }
+int64_t backward_slots(int D, int sms) {
+  return static_cast<int64_t>(sms) * (D <= 2048 ? norm_grad_ctas(128, 4) : D <= 4096 ? norm_grad_ctas(128, 8) : 1);
+}
 
 // Shared-memory opt-in of a kernel and its resident CTAs per SM, once per
 // kernel and device.
@@ -105,6 +107,21 @@ template <int THREADS, int NPT>
 int launch_backward(const NormGradArgs& a, int64_t B, cudaStream_t st) {
   return a.D == 4 * NPT * THREADS ? launch_backward_npt<THREADS, NPT, true>(a, B, st)
                                   : launch_backward_npt<THREADS, NPT, false>(a, B, st);
+}
+
+// The reduction may start while the last rows are on their way out; it waits
+// for them (griddepcontrol.wait) before it reads the sums.
+int launch_reduce(const NormReduceArgs& q, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(q.D, 32)));
+  cfg.blockDim = dim3(32 * kReduceWarps);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, gated_norm_reduce_kernel, q) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -183,17 +200,17 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
                     ld_ds, ld_dh, ld_s, ld_y, ld_gate, ld_mod, ld_dx, ld_dy, S, D, post, pre,
                     chunks, residual_scale, eps};
   const int runs = D / 4;
-  rc = runs <= 256    ? launch_backward<256, 1>(a, B, st)
-       : runs <= 512  ? launch_backward<256, 2>(a, B, st)
-       : runs <= 768  ? launch_backward<256, 3>(a, B, st)
-       : runs <= 1024 ? launch_backward<256, 4>(a, B, st)
-                      : launch_backward<512, 4>(a, B, st);
+  rc = runs <= 256    ? launch_backward<128, 2>(a, B, st)
+       : runs <= 512  ? launch_backward<128, 4>(a, B, st)
+       : runs <= 768  ? launch_backward<128, 6>(a, B, st)
+       : runs <= 1024 ? launch_backward<128, 8>(a, B, st)
+                      : launch_backward<256, 8>(a, B, st);
   if (rc != DQ_OK) return rc;
   NormReduceArgs q = {a.part, a.gate, a.scale, a.post_w, a.pre_w, dgate, dscale, dshift, dpost_weight, dpre_weight,
                       ld_gate, ld_mod, static_cast<int>(B), chunks, D, residual_scale};
   if (dgate != nullptr || dscale != nullptr || dshift != nullptr || dpost_weight != nullptr || dpre_weight != nullptr)
-    gated_norm_reduce_kernel<<<static_cast<unsigned>(ceil_div(D, 32)), 32 * kReduceWarps, 0, st>>>(q);
-  return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+    return launch_reduce(q, st);
+  return DQ_OK;
 }
 
 }  // extern "C"

@@ -342,9 +342,13 @@ struct NormGradArgs {
 };
 
 // CTA (batch element, chunk): rows chunk, chunk + chunks, ... of the element.
+// Few threads with many features each: a row's reductions and addresses cost
+// every warp the same whatever it owns (4608 x 4096: 63 us with 16 warps per
+// row, 49 with 8, 46 with 4).
 constexpr int kNormGradAhead = 2;
+__host__ __device__ constexpr int norm_grad_ctas(int threads, int npt) { return threads > 128 ? 1 : npt <= 4 ? 4 : 2; }
 template <int THREADS, int NPT, bool FULL>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
+__global__ void __launch_bounds__(THREADS, norm_grad_ctas(THREADS, NPT))
     gated_norm_backward_kernel(const NormGradArgs a) {
   constexpr int W = THREADS / 32;
   __shared__ __align__(16) float2 red[2][4][W];
@@ -533,6 +537,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     }
   }
   copies_wait<0>();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   float4* part = reinterpret_cast<float4*>(a.part + static_cast<int64_t>(blockIdx.x) * 3 * a.D);
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
@@ -573,6 +578,7 @@ __global__ void __launch_bounds__(32 * kReduceWarps) gated_norm_reduce_kernel(co
   const float wq = in && a.pre_w != nullptr ? __bfloat162float(a.pre_w[col]) : 1.0f;
   const float wp = in && a.post_w != nullptr ? __bfloat162float(a.post_w[col]) : 1.0f;
   float dpre = 0.f, dpost = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the chunks' sums
   auto add = [&](int b, int first, int step, float* q) {
     if (!in) return;
     for (int c0 = first; c0 < a.chunks; c0 += 8 * step) {
