@@ -76,40 +76,37 @@ DownPlan down_plan(int64_t M, int64_t R, int A, int64_t F, const int* clusters) 
 
 // Row splits of the weight-gradient kernel: the count (up to 16) that leaves
 // the smallest share of the resident CTA slots idle in its last wave, for
-// splits of at least 256 rows.
+// splits of at least 256 rows.  col_tiles: of all problems of the launch.
 struct WgradPlan {
-  int col_tiles, splits, rows_per_split;
+  int splits, rows_per_split;
 };
-WgradPlan wgrad_plan(int64_t M, int64_t R, int A, int64_t cols, int rc, bool i8, int sms) {
+WgradPlan wgrad_plan(int64_t M, int64_t R, int A, int64_t col_tiles, int rc, bool i8, int sms) {
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
   const int slots = sms * (rc <= 64 || !i8 ? 2 : 1);  // WgradCfg::kMinCtas
-  WgradPlan p;
-  p.col_tiles = static_cast<int>(ceil_div(cols, 128));
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, M / 256));
   double best = 0;
   int splits = 1;
   for (int64_t s = 1; s <= most; ++s) {
-    const int64_t ctas = p.col_tiles * s;
+    const int64_t ctas = col_tiles * s;
     const double fill = static_cast<double>(ctas) / static_cast<double>(ceil_div(ctas, slots) * slots);
     if (fill > best + 0.02) {
       best = fill;
       splits = static_cast<int>(s);
     }
   }
+  WgradPlan p;
   p.rows_per_split = static_cast<int>(ceil_div(ceil_div(lay.cap, splits), 64) * 64);
   p.splits = static_cast<int>(ceil_div(lay.cap, p.rows_per_split));
   return p;
 }
-size_t wgrad_bytes(const WgradPlan& p, int64_t cols, int r) {
-  return up256(static_cast<size_t>(2) * p.splits * r * cols * 4);
-}
+int64_t col_tiles(int64_t cols) { return ceil_div(cols, 128); }
 
 // after: programmatic stream serialization -- the kernel may start while the
 // one before it drains, and waits (griddepcontrol.wait) before it reads that
 // one's results.  cluster: CTAs of a cluster along (x, y).
-template <typename Args, typename... More>
-int launch(void (*kern)(Args, More...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool after,
-           dim3 cluster, Args args, More... more) {
+template <typename Args>
+int launch(void (*kern)(Args), dim3 grid, int threads, size_t smem, cudaStream_t st, bool after, dim3 cluster,
+           Args args) {
   cudaLaunchAttribute attr[2];
   int n = 0;
   if (after) {
@@ -129,7 +126,7 @@ int launch(void (*kern)(Args, More...), dim3 grid, int threads, size_t smem, cud
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kern, args, more...) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, args) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 // Shared-memory opt-in of a kernel, once per device.
@@ -231,17 +228,13 @@ int launch_small(SmallArgs a, int64_t M, int64_t R_, int sms, cudaStream_t st) {
 }
 
 template <int R, bool I8>
-int launch_wgrad(const WgradArgs& a, const WgradPlan& p, cudaStream_t st) {
+int launch_wgrad(const WgradArgs& a, int splits, cudaStream_t st) {
   using C = WgradCfg<R, I8>;
   static std::atomic<int> set[kMaxDevices];
-  int rc = allow_smem(adapter_wgrad_kernel<R, I8>, C::kSmemBytes, set);
+  const int rc = allow_smem(adapter_wgrad_kernel<R, I8>, C::kSmemBytes, set);
   if (rc != DQ_OK) return rc;
-  rc = launch(adapter_wgrad_kernel<R, I8>, dim3(p.col_tiles, p.splits), C::kThreads, C::kSmemBytes, st, true, dim3(1), a);
-  if (rc != DQ_OK) return rc;
-  const int64_t elems = static_cast<int64_t>(a.rank) * a.cols;
-  const unsigned bx = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 1024), 512));
-  return launch(adapter_wgrad_reduce_kernel, dim3(bx, a.A), 256, 0, st, true, dim3(1), a.words, a.lay,
-                a.rows_per_split, static_cast<const float*>(a.part), a.dbank, elems);
+  return launch(adapter_wgrad_kernel<R, I8>, dim3(a.first.col_tiles + a.second.col_tiles, splits), C::kThreads,
+                C::kSmemBytes, st, true, dim3(1), a);
 }
 
 // Calls f.template operator()<R>() for the rank class.
@@ -255,47 +248,27 @@ int by_rank(int r, F&& f) {
   return f(std::integral_constant<int, 128>());
 }
 
-int wgrad(const void* x, int64_t ldx, const float* x_scales, const void* g, const float* g32, int64_t M, int64_t R, int64_t cols,
-          int r, int A, const int32_t* words, const AdapterPlan& lay, void* ws, void* dbank, int sms,
-          cudaStream_t st) {
-  const bool i8 = x_scales != nullptr;
-  const WgradPlan p = wgrad_plan(M, R, A, cols, rank_class(r), i8, sms);
-  WgradArgs a = {};
-  a.x = x;
-  a.x_scales = x_scales;
-  a.g = static_cast<const __nv_bfloat16*>(g);
-  a.g32 = g32;
-  int e = error_word(&a.error);
-  if (e != DQ_OK) return e;
-  a.words = words;
-  a.part = static_cast<float*>(ws);
-  a.dbank = static_cast<__nv_bfloat16*>(dbank);
-  a.lay = lay;
-  a.ldx = ldx;
-  a.cols = static_cast<int>(cols);
-  a.rank = r;
-  a.A = A;
-  a.rows_per_split = p.rows_per_split;
-  return by_rank(r, [&](auto rc) {
-    constexpr int R_ = decltype(rc)::value;
-    return i8 ? launch_wgrad<R_, true>(a, p, st) : launch_wgrad<R_, false>(a, p, st);
-  });
-}
-
 // Workspace of the backward pass: g [M, r] in bf16 and in f32, and one region
 // for each weight gradient's partial sums.
 struct BackwardWs {
-  size_t g, g32, up, down, total;
+  WgradPlan up, down;  // splits of dup and of ddown
+  size_t g, g32, up_bytes, down_bytes, total;
 };
-BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A, int sms) {
+BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A, bool i8, int sms) {
   BackwardWs w;
   const int rc = rank_class(r);
+  if (i8) {  // a launch each
+    w.up = wgrad_plan(M, R, A, col_tiles(N), rc, false, sms);
+    w.down = wgrad_plan(M, R, A, col_tiles(K), rc, true, sms);
+  } else {  // one launch
+    w.up = w.down = wgrad_plan(M, R, A, col_tiles(N) + col_tiles(K), rc, false, sms);
+  }
+  auto part = [&](const WgradPlan& p, int64_t cols) { return up256(static_cast<size_t>(2) * p.splits * r * cols * 4); };
   w.g = up256(static_cast<size_t>(M) * r * 2);
-  w.up = wgrad_bytes(wgrad_plan(M, R, A, N, rc, false, sms), N, r);
-  w.down = std::max(wgrad_bytes(wgrad_plan(M, R, A, K, rc, false, sms), K, r),
-                    wgrad_bytes(wgrad_plan(M, R, A, K, rc, true, sms), K, r));
-  w.g32 = up256(static_cast<size_t>(M) * r * 4);
-  w.total = w.g + w.g32 + w.up + w.down;
+  w.g32 = i8 ? up256(static_cast<size_t>(M) * r * 4) : 0;
+  w.up_bytes = part(w.up, N);
+  w.down_bytes = part(w.down, K);
+  w.total = w.g + w.g32 + w.up_bytes + w.down_bytes;
   return w;
 }
 
@@ -436,7 +409,7 @@ int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64
 size_t dq_adapter_backward_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
   int sms = 0;
   if (bank_shape(M, R, K, N, r, A) != DQ_OK || device_sms(&sms) != DQ_OK) return 0;
-  return backward_ws(M, R, K, N, r, A, sms).total;
+  return std::max(backward_ws(M, R, K, N, r, A, false, sms).total, backward_ws(M, R, K, N, r, A, true, sms).total);
 }
 
 int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* x_scales,
@@ -470,19 +443,57 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
     return DQ_ERR_ALIGN;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
-  const BackwardWs w = backward_ws(M, R, K, N, r, A, sms);
+  const BackwardWs w = backward_ws(M, R, K, N, r, A, i8, sms);
   if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < w.total) return DQ_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int32_t* words = static_cast<const int32_t*>(plan);
-  const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  float* g32 = reinterpret_cast<float*>(ws + w.g);
-  uint8_t* parts = ws + w.g + w.g32;
+  float* g32 = i8 ? reinterpret_cast<float*>(ws + w.g) : nullptr;
   rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo, ws, want_w,
-               want_w && i8 ? g32 : nullptr, sms, st);
+               want_w ? g32 : nullptr, sms, st);
   if (rc != DQ_OK || !want_w) return rc;
-  rc = wgrad(dy, lddy, nullptr, hidden, nullptr, M, R, N, r, A, words, lay, parts, dup, sms, st);
+
+  WgradArgs a = {};
+  if ((rc = error_word(&a.error)) != DQ_OK) return rc;
+  a.words = words;
+  a.lay = adapter_plan_layout(M, R, A);
+  a.rank = r;
+  a.A = A;
+  WgradProblem pu = {}, pd = {};
+  pu.x = dy;
+  pu.ldx = lddy;
+  pu.g = static_cast<const __nv_bfloat16*>(hidden);
+  pu.part = reinterpret_cast<float*>(ws + w.g + w.g32);
+  pu.dbank = static_cast<__nv_bfloat16*>(dup);
+  pu.cols = static_cast<int>(N);
+  pu.col_tiles = static_cast<int>(col_tiles(N));
+  pu.rows_per_split = w.up.rows_per_split;
+  pd.x = x;
+  pd.ldx = ldx;
+  pd.x_scales = x_scales;
+  pd.g = reinterpret_cast<const __nv_bfloat16*>(ws);
+  pd.g32 = g32;
+  pd.part = reinterpret_cast<float*>(ws + w.g + w.g32 + w.up_bytes);
+  pd.dbank = static_cast<__nv_bfloat16*>(ddown);
+  pd.cols = static_cast<int>(K);
+  pd.col_tiles = static_cast<int>(col_tiles(K));
+  pd.rows_per_split = w.down.rows_per_split;
+  rc = by_rank(r, [&](auto rank) {
+    constexpr int R_ = decltype(rank)::value;
+    a.first = pu;
+    if (!i8) {
+      a.second = pd;
+      return launch_wgrad<R_, false>(a, w.up.splits, st);
+    }
+    const int e = launch_wgrad<R_, false>(a, w.up.splits, st);
+    a.first = pd;
+    return e != DQ_OK ? e : launch_wgrad<R_, true>(a, w.down.splits, st);
+  });
   if (rc != DQ_OK) return rc;
-  return wgrad(x, ldx, x_scales, ws, g32, M, R, K, r, A, words, lay, parts + w.up, ddown, sms, st);
+  a.first = pu;
+  a.second = pd;
+  const int64_t elems = static_cast<int64_t>(r) * std::max(K, N);
+  const unsigned bx = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 1024), 512));
+  return launch(adapter_wgrad_reduce_kernel, dim3(bx, A, 2), 256, 0, st, true, dim3(1), a);
 }
 
 int dq_checkpoint_pack(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* codes, float* scales,

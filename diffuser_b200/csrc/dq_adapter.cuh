@@ -1030,18 +1030,26 @@ struct WgradCfg {
   static constexpr int kTmemCols = 2 * R;
 };
 
-struct WgradArgs {
+// One weight gradient: X [M, cols] with its scales if it is in 8 bits, G [M, rank]
+// (g32 with an 8-bit X), the partial sums and the result.
+struct WgradProblem {
   const void* x;
   const float* x_scales;
   const __nv_bfloat16* g;
-  const float* g32;  // with an 8-bit X
-  const int32_t* words;
+  const float* g32;
   float* part;
   __nv_bfloat16* dbank;
+  int64_t ldx;
+  int cols, col_tiles, rows_per_split;
+};
+// One launch computes one or two of them: CTAs past the first's column tiles
+// take the second.
+struct WgradArgs {
+  WgradProblem first, second;
+  const int32_t* words;
   unsigned int* error;
   AdapterPlan lay;
-  int64_t ldx;
-  int cols, rank, A, rows_per_split;
+  int rank, A;
 };
 
 // Descriptor of an MN-major operand in 128-byte-swizzled blocks of 64 MN
@@ -1094,6 +1102,9 @@ template <int R, bool I8>
 __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kMinCtas)
     adapter_wgrad_kernel(const WgradArgs a) {
   using C = WgradCfg<R, I8>;
+  const bool second = static_cast<int>(blockIdx.x) >= a.first.col_tiles;
+  const WgradProblem w = second ? a.second : a.first;
+  const int col_tile = blockIdx.x - (second ? a.first.col_tiles : 0);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;
@@ -1125,9 +1136,9 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int col0 = blockIdx.x * C::kCols;
-  const int row_lo = blockIdx.y * a.rows_per_split;
-  const int row_hi = min(row_lo + a.rows_per_split, a.words[AdapterPlan::kNoneStart]);
+  const int col0 = col_tile * C::kCols;
+  const int row_lo = blockIdx.y * w.rows_per_split;  // (past the rows: no work)
+  const int row_hi = min(row_lo + w.rows_per_split, a.words[AdapterPlan::kNoneStart]);
   grid_wait();  // G may be the output of the kernel before this one
   RowCursor cur(a.words, a.lay, row_lo, row_hi);
 
@@ -1137,8 +1148,8 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
     const int pt = tid - 160;
     if constexpr (!I8) {
       const int ch = pt & 15;  // 16-byte chunk of a row's 128 columns
-      const bool col_ok = col0 + ch * 8 < a.cols;
-      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x) + col0 + ch * 8;
+      const bool col_ok = col0 + ch * 8 < w.cols;
+      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(w.x) + col0 + ch * 8;
       // the tokens of a stage's rows, looked up one stage ahead
       constexpr int kG = (64 * (R / 8) + 255) / 256;
       int tx[4], tg[kG];
@@ -1165,7 +1176,7 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
           const int row = (pt >> 4) + 16 * i;
           const bool ok = tx[i] >= 0 && col_ok;
           cp_async_16_l2(sx + (ch >> 3) * C::kBlock + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
-                         ok ? x + static_cast<int64_t>(tx[i]) * a.ldx : static_cast<const __nv_bfloat16*>(a.x), ok);
+                         ok ? x + static_cast<int64_t>(tx[i]) * w.ldx : static_cast<const __nv_bfloat16*>(w.x), ok);
         }
 #pragma unroll
         for (int i = 0; i < kG; ++i) {
@@ -1174,7 +1185,7 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
           if (64 * (R / 8) % 256 != 0 && row >= 64) break;
           const bool ok = tg[i] >= 0 && gc * 8 < a.rank;
           cp_async_16(sg + (gc >> 3) * C::kBlock + row * 128 + (((gc & 7) ^ (row & 7)) << 4),
-                      ok ? a.g + static_cast<int64_t>(tg[i]) * a.rank + gc * 8 : a.g, ok);
+                      ok ? w.g + static_cast<int64_t>(tg[i]) * a.rank + gc * 8 : w.g, ok);
         }
         cp_async_commit();
         cur.next();
@@ -1192,10 +1203,10 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
       if (!cur.live() && lane == 0)
         for (int s = max(0, it - C::kAhead); s < it; ++s) mbar_arrive(full_bar(s % C::kStages));
     } else {
-      const int8_t* x = static_cast<const int8_t*>(a.x);
-      const int ncb = (a.cols + 127) / 128;
+      const int8_t* x = static_cast<const int8_t*>(w.x);
+      const int ncb = (w.cols + 127) / 128;
       const int ch = pt & 7;  // 16 codes
-      const bool col_ok = col0 + ch * 16 < a.cols;
+      const bool col_ok = col0 + ch * 16 < w.cols;
       RowCursor rc(a.words, a.lay, row_lo, row_hi);  // raw codes, kRaw stages ahead
       int rit = 0;
       int tx[2];  // tokens of the next stage's rows, looked up one stage ahead
@@ -1214,7 +1225,7 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
             const int token = tx[i];
             const bool ok = token >= 0 && col_ok;
             cp_async_16(sbase + C::kOffRaw + (rit % C::kRaw) * C::kRawStage + (pt + 256 * i) * 16,
-                        ok ? x + static_cast<int64_t>(token) * a.ldx + col0 + ch * 16 : x, ok);
+                        ok ? x + static_cast<int64_t>(token) * w.ldx + col0 + ch * 16 : x, ok);
           }
           rc.next();
           ++rit;
@@ -1235,11 +1246,11 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
         if (gc.live()) {
           const int token = tg;
           if (token >= 0) {
-            gs = __ldg(a.x_scales + static_cast<int64_t>(token) * ncb + blockIdx.x);
+            gs = __ldg(w.x_scales + static_cast<int64_t>(token) * ncb + col_tile);
 #pragma unroll
             for (int i = 0; i < R / 16; ++i)
               if (g0 + 4 * i < a.rank)
-                gv[i] = __ldg(reinterpret_cast<const float4*>(a.g32 + static_cast<int64_t>(token) * a.rank + g0 + 4 * i));
+                gv[i] = __ldg(reinterpret_cast<const float4*>(w.g32 + static_cast<int64_t>(token) * a.rank + g0 + 4 * i));
           }
           gc.next();
           tg = gc.live() && gc.pos + grow < gc.end ? perm[gc.pos + grow] : -1;
@@ -1262,10 +1273,10 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int row = (pt >> 3) + 32 * i;
-          const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+          const uint32_t c4[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
           uint32_t o[8];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) i8_to_bf16(w[q], o[2 * q], o[2 * q + 1]);
+          for (int q = 0; q < 4; ++q) i8_to_bf16(c4[q], o[2 * q], o[2 * q + 1]);
           const uint32_t base = sx + (ch >> 2) * C::kBlock + row * 128;
           const int c0 = (ch & 3) * 2;
           sts128(base + ((c0 ^ (row & 7)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
@@ -1317,23 +1328,23 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
       const int b = seg & 1, ad = cur.adapter;
       if (!mbar_wait(acc_full(b), static_cast<uint32_t>((seg >> 1) & 1), abort_flag)) break;
       tc_fence_after();
-      const bool whole = starts[ad] >= row_lo && starts[ad + 1] <= row_lo + a.rows_per_split;
+      const bool whole = starts[ad] >= row_lo && starts[ad + 1] <= row_lo + w.rows_per_split;
       const int64_t slot = whole ? ad : 2 * static_cast<int>(blockIdx.y) + (starts[ad] < row_lo ? 0 : 1);
-      const int64_t base = slot * a.rank * a.cols + col;
+      const int64_t base = slot * a.rank * w.cols + col;
 #pragma unroll 1
       for (int c = 0; c < R; c += 16) {
         uint32_t v[16];
         tmem_ld_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + b * R + c, v);
         tmem_wait_ld();
-        if (col < a.cols) {
+        if (col < w.cols) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             if (c + (e & 8) >= a.rank) break;
-            const int64_t o = base + static_cast<int64_t>(c + e) * a.cols;
+            const int64_t o = base + static_cast<int64_t>(c + e) * w.cols;
             if (whole)
-              a.dbank[o] = __float2bfloat16_rn(__uint_as_float(v[e]));
+              w.dbank[o] = __float2bfloat16_rn(__uint_as_float(v[e]));
             else
-              a.part[o] = __uint_as_float(v[e]);
+              w.part[o] = __uint_as_float(v[e]);
           }
         }
       }
@@ -1354,27 +1365,27 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
 }
 
 // Adds the slots of adapters that several splits share, in split order; zeros
-// for adapters without rows.  blockIdx.y: adapter.
-__global__ void __launch_bounds__(256)
-    adapter_wgrad_reduce_kernel(const int32_t* __restrict__ words, AdapterPlan lay, int rows_per_split,
-                                const float* __restrict__ part, __nv_bfloat16* __restrict__ dbank,
-                                int64_t elems) {
+// for adapters without rows.  blockIdx.y: adapter; z: problem.
+__global__ void __launch_bounds__(256) adapter_wgrad_reduce_kernel(const WgradArgs a) {
+  const WgradProblem w = blockIdx.z == 0 ? a.first : a.second;
+  const int64_t elems = static_cast<int64_t>(a.rank) * w.cols;
   const int ad = blockIdx.y;
-  const int lo = words[lay.off_start + ad], hi = words[lay.off_start + ad + 1];
+  const int lo = a.words[a.lay.off_start + ad], hi = a.words[a.lay.off_start + ad + 1];
   grid_wait();
-  const int s0 = lo / rows_per_split, s1 = hi > lo ? (hi - 1) / rows_per_split : s0;
+  const int s0 = lo / w.rows_per_split, s1 = hi > lo ? (hi - 1) / w.rows_per_split : s0;
   if (hi > lo && s0 == s1) return;
   for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < elems; i += gridDim.x * 1024ll) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (hi > lo)
       for (int s = s0; s <= s1; ++s) {
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(2 * s + (s == s0 ? 1 : 0)) * elems + i));
+        const float4 u =
+            __ldcg(reinterpret_cast<const float4*>(w.part + static_cast<int64_t>(2 * s + (s == s0 ? 1 : 0)) * elems + i));
         v.x += u.x;
         v.y += u.y;
         v.z += u.z;
         v.w += u.w;
       }
-    *reinterpret_cast<uint2*>(dbank + static_cast<int64_t>(ad) * elems + i) =
+    *reinterpret_cast<uint2*>(w.dbank + static_cast<int64_t>(ad) * elems + i) =
         make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   }
 }
