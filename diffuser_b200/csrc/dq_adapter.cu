@@ -274,10 +274,14 @@ BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A,
 
 // hidden = scale x . P^T (down), out = act(y + hidden . Q) (up), on one plan.
 // hidden: where the low-rank intermediate goes, complete (zero rows without an
-// adapter) if want_hidden; the small-batch kernel takes NULL.
+// adapter) if want_hidden; the small-batch kernel takes NULL.  between: launches
+// that read x again, put right behind the large-tile down kernel while x is
+// still in L2 (behind everything for small batches).
+template <typename Between>
 int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void* y, int64_t ldy, int64_t F_out,
             const void* Q, const float* scale, int64_t M, int64_t R, int r, int A, const int32_t* words, int act,
-            void* out, int64_t ldo, void* hidden, bool want_hidden, float* hidden32, int sms, cudaStream_t st) {
+            void* out, int64_t ldo, void* hidden, bool want_hidden, float* hidden32, int sms, cudaStream_t st,
+            Between between) {
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
   const int with_none = act != kActNone || out != y || want_hidden;
   if (!large_tiles(M, R, A)) {
@@ -301,7 +305,8 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
     a.A = A;
     a.act = act;
     a.with_none = with_none;
-    return by_rank(r, [&](auto rc) { return launch_small<decltype(rc)::value>(a, M, R, sms, st); });
+    const int e = by_rank(r, [&](auto rc) { return launch_small<decltype(rc)::value>(a, M, R, sms, st); });
+    return e != DQ_OK ? e : between();
   }
   DownArgs d = {};
   int e = error_word(&d.error);
@@ -334,7 +339,8 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
   u.with_none = with_none;
   return by_rank(r, [&](auto rc) {
     constexpr int R_ = decltype(rc)::value;
-    const int e2 = launch_down<R_>(d, M, R, st);
+    int e2 = launch_down<R_>(d, M, R, st);
+    if (e2 == DQ_OK) e2 = between();
     return e2 != DQ_OK ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, sms, st);
   });
 }
@@ -403,7 +409,7 @@ int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64
   if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)) return DQ_ERR_WORKSPACE;
   return down_up(x, ldx, K, down, y, ldy, N, up, scale, M, R, r, A, static_cast<const int32_t*>(plan), act, out,
                  ldo, hidden != nullptr ? hidden : workspace, hidden != nullptr, nullptr, sms,
-                 static_cast<cudaStream_t>(stream));
+                 static_cast<cudaStream_t>(stream), [] { return static_cast<int>(DQ_OK); });
 }
 
 size_t dq_adapter_backward_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
@@ -448,10 +454,6 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int32_t* words = static_cast<const int32_t*>(plan);
   float* g32 = i8 ? reinterpret_cast<float*>(ws + w.g) : nullptr;
-  rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo, ws, want_w,
-               want_w ? g32 : nullptr, sms, st);
-  if (rc != DQ_OK || !want_w) return rc;
-
   WgradArgs a = {};
   if ((rc = error_word(&a.error)) != DQ_OK) return rc;
   a.words = words;
@@ -477,16 +479,24 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
   pd.cols = static_cast<int>(K);
   pd.col_tiles = static_cast<int>(col_tiles(K));
   pd.rows_per_split = w.down.rows_per_split;
+  // dup needs hidden and dy alone: it follows the product that has just read dy
+  // (an 8-bit x takes its own kernel; with a bf16 x one launch computes both)
+  a.first = pu;
+  auto first = [&] {
+    if (!want_w || !i8) return static_cast<int>(DQ_OK);
+    return by_rank(r, [&](auto rank) { return launch_wgrad<decltype(rank)::value, false>(a, w.up.splits, st); });
+  };
+  rc = down_up(dy, lddy, N, up, dx, lddx, K, down, scale, M, R, r, A, words, kActNone, dx_out, lddxo, ws, want_w,
+               want_w ? g32 : nullptr, sms, st, first);
+  if (rc != DQ_OK || !want_w) return rc;
   rc = by_rank(r, [&](auto rank) {
     constexpr int R_ = decltype(rank)::value;
-    a.first = pu;
-    if (!i8) {
-      a.second = pd;
-      return launch_wgrad<R_, false>(a, w.up.splits, st);
+    if (i8) {
+      a.first = pd;
+      return launch_wgrad<R_, true>(a, w.down.splits, st);
     }
-    const int e = launch_wgrad<R_, false>(a, w.up.splits, st);
-    a.first = pd;
-    return e != DQ_OK ? e : launch_wgrad<R_, true>(a, w.down.splits, st);
+    a.second = pd;
+    return launch_wgrad<R_, false>(a, w.up.splits, st);
   });
   if (rc != DQ_OK) return rc;
   a.first = pu;
