@@ -194,17 +194,22 @@ int launch_down(DownArgs a, int64_t M, int64_t requests, cudaStream_t st) {
 }
 
 template <int R>
-int launch_up(UpArgs a, int tiles, int64_t M, int sms, cudaStream_t st) {
+int launch_up(UpArgs a, int tiles, int64_t M, int64_t requests, int sms, cudaStream_t st) {
   using C = UpCfg<R>;
   static std::atomic<int> set[kMaxDevices];
   const int rc = allow_smem(adapter_up_kernel<R>, C::kSmemBytes, set);
   if (rc != DQ_OK) return rc;
-  // columns per CTA: 256 where that leaves four CTAs per SM, else 128 (wider
-  // ones spread a CTA's fixed cost, its rows of hidden and its first loads'
-  // latency, over more steps but leave the last wave emptier)
-  const int cols = ceil_div(M, kTileRows) * ceil_div(a.N, 256) < 4 * sms ? 128 : 256;
-  a.cols_per_cta = cols;
-  return launch(adapter_up_kernel<R>, dim3(tiles, static_cast<unsigned>(ceil_div(a.N, cols))), 256, C::kSmemBytes, st,
+  // 64-column steps per CTA: the fewest that put the whole launch into one wave
+  // if eight are enough (4608 x 4096 at r = 64: six steps 22 us, four, a wave
+  // and a third, 25), else four (4613 x 16384 with its GELU: 80 us; nineteen
+  // steps, one wave of long CTAs that nothing evens out, 92)
+  const int64_t total = ceil_div(a.N, C::kStepCols), slots = static_cast<int64_t>(sms) * C::kMinCtas;
+  const int64_t most = ceil_div(M, kTileRows) + std::min<int64_t>(a.A, requests) + 1;
+  int64_t steps = 1;
+  while (steps <= 8 && most * ceil_div(total, steps) > slots) ++steps;
+  if (steps > 8) steps = 4;
+  a.cols_per_cta = static_cast<int>(steps * C::kStepCols);
+  return launch(adapter_up_kernel<R>, dim3(tiles, static_cast<unsigned>(ceil_div(total, steps))), 256, C::kSmemBytes, st,
                 true, dim3(1), a);
 }
 
@@ -341,7 +346,7 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
     constexpr int R_ = decltype(rc)::value;
     int e2 = launch_down<R_>(d, M, R, st);
     if (e2 == DQ_OK) e2 = between();
-    return e2 != DQ_OK ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, sms, st);
+    return e2 != DQ_OK ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, R, sms, st);
   });
 }
 
