@@ -201,13 +201,14 @@ int launch_up(UpArgs a, int tiles, int64_t M, int64_t requests, int sms, cudaStr
   if (rc != DQ_OK) return rc;
   // 64-column steps per CTA: the fewest that put the whole launch into one wave
   // if eight are enough (4608 x 4096 at r = 64: six steps 22 us, four, a wave
-  // and a third, 25), else four (4613 x 16384 with its GELU: 80 us; nineteen
-  // steps, one wave of long CTAs that nothing evens out, 92)
+  // and a third, 25), else six (4613 x 16384 at r = 32, with / without GELU: six
+  // 82.5 / 69 us, four, whose CTAs' first loads weigh more, 85.7 / 73.8, sixteen,
+  // which leave the last wave emptier, 91 / 78)
   const int64_t total = ceil_div(a.N, C::kStepCols), slots = static_cast<int64_t>(sms) * C::kMinCtas;
   const int64_t most = ceil_div(M, kTileRows) + std::min<int64_t>(a.A, requests) + 1;
   int64_t steps = 1;
   while (steps <= 8 && most * ceil_div(total, steps) > slots) ++steps;
-  if (steps > 8) steps = 4;
+  if (steps > 8) steps = 6;
   a.cols_per_cta = static_cast<int>(steps * C::kStepCols);
   return launch(adapter_up_kernel<R>, dim3(tiles, static_cast<unsigned>(ceil_div(total, steps))), 256, C::kSmemBytes, st,
                 true, dim3(1), a);

@@ -25,6 +25,7 @@
 #include <cstdint>
 
 #include "dq_codec.cuh"
+#include "dq_f32x2.cuh"
 #include "dq_ptx.cuh"
 #include "dq_smallm.cuh"
 
@@ -261,21 +262,19 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
-// mma_16816_bf16 onto zeros (no accumulator registers to clear).
-__device__ __forceinline__ void mma_16816_bf16_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                    uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
 }
 // 2^x by the special-function unit (relative error 2^-22, subnormals to zero).
 __device__ __forceinline__ float exp2f_approx(float x) {
@@ -537,64 +536,44 @@ __global__ void __launch_bounds__(DownCfg<R>::kThreads, 2) adapter_down_kernel(c
   }
 }
 
-__device__ __forceinline__ void unpack8(uint4 u, float* v) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-__device__ __forceinline__ uint4 pack8(const float* v) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
-}
-
 // Activations of the sum y + delta, float32 in and out (rounded once, with the
 // result): gelu_tanh(x) = x sigmoid(2 u), u = sqrt(2/pi) (x + 0.044715 x^3), and
 // silu(x) = x sigmoid(x), sigmoid(z) = 1 / (1 + 2^(-z log2 e)): an exponential
 // and a reciprocal of the special-function unit, whose 16 results a cycle and
 // SM stay below the stream's time (2^inf gives 1 / inf = 0: no clamp).
-__device__ __forceinline__ float sigmoid_of_neg_log2(float z) { return rcp_approx(1.0f + exp2f_approx(z)); }
-__device__ __forceinline__ void gelu_tanh4(float* x) {
+// Two at a time, the products in packed instructions.
+__device__ __forceinline__ F2 sigmoid2_of_neg_log2(F2 z) {
+  const float2 e = unpair(z);
+  const float2 d = unpair(add2(f2(exp2f_approx(e.x), exp2f_approx(e.y)), f2(1.0f)));
+  return f2(rcp_approx(d.x), rcp_approx(d.y));
+}
+__device__ __forceinline__ F2 gelu_tanh2(F2 x) {
   constexpr float k = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] *= sigmoid_of_neg_log2(x[i] * fmaf(x[i] * x[i], 0.044715f * k, k));
+  return mul2(x, sigmoid2_of_neg_log2(mul2(x, fma2(mul2(x, x), f2(0.044715f * k), f2(k)))));
 }
-__device__ __forceinline__ void silu4(float* x) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] *= sigmoid_of_neg_log2(x[i] * -1.4426950408889634f);
-}
-__device__ __forceinline__ void gate4(float* x, int act) {
-  if (act == kActSwiGlu)
-    silu4(x);
-  else
-    gelu_tanh4(x);
-}
+__device__ __forceinline__ F2 silu2(F2 x) { return mul2(x, sigmoid2_of_neg_log2(mul2(x, f2(-1.4426950408889634f)))); }
+__device__ __forceinline__ F2 gate2(F2 x, int act) { return act == kActSwiGlu ? silu2(x) : gelu_tanh2(x); }
 
 // --------------------------------------------------------------------- up
 // O[m, :] = act(Y[m, :] + hidden[m, :] . P_a): 128-row tiles, one warp per 16.
 //
 // Bound: the stream of Y and O (P and hidden are small and reread from L2).
 // The products take a sixteenth of the warp MMA rate at the copy bandwidth,
-// so they stay warp-level with their sums in registers, and the layout is
-// arranged for the stream: P's 64-column pieces are staged in shared memory
-// with their columns permuted -- 4-byte pair j of the 16-byte chunk t of a
-// 32-column group is stored as pair t of chunk j -- so that MMA column
-// 2 tig + e of n-tile j is column 8 tig + 2 j + e of the group and each
-// thread's sums are 16 consecutive bytes of a row of O: Y is read and O
-// written in 16-byte pieces, the next step's Y and P while this one computes.
+// so they stay warp-level with their sums in registers, and what counts is
+// that nothing waits and that few instructions surround the stream: Y and P
+// arrive by cp.async in a ring of 64-column steps, two ahead; Y's tile is read
+// as accumulators with ldmatrix (its fragment is the MMA's own layout), the
+// result returns to the same place with stmatrix and leaves in whole 128-byte
+// rows.  A warp touches only its own 16 rows of Y and O, so the one barrier
+// of a step is the ring's.
 template <int R>
 struct UpCfg {
   static constexpr int kStepCols = 64;
-  static constexpr int kChunks = R * kStepCols / 8;  // 16-byte pieces of P per step
-  static constexpr int kPerThread = (kChunks + 255) / 256;
-  static constexpr int kBuf = R * kStepCols * 2;
-  static constexpr int kYStages = R <= 32 ? 2 : 3;
   static constexpr int kYStage = kTileRows * kStepCols * 2;
-  static constexpr int kOffY = 2 * kBuf;
-  static constexpr int kSmemBytes = kOffY + kYStages * kYStage;
-  static constexpr int kMinCtas = R <= 32 ? 4 : R <= 64 ? 3 : 2;
+  static constexpr int kStage = kYStage + R * kStepCols * 2;
+  static constexpr int kStages = 3;
+  static constexpr int kSmemBytes = kStages * kStage;
+  static constexpr int kMinCtas = R <= 16 ? 4 : R <= 64 ? 3 : 2;
 };
 
 struct UpArgs {
@@ -623,138 +602,138 @@ __global__ void __launch_bounds__(256, UpCfg<R>::kMinCtas) adapter_up_kernel(con
   const int g4 = lane >> 2, tig = lane & 3;
   const int n_lo = blockIdx.y * a.cols_per_cta;
   const int n_hi = min(a.N, n_lo + a.cols_per_cta);
-  const bool none = t.adapter >= a.A;
-  const int tok0 = t.token(a.words + a.lay.off_perm, warp * 16 + g4);
-  const int tok1 = t.token(a.words + a.lay.off_perm, warp * 16 + g4 + 8);
-  const __nv_bfloat16* P = none ? a.bank : a.bank + static_cast<int64_t>(t.adapter) * a.rank * a.N;
-  // this lane copies chunk lane % 8 of its warp's rows lane / 8 + 4 i
+  const bool none = t.adapter >= a.A, gated = act_is_gated(a.act);
+  const int32_t* perm = a.words + a.lay.off_perm;
+  const __nv_bfloat16* P = a.bank + static_cast<int64_t>(none ? 0 : t.adapter) * a.rank * a.N;
+  // this lane moves chunk lane % 8 of its warp's rows lane / 8 + 4 i (gated
+  // results: chunk lane % 4 of rows lane / 4 + 8 i)
+  const int ch = lane & 7;
   const __nv_bfloat16* ysrc[4];
+  __nv_bfloat16* dst[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int tok = t.token(a.words + a.lay.off_perm, warp * 16 + (lane >> 3) + 4 * i);
-    ysrc[i] = tok >= 0 ? a.y + static_cast<int64_t>(tok) * a.ldy + (lane & 7) * 8 : nullptr;
+    const int tok = t.token(perm, warp * 16 + (lane >> 3) + 4 * i);
+    ysrc[i] = tok >= 0 ? a.y + static_cast<int64_t>(tok) * a.ldy + ch * 8 : nullptr;
+    const int to = !gated ? tok : i < 2 ? t.token(perm, warp * 16 + g4 + 8 * i) : -1;
+    dst[i] = to >= 0 ? a.out + static_cast<int64_t>(to) * a.ldo + (gated ? tig : ch) * 8 : nullptr;
   }
-  const bool gated = act_is_gated(a.act);
-  // gated: lanes 0, 1 of a quad write its 16 output columns of a 32-column group
-  __nv_bfloat16* o0 = a.out + static_cast<int64_t>(tok0) * a.ldo + 8 * tig;
-  __nv_bfloat16* o1 = a.out + static_cast<int64_t>(tok1) * a.ldo + 8 * tig;
-  const bool st0 = tok0 >= 0 && (!gated || tig < 2), st1 = tok1 >= 0 && (!gated || tig < 2);
-
-  uint4 preg[C::kPerThread];
-  auto load_p = [&](int n0) {
+  auto load = [&](int n0, int stage) {
+    const bool in = n0 + ch * 8 < n_hi;
+    const uint32_t sy = sbase + stage * C::kStage, sp = sy + C::kYStage;
 #pragma unroll
-    for (int i = 0; i < C::kPerThread; ++i) {
-      const int c = tid + 256 * i;
-      const int row = c >> 3, col = n0 + (c & 7) * 8;
-      const bool ok = !none && row < a.rank && col < n_hi && c < C::kChunks;
-      preg[i] = ok ? __ldg(reinterpret_cast<const uint4*>(P + static_cast<int64_t>(row) * a.N + col))
-                   : make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < 4; ++i) {
+      const int row = warp * 16 + (lane >> 3) + 4 * i;
+      if (in && ysrc[i] != nullptr) cp_async_16_l2(sy + row * 128 + ((ch ^ (row & 7)) << 4), ysrc[i] + n0, true);
     }
-  };
-  auto store_p = [&](int buf) {
+    if (!none && n0 < n_hi) {
 #pragma unroll
-    for (int i = 0; i < C::kPerThread; ++i) {
-      const int c = tid + 256 * i;
-      if (C::kChunks % 256 != 0 && c >= C::kChunks) break;
-      const int row = c >> 3, cc = c & 7;  // 32-column group cc / 4, chunk cc % 4 of it
-      const uint32_t base = sbase + buf * C::kBuf + row * 128 + 4 * (cc & 3);
-      const uint32_t w[4] = {preg[i].x, preg[i].y, preg[i].z, preg[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sts32(base + ((((cc >> 2) * 4 + j) ^ (row & 7)) << 4), w[j]);
-    }
-  };
-  auto load_y = [&](int n0, int stage) {
-    if (n0 + (lane & 7) * 8 < n_hi) {
-      const uint32_t dst = sbase + C::kOffY + stage * C::kYStage + (warp * 16 + (lane >> 3)) * 128;
-      const uint32_t c = static_cast<uint32_t>(((lane & 7) ^ ((lane >> 1) & 4)) << 4);  // row % 2 = (lane / 8) % 2
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (ysrc[i] != nullptr) cp_async_16_l2(dst + i * 512 + c, ysrc[i] + n0, true);
+      for (int i = 0; i < (R * 8 + 255) / 256; ++i) {
+        const int row = (tid >> 3) + 32 * i;
+        const bool ok = in && row < a.rank;
+        if (R % 32 == 0 || row < R)
+          cp_async_16(sp + row * 128 + ((ch ^ (row & 7)) << 4),
+                      ok ? P + static_cast<int64_t>(row) * a.N + n0 + ch * 8 : a.bank, ok);
+      }
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < C::kYStages - 1; ++i) load_y(n_lo + i * C::kStepCols, i);
-  load_p(n_lo);
-  store_p(0);
+  for (int i = 0; i < C::kStages - 1; ++i) load(n_lo + i * C::kStepCols, i);
 
   grid_wait();  // hidden is the down kernel's
   uint32_t vf[R / 16][4];
+  {
+    const int tok0 = t.token(perm, warp * 16 + g4), tok1 = t.token(perm, warp * 16 + g4 + 8);
 #pragma unroll
-  for (int ks = 0; ks < R / 16; ++ks)
+    for (int ks = 0; ks < R / 16; ++ks)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int c = ks * 16 + 8 * (q >> 1);
-      const int tok = (q & 1) ? tok1 : tok0;
-      const bool ok = !none && tok >= 0 && c < a.rank;
-      vf[ks][q] = ok ? __ldcg(reinterpret_cast<const unsigned int*>(a.hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig))
-                     : 0u;
-      if (none && a.zero_hidden != nullptr && blockIdx.y == 0 && tok >= 0 && c < a.rank)
-        *reinterpret_cast<uint32_t*>(a.zero_hidden + static_cast<int64_t>(tok) * a.rank + c + 2 * tig) = 0u;
-    }
+      for (int q = 0; q < 4; ++q) {
+        const int c = ks * 16 + 8 * (q >> 1);
+        const int tok = (q & 1) ? tok1 : tok0;
+        const bool ok = tok >= 0 && c < a.rank;
+        const int64_t o = static_cast<int64_t>(tok) * a.rank + c + 2 * tig;
+        vf[ks][q] = ok && !none ? __ldcg(reinterpret_cast<const unsigned int*>(a.hidden + o)) : 0u;
+        if (ok && none && a.zero_hidden != nullptr && blockIdx.y == 0)
+          *reinterpret_cast<uint32_t*>(a.zero_hidden + o) = 0u;
+      }
+  }
   grid_launch_dependents();
 
-  int buf = 0, ys = 0;
+  // ldmatrix / stmatrix address of this lane: row lane % 16 of 16, column half lane / 16
+  const int lrow = lane & 15, lhalf = lane >> 4;
+  int stage = 0;
   for (int n0 = n_lo; n0 < n_hi; n0 += C::kStepCols) {
-    cp_async_wait<C::kYStages - 2>();
-    __syncthreads();  // this step's P and Y; every warp is done with the last step's
-    load_y(n0 + (C::kYStages - 1) * C::kStepCols, ys == 0 ? C::kYStages - 1 : ys - 1);
-    const bool more = n0 + C::kStepCols < n_hi;
-    if (more) load_p(n0 + C::kStepCols);
-    const uint32_t yrow = sbase + C::kOffY + ys * C::kYStage + (warp * 16 + g4) * 128;
+    cp_async_wait<C::kStages - 2>();
+    __syncthreads();  // this step's Y and P; every warp is done with the last step's
+    load(n0 + (C::kStages - 1) * C::kStepCols, stage == 0 ? C::kStages - 1 : stage - 1);
+    const uint32_t sy = sbase + stage * C::kStage, sp = sy + C::kYStage;
+    const uint32_t ybase = sy + (warp * 16 + lrow) * 128;
+    auto at = [&](int chunk) { return ybase + (((chunk + lhalf) ^ (lrow & 7)) << 4); };
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < 2; ++g) {  // 32 columns: four n-tiles of 8, their sums started from Y (widened exactly)
       float acc[4][4];
-      // (a tile without an adapter multiplies zeros: P's pieces were loaded as such)
-      const int krow = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-      for (int ks = 0; ks < R / 16; ++ks)
+      for (int jp = 0; jp < 2; ++jp) {
+        uint32_t w[4];
+        ldmatrix_x4(at(4 * g + 2 * jp), w);
 #pragma unroll
-        for (int jp = 0; jp < 2; ++jp) {
-          uint32_t bf[4];
-          const int row = ks * 16 + krow;
-          const int ch = g * 4 + 2 * jp + (lane >> 4);
-          ldmatrix_x4_trans(sbase + buf * C::kBuf + row * 128 + ((ch ^ (row & 7)) << 4), bf);
-          if (ks == 0) {
-            mma_16816_bf16_zero(acc[2 * jp], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[0], bf[1]);
-            mma_16816_bf16_zero(acc[2 * jp + 1], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[2], bf[3]);
-          } else {
+        for (int q = 0; q < 4; ++q) {
+          acc[2 * jp + (q >> 1)][2 * (q & 1)] = __uint_as_float(w[q] << 16);
+          acc[2 * jp + (q >> 1)][2 * (q & 1) + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
+        }
+      }
+      if (!none) {
+#pragma unroll
+        for (int ks = 0; ks < R / 16; ++ks)
+#pragma unroll
+          for (int jp = 0; jp < 2; ++jp) {
+            uint32_t bf[4];
+            ldmatrix_x4_trans(sp + (ks * 16 + lrow) * 128 + (((4 * g + 2 * jp + lhalf) ^ (lrow & 7)) << 4), bf);
             mma_16816_bf16(acc[2 * jp], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[0], bf[1]);
             mma_16816_bf16(acc[2 * jp + 1], vf[ks][0], vf[ks][1], vf[ks][2], vf[ks][3], bf[2], bf[3]);
           }
-        }
-      const int col = n0 + g * 32;
-      const bool in = col + 8 * tig < n_hi;
+      }
+      F2 v[4][2];  // [n-tile][row half]
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-        unpack8(lds128(yrow + h * 1024 + (((4 * g + tig) ^ ((g4 & 1) * 4)) << 4)), v);
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] += acc[j][2 * h];
-          v[2 * j + 1] += acc[j][2 * h + 1];
-        }
-        int oc = col;
+        for (int h = 0; h < 2; ++h) v[j][h] = f2(acc[j][2 * h], acc[j][2 * h + 1]);
+      if (gated) {  // n-tiles 0, 1 hold 16 gate columns, 2, 3 their up columns
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) v[j][h] = mul2(gate2(v[j][h], a.act), v[j + 2][h]);
+        stmatrix_x4(at(2 * g), narrow(v[0][0]), narrow(v[0][1]), narrow(v[1][0]), narrow(v[1][1]));
+      } else {
         if (a.act == kActGeluTanh) {
-          gelu_tanh4(v);
-          gelu_tanh4(v + 4);
-        } else if (gated) {
-          // lanes 0, 1 of the quad hold 16 gate columns, lanes 2, 3 their up columns
-          float u[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = __shfl_down_sync(0xffffffffu, v[e], 2, 4);
-          gate4(v, a.act);
-          gate4(v + 4, a.act);
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= u[e];
-          oc = col / 2;
+            for (int h = 0; h < 2; ++h) v[j][h] = gelu_tanh2(v[j][h]);
         }
-        if (in && (h ? st1 : st0)) *reinterpret_cast<uint4*>((h ? o1 : o0) + oc) = pack8(v);
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp)
+          stmatrix_x4(at(4 * g + 2 * jp), narrow(v[2 * jp][0]), narrow(v[2 * jp][1]), narrow(v[2 * jp + 1][0]),
+                      narrow(v[2 * jp + 1][1]));
       }
     }
-    buf ^= 1;
-    if (more) store_p(buf);
-    ys = ys + 1 == C::kYStages ? 0 : ys + 1;
+    __syncwarp();
+    if (gated) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = warp * 16 + g4 + 8 * i;
+        if (dst[i] != nullptr && n0 + tig * 16 < n_hi)
+          *reinterpret_cast<uint4*>(dst[i] + n0 / 2) = lds128(sy + row * 128 + ((tig ^ (row & 7)) << 4));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = warp * 16 + (lane >> 3) + 4 * i;
+        if (dst[i] != nullptr && n0 + ch * 8 < n_hi)
+          *reinterpret_cast<uint4*>(dst[i] + n0) = lds128(sy + row * 128 + ((ch ^ (row & 7)) << 4));
+      }
+    }
+    stage = stage + 1 == C::kStages ? 0 : stage + 1;
   }
   cp_async_wait<0>();
 }
@@ -953,35 +932,31 @@ __global__ void __launch_bounds__(256, R <= 32 ? 3 : 1) adapter_small_kernel(con
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int tok = h ? tok1 : tok0;
-      float v[8];
+      F2 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t u = lds32(sbase + buf * C::kBuf + C::kOffY + (g4 + 8 * h) * C::kYStride + (warp * 32 + 8 * j + 2 * tig) * 2);
-        v[2 * j] = __uint_as_float(u << 16) + acc[j][2 * h];
-        v[2 * j + 1] = __uint_as_float(u & 0xFFFF0000u) + acc[j][2 * h + 1];
-      }
+      for (int j = 0; j < 4; ++j)
+        v[j] = add2(widen(lds32(sbase + buf * C::kBuf + C::kOffY + (g4 + 8 * h) * C::kYStride +
+                                (warp * 32 + 8 * j + 2 * tig) * 2)),
+                    f2(acc[j][2 * h], acc[j][2 * h + 1]));
       const int col = n0 + warp * 32 + 2 * tig;
       if (a.act == kActGeluTanh) {
-        gelu_tanh4(v);
-        gelu_tanh4(v + 4);
-      } else if (a.act != kActNone) {  // n-tiles 0, 1 hold 16 gate columns, 2, 3 their up columns
-        gate4(v, a.act);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= v[4 + e];
+        for (int j = 0; j < 4; ++j) v[j] = gelu_tanh2(v[j]);
+      } else if (a.act != kActNone) {  // n-tiles 0, 1 hold 16 gate columns, 2, 3 their up columns
+        v[0] = mul2(gate2(v[0], a.act), v[2]);
+        v[1] = mul2(gate2(v[1], a.act), v[3]);
       }
       if (tok < 0) continue;
       if (a.act == kActNone || a.act == kActGeluTanh) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (col + 8 * j < n_hi)
-            *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + col + 8 * j) =
-                pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + col + 8 * j) = narrow(v[j]);
       } else if (col < n_hi) {
         const int oc = (n0 + warp * 32) / 2 + 2 * tig;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + oc + 8 * j) =
-              pack_bf16x2(v[2 * j], v[2 * j + 1]);
+          *reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(tok) * a.ldo + oc + 8 * j) = narrow(v[j]);
       }
     }
   }

@@ -147,11 +147,10 @@ __global__ void __launch_bounds__(256)
       uint4 p;
       i8_to_bf16(u[i].x, p.x, p.y);
       i8_to_bf16(u[i].y, p.z, p.w);
-      float v[8];
-      unpack8(p, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= s[i];
-      *reinterpret_cast<uint4*>(out + row[i] * ldo + k[i]) = pack8(v);
+      const F2 by = f2(s[i]);
+      *reinterpret_cast<uint4*>(out + row[i] * ldo + k[i]) =
+          make_uint4(narrow(mul2(widen(p.x), by)), narrow(mul2(widen(p.y), by)), narrow(mul2(widen(p.z), by)),
+                     narrow(mul2(widen(p.w), by)));
     }
   }
 }
