@@ -1,6 +1,6 @@
 // dq_adapter.cu -- host side of include/dq_adapter.h: argument validation,
-// launch planning and launches of the adapter, activation-checkpoint and
-// input-gradient kernels.
+// launch planning and launches of the adapter and activation-checkpoint kernels
+// (the input gradients are in dq_dgrad.cu).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -12,6 +12,7 @@
 #include "dq_adapter.cuh"
 #include "dq_checkpoint.cuh"
 #include "dq_internal.h"
+#include "dq_launch.h"
 
 namespace dq {
 namespace {
@@ -20,10 +21,6 @@ constexpr int64_t kMaxTokens = 1 << 30;
 constexpr int kMaxAdapters = 65535;
 constexpr int kMaxRank = 128;
 constexpr int kMaxCluster = 8;
-
-inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 int plan_shape(int64_t M, int64_t R, int A) {
   return M < 0 || M > kMaxTokens || R < 0 || R > kMaxTokens || A < 1 || A > kMaxAdapters ? DQ_ERR_SHAPE : DQ_OK;
@@ -100,47 +97,6 @@ WgradPlan wgrad_plan(int64_t M, int64_t R, int A, int64_t col_tiles, int rc, boo
   return p;
 }
 int64_t col_tiles(int64_t cols) { return ceil_div(cols, 128); }
-
-// after: programmatic stream serialization -- the kernel may start while the
-// one before it drains, and waits (griddepcontrol.wait) before it reads that
-// one's results.  cluster: CTAs of a cluster along (x, y).
-template <typename Args>
-int launch(void (*kern)(Args), dim3 grid, int threads, size_t smem, cudaStream_t st, bool after, dim3 cluster,
-           Args args) {
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (after) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster.x * cluster.y > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster.x;
-    attr[n].val.clusterDim.y = cluster.y;
-    attr[n++].val.clusterDim.z = 1;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kern, args) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
-}
-
-// Shared-memory opt-in of a kernel, once per device.
-constexpr int kMaxDevices = 64;
-template <typename K>
-int allow_smem(K kern, int bytes, std::atomic<int>* set) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
-  if (set[dev].load(std::memory_order_acquire)) return DQ_OK;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return DQ_ERR_LAUNCH;
-  set[dev].store(1, std::memory_order_release);
-  return DQ_OK;
-}
 
 // Resident clusters of the down kernel by their (even) size, once per device.
 // The runtime's occupancy query counts one CTA per SM for a kernel that
@@ -544,50 +500,6 @@ int dq_checkpoint_unpack(const int8_t* codes, const float* scales, int64_t M, in
       codes, scales, M, static_cast<int>(K), static_cast<int>(ceil_div(K, kCkptRun)),
       static_cast<__nv_bfloat16*>(out), ldo);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
-}
-
-size_t dq_linear_dgrad_workspace(int64_t N, int64_t K) {
-  return N <= 0 || K <= 0 ? 0 : up256(static_cast<size_t>(N) * K * 2);
-}
-
-static int dgrad_impl(int fmt, const void* dy, int64_t M, int64_t N, const uint8_t* w, const void* absmax, int sbf,
-                      float scale, int64_t K, void* dx, void* workspace, size_t workspace_bytes, cudaStream_t st) {
-  if (M < 0 || N <= 0 || K <= 0 || N % 8 != 0 || K % (fmt == kFmtNF4 ? 64 : 16) != 0 || M > INT32_MAX ||
-      N > INT32_MAX || K > INT32_MAX || ceil_div(N, 128) > 65535)
-    return DQ_ERR_SHAPE;
-  if (M == 0) return DQ_OK;
-  if (dy == nullptr || w == nullptr || dx == nullptr || (fmt == kFmtNF4 && absmax == nullptr)) return DQ_ERR_ARG;
-  if (!aligned(dy, 16) || !aligned(w, 16) || !aligned(dx, 16) || !aligned(absmax, sbf ? 2 : 4)) return DQ_ERR_ALIGN;
-  int sms = 0;
-  const int rc = device_sms(&sms);
-  if (rc != DQ_OK) return rc;
-  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_linear_dgrad_workspace(N, K))
-    return DQ_ERR_WORKSPACE;
-  const dim3 grid(static_cast<unsigned>(ceil_div(K, 64)), static_cast<unsigned>(ceil_div(N, 128)));
-  if (fmt == kFmtNF4)
-    decode_transposed_kernel<kFmtNF4><<<grid, 256, 0, st>>>(w, absmax, sbf, 0.f, static_cast<int>(N),
-                                                            static_cast<int>(K),
-                                                            static_cast<__nv_bfloat16*>(workspace));
-  else
-    decode_transposed_kernel<kFmtFP8><<<grid, 256, 0, st>>>(w, nullptr, 0, scale, static_cast<int>(N),
-                                                            static_cast<int>(K),
-                                                            static_cast<__nv_bfloat16*>(workspace));
-  if (cudaGetLastError() != cudaSuccess) return DQ_ERR_LAUNCH;
-  return bf16_gemm(dy, M, N, workspace, K, dx, K, st);
-}
-
-int dq_linear_nf4_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* packed, const void* absmax,
-                        int scale_dtype, int64_t K, void* dx, void* workspace, size_t workspace_bytes,
-                        dq_stream_t stream) {
-  if (scale_dtype != DQ_DTYPE_F32 && scale_dtype != DQ_DTYPE_BF16) return DQ_ERR_ARG;
-  return dgrad_impl(kFmtNF4, dy, M, N, packed, absmax, scale_dtype == DQ_DTYPE_BF16, 0.f, K, dx, workspace,
-                    workspace_bytes, static_cast<cudaStream_t>(stream));
-}
-
-int dq_linear_fp8_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* w8, float scale, int64_t K, void* dx,
-                        void* workspace, size_t workspace_bytes, dq_stream_t stream) {
-  return dgrad_impl(kFmtFP8, dy, M, N, w8, nullptr, 0, scale, K, dx, workspace, workspace_bytes,
-                    static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

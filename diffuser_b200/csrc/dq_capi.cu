@@ -1134,6 +1134,12 @@ int bf16_gemm(const void* x, int64_t M, int64_t K, const void* w, int64_t N, voi
   return launch_bf16_gemm2_bm<-1>(d, p, mx, ma, g, st);
 }
 
+bool bf16_tile_map(void* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                   uint32_t box_outer) {
+  return make_map_2d(static_cast<CUtensorMap*>(map), base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, inner, outer, row_bytes,
+                     64, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 int device_sms(int* sms) {
   DeviceInfo* d = nullptr;
   const int rc = current_device(&d);

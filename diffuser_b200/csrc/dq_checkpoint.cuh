@@ -1,5 +1,4 @@
-// dq_checkpoint.cuh -- activations kept in 8 bits until the backward pass, and
-// the transposed decode of a quantized weight for its input gradient
+// dq_checkpoint.cuh -- activations kept in 8 bits until the backward pass
 // (include/dq_adapter.h).
 #pragma once
 
@@ -152,62 +151,6 @@ __global__ void __launch_bounds__(256)
           make_uint4(narrow(mul2(widen(p.x), by)), narrow(mul2(widen(p.y), by)), narrow(mul2(widen(p.z), by)),
                      narrow(mul2(widen(p.w), by)));
     }
-  }
-}
-
-// ------------------------------------------------- transposed weight decode
-// W [N, K] (NF4 or e4m3) -> bf16 W^T [K, N], the operand the bf16 pair GEMM
-// takes for dx = dy . W.  A CTA decodes 128 weight rows x 64 k (one NF4 block
-// per row): thread (pair p of rows, quarter kc of the 64 k) decodes 16 k of
-// rows 2p and 2p + 1, pairs the two rows' values at each k with byte permutes
-// and stores them at [k][p ^ 8 kc] (conflict-free: the four quarters of a row
-// pair sit in distinct banks), then the CTA writes 256-byte row pieces of W^T.
-// The values are those of dq_dequant_* bit for bit.
-template <int FMT>
-__global__ void __launch_bounds__(256)
-    decode_transposed_kernel(const uint8_t* __restrict__ w, const void* __restrict__ absmax, int sbf,
-                             float fp8_scale, int N, int K, __nv_bfloat16* __restrict__ out) {
-  __shared__ __align__(16) uint32_t tile[64 * 64];  // [k][row pair]
-  const int k0 = blockIdx.x * 64, n0 = blockIdx.y * 128;
-  const int kc = threadIdx.x & 3, p = threadIdx.x >> 2;
-  const int k = k0 + kc * 16;
-  uint32_t o[2][8];  // 16 k of each row as bf16 pairs along k
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int n = n0 + 2 * p + h;
-    if (n < N && k < K) {  // K is a multiple of 16
-      if constexpr (FMT == kFmtNF4) {
-        const uint2 u = *reinterpret_cast<const uint2*>(w + static_cast<int64_t>(n) * (K / 2) + k / 2);
-        const Nf4Planes P =
-            nf4_scaled_planes(nf4_scale2(load_scale(absmax, static_cast<int64_t>(n) * (K / 64) + k / 64, sbf != 0)));
-        nf4_decode_word(u.x, P, o[h]);
-        nf4_decode_word(u.y, P, o[h] + 4);
-      } else {
-        const float s = __bfloat162float(__float2bfloat16_rn(fp8_scale));
-        const uint4 u = *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(n) * K + k);
-        fp8_decode_word(u.x, s, o[h]);
-        fp8_decode_word(u.y, s, o[h] + 2);
-        fp8_decode_word(u.z, s, o[h] + 4);
-        fp8_decode_word(u.w, s, o[h] + 6);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[h][e] = 0u;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    tile[(kc * 16 + 2 * e) * 64 + (p ^ (8 * kc))] = prmt(o[0][e], o[1][e], 0x5410u);
-    tile[(kc * 16 + 2 * e + 1) * 64 + (p ^ (8 * kc))] = prmt(o[0][e], o[1][e], 0x7632u);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (threadIdx.x >> 4) + 16 * i, ch = threadIdx.x & 15;  // 16-byte chunk of 8 weight rows
-    const int n = n0 + ch * 8;
-    if (k0 + row < K && n < N)  // N is a multiple of 8
-      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(k0 + row) * N + n) =
-          *reinterpret_cast<const uint4*>(&tile[row * 64 + ((ch * 4) ^ (8 * (row >> 4)))]);
   }
 }
 

@@ -23,4 +23,10 @@ enum : unsigned int { kErrIndex = 10u };
 int bf16_gemm(const void* x, int64_t M, int64_t K, const void* w, int64_t N, void* y, int64_t ldy,
               cudaStream_t st);
 
+// Tensor map of a row-major bf16 matrix [outer, inner], rows row_bytes apart, in
+// boxes of [box_outer, 64] elements with the 128-byte swizzle (map: a
+// CUtensorMap); false if the driver refuses it.
+bool bf16_tile_map(void* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                   uint32_t box_outer);
+
 }  // namespace dq

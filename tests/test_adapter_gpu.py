@@ -458,3 +458,46 @@ def test_input_gradient_refusals_and_batches():
         ops.nf4_linear_dgrad(dy.float(), packed, absmax, 128)
     with pytest.raises(ValueError, match="% 8"):
         ops.fp8_linear_dgrad(dy[..., :60], torch.zeros(60, 64, dtype=torch.float8_e4m3fn, device="cuda"), 1.0)
+
+
+# few tokens: the weight is decoded next to the product (one launch); one token
+# tile and two, ragged token counts, sums split 1, 2, 4 and 8 ways, ends inside a
+# 64-row step and inside a 128-feature slab
+@pytest.mark.parametrize("m,n,k", [(512, 2048, 192), (333, 2056, 1024), (300, 4168, 4160), (256, 136, 64),
+                                   (48, 200, 4096), (17, 72, 9024), (16, 64, 128), (400, 1000, 256)])
+@pytest.mark.parametrize("fmt", ["nf4", "fp8"])
+def test_input_gradient_of_few_tokens(m, n, k, fmt):
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(m)
+    w = torch.randn(n, k, generator=g, device="cuda") * 0.02
+    dy = _rn(g, m, n)
+    if fmt == "fp8":
+        k -= 16
+        w8, s = ops.fp8_quantize(w[:, :k].contiguous())
+        s = float(s)  # on the host before the capture
+        call, wd = (lambda d: ops.fp8_linear_dgrad(d, w8, s)), ops.fp8_dequantize(w8, s)
+    else:
+        packed, absmax = ops.ltx23_nf4_quantize(w)
+        call, wd = (lambda d: ops.nf4_linear_dgrad(d, packed, absmax, k)), ops.ltx23_nf4_dequantize(packed, absmax, (n, k))
+    got = call(dy)
+    ref = dy.double() @ wd.double()
+    tol = (n + 8) * U * (dy.double().abs() @ wd.double().abs()) + H * ref.abs()
+    _close(got, ref, tol, fmt)
+    # the same sums in the same order on another stream, replayed from a graph
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call(dy)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            again = call(dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, got)
+    # a row that is not finite stays its own row's affair
+    bad = dy.clone()
+    bad[m // 2, 3], bad[m - 1] = float("nan"), float("inf")
+    out = call(bad)
+    keep = [i for i in range(m) if i not in (m // 2, m - 1)]
+    assert torch.equal(out[keep], got[keep]) and out[m // 2].isnan().all() and not out[m - 1].isfinite().any()
+    assert ops.device_error() == 0
