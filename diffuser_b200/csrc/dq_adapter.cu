@@ -18,12 +18,13 @@ namespace dq {
 namespace {
 
 constexpr int64_t kMaxTokens = 1 << 30;
+constexpr int64_t kMaxRequests = 1 << 20;
 constexpr int kMaxAdapters = 65535;
 constexpr int kMaxRank = 128;
 constexpr int kMaxCluster = 8;
 
 int plan_shape(int64_t M, int64_t R, int A) {
-  return M < 0 || M > kMaxTokens || R < 0 || R > kMaxTokens || A < 1 || A > kMaxAdapters ? DQ_ERR_SHAPE : DQ_OK;
+  return M < 0 || M > kMaxTokens || R < 0 || R > kMaxRequests || A < 1 || A > kMaxAdapters ? DQ_ERR_SHAPE : DQ_OK;
 }
 int bank_shape(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A) {
   if (plan_shape(M, R, A) != DQ_OK || K <= 0 || N <= 0 || K % 8 != 0 || N % 8 != 0 || r <= 0 || r % 8 != 0 ||

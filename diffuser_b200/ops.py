@@ -427,12 +427,17 @@ class AdapterPlan:
         lib = _lib.lib()
         nbytes = int(lib.dq_adapter_plan_bytes(self.tokens, self.requests, self.n_adapters))
         if nbytes == 0:
-            raise ValueError("adapter_plan: tokens must be 0..2^30 and n_adapters 1..65535")
+            raise ValueError("adapter_plan: tokens must be 0..2^30, requests at most 2^20 and n_adapters 1..65535")
         # bytes of adapter_add's workspace per unit of rank
         self.add_workspace = int(lib.dq_adapter_add_workspace(self.tokens, self.requests, 1, self.n_adapters))
         self.words = torch.empty(nbytes // 4, dtype=torch.int32, device=ids.device)
         self.address = self.words.data_ptr()
+        self.version = 0  # how often it has been built
         self.update_(ids, offsets)
+
+    def __setstate__(self, state):  # a copy holds its own words
+        self.__dict__.update(state)
+        self.address = self.words.data_ptr()
 
     def update_(self, ids: torch.Tensor, offsets: torch.Tensor) -> "AdapterPlan":
         """Rebuild in place for new ids / offsets of the same counts (also
@@ -447,6 +452,7 @@ class AdapterPlan:
             _lib.check("dq_adapter_plan", _lib.lib().dq_adapter_plan(
                 _ptr(ids), _ptr(offsets), self.requests, self.tokens, self.n_adapters, self.address,
                 self.words.numel() * 4, _raw_stream(self.words)))
+        self.version += 1
         return self
 
 
@@ -472,6 +478,14 @@ def _check_plan(plan: AdapterPlan, m: int, a: int, like: torch.Tensor) -> None:
         _same_device(plan.words, "plan", like)
 
 
+def _refuse_alias(out: torch.Tensor, op: int, others) -> None:
+    """out's rows are written while other tokens of `others` are still read."""
+    for t, p, name in others:
+        if p == op or (out.is_contiguous() and t.is_contiguous() and
+                       op < p + t.numel() * t.element_size() and p < op + out.numel() * out.element_size()):
+            raise ValueError(f"out must not overlap {name}")
+
+
 def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
                 scale: torch.Tensor, plan: AdapterPlan, act: str | None = None,
                 out: torch.Tensor | None = None, return_hidden: bool = False):
@@ -481,8 +495,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
     input.  down bf16 [A, r, K], up bf16 [A, r, N] (the transposed second
     factor), scale float32 [A].  act as nf4_linear's; the gated ones take y and
     up in the gated row order and return N / 2 columns.  out may be y itself
-    (in place, not with a gated act).  With return_hidden also the bf16
-    [tokens, r] scale_a * x . down_a^T that adapter_backward takes."""
+    (in place, not with a gated act) but overlaps no other operand.  With
+    return_hidden also the bf16 [tokens, r] scale_a * x . down_a^T that
+    adapter_backward takes."""
     _require_cuda(y, "y")
     a, r, k, n = _bank(down, up, scale, y)
     code, n_out = (_lib.DQ_ACT_NONE, n) if act is None else _act_code(act, n)
@@ -500,6 +515,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
         _, op, ldo, mo = _row_operand(out, "out", n_out, y, must_alias=True)
         if mo != m:
             raise ValueError(f"out holds {mo} tokens, y {m}")
+        if m:
+            _refuse_alias(out, op, ((x2, xp, "x"),) if op == yp else ((x2, xp, "x"), (y2, yp, "y unless it is y")))
     hidden = torch.empty((m, r), dtype=_BF16, device=y.device) if return_hidden else None
     nbytes = 0 if return_hidden else plan.add_workspace * r
     ws = _scratch(nbytes, y) if nbytes else None
@@ -513,16 +530,17 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
 
 def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
                      scale: torch.Tensor, plan: AdapterPlan, dx: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None):
+                     out: torch.Tensor | None = None, factors: bool = True):
     """Gradients of adapter_add (without act): returns (dx, ddown, dup).
 
     dy [..., N] is the output's gradient; x the forward's input, as bf16
     [..., K] or as checkpoint_pack packed it; hidden what adapter_add returned.
     dx [..., K], if given, is the shared projection's input gradient
     (nf4_linear_dgrad / fp8_linear_dgrad): the adapters' part is added to it, in
-    `out` (which may be dx) or a new tensor.  ddown / dup have the layouts of
-    down / up, zeros for adapters without tokens.  The same inputs give the
-    same bits."""
+    `out` (which may be dx, and overlaps no other operand) or a new tensor.
+    ddown / dup have the layouts of down / up, zeros for adapters without
+    tokens; with factors=False they are None, and neither is computed.  The same
+    inputs give the same bits."""
     _require_cuda(dy, "dy")
     a, r, k, n = _bank(down, up, scale, dy)
     dy2, dyp, lddy, m = _row_operand(dy, "dy", n, dy)
@@ -555,15 +573,18 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
     _, op, ldo, mo = _row_operand(res, "out", k, dy, must_alias=True)
     if mo != m:
         raise ValueError(f"out holds {mo} tokens, dy {m}")
-    ddown, dup = torch.empty_like(down), torch.empty_like(up)
+    if out is not None and m:
+        other = ((dy2, dyp, "dy"), (x2, xp, "x"), (hidden, hidden.data_ptr(), "hidden"))
+        _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
+    ddown, dup = (torch.empty_like(down), torch.empty_like(up)) if factors else (None, None)
     with _on(dy):
         lib = _lib.lib()
         nbytes = lib.dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
         ws = _scratch(nbytes, dy)
         _lib.check("dq_adapter_backward", lib.dq_adapter_backward(
             dyp, lddy, xp, ldx, scales, hidden.data_ptr(), m, plan.requests, k, n, down.data_ptr(), up.data_ptr(),
-            scale.data_ptr(), r, a, plan.address, dxp, lddx, op, ldo, ddown.data_ptr(), dup.data_ptr(),
-            ws.data_ptr(), nbytes, _raw_stream(dy)))
+            scale.data_ptr(), r, a, plan.address, dxp, lddx, op, ldo, None if ddown is None else ddown.data_ptr(),
+            None if dup is None else dup.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy)))
     return res, ddown, dup
 
 
@@ -629,8 +650,10 @@ def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None)
 
 
 # -------------------------------------------------------- input gradients
-def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor):
+def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor, dtypes):
     _same_device(weight, "weight", dy)
+    if weight.dtype not in dtypes or not weight.is_contiguous():
+        raise TypeError(f"the weight must be contiguous {' or '.join(str(t) for t in dtypes)}, got {weight.dtype}")
     if n % 8 != 0:
         raise ValueError("the input gradient needs out_features % 8 == 0")
     if dy.dtype != _BF16:
@@ -651,9 +674,9 @@ def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tenso
     n = packed.numel() * 2 // k
     if n * k != packed.numel() * 2 or absmax.numel() * NF4_BLOCK != n * k:
         raise ValueError("packed / absmax sizes do not match in_features")
-    dy2, dx, nbytes = _prep_dgrad(dy, n, k, packed)
+    dy2, dx, nbytes = _prep_dgrad(dy, n, k, packed, (torch.uint8,))
     _same_device(absmax, "absmax", dy)
-    am = absmax if absmax.dtype in (_F32, _BF16) else absmax.float()
+    am = (absmax if absmax.dtype in (_F32, _BF16) else absmax.float()).contiguous()
     with _on(dy):
         ws = _scratch(nbytes, dy)
         _lib.check("dq_linear_nf4_dgrad", _lib.lib().dq_linear_nf4_dgrad(
@@ -665,8 +688,10 @@ def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tenso
 def fp8_linear_dgrad(dy: torch.Tensor, w8: torch.Tensor, scale: float) -> torch.Tensor:
     """dx = dy . (e4m3(W) * bf16(scale)), the input gradient of fp8_linear."""
     _require_cuda(dy, "dy")
+    if w8.dim() != 2:
+        raise ValueError(f"w8 must be [out_features, in_features], got {tuple(w8.shape)}")
     n, k = int(w8.shape[0]), int(w8.shape[1])
-    dy2, dx, nbytes = _prep_dgrad(dy, n, k, w8)
+    dy2, dx, nbytes = _prep_dgrad(dy, n, k, w8, (torch.float8_e4m3fn, torch.uint8))
     with _on(dy):
         ws = _scratch(nbytes, dy)
         _lib.check("dq_linear_fp8_dgrad", _lib.lib().dq_linear_fp8_dgrad(

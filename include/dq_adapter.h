@@ -30,7 +30,7 @@ extern "C" {
  * request have no adapter.  Both arrays are device memory and are not read by
  * the host.  An id outside -1..A-1 counts as none, and offsets that decrease
  * or leave 0..M leave every token without an adapter; either is recorded as
- * DQ_ERR_INDEX for dq_device_error.  M <= 2^30, 1 <= A <= 65535, R >= 0.
+ * DQ_ERR_INDEX for dq_device_error.  M <= 2^30, 1 <= A <= 65535, 0 <= R <= 2^20.
  * The plan buffer (dq_adapter_plan_bytes) is 16-byte aligned and needs no
  * initialization; it may be rebuilt in place, also inside a captured graph,
  * as long as M, R and A stay the same. */

@@ -501,3 +501,37 @@ def test_input_gradient_of_few_tokens(m, n, k, fmt):
     keep = [i for i in range(m) if i not in (m // 2, m - 1)]
     assert torch.equal(out[keep], got[keep]) and out[m // 2].isnan().all() and not out[m - 1].isfinite().any()
     assert ops.device_error() == 0
+
+
+def test_outputs_may_not_overlap_what_is_still_read():
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    ids, off = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0], [0, 20]))
+    plan = ops.adapter_plan(ids, off, 20, 1)
+    down, up, scale = _rn(g, 1, 8, 64), _rn(g, 1, 8, 64), torch.ones(1, device="cuda")
+    x, y = _rn(g, 20, 64), _rn(g, 20, 64)
+    want, hidden = ops.adapter_add(y, x, down, up, scale, plan, return_hidden=True)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.adapter_add(y, x, down, up, scale, plan, out=x)
+    both = torch.empty(40, 64, dtype=torch.bfloat16, device="cuda")
+    both[1:21].copy_(y)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.adapter_add(both[1:21], x, down, up, scale, plan, out=both[:20])
+    assert torch.equal(ops.adapter_add(both[1:21], x, down, up, scale, plan, out=both[1:21]), want)
+    dx = ops.adapter_backward(y, x, hidden, down, up, scale, plan)[0]
+    for out in (y, x):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.adapter_backward(y, x, hidden, down, up, scale, plan, out=out)
+    only, none, none2 = ops.adapter_backward(y, x, hidden, down, up, scale, plan, factors=False)
+    assert torch.equal(only, dx) and none is none2 is None
+    # weights whose elements do not follow one another
+    w8 = torch.zeros(64, 128, device="cuda").to(torch.float8_e4m3fn)
+    with pytest.raises(TypeError):
+        ops.fp8_linear_dgrad(_rn(g, 2, 128), w8.t(), 1.0)
+    packed, absmax = ops.ltx23_nf4_quantize(torch.randn(64, 128, generator=g, device="cuda"))
+    with pytest.raises(TypeError):
+        ops.nf4_linear_dgrad(y, torch.stack([packed, packed], 1)[:, 0], absmax, 128)
+    with pytest.raises(TypeError):
+        ops.nf4_linear_dgrad(y, packed.to(torch.int8), absmax, 128)
+    twice = torch.stack([absmax, absmax], 1)
+    assert torch.equal(ops.nf4_linear_dgrad(y, packed, twice[:, 0], 128), ops.nf4_linear_dgrad(y, packed, absmax, 128))
