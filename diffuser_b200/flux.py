@@ -16,6 +16,7 @@ import math
 
 import torch
 import torch.nn.functional as F
+from torch.nn.attention import SDPBackend, sdpa_kernel
 from torch import nn
 
 from . import _lib, modules, ops
@@ -333,40 +334,68 @@ class _GatedNorm(torch.autograd.Function):
                 low(g["dpre_weight"]), None, None, None, None, None)
 
 
+class _Recomputed(torch.autograd.Function):
+    """fused(*tensors) whose backward pass differentiates plain(*tensors), the
+    same result (or tuple) in tensor ops, computed again from the inputs."""
+
+    @staticmethod
+    def forward(ctx, fused, plain, *tensors):
+        ctx.plain = plain
+        ctx.save_for_backward(*tensors)
+        return fused(*tensors)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        wanted = ctx.needs_input_grad[2:]
+        with torch.enable_grad():
+            ins = [t if t is None else t.detach().requires_grad_(w) for t, w in zip(ctx.saved_tensors, wanted)]
+            grads = iter(torch.autograd.grad(ctx.plain(*ins), [t for t, w in zip(ins, wanted) if w], dy))
+        return (None, None, *(next(grads) if w else None for w in wanted))
+
+
+def _recorded(module, *tensors) -> bool:
+    """Whether a call inside a model with adapters is recorded for a backward
+    pass (elsewhere the fused kernels stay outside autograd)."""
+    return getattr(module, "differentiable", False) and torch.is_grad_enabled() and \
+        any(t is not None and t.requires_grad for t in tensors)
+
+
+def _fuse(module, fused, plain, *tensors):
+    """fused(*tensors), through autograd if the call is recorded."""
+    return _Recomputed.apply(fused, plain, *tensors) if _recorded(module, *tensors) else fused(*tensors)
+
+
 def _adaln_ok(x):
     return FUSED_ADALN and x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.shape[-1] % 4 == 0
 
 
 def _modulate(norm, x, scale, shift):
+    plain = lambda x, scale, shift: norm(x) * (scale[:, None] + 1) + shift[:, None]  # noqa: E731
     if _adaln_ok(x) and norm.weight is None and norm.bias is None:
-        return adaln_modulate(x, scale, shift, norm.eps)
-    return norm(x) * (scale[:, None] + 1) + shift[:, None]
+        return _fuse(norm, lambda x, scale, shift: adaln_modulate(x, scale, shift, norm.eps), plain, x, scale, shift)
+    return plain(x, scale, shift)
 
 
-def _gated_add(x, gate, y):
+def _gated_add(x, gate, y, module=None):
+    plain = lambda x, gate, y: x + gate[:, None] * y  # noqa: E731
     if _adaln_ok(x) and y.shape == x.shape:
-        return gated_residual(x, gate, y)
-    return x + gate[:, None] * y
+        return _fuse(module, gated_residual, plain, x, gate, y)
+    return plain(x, gate, y)
 
 
 def _add_and_modulate(x, gate, y, norm, scale, shift):
     """(x + gate * y, norm(that) * (1 + scale) + shift)."""
     if FUSED_BOUNDARY and _adaln_ok(x) and y.shape == x.shape and norm.weight is None and norm.bias is None and \
             x.shape[-1] <= 8192:
-        return gated_norm(x, y, gate, pre="layer", scale=scale, shift=shift, eps=norm.eps, rounding="ops")
-    s = _gated_add(x, gate, y)
+        with torch.set_grad_enabled(_recorded(norm, x, gate, y, scale, shift)):
+            return gated_norm(x, y, gate, pre="layer", scale=scale, shift=shift, eps=norm.eps, rounding="ops")
+    s = _gated_add(x, gate, y, norm)
     return s, _modulate(norm, s, scale, shift)
 
 
 # The linears that take an activation and an output view.
 _ENGINE_LINEARS = (modules.Ltx23Nf4Linear, modules.Ltx23Fp8Linear, modules.AdapterLinear)
-
-
-def _differentiable(x, proj):
-    """Whether an adapted linear's call is recorded for a backward pass (it
-    then writes no caller-given output)."""
-    return isinstance(proj, modules.AdapterLinear) and torch.is_grad_enabled() and \
-        (x.requires_grad or proj.down.requires_grad)
 
 
 # GELU-tanh after the up-projections runs in the quantized linear's epilogue
@@ -607,6 +636,28 @@ class FluxAttention(nn.Module):
             return y[..., :n], y[..., n:2 * n], y[..., 2 * n:]
         return q_proj(x), k_proj(x), v_proj(x)
 
+    def _norm_rope(self, img, txt, norm_img, norm_txt, rope):
+        """One of q, k, v through qk_norm_rope, recorded for a backward pass."""
+        h = self.heads
+        w_img, w_txt = (None if n is None else n.weight for n in (norm_img, norm_txt))
+        eps = 1e-6 if norm_img is None else norm_img.eps
+
+        def rms(t, w):  # RMSNorm.forward
+            if w is None:
+                return t
+            t = t * torch.rsqrt(t.to(torch.float32).pow(2).mean(dim=-1, keepdim=True) + eps)
+            return t.to(w.dtype) * w
+
+        def plain(img, txt, w_img, w_txt):
+            t = rms(img.unflatten(-1, (h, -1)), w_img)
+            if txt is not None:
+                t = torch.cat([rms(txt.unflatten(-1, (h, -1)), w_txt), t], dim=1)
+            t = t.transpose(1, 2)
+            return t if rope is None else apply_rotary_emb(t, rope)
+
+        fused = lambda img, txt, w_img, w_txt: qk_norm_rope(img, txt, h, w_img, w_txt, rope, eps)  # noqa: E731
+        return _Recomputed.apply(fused, plain, img, txt, w_img, w_txt)
+
     def _forward_fused(self, x, ctx, rope, out=None):
         """The same computation with the norm / concat / transpose / rotary
         chain in one kernel per tensor and the split back in one more."""
@@ -618,7 +669,12 @@ class FluxAttention(nn.Module):
                                       self.add_k_proj, self.add_v_proj)
             wq_t, wk_t = self.norm_added_q.weight, self.norm_added_k.weight
         q_i, k_i, v_i = self._qkv(x, getattr(self, "to_qkv", None), self.to_q, self.to_k, self.to_v)
-        if self.norm_q.eps == self.norm_k.eps:
+        recorded = _recorded(self, q_i, k_i, v_i, q_t, k_t, v_t)
+        if recorded:
+            q = self._norm_rope(q_i, q_t, self.norm_q, None if ctx is None else self.norm_added_q, rope)
+            k = self._norm_rope(k_i, k_t, self.norm_k, None if ctx is None else self.norm_added_k, rope)
+            v = self._norm_rope(v_i, v_t, None, None, None)
+        elif self.norm_q.eps == self.norm_k.eps:
             q, k, v = qkv_norm_rope((q_i, k_i, v_i), (q_t, k_t, v_t), h,
                                     (self.norm_q.weight, self.norm_k.weight, None), (wq_t, wk_t, None),
                                     (rope is not None, rope is not None, False), rope, self.norm_q.eps)
@@ -626,8 +682,19 @@ class FluxAttention(nn.Module):
             q = qk_norm_rope(q_i, q_t, h, self.norm_q.weight, wq_t, rope, self.norm_q.eps)
             k = qk_norm_rope(k_i, k_t, h, self.norm_k.weight, wk_t, rope, self.norm_k.eps)
             v = qk_norm_rope(v_i, v_t, h)
-        att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
+        if recorded:
+            # not by cuDNN, whose backward pass was seen to return NaN (44 tokens
+            # x 64, from finite operands, outputs and log-sums that were right)
+            with sdpa_kernel([SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION, SDPBackend.MATH]):
+                att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
+        else:
+            att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
         txt_len = 0 if ctx is None else ctx.shape[1]
+        if recorded:
+            rows = att.transpose(1, 2).flatten(2)
+            if ctx is not None:
+                return self.to_out[0](rows[:, txt_len:].contiguous()), self.to_add_out(rows[:, :txt_len].contiguous())
+            return rows if self.pre_only else self.to_out[0](rows)
         # `out` (pre-only attention): the image tokens go straight there
         txt, img = heads_to_tokens(att, txt_len, out if (self.pre_only and ctx is None) else None)
         if ctx is not None:
@@ -655,9 +722,9 @@ class DoubleBlock(nn.Module):
         nc, cg_msa, csh_mlp, csc_mlp, cg_mlp = self.norm1_context(ctx, temb)
         a_img, a_txt = self.attn(nx, nc, rope)
         x, h = _add_and_modulate(x, g_msa, a_img, self.norm2, sc_mlp, sh_mlp)
-        x = _gated_add(x, g_mlp, self.ff(h))
+        x = _gated_add(x, g_mlp, self.ff(h), self)
         ctx, h = _add_and_modulate(ctx, cg_msa, a_txt, self.norm2_context, csc_mlp, csh_mlp)
-        ctx = _gated_add(ctx, cg_mlp, self.ff_context(h))
+        ctx = _gated_add(ctx, cg_mlp, self.ff_context(h), self)
         if ctx.dtype == torch.float16:
             ctx = ctx.clamp(-65504, 65504)
         return ctx, x
@@ -677,7 +744,8 @@ class SingleBlock(nn.Module):
     def forward(self, x, temb, rope):
         n, gate = self.norm(x, temb)
         if FUSED_CONCAT and _fused_ok(n, self.attn.norm_q.weight.shape[0]) and \
-                isinstance(self.proj_mlp, _ENGINE_LINEARS) and not _differentiable(n, self.proj_mlp):
+                isinstance(self.proj_mlp, _ENGINE_LINEARS) and \
+                not (getattr(self, "differentiable", False) and torch.is_grad_enabled()):
             # attention and MLP outputs land in the two column ranges of the
             # proj_out input, which is then read whole (no concatenation pass)
             d_attn = self.attn.to_q.out_features
@@ -685,10 +753,10 @@ class SingleBlock(nn.Module):
                               dtype=torch.bfloat16, device=n.device)
             _proj_gelu_tanh(self.proj_mlp, n, out=cat[..., d_attn:])
             self.attn(n, rope=rope, out=cat[..., :d_attn])
-            return _gated_add(x, gate, self.proj_out(cat))
+            return _gated_add(x, gate, self.proj_out(cat), self)
         mlp = _proj_gelu_tanh(self.proj_mlp, n)
         a = self.attn(n, rope=rope)
-        x = _gated_add(x, gate, self.proj_out(torch.cat([a, mlp], dim=2)))
+        x = _gated_add(x, gate, self.proj_out(torch.cat([a, mlp], dim=2)), self)
         if x.dtype == torch.float16:
             x = x.clamp(-65504, 65504)
         return x

@@ -19,6 +19,45 @@ from . import ops
 NF4_BLOCK = ops.NF4_BLOCK
 
 
+def _activate(y: torch.Tensor, act: str) -> torch.Tensor:
+    """The activation of a projection's output, in tensor ops."""
+    if act == "gelu_tanh":
+        return nn.functional.gelu(y, approximate="tanh")
+    gate, up = y.unflatten(-1, (-1, 2, 16)).unbind(-2)  # the gated row order
+    gate = nn.functional.silu(gate) if act == "swiglu" else nn.functional.gelu(gate, approximate="tanh")
+    return (gate * up).flatten(-2)
+
+
+class _FrozenProjection(torch.autograd.Function):
+    """A quantized linear whose input takes a gradient: the forward pass is the
+    engine's, the backward pass its input gradient (behind an activation, whose
+    argument is computed again)."""
+
+    @staticmethod
+    def forward(ctx, x, linear, act):
+        ctx.linear, ctx.act = linear, act
+        if act is not None:
+            ctx.save_for_backward(x)
+        return linear._run(x, act, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        if ctx.act is not None:
+            with torch.enable_grad():
+                y = ctx.linear._run(ctx.saved_tensors[0], None, None).requires_grad_()
+                dy, = torch.autograd.grad(_activate(y, ctx.act), y, dy)
+        return ctx.linear.input_grad(dy), None, None
+
+
+def _run_linear(linear, x, act, out):
+    if getattr(linear, "differentiable", False) and torch.is_grad_enabled() and x.requires_grad:
+        if out is not None:
+            raise RuntimeError("a differentiable call takes no out")
+        return _FrozenProjection.apply(x, linear, act)
+    return linear._run(x, act, out)
+
+
 class Ltx23Nf4Linear(nn.Module):
     """NF4 linear (R/nf4_ltx23.R:211-247).
 
@@ -40,6 +79,7 @@ class Ltx23Nf4Linear(nn.Module):
         else:
             self.register_parameter("bias", None)
         self.gated_act = None
+        self.differentiable = False  # in its input (attach_adapters sets it)
 
     def set_nf4_weight(self, packed: torch.Tensor, absmax: torch.Tensor):
         """Copy packed codes and block scales into the buffers (R/nf4_ltx23.R:228-234)."""
@@ -81,8 +121,15 @@ class Ltx23Nf4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor, act: str | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
+        return _run_linear(self, x, act or self.gated_act, out)
+
+    def _run(self, x, act, out):
         return ops.nf4_linear(x, self.weight_nf4, self.weight_absmax, self.out_features, self.bias,
-                              act=act or self.gated_act, out=out)
+                              act=act, out=out)
+
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        """dy . W for a gradient dy of the projection's output."""
+        return ops.nf4_linear_dgrad(dy, self.weight_nf4, self.weight_absmax, self.in_features)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, format=nf4"
@@ -110,6 +157,7 @@ class Ltx23Fp8Linear(nn.Module):
         else:
             self.register_parameter("bias", None)
         self.gated_act = None
+        self.differentiable = False  # in its input (attach_adapters sets it)
 
     def set_fp8_weight(self, weight: torch.Tensor, scale, pin: bool = False):
         """Store the e4m3 weight and float32 scale (R/fp8_ltx23.R:60-68)."""
@@ -141,8 +189,14 @@ class Ltx23Fp8Linear(nn.Module):
 
     def forward(self, x: torch.Tensor, act: str | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-        act = act or self.gated_act
+        return _run_linear(self, x, act or self.gated_act, out)
+
+    def _run(self, x, act, out):
         return ops.fp8_linear(x, self._weight_on(x.device), self._scale_f, self.bias, act=act, out=out)
+
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        """dy . W for a gradient dy of the projection's output."""
+        return ops.fp8_linear_dgrad(dy, self._weight_on(dy.device), self._scale_f)
 
     def _weight_on(self, device: torch.device) -> torch.Tensor:
         if self.weight_fp8 is None:
@@ -224,15 +278,29 @@ class AdapterSelection:
     """Which adapter each batch element uses: ids, int32 on the GPU, one per
     element (-1: none).  Every adapted linear of a model shares it; the plan for
     a token count is built at its first use (an element's tokens follow one
-    another, equally many for each)."""
+    another, equally many for each), on the stream of that use, which the other
+    streams that use it wait for.  A graph capture takes plans that were built
+    before it (by a call, or by plan(tokens))."""
 
     def __init__(self, ids: torch.Tensor, n_adapters: int):
         if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or \
                 ids.numel() == 0:
             raise ValueError("ids must be a 1-d int32 CUDA tensor, one entry per batch element")
-        self.ids = ids.contiguous()
+        self.ids = ids.clone()
         self.n_adapters = int(n_adapters)
-        self._plans: dict = {}
+        self._plans: dict = {}  # tokens -> plan
+        self._built: dict = {}  # tokens -> stream handle, event
+
+    def __getstate__(self):  # a copy builds its own plans
+        return dict(self.__dict__, _plans={}, _built={})
+
+    def _offsets(self, tokens: int) -> torch.Tensor:
+        batch = self.ids.numel()
+        return torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
+
+    def _mark(self, tokens: int) -> None:
+        stream = torch.cuda.current_stream(self.ids.device)
+        self._built[tokens] = (stream.cuda_stream, stream.record_event())
 
     def plan(self, tokens: int) -> ops.AdapterPlan:
         plan = self._plans.get(tokens)
@@ -240,18 +308,34 @@ class AdapterSelection:
             batch = self.ids.numel()
             if tokens % batch != 0:
                 raise ValueError(f"{tokens} tokens are not a whole number per element of a batch of {batch}")
-            offsets = torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
-            plan = self._plans[tokens] = ops.adapter_plan(self.ids, offsets, tokens, self.n_adapters)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the plan for {tokens} tokens must be built before a capture: run the call once, "
+                                   "or selection.plan(tokens)")
+            with torch.cuda.device(self.ids.device):
+                plan = ops.adapter_plan(self.ids, self._offsets(tokens), tokens, self.n_adapters)
+                self._mark(tokens)
+            self._plans[tokens] = plan
+            return plan
+        handle, event = self._built[tokens]
+        if handle != ops._raw_stream(self.ids) and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.ids.device)
+            stream.wait_event(event)
+            plan.words.record_stream(stream)
         return plan
 
     def update_(self, ids: torch.Tensor) -> "AdapterSelection":
         """Other adapters for the same batch size: the plans built so far are
-        rebuilt in place (captured graphs that read them see the new ones)."""
-        self.ids.copy_(ids)
-        batch = self.ids.numel()
-        for tokens, plan in self._plans.items():
-            offsets = torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
-            plan.update_(self.ids, offsets)
+        rebuilt in place (captured graphs that read them see the new ones).  Not
+        between a call and its backward pass, which then raises; calls on other
+        streams must have finished."""
+        if not isinstance(ids, torch.Tensor) or ids.shape != self.ids.shape or ids.dtype != torch.int32:
+            raise ValueError(f"ids must hold {self.ids.numel()} int32 entries, as before")
+        with torch.cuda.device(self.ids.device):
+            self.ids.copy_(ids)
+            for tokens, plan in self._plans.items():
+                plan.update_(self.ids, self._offsets(tokens))
+                if not torch.cuda.is_current_stream_capturing():
+                    self._mark(tokens)
         return self
 
 
@@ -267,16 +351,19 @@ class _AdaptedProjection(torch.autograd.Function):
             ctx.save_for_backward(hidden, down, up, scale, packed.codes, packed.scales)
         else:
             ctx.save_for_backward(hidden, down, up, scale, x)
-        ctx.plan, ctx.base, ctx.pack = plan, base, pack
+        ctx.plan, ctx.version, ctx.base, ctx.pack = plan, plan.version, base, pack
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if ctx.plan.version != ctx.version:
+            raise RuntimeError("the adapter plan was rebuilt for another batch after this call")
         hidden, down, up, scale, *x = ctx.saved_tensors
         x = ops.PackedActivation(*x) if ctx.pack else x[0]
         dx = ctx.base.input_grad(dy) if ctx.needs_input_grad[0] else None
-        dx, ddown, dup = ops.adapter_backward(dy, x, hidden, down, up, scale, ctx.plan, dx=dx, out=dx)
+        dx, ddown, dup = ops.adapter_backward(dy, x, hidden, down, up, scale, ctx.plan, dx=dx, out=dx,
+                                              factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return dx if ctx.needs_input_grad[0] else None, ddown, dup, None, None, None, None
 
 
@@ -290,7 +377,9 @@ class AdapterLinear(nn.Module):
     pass a plan, before calling; without either the base runs alone.  With
     gradients enabled the call is differentiable in x and the factors, and
     keeps its input for the backward pass as it is or, with
-    ``pack_activations``, in 8 bits."""
+    ``pack_activations``, in 8 bits.  (As for any leaf of PyTorch's autograd: do
+    not capture a backward pass into a CUDA graph while an eager graph over the
+    same factors is alive; delete its results first.)"""
 
     def __init__(self, base: nn.Module, n_adapters: int, rank: int, pack_activations: bool = False):
         super().__init__()
@@ -302,6 +391,7 @@ class AdapterLinear(nn.Module):
         if pack_activations and base.in_features % 16 != 0:
             raise ValueError("8-bit activations need in_features % 16 == 0")
         self.base = base
+        base.differentiable = True
         self.in_features, self.out_features = base.in_features, base.out_features
         self.pack_activations = bool(pack_activations)
         dev = base.weight_nf4.device if isinstance(base, Ltx23Nf4Linear) else \
@@ -344,16 +434,10 @@ class AdapterLinear(nn.Module):
 
     def project(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """The base's projection alone, without an activation."""
-        b = self.base
-        if isinstance(b, Ltx23Nf4Linear):
-            return ops.nf4_linear(x, b.weight_nf4, b.weight_absmax, b.out_features, b.bias, out=out)
-        return ops.fp8_linear(x, b._weight_on(x.device), b._scale_f, b.bias, out=out)
+        return self.base._run(x, None, out)
 
     def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
-        b = self.base
-        if isinstance(b, Ltx23Nf4Linear):
-            return ops.nf4_linear_dgrad(dy, b.weight_nf4, b.weight_absmax, b.in_features)
-        return ops.fp8_linear_dgrad(dy, b._weight_on(dy.device), b._scale_f)
+        return self.base.input_grad(dy)
 
     def forward(self, x: torch.Tensor, act: str | None = None, out: torch.Tensor | None = None,
                 plan: ops.AdapterPlan | None = None) -> torch.Tensor:
@@ -366,7 +450,7 @@ class AdapterLinear(nn.Module):
             if out is not None or act in ops.GATED_ACTS:
                 raise RuntimeError("a differentiable call takes neither out nor a gated activation")
             y = _AdaptedProjection.apply(x, self.down, self.up, self.scale, plan, self, self.pack_activations)
-            return y if act is None else nn.functional.gelu(y, approximate="tanh")
+            return y if act is None else _activate(y, act)
         down, up = self.down.detach(), self.up.detach()
         if act is None:
             y = self.project(x, out=out)
@@ -382,12 +466,19 @@ def attach_adapters(model: nn.Module, n_adapters: int, rank: int, is_adapted_key
     """Wrap the model's quantized linears (those whose ``<name>.weight`` key
     is_adapted_key accepts; all of them without it) in AdapterLinear.  Linears
     that flux.fuse_qkv_projections concatenated are dropped where one of their
-    parts is wrapped.  Returns the wrapped names."""
+    parts is wrapped; linears that have a bank already keep it.  The model's
+    modules are marked differentiable: with gradients enabled, the quantized
+    linears that were not wrapped and the FLUX blocks' fused kernels then pass
+    gradients on too.  Returns the wrapped names."""
     wrapped = []
+    for mod in model.modules():
+        mod.differentiable = True
     for name, mod in list(model.named_modules()):
         if not isinstance(mod, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
             continue
         segs = name.split(".")
+        if len(segs) > 1 and isinstance(_walk(model, segs[:-1]), AdapterLinear):
+            continue
         if segs[-1] in ("to_qkv", "add_qkv") or (is_adapted_key is not None and not is_adapted_key(name + ".weight")):
             continue
         parent = _walk(model, segs[:-1]) if len(segs) > 1 else model

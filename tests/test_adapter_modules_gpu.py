@@ -234,3 +234,175 @@ def test_flux_with_adapters_serves_every_element_its_own():
         assert torch.equal(model(*inputs), none)
         with pytest.raises(ValueError):
             modules.select_adapters(nn.Linear(2, 2), ids)
+
+
+def _reference64(model, ids):
+    """The model in 64 bits: dequantized weights, plain adapters, tensor ops."""
+    import copy
+    from diffuser_b200 import modules, ops
+
+    class Plain(nn.Module):
+        def __init__(self, m):
+            super().__init__()
+            base = m.base if isinstance(m, modules.AdapterLinear) else m
+            self.out_features = base.out_features
+            w = ops.ltx23_nf4_dequantize(base.weight_nf4, base.weight_absmax.float(),
+                                         (base.out_features, base.in_features))
+            self.weight = nn.Parameter(w.double(), requires_grad=False)
+            self.bias = None if base.bias is None else nn.Parameter(base.bias.detach().double(), requires_grad=False)
+            self.bank = None
+            if base is not m:
+                self.down, self.up = (nn.Parameter(t.detach().double()) for t in (m.down, m.up))
+                self.bank = m.scale.double()
+
+        def forward(self, x):
+            y = nn.functional.linear(x, self.weight, self.bias)
+            if self.bank is None:
+                return y
+            rows = x.view(len(ids), -1, x.shape[-1])
+            add = [self.bank[a] * (r @ self.down[a].T) @ self.up[a] if a >= 0 else r.new_zeros(r.shape[0], y.shape[-1])
+                   for r, a in zip(rows, ids)]
+            return y + torch.stack(add).view(y.shape)
+
+    ref = copy.deepcopy(model)
+    for name, mod in list(ref.named_modules()):
+        inner = isinstance(mod, (modules.Ltx23Nf4Linear, modules.AdapterLinear))
+        if inner and not name.endswith(".base") and not name.endswith("_qkv"):
+            parent = modules._walk(ref, name.split(".")[:-1])
+            leaf = name.split(".")[-1]
+            if leaf.isdigit():
+                parent[int(leaf)] = Plain(mod)
+            else:
+                setattr(parent, leaf, Plain(mod))
+    return ref.double()
+
+
+# all linears, those of the attentions (the rest pass gradients on), and those
+# of the feed-forwards alone (next to the concatenated q, k, v)
+@pytest.mark.parametrize("which", ["all", "attn", "ff"])
+def test_flux_trains_its_adapters(which):
+    from diffuser_b200 import modules
+    model, inputs = _tiny_flux(), _flux_inputs(3)
+    bare = model(*inputs).detach()
+    accept = {"all": None, "attn": lambda key: ".attn." in key,
+              "ff": lambda key: ".ff" in key or "proj_mlp" in key}[which]
+    assert modules.attach_adapters(model, 3, 8, accept, pack_activations=False)
+    for i, m in enumerate(m for m in model.modules() if isinstance(m, modules.AdapterLinear)):
+        _fill(m, 40 + i)
+    assert modules.attach_adapters(model, 3, 8, accept if accept else lambda key: False) == []  # they keep theirs
+    ids = [2, -1, 0]
+    x = inputs[0].clone().requires_grad_()
+    if which == "ff":  # (the concatenated q, k, v stay) the bits of the bare model, differentiable now
+        assert torch.equal(model(*inputs).detach(), bare)
+    modules.select_adapters(model, torch.tensor(ids, dtype=torch.int32, device="cuda"))
+    out = model(x, *inputs[1:])
+    with torch.no_grad():
+        assert _far(out, model(*inputs).double()) <= 8 * H  # the recorded call's values
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dout = torch.randn(out.shape, generator=g, device="cuda").to(torch.bfloat16)
+    out.backward(dout)
+    ref = _reference64(model, ids)
+    x64 = inputs[0].double().requires_grad_()
+    want = ref(x64, *(t.double() for t in inputs[1:4]), inputs[4])
+    want.backward(dout.double())
+    # About 40 roundings lie on a path through the blocks and as many on the way
+    # back, each of at most H and H / sqrt(3) in the mean square: independent
+    # ones add up to sqrt(80 / 3) H = 0.02, and sums of paths that partly cancel
+    # (the residual adds, the norms' means) to a few times that.  A path that is
+    # cut loses a share of the gradient, not a few per cent of it.
+    assert _far(out, want.detach()) <= 0.1
+    assert _far(x.grad, x64.grad) <= 0.1
+    plain = dict(ref.named_modules())
+    banks = [(n, m) for n, m in model.named_modules() if isinstance(m, modules.AdapterLinear)]
+    assert len(banks) == {"all": 26, "attn": 8 + 2 * 3, "ff": 4 + 2}[which]
+    for name, m in banks:
+        for mine, theirs in ((m.down.grad, plain[name].down.grad), (m.up.grad, plain[name].up.grad)):
+            assert _far(mine, theirs) <= 0.1, name
+            assert not mine[1].any() and mine[0].any() and mine[2].any(), name
+
+
+def test_selections_and_plans_are_guarded():
+    from diffuser_b200 import modules, ops
+    lin, _, _ = _linear("nf4", 64, 64, 3)
+    mod = modules.AdapterLinear(lin, 2, 8)
+    _fill(mod, 1)
+    ids = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    sel = mod.selection = modules.AdapterSelection(ids, 2)
+    x = torch.randn(2, 6, 64, device="cuda").to(torch.bfloat16).requires_grad_()
+    before = mod(x).detach()
+    ids.zero_()  # the caller's own tensor
+    assert torch.equal(mod(x), before) and sel.ids.tolist() == [1, 0]
+    # a plan rebuilt between a call and its backward pass
+    y = mod(x)
+    sel.update_(torch.tensor([0, 0], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="rebuilt"):
+        y.sum().backward()
+    mod(x).sum().backward()
+    for bad in (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda"), [0, 1]):
+        with pytest.raises(ValueError):
+            sel.update_(bad)
+    # a plan made inside a capture would hold nothing until its replay
+    stream = torch.cuda.Stream()
+    with torch.no_grad(), torch.cuda.stream(stream):
+        stream.wait_stream(torch.cuda.default_stream())
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            with pytest.raises(RuntimeError, match="before a capture"):
+                sel.plan(2)
+        finally:
+            graph.capture_end()
+        want = mod(x)  # its plan from another stream
+    torch.cuda.default_stream().wait_stream(stream)
+    assert torch.equal(want, mod(x).detach())
+    # one factor frozen, both frozen, the input frozen
+    d = torch.randn(2, 6, 64, device="cuda").to(torch.bfloat16)
+    grads = {}
+    for frozen in ((), ("down",), ("down", "up"), ("x",)):
+        for n, t in (("down", mod.down), ("up", mod.up), ("x", x)):
+            t.requires_grad_(n not in frozen)
+            t.grad = None
+        mod(x).backward(d)
+        for n, t in (("down", mod.down), ("up", mod.up), ("x", x)):
+            assert (t.grad is None) == (n in frozen), (frozen, n)
+            if t.grad is not None:
+                assert torch.equal(t.grad, grads.setdefault(n, t.grad.clone())), (frozen, n)
+    # a copy of the module has its own plans
+    import copy
+    twin = copy.deepcopy(mod)
+    assert twin.selection is not sel and not twin.selection._plans and torch.equal(twin(x).detach(), mod(x).detach())
+    plan = copy.deepcopy(sel.plan(12))
+    assert plan.address == plan.words.data_ptr() != sel.plan(12).address
+    # no tokens
+    with torch.no_grad():
+        assert mod(x[:, :0]).shape == (2, 0, 64)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("act", [None, "gelu_tanh", "swiglu"])
+@pytest.mark.parametrize("fmt", ["nf4", "fp8"])
+def test_a_frozen_linear_passes_gradients_on(fmt, act):
+    from diffuser_b200 import modules
+    lin, wd, bias = _linear(fmt, 128, 192, 6)
+    if act == "swiglu":
+        lin.to_gated("swiglu")
+    x = torch.randn(3, 7, 192, device="cuda").to(torch.bfloat16).requires_grad_()
+    call = lambda: lin(x, act=act if act == "gelu_tanh" else None)  # noqa: E731
+    assert not call().requires_grad  # outside autograd, as ever
+    lin.differentiable = True
+    y = call()
+    with torch.no_grad():
+        assert torch.equal(y, call())
+    dy = torch.randn(y.shape, device="cuda").to(torch.bfloat16)
+    y.backward(dy)
+    x64 = x.detach().double().requires_grad_()
+    z = x64 @ wd.T + bias
+    if act == "gelu_tanh":
+        z = nn.functional.gelu(z, approximate="tanh")
+    elif act == "swiglu":
+        z = nn.functional.silu(z[..., :64]) * z[..., 64:]
+    z.backward(dy.double())
+    # roundings: the projection, two of the activation, its gradient's three and dx
+    assert _far(y, z.detach()) <= 8 * H and _far(x.grad, x64.grad) <= 2 * 8 * H
+    with pytest.raises(RuntimeError, match="out"):
+        lin(x, out=torch.empty(21, 128 if act != "swiglu" else 64, device="cuda", dtype=torch.bfloat16))
