@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 from .build import LIB_PATH
 
@@ -135,6 +136,14 @@ SIGNATURES = {
     "dq_plan_info": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, ctypes.c_int] + [ctypes.POINTER(ctypes.c_int)] * 4),
 }
 
+# Entries that call() reaches through their packed form (include/dq_packed.h):
+# one string of 8-byte words instead of an argument list, which ctypes converts
+# one by one.
+PACKED = ("dq_adapter_add", "dq_adapter_backward", "dq_checkpoint_pack", "dq_checkpoint_unpack",
+          "dq_linear_nf4_dgrad", "dq_linear_fp8_dgrad", "dq_gated_norm", "dq_gated_norm_backward")
+SIGNATURES.update({name + "_packed": (ctypes.c_int, [ctypes.c_char_p]) for name in PACKED})
+_CALLS: dict = {}  # name -> (function, packer)
+
 DQ_OK = 0
 DQ_ERR_TIMEOUT = 5
 DQ_ERR_SCRATCH_LIMIT = 9
@@ -170,6 +179,9 @@ def lib() -> ctypes.CDLL:
             fn = getattr(h, name)
             fn.restype = res
             fn.argtypes = args
+        for name in PACKED:
+            form = "=" + "".join("d" if t is ctypes.c_float else "q" for t in SIGNATURES[name][1])
+            _CALLS[name] = getattr(h, name + "_packed"), struct.Struct(form).pack
         _LIB = h
     return _LIB
 
@@ -181,6 +193,16 @@ def status_string(status: int) -> str:
 def check(fn: str, status: int) -> None:
     if status != DQ_OK:
         raise DqError(fn, status)
+
+
+def call(name: str, *args) -> None:
+    """The entry `name` of PACKED with its arguments (0 for a null pointer)."""
+    if _LIB is None:
+        lib()
+    fn, pack = _CALLS[name]
+    status = fn(pack(*args))
+    if status != DQ_OK:
+        raise DqError(name, status)
 
 
 def version() -> str:

@@ -172,7 +172,7 @@ _ROUNDINGS = {"once": _lib.DQ_ROUND_ONCE, "ops": _lib.DQ_ROUND_OPS}
 
 
 def _address(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _token_rows(t, name, like):
@@ -250,8 +250,8 @@ def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_w
     followed by adaln_modulate).  Returns (s, h), differentiable in every
     tensor where gradients are enabled (with the gradients of the formula,
     whatever the rounding)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, y, gate, scale, shift, post_weight, pre_weight)):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad
+                                        for t in (x, y, gate, scale, shift, post_weight, pre_weight)]):
         return _GatedNorm.apply(x, y, gate, scale, shift, post_weight, pre_weight, post, pre, residual_scale, eps,
                                 rounding)
     gate, ldg, scale, shift, ldm, pw, qw = _norm_args(x, gate, scale, shift, post, pre, post_weight, pre_weight)
@@ -265,10 +265,9 @@ def gated_norm(x, y, gate=None, *, post=None, pre="rms", post_weight=None, pre_w
     if x.numel() == 0:
         return s, h
     with ops._on(x):
-        _lib.check("dq_gated_norm", _lib.lib().dq_gated_norm(
-            x2.data_ptr(), ldx, y2.data_ptr(), ldy, b * n, n, d, _address(gate), ldg, _address(scale), _address(shift),
-            ldm, _address(pw), _address(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, _ROUNDINGS[rounding],
-            s.data_ptr(), d, h.data_ptr(), d, ops._raw_stream(x)))
+        _lib.call("dq_gated_norm", x2.data_ptr(), ldx, y2.data_ptr(), ldy, b * n, n, d, _address(gate), ldg,
+                  _address(scale), _address(shift), ldm, _address(pw), _address(qw), _NORMS[post], _NORMS[pre],
+                  residual_scale, eps, _ROUNDINGS[rounding], s.data_ptr(), d, h.data_ptr(), d, ops._raw_stream(x))
     return s, h
 
 
@@ -298,15 +297,14 @@ def gated_norm_backward(ds, dh, s, y, gate=None, *, post=None, pre="rms", post_w
                 g.zero_()
         return out
     with ops._on(s):
-        lib = _lib.lib()
-        nbytes = lib.dq_gated_norm_backward_workspace(b * n, n, d)
+        nbytes = _lib.lib().dq_gated_norm_backward_workspace(b * n, n, d)
         ws = ops._scratch(nbytes, s)
-        _lib.check("dq_gated_norm_backward", lib.dq_gated_norm_backward(
-            _address(ds2), ldds, dh2.data_ptr(), lddh, s2.data_ptr(), lds, y2.data_ptr(), ldy, b * n, n, d,
-            _address(gate), ldg, _address(scale), ldm, _address(pw), _address(qw), _NORMS[post], _NORMS[pre],
-            residual_scale, eps, dx.data_ptr(), d, dy.data_ptr(), d, _address(out["dgate"]), _address(out["dscale"]),
-            _address(out["dshift"]), _address(out["dpost_weight"]), _address(out["dpre_weight"]), ws.data_ptr(), nbytes,
-            ops._raw_stream(s)))
+        _lib.call("dq_gated_norm_backward", _address(ds2), ldds, dh2.data_ptr(), lddh, s2.data_ptr(), lds,
+                  y2.data_ptr(), ldy, b * n, n, d, _address(gate), ldg, _address(scale), ldm, _address(pw),
+                  _address(qw), _NORMS[post], _NORMS[pre], residual_scale, eps, dx.data_ptr(), d, dy.data_ptr(), d,
+                  _address(out["dgate"]), _address(out["dscale"]), _address(out["dshift"]),
+                  _address(out["dpost_weight"]), _address(out["dpre_weight"]), ws.data_ptr(), nbytes,
+                  ops._raw_stream(s))
     return out
 
 

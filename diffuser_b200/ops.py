@@ -521,10 +521,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
     nbytes = 0 if return_hidden else plan.add_workspace * r
     ws = _scratch(nbytes, y) if nbytes else None
     with _on(y):
-        _lib.check("dq_adapter_add", _lib.lib().dq_adapter_add(
-            yp, ldy, xp, ldx, m, plan.requests, k, n, down.data_ptr(), up.data_ptr(), scale.data_ptr(), r, a,
-            plan.address, code, op, ldo, None if hidden is None else hidden.data_ptr(),
-            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(y)))
+        _lib.call("dq_adapter_add", yp, ldy, xp, ldx, m, plan.requests, k, n, down.data_ptr(), up.data_ptr(),
+                  scale.data_ptr(), r, a, plan.address, code, op, ldo, 0 if hidden is None else hidden.data_ptr(),
+                  0 if ws is None else ws.data_ptr(), nbytes, _raw_stream(y))
     return (res, hidden) if return_hidden else res
 
 
@@ -552,7 +551,7 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
         x2, xp, ldx, scales = x.codes, x.codes.data_ptr(), k, x.scales.data_ptr()
     else:
         x2, xp, ldx, mx = _row_operand(x, "x", k, dy)
-        scales = None
+        scales = 0
         if mx != m:
             raise ValueError(f"x holds {mx} tokens, dy {m}")
     _same_device(hidden, "hidden", dy)
@@ -578,13 +577,12 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
         _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
     ddown, dup = (torch.empty_like(down), torch.empty_like(up)) if factors else (None, None)
     with _on(dy):
-        lib = _lib.lib()
-        nbytes = lib.dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
+        nbytes = _lib.lib().dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
         ws = _scratch(nbytes, dy)
-        _lib.check("dq_adapter_backward", lib.dq_adapter_backward(
-            dyp, lddy, xp, ldx, scales, hidden.data_ptr(), m, plan.requests, k, n, down.data_ptr(), up.data_ptr(),
-            scale.data_ptr(), r, a, plan.address, dxp, lddx, op, ldo, None if ddown is None else ddown.data_ptr(),
-            None if dup is None else dup.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy)))
+        _lib.call("dq_adapter_backward", dyp, lddy, xp, ldx, scales, hidden.data_ptr(), m, plan.requests, k, n,
+                  down.data_ptr(), up.data_ptr(), scale.data_ptr(), r, a, plan.address, dxp, lddx, op, ldo,
+                  0 if ddown is None else ddown.data_ptr(), 0 if dup is None else dup.data_ptr(), ws.data_ptr(),
+                  nbytes, _raw_stream(dy))
     return res, ddown, dup
 
 
@@ -624,8 +622,7 @@ def checkpoint_pack(x: torch.Tensor) -> PackedActivation:
     packed.codes = codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     packed.scales = scales = x.new_empty((m, -(-k // CHECKPOINT_RUN)), dtype=_F32)
     with _on(x):
-        _lib.check("dq_checkpoint_pack", _lib.lib().dq_checkpoint_pack(
-            xp, ldx, m, k, codes.data_ptr(), scales.data_ptr(), _raw_stream(x)))
+        _lib.call("dq_checkpoint_pack", xp, ldx, m, k, codes.data_ptr(), scales.data_ptr(), _raw_stream(x))
     return packed
 
 
@@ -644,8 +641,8 @@ def checkpoint_unpack(packed: PackedActivation, out: torch.Tensor | None = None)
         if m != codes.numel() // k:
             raise ValueError("out must hold the packed rows")
     with _on(codes):
-        _lib.check("dq_checkpoint_unpack", _lib.lib().dq_checkpoint_unpack(
-            codes.data_ptr(), packed.scales.data_ptr(), m, k, op, ldo, _raw_stream(codes)))
+        _lib.call("dq_checkpoint_unpack", codes.data_ptr(), packed.scales.data_ptr(), m, k, op, ldo,
+                  _raw_stream(codes))
     return res
 
 
@@ -679,9 +676,8 @@ def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tenso
     am = (absmax if absmax.dtype in (_F32, _BF16) else absmax.float()).contiguous()
     with _on(dy):
         ws = _scratch(nbytes, dy)
-        _lib.check("dq_linear_nf4_dgrad", _lib.lib().dq_linear_nf4_dgrad(
-            dy2.data_ptr(), dy2.numel() // n, n, packed.data_ptr(), am.data_ptr(), _dtype_code(am), k,
-            dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy)))
+        _lib.call("dq_linear_nf4_dgrad", dy2.data_ptr(), dy2.numel() // n, n, packed.data_ptr(), am.data_ptr(),
+                  _dtype_code(am), k, dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy))
     return dx
 
 
@@ -694,9 +690,8 @@ def fp8_linear_dgrad(dy: torch.Tensor, w8: torch.Tensor, scale: float) -> torch.
     dy2, dx, nbytes = _prep_dgrad(dy, n, k, w8, (torch.float8_e4m3fn, torch.uint8))
     with _on(dy):
         ws = _scratch(nbytes, dy)
-        _lib.check("dq_linear_fp8_dgrad", _lib.lib().dq_linear_fp8_dgrad(
-            dy2.data_ptr(), dy2.numel() // n, n, w8.data_ptr(), float(scale), k, dx.data_ptr(), ws.data_ptr(),
-            nbytes, _raw_stream(dy)))
+        _lib.call("dq_linear_fp8_dgrad", dy2.data_ptr(), dy2.numel() // n, n, w8.data_ptr(), float(scale), k,
+                  dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy))
     return dx
 
 

@@ -152,3 +152,26 @@ def test_python_entry_points_refuse_cpu_tensors():
         flux.gated_norm(b(1, 2, 64), b(1, 2, 64))
     with pytest.raises(RuntimeError, match="CUDA"):
         flux.gated_norm_backward(None, b(1, 2, 64), b(1, 2, 64), b(1, 2, 64))
+
+
+def test_packed_calls_carry_every_argument(lib):
+    """The packed form of an entry refuses what the entry itself refuses, so a
+    word out of place shows: each argument is spoilt in turn."""
+    from diffuser_b200 import _lib as L
+    assert all(getattr(lib, name + "_packed")(None) == ARG for name in L.PACKED)
+    # dq_checkpoint_pack: x, ldx, M, K, codes, scales, stream
+    good = [1 << 20, 64, 0, 64, 1 << 20, 1 << 20, 0]
+    L.call("dq_checkpoint_pack", *good)
+    for at, bad in ((1, 60), (2, -1), (3, 40), (3, -16)):
+        words = list(good)
+        words[at] = bad
+        with pytest.raises(L.DqError, match="dq_checkpoint_pack.*shape"):
+            L.call("dq_checkpoint_pack", *words)
+    # dq_gated_norm: a float past the integers, then an alignment
+    norm = [16, 64, 16, 64, 4, 2, 64, 0, 0, 0, 0, 0, 0, 0, 0, 1, 1.0, 1e-6, 0, 16, 64, 16, 64, 0]
+    for at, bad, status in ((4, 3, "shape"), (6, 62, "shape"), (14, 7, ""), (18, 5, ""), (20, 63, "shape"),
+                            (21, 17, "align"), (0, 20, "align")):
+        words = list(norm)
+        words[at] = bad
+        with pytest.raises(L.DqError, match=f"dq_gated_norm.*{status}"):
+            L.call("dq_gated_norm", *words)
