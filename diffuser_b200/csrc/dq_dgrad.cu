@@ -18,10 +18,12 @@ namespace {
 constexpr int kFusedTokens = 512;  // tokens per CTA: the columns of tensor memory
 
 // Whether decode and product go in one launch.  Two launches (NF4, us against
-// the fused one): 333 x 4096 x 4096 28 / 21, 512 tokens 28 / 28; 512 x 16384 x
-// 4096 97 / 72, x 1024 x 2048 12 / 17 (the sums' way out does not shrink with
+// the fused one): 333 x 4096 x 4096 28 / 20, 512 tokens 28 / 28; 512 x 16384 x
+// 4096 97 / 71, x 1024 x 2048 12 / 17 (the sums' way out does not shrink with
 // N), 256 x 1024 x 2048 12 / 11; 1024 x 4096 x 4096, decoded twice, 37 / 38.
-bool fused_wins(int64_t M, int64_t N) { return M <= 256 || (M <= kFusedTokens && N >= 2048); }
+bool fused_wins(int64_t M, int64_t N) {
+  return N <= (1 << 30) && (M <= 256 || (M <= kFusedTokens && N >= 2048));  // (rows are counted in 32 bits)
+}
 
 // Tokens per CTA (all of them), ring stages and CTAs of a cluster along N: the
 // size with the least waves x (steps of 64 n per CTA + a fixed cost of eight).
@@ -41,7 +43,9 @@ FusedPlan fused_plan(int fmt, int64_t M, int64_t N, int64_t K, int sms) {
   p.feature_tiles = static_cast<int>(ceil_div(K, kDgradFeatures));
   p.stage_bytes = kDgradWBytes + tokens * 128;
   const int behind = kDgradLutAt + (fmt == kFmtNF4 ? kNf4LutBytes : 0), room = 226 * 1024 - behind;
-  p.stages = std::min(kDgradMaxStages, room / p.stage_bytes);
+  p.stages = std::min(kDgradMaxStages, room / p.stage_bytes);  // 2 (512 tokens) or more
+  static_assert(2 * (kDgradWBytes + kFusedTokens * 128) <= 226 * 1024 - kDgradLutAt - kNf4LutBytes &&
+                kDgradGroups <= 2, "a stage per group of decoding warps");
   p.smem = static_cast<size_t>(p.stages) * p.stage_bytes + behind + 1024;
   p.red_tokens = std::min(tokens, p.stages * p.stage_bytes / (kDgradFeatures * 4) / 16 * 16);
   p.tmem_cols = 32;

@@ -90,11 +90,12 @@ __global__ void __launch_bounds__(256)
 // CTA each; their partial sums meet through distributed shared memory, in rank
 // order, and are rounded to bf16 once.
 //
-// Measured (NF4, against the two launches): 333 tokens x 4096 x 4096 21 us (28),
-// one token 12.6 (26); 16384 x 4096: 48 (95), 34 (93).  A step of 64 n takes
-// 0.42 us with few tokens (the decode's instructions) and 0.55 with 333 (dy's
-// boxes come from L2 for every slab); of the rest about 4 us are the sums' way
-// out and 3 the first loads.
+// Measured (NF4, against the two launches): 333 tokens x 4096 x 4096 20 us (28),
+// one token 12.3 (26); 16384 x 4096: 46 (95), 33 (93).  A step of 64 n takes
+// 0.43 us with few tokens, the decoding warps' instructions (e4m3 0.38), and
+// 0.54 with 333, of which dy's boxes come from L2 for every slab (85 bytes a
+// nanosecond and SM); of the rest about 4 us are the sums' way out and 3 the
+// first loads.
 struct DgradArgs {
   const uint8_t* w;
   const void* absmax;
@@ -111,10 +112,12 @@ struct DgradArgs {
 
 constexpr int kDgradRows = 64, kDgradFeatures = 128;
 constexpr int kDgradWBytes = kDgradRows * kDgradFeatures * 2;
-constexpr int kDgradMaxStages = 6;
+constexpr int kDgradMaxStages = 12;
 constexpr int kDgradBars = 16 * kDgradMaxStages + 8;  // full, empty, done
-constexpr int kDgradLutAt = 128;                      // the NF4 table, behind the barriers
-constexpr int kDgradThreads = 10 * 32;
+constexpr int kDgradLutAt = 256;                      // the NF4 table, behind the barriers
+constexpr int kDgradGroups = 2;                       // of four decoding warps
+constexpr int kDgradMmaWarp = 4 * kDgradGroups, kDgradTmaWarp = kDgradMmaWarp + 1;
+constexpr int kDgradThreads = (kDgradTmaWarp + 1) * 32;
 
 template <int FMT>
 __global__ void __launch_bounds__(kDgradThreads, 1)
@@ -140,8 +143,8 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
     fence_barrier_init();
   }
   if constexpr (FMT == kFmtNF4) nf4_lut_fill(reinterpret_cast<uint32_t*>(smem + off_bar + kDgradLutAt));
-  if (tid == 288) prefetch_tensormap(&tdy);
-  if (warp == 8) {
+  if (warp == kDgradTmaWarp && lane == 0) prefetch_tensormap(&tdy);
+  if (warp == kDgradMmaWarp) {
     tmem_alloc(smem_u32(tmem_slot), a.tmem_cols);
     tmem_relinquish();
   }
@@ -155,12 +158,17 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
   const int b_lo = me * a.per_split;
   const int steps = min((a.N + kDgradRows - 1) / kDgradRows, b_lo + a.per_split) - b_lo;  // at least one
 
-  if (warp < 8) {
+  if (warp < kDgradMmaWarp) {
     // ---------------------------------------------------------------- decode
     // Two groups of four warps take the steps in turn, so that one's latencies
     // (barrier, lookups, the fence towards the MMAs) pass under the other's.
-    // This thread: 32 features (quarter q) of rows t / 4 and t / 4 + 32 of every
-    // second step, its weight words two own steps ahead in registers.
+    // (No more groups than ring stages, of which there are at least two: a group
+    // that comes to step i has seen step i - groups - stages consumed, and its
+    // parity wait for i - stages is unambiguous only if i - 2 stages is among
+    // those.  Four groups, where the ring has the stages: NF4 2-7% faster at
+    // 12288 x 4096 and more, 3% slower at 4096 x 4096, e4m3 3% slower.)
+    // This thread: 32 features (quarter q) of rows t / 4 and t / 4 + 32 of its
+    // group's steps, the weight words two own steps ahead in registers.
     constexpr int kAhead = 2;
     const uint32_t lut_lane = sbase + a.stages * a.stage_bytes + kDgradLutAt + 4u * lane;
     constexpr int kWords = FMT == kFmtNF4 ? 1 : 2;
@@ -172,35 +180,41 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
       uint4 u[2][kWords];
       float scale[2];
     };
-    auto load = [&](int it, Own& w) {
+    // walking pointers: this thread's next row (and that + 32), of rows below
+    // n_end (0: its features are past K; NF4's K % 64 == 0 puts a quarter all in
+    // or all out, an e4m3 one's second half may be past it)
+    const int64_t row_bytes = FMT == kFmtNF4 ? a.K / 2 : a.K;
+    int n = (b_lo + group) * kDgradRows + row0;
+    const int n_end = f < a.K ? min(a.N, (b_lo + steps) * kDgradRows) : 0;
+    const bool upper = f + 16 < a.K;
+    const uint8_t* src = a.w + n * row_bytes + (FMT == kFmtNF4 ? f / 2 : f);
+    const int64_t src_step = static_cast<int64_t>(kDgradGroups) * kDgradRows * row_bytes;
+    int64_t block = static_cast<int64_t>(n) * (a.K / 64) + f / 64;
+    auto load = [&](Own& w) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int n = (b_lo + it) * kDgradRows + row0 + 32 * h;
-        const bool in = it < steps && n < a.N;
-        if constexpr (FMT == kFmtNF4) {  // K % 64 == 0: a quarter is all in or all out
-          const bool ok = in && f < a.K;
-          w.u[h][0] = ok ? __ldg(reinterpret_cast<const uint4*>(a.w + (static_cast<int64_t>(n) * a.K + f) / 2))
-                         : make_uint4(0u, 0u, 0u, 0u);
-          w.scale[h] = ok ? load_scale(a.absmax, (static_cast<int64_t>(n) * a.K + f) / 64, a.scale_bf16 != 0) : 0.f;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            w.u[h][i] = in && f + 16 * i < a.K
-                            ? __ldg(reinterpret_cast<const uint4*>(a.w + static_cast<int64_t>(n) * a.K + f + 16 * i))
-                            : make_uint4(0u, 0u, 0u, 0u);
-        }
+        const bool in = n + 32 * h < n_end;
+        const uint4* p = reinterpret_cast<const uint4*>(src + 32 * h * row_bytes);
+        w.u[h][0] = in ? __ldg(p) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (FMT == kFmtNF4)
+          w.scale[h] = in ? load_scale(a.absmax, block + 32 * h * (a.K / 64), a.scale_bf16 != 0) : 0.f;
+        else
+          w.u[h][kWords - 1] = in && upper ? __ldg(p + 1) : make_uint4(0u, 0u, 0u, 0u);
       }
+      n += kDgradGroups * kDgradRows;
+      src += src_step;
+      block += static_cast<int64_t>(kDgradGroups) * kDgradRows * (a.K / 64);
     };
     Own ahead[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(group + 2 * i, ahead[i]);
+    for (int i = 0; i < kAhead; ++i) load(ahead[i]);
+    int slot = group;
+    uint32_t parity = 1;
     bool live = true;
-    for (int base = group; base < steps && live; base += 2 * kAhead) {
+    for (int base = group; base < steps && live; base += kDgradGroups * kAhead) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int it = base + 2 * i;
-        if (it >= steps || !live) break;
-        const int slot = it % a.stages;
+        if (base + kDgradGroups * i >= steps || !live) break;
         uint32_t o[2][16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -225,8 +239,8 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
             fp8_decode_word(v.w, s8, o[h] + 14);
           }
         }
-        load(it + 2 * kAhead, ahead[i]);
-        if (!mbar_wait(empty_bar(slot), static_cast<uint32_t>(((it / a.stages) & 1) ^ 1), abort_flag)) {
+        load(ahead[i]);
+        if (!mbar_wait(empty_bar(slot), parity, abort_flag)) {
           live = false;
           break;
         }
@@ -244,37 +258,61 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full_bar(slot));
+        slot += kDgradGroups;
+        if (slot >= a.stages) {
+          slot -= a.stages;
+          parity ^= 1u;
+        }
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == kDgradMmaWarp) {
     // ------------------------------------------------------------------- MMA
-    const uint32_t idesc = make_idesc_bf16(128, a.tok_n) | (1u << 15);  // A MN-major
-    for (int it = 0; it < steps; ++it) {
-      const int slot = it % a.stages;
-      if (!mbar_wait(full_bar(slot), static_cast<uint32_t>((it / a.stages) & 1), abort_flag)) break;
-      tc_fence_after();
-      const uint32_t sw = sbase + slot * a.stage_bytes;
-      const uint64_t ad = make_sw128_mnmajor_desc(sw, kDgradWBytes / 2);
-      for (int m = 0; m < a.n_mma; ++m) {
-        const uint64_t bd = make_sw128_kmajor_desc(sw + kDgradWBytes + m * a.tok_n * 128);
+    // one thread: it alone issues, commits and waits
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc_bf16(128, a.tok_n) | (1u << 15);  // A MN-major
+      const uint32_t x_mma = static_cast<uint32_t>(a.tok_n) * 128 / 16;   // descriptor units per MMA's tokens
+      uint32_t at = sbase, parity = 0;
+      int slot = 0;
+      for (int it = 0; it < steps; ++it) {
+        if (!mbar_wait(full_bar(slot), parity, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t ad = make_sw128_mnmajor_desc(at, kDgradWBytes / 2);
+        uint64_t bd = make_sw128_kmajor_desc(at + kDgradWBytes);
+        uint32_t d = tmem;
+        for (int m = 0; m < a.n_mma; ++m) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)  // 16 n: two 8-row groups of W, 32 bytes of dy's rows
-          tc_mma_ss_elect(tmem + m * a.tok_n, ad + 128 * ks, bd + 2 * ks, idesc, (it | ks) != 0);
+          for (int ks = 0; ks < 4; ++ks)  // 16 n: two 8-row groups of W, 32 bytes of dy's rows
+            tc_mma_ss(d, ad + 128 * ks, bd + 2 * ks, idesc, (it | ks) != 0);
+          d += a.tok_n;
+          bd += x_mma;
+        }
+        tc_commit(empty_bar(slot));
+        at += a.stage_bytes;
+        if (++slot == a.stages) {
+          slot = 0;
+          at = sbase;
+          parity ^= 1u;
+        }
       }
-      tc_commit_elect(empty_bar(slot));
+      tc_commit(done_bar);
     }
-    tc_commit_elect(done_bar);
     __syncwarp();
   } else {
     // ------------------------------------------------------------------- TMA
     if (lane == 0) {
+      uint32_t dst = sbase + kDgradWBytes, parity = 1;
+      int slot = 0;
       for (int it = 0; it < steps; ++it) {
-        const int slot = it % a.stages;
-        if (!mbar_wait(empty_bar(slot), static_cast<uint32_t>(((it / a.stages) & 1) ^ 1), abort_flag)) break;
-        const uint32_t dst = sbase + slot * a.stage_bytes + kDgradWBytes;
+        if (!mbar_wait(empty_bar(slot), parity, abort_flag)) break;
         mbar_arrive_expect_tx(full_bar(slot), static_cast<uint32_t>(tokens * 128));
         for (int m = 0; m < a.n_mma; ++m)
           tma_load_2d(dst + m * a.tok_n * 128, &tdy, full_bar(slot), (b_lo + it) * kDgradRows, m * a.tok_n);
+        dst += a.stage_bytes;
+        if (++slot == a.stages) {
+          slot = 0;
+          dst = sbase + kDgradWBytes;
+          parity ^= 1u;
+        }
       }
     }
     __syncwarp();
@@ -286,9 +324,9 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
   __syncthreads();
   for (int t0 = 0; t0 < tokens; t0 += a.red_tokens) {
     const int tn = min(a.red_tokens, tokens - t0);
-    if (ok && warp < 8) {
+    if (ok && warp < kDgradMmaWarp) {
       const int quad = warp & 3;
-      for (int c = (warp >> 2) * 16; c < tn; c += 32) {
+      for (int c = (warp >> 2) * 16; c < tn; c += 16 * kDgradGroups) {
         uint32_t v[16];
         tmem_ld_x16(tmem + (static_cast<uint32_t>(32 * quad) << 16) + t0 + c, v);
         tmem_wait_ld();
@@ -338,7 +376,7 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
     if (tid == 0) atomicOr(a.error, 1u << 5);
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kDgradMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, a.tmem_cols);
   }
