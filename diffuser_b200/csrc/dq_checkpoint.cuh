@@ -33,13 +33,15 @@ struct RowWalk {
 };
 
 // Pack: 8 lanes per run of 128 features, two 16-byte pieces per lane, four runs
-// per warp (16 lanes per run spend more on the maximum and the scale: 75 us).  The maximum is taken
-// over bf16 pairs and keeps NaN, so a run that is not finite is seen.  HBM-bound: 3 bytes per feature, 47 us at 6144 x 16384.  An IEEE
-// division per feature made it 127 us, so the quotient is taken as
-// x (1 / scale), off by at most 127 (2^-23 + 2^-24) = 2.3e-5 from the exact one,
-// and divided only where that could round to another integer: within 1e-4 of a
-// half.  Adding 1.5 2^23 rounds to an integer (ties to even) and leaves it in
-// the low bits, without the special-function unit's conversions.
+// per warp (16 lanes per run spend more on the maximum and the scale: 75 us).
+// The maximum is taken over bf16 pairs and keeps NaN, so a run that is not
+// finite is seen.  Bound: HBM, 3 bytes per feature, 47 us at 6144 x 16384, where
+// pack takes 60 and unpack 59.  An IEEE division per feature made pack 127 us, so
+// the quotient is taken as x (1 / scale), off by at most 127 (2^-23 + 2^-24) =
+// 2.3e-5 from the exact one, and divided only where that could round to another
+// integer: within 1e-4 of a half.  Adding 1.5 2^23 rounds to an integer (ties to
+// even) and leaves it in the low bits, without the special-function unit's
+// conversions.
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
 __device__ __forceinline__ void pack_pair(uint32_t w, float scale, F2 inv, uint32_t& c0, uint32_t& c1) {
   const F2 v = widen(w), t = mul2(v, inv);

@@ -14,7 +14,8 @@
 // reads (no barrier).  Each block reduction has shared words of its own,
 // doubled by row parity, so it takes one barrier.  (With scalar arithmetic,
 // bf16 factors from L1 and the next row prefetched in registers: 42 instructions
-// per element and 35 us forward, 68 and 98 us backward at 4608 x 4096.)
+// per element and 35 us forward, 68 and 98 us backward at 4608 x 4096, where
+// forward now takes 26.0, 5.8 TB/s, and backward with its reduction 51.5.)
 //
 // Backward.  With t = Npre(s), m = wpre (1 + scale), dt = dh m, and yh = Npost(y):
 //   dx = ds + rstd_s (dt - [mean dt] - t mean(dt t))            (mean dt: LayerNorm only)

@@ -44,7 +44,8 @@ int dq_adapter_plan(const int32_t* ids, const int32_t* offsets, int64_t R, int64
  * asks for them).  act as dq_linear_*_ex; with a gated activation up's and y's
  * columns are in the gated row order, N % 32 == 0 and out has N / 2 columns.
  * hidden (or NULL): bf16 [M, r], receives scale_a * x . down_a^T (zero rows
- * where there is none), which the backward pass takes.
+ * where there is none), which the backward pass takes.  Apart from y, out
+ * overlaps no operand (dx_out below: apart from dx).
  * The sums of the down projection are kept in float32 over K, rounded once
  * to bf16 for the up projection, which accumulates in float32 onto y; out is
  * rounded once.  The workspace (16-byte aligned, at most M * r * 2 bytes; none
@@ -88,9 +89,11 @@ int dq_checkpoint_unpack(const int8_t* codes, const float* scales, int64_t M, in
 
 /* Input gradient of the quantized linears: dx[M, K] = dy[M, N] . dequant(W),
  * W as dq_linear_nf4 / dq_linear_fp8 take it (absmax f32 or, scale_dtype
- * DQ_DTYPE_BF16, bf16).  The weight is decoded once, transposed, into the
- * workspace (dq_linear_dgrad_workspace bytes, 16-byte aligned), then
- * multiplied by the bf16 CTA-pair GEMM.  N % 8 == 0, K % 64 == 0 (NF4) or
+ * DQ_DTYPE_BF16, bf16).  Up to 512 tokens the weight is decoded next to the
+ * product, in one launch; beyond, once, transposed, into the workspace
+ * (dq_linear_dgrad_workspace bytes, 16-byte aligned, asked for in either case)
+ * and multiplied by the bf16 CTA-pair GEMM.  Sums are float32, dx is rounded
+ * once; the same inputs give the same bits.  N % 8 == 0, K % 64 == 0 (NF4) or
  * K % 16 == 0 (fp8); dy and dx contiguous, 16-byte aligned. */
 size_t dq_linear_dgrad_workspace(int64_t N, int64_t K);
 int dq_linear_nf4_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* packed,
