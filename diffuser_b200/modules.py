@@ -470,6 +470,8 @@ def attach_adapters(model: nn.Module, n_adapters: int, rank: int, is_adapted_key
     modules are marked differentiable: with gradients enabled, the quantized
     linears that were not wrapped and the FLUX blocks' fused kernels then pass
     gradients on too.  Returns the wrapped names."""
+    if isinstance(model, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
+        raise TypeError("a linear by itself is wrapped by AdapterLinear(linear, ...)")
     wrapped = []
     for mod in model.modules():
         mod.differentiable = True

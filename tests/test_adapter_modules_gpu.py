@@ -406,3 +406,53 @@ def test_a_frozen_linear_passes_gradients_on(fmt, act):
     assert _far(y, z.detach()) <= 8 * H and _far(x.grad, x64.grad) <= 2 * 8 * H
     with pytest.raises(RuntimeError, match="out"):
         lin(x, out=torch.empty(21, 128 if act != "swiglu" else 64, device="cuda", dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("pack", [False, True])
+@pytest.mark.parametrize("seq", [5, 150])
+def test_a_training_step_captured_and_replayed(seq, pack):
+    """Two linears with an activation between them, forward and backward in one
+    graph (no eager graph over the same factors alive), on other inputs and for
+    another selection."""
+    from diffuser_b200 import modules, ops
+    mods = [modules.AdapterLinear(_linear("nf4", n, k, 5 + i)[0], 3, 8, pack) for i, (n, k) in enumerate([(256, 128), (64, 256)])]
+    for i, m in enumerate(mods):
+        _fill(m, 11 + i)
+    sel = modules.AdapterSelection(torch.tensor([2, -1, 0], dtype=torch.int32, device="cuda"), 3)
+    for m in mods:
+        m.selection = sel
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    leaves = [p for m in mods for p in (m.down, m.up)]
+    x, dy = rn(3, seq, 128).requires_grad_(), rn(3, seq, 64)
+
+    def step():
+        for t in (*leaves, x):
+            t.grad = None
+        y = mods[1](mods[0](x, act="gelu_tanh"))
+        y.backward(dy)
+        return y.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    held = [t.grad for t in (*leaves, x)]
+    for ids in ([0, 1, -1], [1, 1, 1]):
+        with torch.no_grad():
+            x.copy_(rn(3, seq, 128))
+        dy.copy_(rn(3, seq, 64))
+        sel.update_(torch.tensor(ids, dtype=torch.int32, device="cuda"))
+        graph.replay()
+        replayed = [out.clone(), *(t.clone() for t in held)]
+        eager = [step(), *(t.grad for t in (*leaves, x))]
+        for i, (a, b) in enumerate(zip(replayed, eager)):
+            assert torch.equal(a, b), (ids, i)
+    assert ops.device_error() == 0
+    with pytest.raises(TypeError):
+        modules.attach_adapters(_linear("nf4", 64, 64, 1)[0], 1, 8)
