@@ -84,18 +84,18 @@ __global__ void __launch_bounds__(256)
 // tensor memory, up to all 512 columns.  Every weight element is decoded once.
 // Eight warps decode (NF4 through the per-lane byte table: a lookup and a
 // product per two weights), their weight words four steps ahead in registers,
-// one issues the MMAs, one the TMA loads.
+// two issue the MMAs, one the TMA loads.
 //
 // The sum over N is split over the CTAs of a cluster so that the SMs have one
 // CTA each; their partial sums meet through distributed shared memory, in rank
 // order, and are rounded to bf16 once.
 //
 // Measured (NF4, against the two launches): 333 tokens x 4096 x 4096 20 us (28),
-// one token 12.3 (26); 16384 x 4096: 46 (95), 33 (93).  A step of 64 n takes
-// 0.43 us with few tokens, the decoding warps' instructions (e4m3 0.38), and
-// 0.54 with 333, of which dy's boxes come from L2 for every slab (85 bytes a
-// nanosecond and SM); of the rest about 4 us are the sums' way out and 3 the
-// first loads.
+// one token 12.0 (26); 16384 x 4096: 46 (95), 31 (93).  A step of 64 n takes
+// 0.40 us with few tokens, in which the decoding warps hardly wait, and 0.53 with
+// 333, near what its shared-memory traffic needs: dy's boxes in and out, W's tile
+// in and twice out, the table's lookups, 150 KB at 128 bytes a cycle.  Of the
+// rest about 4 us are the sums' way out and 3 the first loads.
 struct DgradArgs {
   const uint8_t* w;
   const void* absmax;
@@ -116,7 +116,7 @@ constexpr int kDgradMaxStages = 12;
 constexpr int kDgradBars = 16 * kDgradMaxStages + 8;  // full, empty, done
 constexpr int kDgradLutAt = 256;                      // the NF4 table, behind the barriers
 constexpr int kDgradGroups = 2;                       // of four decoding warps
-constexpr int kDgradMmaWarp = 4 * kDgradGroups, kDgradTmaWarp = kDgradMmaWarp + 1;
+constexpr int kDgradMmaWarp = 4 * kDgradGroups, kDgradTmaWarp = kDgradMmaWarp + 2;  // two issue MMAs
 constexpr int kDgradThreads = (kDgradTmaWarp + 1) * 32;
 
 template <int FMT>
@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
       mbar_init(full_bar(s), 5);  // four decoding warps, the TMA issuer
-      mbar_init(empty_bar(s), 1);
+      mbar_init(empty_bar(s), a.n_mma);
     }
-    mbar_init(done_bar, 1);
+    mbar_init(done_bar, a.n_mma);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -265,27 +265,25 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
         }
       }
     }
-  } else if (warp == kDgradMmaWarp) {
+  } else if (warp < kDgradTmaWarp) {
     // ------------------------------------------------------------------- MMA
-    // one thread: it alone issues, commits and waits
-    if (lane == 0) {
+    // Each half of more than 256 tokens, with its own sums, has its own issuing
+    // thread (one for both: 333 x 4096 x 4096 20.4 us, two 20.0; two halves for
+    // fewer tokens read W's tile twice: 16384 x 4096 3% slower)
+    const int m = warp - kDgradMmaWarp;
+    if (m < a.n_mma && lane == 0) {
       const uint32_t idesc = make_idesc_bf16(128, a.tok_n) | (1u << 15);  // A MN-major
-      const uint32_t x_mma = static_cast<uint32_t>(a.tok_n) * 128 / 16;   // descriptor units per MMA's tokens
+      const uint32_t d = tmem + m * a.tok_n, x_at = kDgradWBytes + m * a.tok_n * 128;
       uint32_t at = sbase, parity = 0;
       int slot = 0;
       for (int it = 0; it < steps; ++it) {
         if (!mbar_wait(full_bar(slot), parity, abort_flag)) break;
         tc_fence_after();
         const uint64_t ad = make_sw128_mnmajor_desc(at, kDgradWBytes / 2);
-        uint64_t bd = make_sw128_kmajor_desc(at + kDgradWBytes);
-        uint32_t d = tmem;
-        for (int m = 0; m < a.n_mma; ++m) {
+        const uint64_t bd = make_sw128_kmajor_desc(at + x_at);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)  // 16 n: two 8-row groups of W, 32 bytes of dy's rows
-            tc_mma_ss(d, ad + 128 * ks, bd + 2 * ks, idesc, (it | ks) != 0);
-          d += a.tok_n;
-          bd += x_mma;
-        }
+        for (int ks = 0; ks < 4; ++ks)  // 16 n: two 8-row groups of W, 32 bytes of dy's rows
+          tc_mma_ss(d, ad + 128 * ks, bd + 2 * ks, idesc, (it | ks) != 0);
         tc_commit(empty_bar(slot));
         at += a.stage_bytes;
         if (++slot == a.stages) {
