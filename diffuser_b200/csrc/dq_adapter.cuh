@@ -945,6 +945,7 @@ struct WgradArgs {
   unsigned int* error;
   AdapterPlan lay;
   int rank, A;
+  int alone;  // one split and few adapters: no reduce kernel follows
 };
 
 // Four int8 codes -> two bf16 pairs, exact.
@@ -1235,6 +1236,12 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
       if (lane == 0) mbar_arrive(acc_empty(b));
       cur.pos = cur.end;
       cur.open();
+    }
+    if (a.alone && col < w.cols) {  // zeros for adapters without rows
+      for (int ad = 0; ad < a.A; ++ad)
+        if (starts[ad] == starts[ad + 1])
+          for (int r = 0; r < a.rank; ++r)
+            w.dbank[(static_cast<int64_t>(ad) * a.rank + r) * w.cols + col] = __float2bfloat16_rn(0.f);
     }
   }
   tc_fence_before();

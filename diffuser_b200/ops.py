@@ -566,12 +566,14 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
     if md != m:
         raise ValueError(f"dx holds {md} tokens, dy {m}")
     if out is None:
-        res = base if dx is None else torch.empty(shape, dtype=_BF16, device=dy.device)
+        res = base if dx is None else torch.empty_like(dx) if dx2 is dx and dx.shape == shape else \
+            torch.empty(shape, dtype=_BF16, device=dy.device)
+        op, ldo = res.data_ptr(), k
     else:
         res = out
-    _, op, ldo, mo = _row_operand(res, "out", k, dy, must_alias=True)
-    if mo != m:
-        raise ValueError(f"out holds {mo} tokens, dy {m}")
+        _, op, ldo, mo = _row_operand(out, "out", k, dy, must_alias=True)
+        if mo != m:
+            raise ValueError(f"out holds {mo} tokens, dy {m}")
     if out is not None and m:
         other = ((dy2, dyp, "dy"), (x2, xp, "x"), (hidden, hidden.data_ptr(), "hidden"))
         _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
