@@ -93,9 +93,9 @@ __global__ void __launch_bounds__(256)
 // Measured (NF4, against the two launches): 333 tokens x 4096 x 4096 20 us (28),
 // one token 12.0 (26); 16384 x 4096: 46 (95), 31 (93).  A step of 64 n takes
 // 0.40 us with few tokens, in which the decoding warps hardly wait, and 0.53 with
-// 333, near what its shared-memory traffic needs: dy's boxes in and out, W's tile
-// in and twice out, the table's lookups, 150 KB at 128 bytes a cycle.  Of the
-// rest about 4 us are the sums' way out and 3 the first loads.
+// 333, of the order of its shared-memory traffic (dy's boxes in and out, W's tile
+// in and twice out, the table's lookups: some 150 KB).  Of the rest about 4 us
+// are the sums' way out and 3 the first loads.
 struct DgradArgs {
   const uint8_t* w;
   const void* absmax;
