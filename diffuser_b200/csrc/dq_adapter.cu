@@ -486,7 +486,8 @@ int dq_checkpoint_pack(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t*
   const int64_t runs = M * nrun;
   const int grid = static_cast<int>(std::min<int64_t>(ceil_div(runs, 32), static_cast<int64_t>(sms) * 6));  // resident CTAs
   checkpoint_pack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const __nv_bfloat16*>(x), ldx, M, nrun, static_cast<int>(K), codes, scales);
+      static_cast<const __nv_bfloat16*>(x), ldx, M, nrun, static_cast<int>(K), aligned(x, 32) && ldx % 16 == 0, codes,
+      scales);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
@@ -499,11 +500,11 @@ int dq_checkpoint_unpack(const int8_t* codes, const float* scales, int64_t M, in
   int sms = 0;
   const int rc = device_sms(&sms);
   if (rc != DQ_OK) return rc;
-  const int64_t total = M * (K / 8);
-  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(total, 256), static_cast<int64_t>(sms) * 8));
+  const int64_t total = M * (K / 16);
+  const int grid = static_cast<int>(std::min<int64_t>(ceil_div(total, 256), static_cast<int64_t>(sms) * 4));  // resident CTAs
   checkpoint_unpack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
       codes, scales, M, static_cast<int>(K), static_cast<int>(ceil_div(K, kCkptRun)),
-      static_cast<__nv_bfloat16*>(out), ldo);
+      aligned(out, 32) && ldo % 16 == 0, static_cast<__nv_bfloat16*>(out), ldo);
   return cudaGetLastError() == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 

@@ -32,14 +32,15 @@ struct RowWalk {
   }
 };
 
-// Pack: 8 lanes per run of 128 features, two 16-byte pieces per lane, four runs
-// per warp (16 lanes per run spend more on the maximum and the scale: 75 us).
+// Pack: 8 lanes per run of 128 features, 16 features per lane (one 32-byte load
+// where the rows are 32-byte aligned: 58 us at 6144 x 16384, two of 16 bytes 60),
+// four runs per warp (16 lanes per run spend more on the maximum and the scale:
+// 75 us; the next run's load issued ahead, or two runs at a time: 63).
 // The maximum is taken over bf16 pairs and keeps NaN, so a run that is not
-// finite is seen.  Bound: HBM, 3 bytes per feature, 47 us at 6144 x 16384, where
-// pack takes 60 and unpack 59.  An IEEE division per feature made pack 127 us, so
-// the quotient is taken as x (1 / scale), off by at most 127 (2^-23 + 2^-24) =
-// 2.3e-5 from the exact one, and divided only where that could round to another
-// integer: within 1e-4 of a half.  Adding 1.5 2^23 rounds to an integer (ties to
+// finite is seen.  Bound: HBM, 3 bytes per feature, 47 us.  An IEEE division per
+// feature made pack 127 us, so the quotient is taken as x (1 / scale), off by at
+// most 127 (2^-23 + 2^-24) = 2.3e-5 from the exact one, and divided only where
+// that could round to another integer: within 1e-4 of a half.  Adding 1.5 2^23 rounds to an integer (ties to
 // even) and leaves it in the low bits, without the special-function unit's
 // conversions.
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
@@ -66,6 +67,19 @@ __device__ __forceinline__ float over_127(float amax) {
   return fmaf(fmaf(-127.0f, q, amax), c, q);
 }
 
+// 32 streamed bytes in one instruction (32-byte aligned).
+__device__ __forceinline__ void ld_stream32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+
+__device__ __forceinline__ void st_global32(void* p, uint4 a, uint4 b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -74,18 +88,22 @@ __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
 
 __global__ void __launch_bounds__(256)
     checkpoint_pack_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int64_t M, int nrun, int K,
-                           int8_t* __restrict__ codes, float* __restrict__ scales) {
+                           bool wide, int8_t* __restrict__ codes, float* __restrict__ scales) {
   const int sub = threadIdx.x & 7;  // lane of the run's eight
   RowWalk at(blockIdx.x * 32ll + (threadIdx.x >> 3), static_cast<int64_t>(gridDim.x) * 32, nrun);
   while (__any_sync(0xffffffffu, at.row < M)) {
     const int64_t row = at.row;
-    const int run = at.col, k = run * kCkptRun + sub * 8;  // and k + 64
-    uint4 u[2];
-    bool in[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      in[i] = row < M && k + 64 * i < K;
-      u[i] = in[i] ? ld_stream16(x + row * ldx + k + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
+    const int run = at.col, k = run * kCkptRun + sub * 16;
+    const bool in = row < M && k < K;  // K % 16 == 0
+    uint4 u[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (in) {
+      const __nv_bfloat16* p = x + row * ldx + k;
+      if (wide) {
+        ld_stream32(p, u[0], u[1]);
+      } else {
+        u[0] = ld_stream16(p);
+        u[1] = ld_stream16(p + 8);
+      }
     }
     at.next();
     constexpr uint32_t kAbs = 0x7FFF7FFFu;
@@ -100,58 +118,72 @@ __global__ void __launch_bounds__(256)
     const bool finite = top < 0x7F80u;
     const float scale = finite ? over_127(fmaxf(__uint_as_float(top << 16), 1e-12f)) : __uint_as_float(0x7FC00000u);
     const F2 inv = f2(finite ? rcp_approx(scale) : 0.f);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (!in[i]) continue;
-      uint32_t w[2] = {0u, 0u};
+    if (in) {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
       if (finite) {
-        uint32_t c[8];
-        pack_pair(u[i].x, scale, inv, c[0], c[1]);
-        pack_pair(u[i].y, scale, inv, c[2], c[3]);
-        pack_pair(u[i].z, scale, inv, c[4], c[5]);
-        pack_pair(u[i].w, scale, inv, c[6], c[7]);
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-          w[q] = prmt(prmt(c[4 * q], c[4 * q + 1], 0x0040u), prmt(c[4 * q + 2], c[4 * q + 3], 0x0040u), 0x5410u);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t c[8];
+          pack_pair(u[i].x, scale, inv, c[0], c[1]);
+          pack_pair(u[i].y, scale, inv, c[2], c[3]);
+          pack_pair(u[i].z, scale, inv, c[4], c[5]);
+          pack_pair(u[i].w, scale, inv, c[6], c[7]);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            w[2 * i + q] = prmt(prmt(c[4 * q], c[4 * q + 1], 0x0040u), prmt(c[4 * q + 2], c[4 * q + 3], 0x0040u), 0x5410u);
+        }
       }
-      *reinterpret_cast<uint2*>(codes + row * K + k + 64 * i) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint4*>(codes + row * K + k) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (sub == 0 && row < M) scales[row * nrun + run] = scale;
   }
 }
 
-// Unpack: 8 codes per thread, two pieces in flight.  The codes become bf16
-// exactly, so float32 by a shift, without integer conversions.
+// Unpack: 16 codes per thread, two pieces in flight, 32 bytes per store where the
+// rows are 32-byte aligned: 47 us at 6144 x 16384, 6.5 TB/s (8 codes and 16-byte
+// stores: 51; four pieces of 16: 54; two of 8 on twice the resident CTAs: 59).
+// The codes become bf16 exactly, so float32 by a shift, without integer
+// conversions.
+__device__ __forceinline__ uint4 restore8(uint32_t lo, uint32_t hi, F2 by) {
+  uint4 p;
+  i8_to_bf16(lo, p.x, p.y);
+  i8_to_bf16(hi, p.z, p.w);
+  return make_uint4(narrow(mul2(widen(p.x), by)), narrow(mul2(widen(p.y), by)), narrow(mul2(widen(p.z), by)),
+                    narrow(mul2(widen(p.w), by)));
+}
 __global__ void __launch_bounds__(256)
     checkpoint_unpack_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
-                             int64_t M, int K, int nrun, __nv_bfloat16* __restrict__ out, int64_t ldo) {
+                             int64_t M, int K, int nrun, bool wide, __nv_bfloat16* __restrict__ out, int64_t ldo) {
+  constexpr int kPieces = 2;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  RowWalk at(blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x, stride, K / 8);
+  RowWalk at(blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x, stride, K / 16);
   while (at.row < M) {
-    uint2 u[2];
-    float s[2];
-    int64_t row[2];
-    int k[2];
+    uint4 u[kPieces];
+    float s[kPieces];
+    int64_t row[kPieces];
+    int k[kPieces];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPieces; ++i) {
       row[i] = at.row;
-      k[i] = at.col * 8;
+      k[i] = at.col * 16;
       if (row[i] < M) {
-        u[i] = __ldg(reinterpret_cast<const uint2*>(codes + row[i] * K + k[i]));
+        u[i] = __ldg(reinterpret_cast<const uint4*>(codes + row[i] * K + k[i]));
         s[i] = __ldg(scales + row[i] * nrun + k[i] / kCkptRun);
       }
       at.next();
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPieces; ++i) {
       if (row[i] >= M) break;
-      uint4 p;
-      i8_to_bf16(u[i].x, p.x, p.y);
-      i8_to_bf16(u[i].y, p.z, p.w);
       const F2 by = f2(s[i]);
-      *reinterpret_cast<uint4*>(out + row[i] * ldo + k[i]) =
-          make_uint4(narrow(mul2(widen(p.x), by)), narrow(mul2(widen(p.y), by)), narrow(mul2(widen(p.z), by)),
-                     narrow(mul2(widen(p.w), by)));
+      __nv_bfloat16* p = out + row[i] * ldo + k[i];
+      const uint4 a = restore8(u[i].x, u[i].y, by), b = restore8(u[i].z, u[i].w, by);
+      if (wide) {
+        st_global32(p, a, b);
+      } else {
+        *reinterpret_cast<uint4*>(p) = a;
+        *reinterpret_cast<uint4*>(p + 8) = b;
+      }
     }
   }
 }

@@ -535,3 +535,24 @@ def test_outputs_may_not_overlap_what_is_still_read():
         ops.nf4_linear_dgrad(y, packed.to(torch.int8), absmax, 128)
     twice = torch.stack([absmax, absmax], 1)
     assert torch.equal(ops.nf4_linear_dgrad(y, packed, twice[:, 0], 128), ops.nf4_linear_dgrad(y, packed, absmax, 128))
+
+
+# rows that start 16 but not 32 bytes aligned, by address and by stride
+@pytest.mark.parametrize("offset,stride", [(8, 336), (0, 328), (16, 344)])
+def test_checkpoint_rows_of_either_alignment(offset, stride):
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = _rn(g, 37, 304)
+    want = ops.checkpoint_pack(x)
+    wide = torch.zeros(37 * stride + 64, dtype=torch.bfloat16, device="cuda")
+    view = wide[offset:].as_strided((37, 304), (stride, 1))
+    view.copy_(x)
+    got = ops.checkpoint_pack(view)
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    back = torch.full_like(wide, 7.0)
+    out = back[offset:].as_strided((37, 304), (stride, 1))
+    ops.checkpoint_unpack(want, out=out)
+    assert torch.equal(out, ops.checkpoint_unpack(want))
+    gaps = torch.ones_like(back, dtype=torch.bool)
+    gaps[offset:].as_strided((37, 304), (stride, 1)).fill_(False)
+    assert (back[gaps] == 7.0).all()
