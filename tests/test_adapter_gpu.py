@@ -556,3 +556,30 @@ def test_checkpoint_rows_of_either_alignment(offset, stride):
     gaps = torch.ones_like(back, dtype=torch.bool)
     gaps[offset:].as_strided((37, 304), (stride, 1)).fill_(False)
     assert (back[gaps] == 7.0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(7, 8, 64), (300, 24, 128), (600, 16, 64)])
+@pytest.mark.parametrize("fmt", ["nf4", "fp8"])
+def test_input_gradient_of_few_outputs(m, n, k, fmt):
+    """Sums shorter than a step of 64 (the rest of dy's boxes and of the weight's
+    tile is past their end), every dx written, nothing behind it."""
+    from diffuser_b200 import _lib, ops
+    g = torch.Generator(device="cuda").manual_seed(n)
+    w, dy = torch.randn(n, k, generator=g, device="cuda") * 0.02, _rn(g, m, n)
+    ws = torch.empty(2 * n * k + 256, dtype=torch.uint8, device="cuda")
+    dx = torch.full((m + 3, k), 5.0, dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    if fmt == "nf4":
+        packed, absmax = ops.ltx23_nf4_quantize(w)
+        wd = ops.ltx23_nf4_dequantize(packed, absmax, (n, k))
+        _lib.call("dq_linear_nf4_dgrad", dy.data_ptr(), m, n, packed.data_ptr(), absmax.data_ptr(), 0, k, dx.data_ptr(),
+                  ws.data_ptr(), ws.numel(), stream)
+    else:
+        w8, s = ops.fp8_quantize(w)
+        wd = ops.fp8_dequantize(w8, float(s))
+        _lib.call("dq_linear_fp8_dgrad", dy.data_ptr(), m, n, w8.data_ptr(), float(s), k, dx.data_ptr(), ws.data_ptr(),
+                  ws.numel(), stream)
+    ref = dy.double() @ wd.double()
+    tol = (n + 8) * U * (dy.double().abs() @ wd.double().abs()) + H * ref.abs()
+    _close(dx[:m], ref, tol, fmt)
+    assert (dx[m:] == 5.0).all() and ops.device_error() == 0
