@@ -881,7 +881,7 @@ def dit_section(ctx, reference: bool = True, profile: bool = False) -> dict:
     with ClockSampler(ctx.local) as clk:
         eager_ms, eager_ranks = ctx.timed(step, steps)
         # the same step captured once in a CUDA graph and replayed (the engine
-        # launches on torch's current stream with cached workspaces, so the
+        # launches on torch's current stream, its scratch from the graph's pool, so the
         # whole step captures)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()

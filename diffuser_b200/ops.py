@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import threading
 
 import torch
 
@@ -40,29 +39,23 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 
 # ------------------------------------------------------------- workspaces
-_WS_LOCK = threading.Lock()
-_WS: dict = {}
-
-
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
-    """Per-device scratch for split-K partial sums, grown on demand and reused
-    (the analogue of the reference's per-shape dequant buffers,
-    R/nf4_ltx23.R:160-175, except that it holds f32 partials, not weights)."""
+    """Scratch of one call (split-K partial sums, or a weight decoded to bf16 and
+    its ready counters), from torch's allocator.  The allocator keeps it for the
+    next call on the same stream, as the reference's per-shape dequant buffers
+    are kept (R/nf4_ltx23.R:160-175), but calls on several streams never meet in
+    it, and a captured graph owns what it replays into: one buffer per device,
+    grown on demand, was written by two streams at once and freed under the
+    graphs that held its address."""
     if nbytes == 0:
         return None
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    with _WS_LOCK:
-        buf = _WS.get(idx)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", idx))
-            _WS[idx] = buf
-        return buf
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def release_workspaces() -> None:
-    """Drop the cached scratch (ltx23_release_dequant_buffers, R/nf4_ltx23.R:185-194)."""
-    with _WS_LOCK:
-        _WS.clear()
+    """Give unused scratch back to the device
+    (ltx23_release_dequant_buffers, R/nf4_ltx23.R:185-194)."""
+    torch.cuda.empty_cache()
 
 
 def workspace_size(M: int, N: int, K: int, fmt: int = _lib.DQ_FMT_NF4) -> int:
