@@ -278,29 +278,51 @@ class AdapterSelection:
     """Which adapter each batch element uses: ids, int32 on the GPU, one per
     element (-1: none).  Every adapted linear of a model shares it; the plan for
     a token count is built at its first use (an element's tokens follow one
-    another, equally many for each), on the stream of that use, which the other
-    streams that use it wait for.  A graph capture takes plans that were built
-    before it (by a call, or by plan(tokens))."""
+    another, equally many for each).  Streams wait for one another here: a plan's
+    build for the stream that set the ids, a use for the stream of the build.  A
+    graph capture takes a selection and plans that were made before it (by a
+    call, or by plan(tokens)); the graph reads their memory at every replay, so
+    keep the selection for as long as the graph."""
 
     def __init__(self, ids: torch.Tensor, n_adapters: int):
         if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or \
                 ids.numel() == 0:
             raise ValueError("ids must be a 1-d int32 CUDA tensor, one entry per batch element")
-        self.ids = ids.clone()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a selection made inside a capture would hold nothing until its replay")
         self.n_adapters = int(n_adapters)
+        with torch.cuda.device(ids.device):
+            self.ids = ids.clone()
+            self._set = self._now()  # stream and event behind the last write of ids
         self._plans: dict = {}  # tokens -> plan
-        self._built: dict = {}  # tokens -> stream handle, event
+        self._built: dict = {}  # tokens -> stream and event behind its last build
 
     def __getstate__(self):  # a copy builds its own plans
-        return dict(self.__dict__, _plans={}, _built={})
+        with torch.cuda.device(self.ids.device):
+            self._after(self._set, self.ids)
+        return dict(self.__dict__, _plans={}, _built={}, _set=None)
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        with torch.cuda.device(self.ids.device):
+            self._set = self._now()
 
     def _offsets(self, tokens: int) -> torch.Tensor:
         batch = self.ids.numel()
         return torch.arange(batch + 1, dtype=torch.int32, device=self.ids.device) * (tokens // batch)
 
-    def _mark(self, tokens: int) -> None:
+    def _now(self):
         stream = torch.cuda.current_stream(self.ids.device)
-        self._built[tokens] = (stream.cuda_stream, stream.record_event())
+        return stream.cuda_stream, stream.record_event()
+
+    def _after(self, mark, *written: torch.Tensor) -> None:
+        """The current stream goes on behind `mark`, whose stream wrote these."""
+        handle, event = mark
+        if handle != ops._raw_stream(self.ids) and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.ids.device)
+            stream.wait_event(event)
+            for t in written:
+                t.record_stream(stream)
 
     def plan(self, tokens: int) -> ops.AdapterPlan:
         plan = self._plans.get(tokens)
@@ -312,15 +334,12 @@ class AdapterSelection:
                 raise RuntimeError(f"the plan for {tokens} tokens must be built before a capture: run the call once, "
                                    "or selection.plan(tokens)")
             with torch.cuda.device(self.ids.device):
+                self._after(self._set, self.ids)
                 plan = ops.adapter_plan(self.ids, self._offsets(tokens), tokens, self.n_adapters)
-                self._mark(tokens)
+                self._built[tokens] = self._now()
             self._plans[tokens] = plan
             return plan
-        handle, event = self._built[tokens]
-        if handle != ops._raw_stream(self.ids) and not torch.cuda.is_current_stream_capturing():
-            stream = torch.cuda.current_stream(self.ids.device)
-            stream.wait_event(event)
-            plan.words.record_stream(stream)
+        self._after(self._built[tokens], plan.words)
         return plan
 
     def update_(self, ids: torch.Tensor) -> "AdapterSelection":
@@ -331,11 +350,16 @@ class AdapterSelection:
         if not isinstance(ids, torch.Tensor) or ids.shape != self.ids.shape or ids.dtype != torch.int32:
             raise ValueError(f"ids must hold {self.ids.numel()} int32 entries, as before")
         with torch.cuda.device(self.ids.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+            self._after(self._set, self.ids)
             self.ids.copy_(ids)
+            if not capturing:
+                self._set = self._now()
             for tokens, plan in self._plans.items():
+                self._after(self._built[tokens], plan.words)
                 plan.update_(self.ids, self._offsets(tokens))
-                if not torch.cuda.is_current_stream_capturing():
-                    self._mark(tokens)
+                if not capturing:
+                    self._built[tokens] = self._now()
         return self
 
 
