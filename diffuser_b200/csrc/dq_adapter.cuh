@@ -795,7 +795,9 @@ __global__ void __launch_bounds__(256, R <= 32 ? 3 : 1) adapter_small_kernel(con
     for (int i = tid; i < 16 * (R / 2); i += 256) {
       const int row = i / (R / 2), c = (i % (R / 2)) * 2;
       float2 v = make_float2(0.f, 0.f);
-      if (!none) {
+      // (columns past the rank are an infinite x times zeros: NaN, which would
+      // meet the zeros of P's rows there)
+      if (!none && c < a.rank) {
         float2 u[kSmallCluster];
 #pragma unroll
         for (int q = 0; q < kSmallCluster; ++q)

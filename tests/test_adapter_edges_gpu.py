@@ -1,0 +1,44 @@
+"""Adapter calls at their edges, against 64-bit formulas."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H = torch.finfo(torch.bfloat16).eps / 2
+U = 2.0 ** -23
+
+
+def _rn(g, *shape, std=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(torch.bfloat16)
+
+
+def _one_adapter(m):
+    from diffuser_b200 import ops
+    off = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    return ops.adapter_plan(torch.zeros(1, dtype=torch.int32, device="cuda"), off, m, 1)
+
+
+# 16-row tiles (3 tokens) and 128-row ones (200), ranks that fill their class and not
+@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("r", [8, 16, 24, 40, 64, 96, 128])
+def test_an_infinite_input_gives_an_infinity(m, r):
+    """One infinity in x, positive weights where it is multiplied: every v of
+    its row is infinite and so is every out, and none is NaN, whatever the rank
+    is padded to."""
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(r)
+    k, n, at = 256, 264, m // 2
+    x, y = _rn(g, m, k), _rn(g, m, n)
+    down, up = _rn(g, 1, r, k, std=k ** -0.5), _rn(g, 1, r, n).abs() + 0.125
+    down[0, :, 5] = 0.5
+    x[at, 5] = float("inf")
+    one, plan = torch.ones(1, device="cuda"), _one_adapter(m)
+    out, hidden = ops.adapter_add(y, x, down, up, one, plan, return_hidden=True)
+    keep = torch.arange(m, device="cuda") != at
+    assert (hidden[at] == float("inf")).all() and (out[at] == float("inf")).all()
+    assert out[keep].isfinite().all() and hidden[keep].isfinite().all()
+    # and back: the same products with the factors' parts exchanged
+    dy = _rn(g, m, n)
+    dy[at, 7] = float("inf")
+    dx, _, _ = ops.adapter_backward(dy, x, hidden, down.abs() + 0.125, up, one, plan)
+    assert (dx[at] == float("inf")).all() and dx[keep].isfinite().all()
