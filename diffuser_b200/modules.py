@@ -28,6 +28,23 @@ def _activate(y: torch.Tensor, act: str) -> torch.Tensor:
     return (gate * up).flatten(-2)
 
 
+class _Frozen:
+    """The tensors of a frozen linear that a call used and its backward pass
+    reads again: held until then, and not to be written in between."""
+
+    def __init__(self, tensors):
+        self.tensors = tensors
+        self.versions = self._versions()
+
+    def _versions(self):  # (inference tensors count none)
+        return [None if t is None or t.is_inference() else t._version for t in self.tensors]
+
+    def again(self):
+        if self._versions() != self.versions:
+            raise RuntimeError("a frozen linear's weight was changed after the call whose backward pass needs it")
+        return self.tensors
+
+
 class _FrozenProjection(torch.autograd.Function):
     """A quantized linear whose input takes a gradient: the forward pass is the
     engine's, the backward pass its input gradient (behind an activation, whose
@@ -35,19 +52,23 @@ class _FrozenProjection(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, linear, act):
-        ctx.linear, ctx.act = linear, act
+        weight, bias, factor = linear._operands(x.device)
+        ctx.linear, ctx.act, ctx.factor = linear, act, factor
+        ctx.frozen = _Frozen((*weight, *(() if act is None else (bias,))))
         if act is not None:
             ctx.save_for_backward(x)
-        return linear._run(x, act, None)
+        return linear._run(x, act, None, (weight, bias, factor))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        weight = ctx.frozen.again()
         if ctx.act is not None:
+            *weight, bias = weight
             with torch.enable_grad():
-                y = ctx.linear._run(ctx.saved_tensors[0], None, None).requires_grad_()
+                y = ctx.linear._run(ctx.saved_tensors[0], None, None, (weight, bias, ctx.factor)).requires_grad_()
                 dy, = torch.autograd.grad(_activate(y, ctx.act), y, dy)
-        return ctx.linear.input_grad(dy), None, None
+        return ctx.linear._input_grad(dy, weight, ctx.factor), None, None
 
 
 def _run_linear(linear, x, act, out):
@@ -123,13 +144,21 @@ class Ltx23Nf4Linear(nn.Module):
                 out: torch.Tensor | None = None) -> torch.Tensor:
         return _run_linear(self, x, act or self.gated_act, out)
 
-    def _run(self, x, act, out):
-        return ops.nf4_linear(x, self.weight_nf4, self.weight_absmax, self.out_features, self.bias,
-                              act=act, out=out)
+    def _operands(self, device):
+        """(weight tensors, bias, per-tensor factor) of a call."""
+        return (self.weight_nf4, self.weight_absmax), self.bias, None
+
+    def _run(self, x, act, out, operands=None):
+        (packed, absmax), bias, _ = operands or self._operands(x.device)
+        return ops.nf4_linear(x, packed, absmax, self.out_features, bias, act=act, out=out)
+
+    def _input_grad(self, dy, weight, factor):
+        return ops.nf4_linear_dgrad(dy, *weight, self.in_features)
 
     def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
         """dy . W for a gradient dy of the projection's output."""
-        return ops.nf4_linear_dgrad(dy, self.weight_nf4, self.weight_absmax, self.in_features)
+        weight, _, factor = self._operands(dy.device)
+        return self._input_grad(dy, weight, factor)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, format=nf4"
@@ -191,12 +220,21 @@ class Ltx23Fp8Linear(nn.Module):
                 out: torch.Tensor | None = None) -> torch.Tensor:
         return _run_linear(self, x, act or self.gated_act, out)
 
-    def _run(self, x, act, out):
-        return ops.fp8_linear(x, self._weight_on(x.device), self._scale_f, self.bias, act=act, out=out)
+    def _operands(self, device):
+        """(weight tensors, bias, per-tensor factor) of a call."""
+        return (self._weight_on(device),), self.bias, self._scale_f
+
+    def _run(self, x, act, out, operands=None):
+        (w8,), bias, factor = operands or self._operands(x.device)
+        return ops.fp8_linear(x, w8, factor, bias, act=act, out=out)
+
+    def _input_grad(self, dy, weight, factor):
+        return ops.fp8_linear_dgrad(dy, *weight, factor)
 
     def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
         """dy . W for a gradient dy of the projection's output."""
-        return ops.fp8_linear_dgrad(dy, self._weight_on(dy.device), self._scale_f)
+        weight, _, factor = self._operands(dy.device)
+        return self._input_grad(dy, weight, factor)
 
     def _weight_on(self, device: torch.device) -> torch.Tensor:
         if self.weight_fp8 is None:
@@ -368,14 +406,16 @@ class _AdaptedProjection(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, down, up, scale, plan, base, pack):
-        y = base.project(x)
+        operands = base.base._operands(x.device)
+        y = base.base._run(x, None, None, operands)
         y, hidden = ops.adapter_add(y, x, down, up, scale, plan, out=y, return_hidden=True)
         if pack:
             packed = ops.checkpoint_pack(x)
             ctx.save_for_backward(hidden, down, up, scale, packed.codes, packed.scales)
         else:
             ctx.save_for_backward(hidden, down, up, scale, x)
-        ctx.plan, ctx.version, ctx.base, ctx.pack = plan, plan.version, base, pack
+        ctx.plan, ctx.version, ctx.base, ctx.pack = plan, plan.version, base.base, pack
+        ctx.frozen, ctx.factor = _Frozen(operands[0]), operands[2]
         return y
 
     @staticmethod
@@ -385,7 +425,7 @@ class _AdaptedProjection(torch.autograd.Function):
             raise RuntimeError("the adapter plan was rebuilt for another batch after this call")
         hidden, down, up, scale, *x = ctx.saved_tensors
         x = ops.PackedActivation(*x) if ctx.pack else x[0]
-        dx = ctx.base.input_grad(dy) if ctx.needs_input_grad[0] else None
+        dx = ctx.base._input_grad(dy, ctx.frozen.again(), ctx.factor) if ctx.needs_input_grad[0] else None
         dx, ddown, dup = ops.adapter_backward(dy, x, hidden, down, up, scale, ctx.plan, dx=dx, out=dx,
                                               factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return dx if ctx.needs_input_grad[0] else None, ddown, dup, None, None, None, None

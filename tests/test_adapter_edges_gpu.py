@@ -42,3 +42,57 @@ def test_an_infinite_input_gives_an_infinity(m, r):
     dy[at, 7] = float("inf")
     dx, _, _ = ops.adapter_backward(dy, x, hidden, down.abs() + 0.125, up, one, plan)
     assert (dx[at] == float("inf")).all() and dx[keep].isfinite().all()
+
+
+def _linear(fmt, seed):
+    from diffuser_b200 import modules
+    lin = (modules.Ltx23Nf4Linear if fmt == "nf4" else modules.Ltx23Fp8Linear)(64, 128, bias=True).cuda()
+    _set(lin, fmt, seed)
+    return lin
+
+
+def _set(lin, fmt, seed):
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn(64, 128, generator=g, device="cuda") * 0.1
+    if fmt == "nf4":
+        lin.set_nf4_weight(*ops.ltx23_nf4_quantize(w))
+    else:
+        w8, s = ops.fp8_quantize(w)
+        lin.set_fp8_weight(w8, s.cpu())
+
+
+@pytest.mark.parametrize("adapted", [False, True])
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+@pytest.mark.parametrize("fmt", ["nf4", "fp8"])
+def test_a_weight_replaced_before_the_backward_pass(fmt, act, adapted):
+    """The gradient is that of the weight the forward pass used, or none."""
+    from diffuser_b200 import modules
+    lin = _linear(fmt, 1)
+    mod = modules.AdapterLinear(lin, 1, 8) if adapted else lin
+    lin.differentiable = True
+    if adapted:
+        mod.selection = modules.AdapterSelection(torch.zeros(1, dtype=torch.int32, device="cuda"), 1)
+    x = torch.randn(9, 128, device="cuda").to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(9, 64, device="cuda").to(torch.bfloat16)
+    want, = torch.autograd.grad(mod(x, act=act), x, dy)
+    y = mod(x, act=act)
+    _set(lin, fmt, 2)
+    if fmt == "nf4":  # in place: the old weight is gone
+        with pytest.raises(RuntimeError, match="changed"):
+            y.backward(dy)
+    else:  # another tensor: the old one is still held
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+    assert not torch.equal(torch.autograd.grad(mod(x, act=act), x, dy)[0], want)
+
+
+def test_a_bias_replaced_before_the_backward_pass():
+    lin = _linear("nf4", 3)
+    lin.differentiable = True
+    x = torch.randn(9, 128, device="cuda").to(torch.bfloat16).requires_grad_()
+    y = lin(x, act="gelu_tanh")
+    with torch.no_grad():
+        lin.bias.add_(1)
+    with pytest.raises(RuntimeError, match="changed"):
+        y.sum().backward()
+    lin(x).sum().backward()  # without an activation the bias is not read again
