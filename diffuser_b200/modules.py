@@ -10,6 +10,7 @@ loader swap ``do.call(`$<-`, list(parent, leaf, quant_mod))``
 from __future__ import annotations
 
 import re
+import weakref
 
 import torch
 from torch import nn
@@ -320,7 +321,10 @@ class AdapterSelection:
     build for the stream that set the ids, a use for the stream of the build.  A
     graph capture takes a selection and plans that were made before it (by a
     call, or by plan(tokens)); the graph reads their memory at every replay, so
-    keep the selection for as long as the graph."""
+    keep the selection for as long as the graph.  Of the plans that no capture
+    took, the sixteen used last are kept, and those that are in use elsewhere."""
+
+    KEPT = 16
 
     def __init__(self, ids: torch.Tensor, n_adapters: int):
         if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32 or ids.dim() != 1 or \
@@ -332,16 +336,22 @@ class AdapterSelection:
         with torch.cuda.device(ids.device):
             self.ids = ids.clone()
             self._set = self._now()  # stream and event behind the last write of ids
-        self._plans: dict = {}  # tokens -> plan
-        self._built: dict = {}  # tokens -> stream and event behind its last build
+        self._no_plans()
+
+    def _no_plans(self):
+        self._plans = weakref.WeakValueDictionary()  # tokens -> plan, every one alive
+        self._built = weakref.WeakKeyDictionary()    # plan -> stream and event behind its last build
+        self._recent: dict = {}                      # tokens -> plan, the KEPT used last, oldest first
+        self._captured: dict = {}                    # tokens -> plan
 
     def __getstate__(self):  # a copy builds its own plans
         with torch.cuda.device(self.ids.device):
             self._after(self._set, self.ids)
-        return dict(self.__dict__, _plans={}, _built={}, _set=None)
+        return {"ids": self.ids, "n_adapters": self.n_adapters}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
+        self._no_plans()
         with torch.cuda.device(self.ids.device):
             self._set = self._now()
 
@@ -374,10 +384,16 @@ class AdapterSelection:
             with torch.cuda.device(self.ids.device):
                 self._after(self._set, self.ids)
                 plan = ops.adapter_plan(self.ids, self._offsets(tokens), tokens, self.n_adapters)
-                self._built[tokens] = self._now()
+                self._built[plan] = self._now()
             self._plans[tokens] = plan
-            return plan
-        self._after(self._built[tokens], plan.words)
+        else:
+            self._after(self._built[plan], plan.words)
+        if torch.cuda.is_current_stream_capturing():
+            self._captured[tokens] = plan
+        self._recent.pop(tokens, None)
+        self._recent[tokens] = plan
+        if len(self._recent) > self.KEPT:
+            del self._recent[next(iter(self._recent))]
         return plan
 
     def update_(self, ids: torch.Tensor) -> "AdapterSelection":
@@ -393,11 +409,11 @@ class AdapterSelection:
             self.ids.copy_(ids)
             if not capturing:
                 self._set = self._now()
-            for tokens, plan in self._plans.items():
-                self._after(self._built[tokens], plan.words)
+            for tokens, plan in list(self._plans.items()):
+                self._after(self._built[plan], plan.words)
                 plan.update_(self.ids, self._offsets(tokens))
                 if not capturing:
-                    self._built[tokens] = self._now()
+                    self._built[plan] = self._now()
         return self
 
 

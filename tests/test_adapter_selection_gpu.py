@@ -100,3 +100,31 @@ def test_no_selection_is_made_inside_a_capture():
             modules.AdapterSelection(ids, 2)
     graph.replay()
     assert out.item() == 1
+
+
+def test_plans_of_many_lengths_are_not_all_kept():
+    """Prompts of ever other lengths: the plans used last are kept, with those a
+    capture took and those in use, and every one alive follows an update."""
+    import gc
+    import weakref
+    from diffuser_b200 import modules, ops
+    ids = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    sel = modules.AdapterSelection(ids, 3)
+    operands = _operands(2, 3)
+    sel.plan(6)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.adapter_add(*operands, sel.plan(6))
+    mine = sel.plan(10)
+    seen = [weakref.ref(sel.plan(2 * n)) for n in range(10, 60)]
+    gc.collect()
+    alive = [r for r in seen if r() is not None]
+    assert len(alive) == sel.KEPT and alive == seen[-sel.KEPT:]
+    assert sel.plan(10) is mine  # held here
+    sel.update_(torch.tensor([2, -1], dtype=torch.int32, device="cuda"))
+    graph.replay()
+    offsets = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+    assert torch.equal(out, ops.adapter_add(*operands, ops.adapter_plan(sel.ids, offsets, 6, 3)))
+    fresh = ops.adapter_plan(sel.ids, torch.tensor([0, 5, 10], dtype=torch.int32, device="cuda"), 10, 3)
+    wide = [torch.cat([t, t])[:10] for t in operands[:2]]
+    assert torch.equal(ops.adapter_add(*wide, *operands[2:], mine), ops.adapter_add(*wide, *operands[2:], fresh))
