@@ -129,6 +129,7 @@ SIGNATURES = {
     "dq_checkpoint_pack": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
     "dq_checkpoint_unpack": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p]),
     "dq_linear_dgrad_workspace": (_c_sz, [_c_i64, _c_i64]),
+    "dq_linear_dgrad_workspace_for": (_c_sz, [_c_i64, _c_i64, _c_i64]),
     "dq_linear_nf4_dgrad": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p, ctypes.c_int, _c_i64, _c_p, _c_p,
                                            _c_sz, _c_p]),
     "dq_linear_fp8_dgrad": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_p, ctypes.c_float, _c_i64, _c_p, _c_p, _c_sz,

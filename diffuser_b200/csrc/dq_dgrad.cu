@@ -106,13 +106,13 @@ int dgrad_impl(int fmt, const void* dy, int64_t M, int64_t N, const uint8_t* w, 
   int sms = 0;
   const int rc = device_sms(&sms);
   if (rc != DQ_OK) return rc;
-  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_linear_dgrad_workspace(N, K))
-    return DQ_ERR_WORKSPACE;
   if (fused_wins(M, N)) {
     const FusedPlan p = fused_plan(fmt, M, N, K, sms);
     return fmt == kFmtNF4 ? launch_fused<kFmtNF4>(p, dy, M, N, w, absmax, sbf, scale, K, dx, st)
                           : launch_fused<kFmtFP8>(p, dy, M, N, w, absmax, sbf, scale, K, dx, st);
   }
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < dq_linear_dgrad_workspace(N, K))
+    return DQ_ERR_WORKSPACE;
   const dim3 grid(static_cast<unsigned>(ceil_div(K, 64)), static_cast<unsigned>(ceil_div(N, 128)));
   if (fmt == kFmtNF4)
     decode_transposed_kernel<kFmtNF4><<<grid, 256, 0, st>>>(w, absmax, sbf, 0.f, static_cast<int>(N),
@@ -135,6 +135,10 @@ extern "C" {
 
 size_t dq_linear_dgrad_workspace(int64_t N, int64_t K) {
   return N <= 0 || K <= 0 ? 0 : up256(static_cast<size_t>(N) * K * 2);
+}
+
+size_t dq_linear_dgrad_workspace_for(int64_t M, int64_t N, int64_t K) {
+  return M <= 0 || fused_wins(M, N) ? 0 : dq_linear_dgrad_workspace(N, K);
 }
 
 int dq_linear_nf4_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* packed, const void* absmax,

@@ -646,7 +646,7 @@ def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor, dtypes):
     _same_device(weight, "weight", dy)
     if weight.dtype not in dtypes or not weight.is_contiguous():
         raise TypeError(f"the weight must be contiguous {' or '.join(str(t) for t in dtypes)}, got {weight.dtype}")
-    if n % 8 != 0:
+    if n == 0 or n % 8 != 0:
         raise ValueError("the input gradient needs out_features % 8 == 0")
     if dy.dtype != _BF16:
         raise TypeError(f"gradients must be bfloat16 on the GPU path, got {dy.dtype}")
@@ -654,7 +654,10 @@ def _prep_dgrad(dy: torch.Tensor, n: int, k: int, weight: torch.Tensor, dtypes):
         raise ValueError(f"last dim of dy is {tuple(dy.shape)[-1:]}, expected out_features={n}")
     dy2 = dy if dy.is_contiguous() and dy.data_ptr() % 16 == 0 else dy.new_empty(dy.shape).copy_(dy)
     dx = torch.empty((*dy.shape[:-1], k), dtype=_BF16, device=dy.device)
-    return dy2, dx, 2 * n * k + 255 & ~255  # dq_linear_dgrad_workspace
+    m = dy2.numel() // n
+    nbytes = _lib.lib().dq_linear_dgrad_workspace_for(m, n, k)
+    ws = _scratch(nbytes, dy) if nbytes else None
+    return dy2, dx, m, ws, 0 if ws is None else ws.data_ptr(), nbytes
 
 
 def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
@@ -663,16 +666,15 @@ def nf4_linear_dgrad(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tenso
     [..., N] -> [..., K].  absmax float32 or bf16 as for the forward."""
     _require_cuda(dy, "dy")
     k = int(in_features)
-    n = packed.numel() * 2 // k
+    n = packed.numel() * 2 // max(k, 1)
     if n * k != packed.numel() * 2 or absmax.numel() * NF4_BLOCK != n * k:
         raise ValueError("packed / absmax sizes do not match in_features")
-    dy2, dx, nbytes = _prep_dgrad(dy, n, k, packed, (torch.uint8,))
+    dy2, dx, m, ws, wsp, nbytes = _prep_dgrad(dy, n, k, packed, (torch.uint8,))
     _same_device(absmax, "absmax", dy)
     am = (absmax if absmax.dtype in (_F32, _BF16) else absmax.float()).contiguous()
     with _on(dy):
-        ws = _scratch(nbytes, dy)
-        _lib.call("dq_linear_nf4_dgrad", dy2.data_ptr(), dy2.numel() // n, n, packed.data_ptr(), am.data_ptr(),
-                  _dtype_code(am), k, dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy))
+        _lib.call("dq_linear_nf4_dgrad", dy2.data_ptr(), m, n, packed.data_ptr(), am.data_ptr(),
+                  _dtype_code(am), k, dx.data_ptr(), wsp, nbytes, _raw_stream(dy))
     return dx
 
 
@@ -682,11 +684,10 @@ def fp8_linear_dgrad(dy: torch.Tensor, w8: torch.Tensor, scale: float) -> torch.
     if w8.dim() != 2:
         raise ValueError(f"w8 must be [out_features, in_features], got {tuple(w8.shape)}")
     n, k = int(w8.shape[0]), int(w8.shape[1])
-    dy2, dx, nbytes = _prep_dgrad(dy, n, k, w8, (torch.float8_e4m3fn, torch.uint8))
+    dy2, dx, m, ws, wsp, nbytes = _prep_dgrad(dy, n, k, w8, (torch.float8_e4m3fn, torch.uint8))
     with _on(dy):
-        ws = _scratch(nbytes, dy)
-        _lib.call("dq_linear_fp8_dgrad", dy2.data_ptr(), dy2.numel() // n, n, w8.data_ptr(), float(scale), k,
-                  dx.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dy))
+        _lib.call("dq_linear_fp8_dgrad", dy2.data_ptr(), m, n, w8.data_ptr(), float(scale), k,
+                  dx.data_ptr(), wsp, nbytes, _raw_stream(dy))
     return dx
 
 

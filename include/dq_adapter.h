@@ -89,12 +89,15 @@ int dq_checkpoint_unpack(const int8_t* codes, const float* scales, int64_t M, in
 
 /* Input gradient of the quantized linears: dx[M, K] = dy[M, N] . dequant(W),
  * W as dq_linear_nf4 / dq_linear_fp8 take it (absmax f32 or, scale_dtype
- * DQ_DTYPE_BF16, bf16).  Up to 512 tokens the weight is decoded next to the
- * product, in one launch; beyond, once, transposed, into the workspace
- * (dq_linear_dgrad_workspace bytes, 16-byte aligned, asked for in either case)
- * and multiplied by the bf16 CTA-pair GEMM.  Sums are float32, dx is rounded
- * once; the same inputs give the same bits.  N % 8 == 0, K % 64 == 0 (NF4) or
- * K % 16 == 0 (fp8); dy and dx contiguous, 16-byte aligned. */
+ * DQ_DTYPE_BF16, bf16).  Up to 256 tokens, and up to 512 where N >= 2048, the
+ * weight is decoded next to the product, in one launch without a workspace;
+ * beyond, once, transposed, into the workspace (16-byte aligned) and
+ * multiplied by the bf16 CTA-pair GEMM.  dq_linear_dgrad_workspace_for: the
+ * bytes that a call with M tokens needs (0: none, workspace may be NULL);
+ * dq_linear_dgrad_workspace: enough for any number of tokens.  Sums are float32, dx is
+ * rounded once; the same inputs give the same bits.  N % 8 == 0, K % 64 == 0
+ * (NF4) or K % 16 == 0 (fp8); dy and dx contiguous, 16-byte aligned. */
+size_t dq_linear_dgrad_workspace_for(int64_t M, int64_t N, int64_t K);
 size_t dq_linear_dgrad_workspace(int64_t N, int64_t K);
 int dq_linear_nf4_dgrad(const void* dy, int64_t M, int64_t N, const uint8_t* packed,
                         const void* absmax, int scale_dtype, int64_t K, void* dx, void* workspace,
