@@ -235,7 +235,8 @@ BackwardWs backward_ws(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A,
   return w;
 }
 
-// hidden = scale x . P^T (down), out = act(y + hidden . Q) (up), on one plan.
+// hidden = scale x . P^T (down), out = act(y + hidden . Q) (up), on one plan;
+// without an out the first alone.
 // hidden: where the low-rank intermediate goes, complete (zero rows without an
 // adapter) if want_hidden; the small-batch kernel takes NULL.  between: launches
 // that read x again, put right behind the large-tile down kernel while x is
@@ -246,7 +247,7 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
             void* out, int64_t ldo, void* hidden, bool want_hidden, float* hidden32, int sms, cudaStream_t st,
             Between between) {
   const AdapterPlan lay = adapter_plan_layout(M, R, A);
-  const int with_none = act != kActNone || out != y || want_hidden;
+  const int with_none = out != nullptr && (act != kActNone || out != y || want_hidden);
   if (!large_tiles(M, R, A)) {
     SmallArgs a = {};
     a.x = static_cast<const __nv_bfloat16*>(x);
@@ -263,7 +264,7 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
     a.ldy = ldy;
     a.ldo = ldo;
     a.K = static_cast<int>(F_in);
-    a.N = static_cast<int>(F_out);
+    a.N = out == nullptr ? 0 : static_cast<int>(F_out);  // (no columns: the hidden tile is all)
     a.rank = r;
     a.A = A;
     a.act = act;
@@ -304,7 +305,7 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
     constexpr int R_ = decltype(rc)::value;
     int e2 = launch_down<R_>(d, M, R, st);
     if (e2 == DQ_OK) e2 = between();
-    return e2 != DQ_OK ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, R, sms, st);
+    return e2 != DQ_OK || out == nullptr ? e2 : launch_up<R_>(u, static_cast<int>(lay.max_tiles), M, R, sms, st);
   });
 }
 
@@ -389,12 +390,12 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
   int rc = bank_shape(M, R, K, N, r, A);
   if (rc != DQ_OK) return rc;
   const bool i8 = x_scales != nullptr;
-  const bool want_w = ddown != nullptr;
+  const bool want_w = ddown != nullptr, want_x = dx != nullptr || dx_out != nullptr;
   if (!row_stride_ok(lddy, N) || (i8 && (K % 16 != 0 || ldx < K || ldx % 16 != 0)) ||
       (want_w && !i8 && !row_stride_ok(ldx, K)))
     return DQ_ERR_SHAPE;
-  if (!row_stride_ok(lddx, K) || !row_stride_ok(lddxo, K)) return DQ_ERR_SHAPE;
-  if ((ddown == nullptr) != (dup == nullptr)) return DQ_ERR_ARG;
+  if (want_x && (!row_stride_ok(lddx, K) || !row_stride_ok(lddxo, K))) return DQ_ERR_SHAPE;
+  if ((ddown == nullptr) != (dup == nullptr) || (M > 0 && !want_x && !want_w)) return DQ_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (M == 0) {
     if (want_w && (cudaMemsetAsync(ddown, 0, static_cast<size_t>(A) * r * K * 2, st) != cudaSuccess ||
@@ -403,9 +404,9 @@ int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx
     return DQ_OK;
   }
   if (dy == nullptr || down == nullptr || up == nullptr || scale == nullptr || plan == nullptr ||
-      dx == nullptr || dx_out == nullptr || (want_w && (x == nullptr || hidden == nullptr)))
+      (want_x && (dx == nullptr || dx_out == nullptr)) || (want_w && (x == nullptr || hidden == nullptr)))
     return DQ_ERR_ARG;
-  if (dx == dx_out && lddx != lddxo) return DQ_ERR_SHAPE;
+  if (want_x && dx == dx_out && lddx != lddxo) return DQ_ERR_SHAPE;
   if (!aligned(dy, 16) || !aligned(x, 16) || !aligned(x_scales, 4) || !aligned(hidden, 16) || !aligned(down, 16) ||
       !aligned(up, 16) || !aligned(scale, 4) || !aligned(plan, 16) || !aligned(dx, 16) || !aligned(dx_out, 16) ||
       !aligned(ddown, 16) || !aligned(dup, 16))

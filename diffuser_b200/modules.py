@@ -443,8 +443,9 @@ class _AdaptedProjection(torch.autograd.Function):
         x = ops.PackedActivation(*x) if ctx.pack else x[0]
         dx = ctx.base._input_grad(dy, ctx.frozen.again(), ctx.factor) if ctx.needs_input_grad[0] else None
         dx, ddown, dup = ops.adapter_backward(dy, x, hidden, down, up, scale, ctx.plan, dx=dx, out=dx,
-                                              factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
-        return dx if ctx.needs_input_grad[0] else None, ddown, dup, None, None, None, None
+                                              factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2],
+                                              inputs=ctx.needs_input_grad[0])
+        return dx, ddown, dup, None, None, None, None
 
 
 class AdapterLinear(nn.Module):

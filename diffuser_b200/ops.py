@@ -522,7 +522,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
 
 def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
                      scale: torch.Tensor, plan: AdapterPlan, dx: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None, factors: bool = True):
+                     out: torch.Tensor | None = None, factors: bool = True, inputs: bool = True):
     """Gradients of adapter_add (without act): returns (dx, ddown, dup).
 
     dy [..., N] is the output's gradient; x the forward's input, as bf16
@@ -531,8 +531,11 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
     (nf4_linear_dgrad / fp8_linear_dgrad): the adapters' part is added to it, in
     `out` (which may be dx, and overlaps no other operand) or a new tensor.
     ddown / dup have the layouts of down / up, zeros for adapters without
-    tokens; with factors=False they are None, and neither is computed.  The same
-    inputs give the same bits."""
+    tokens; with factors=False they are None, and neither is computed, nor with
+    inputs=False (a first layer's) the gradient of x.  The same inputs give the
+    same bits."""
+    if not inputs and (dx is not None or out is not None or not factors):
+        raise ValueError("inputs=False takes neither dx nor out, nor factors=False")
     _require_cuda(dy, "dy")
     a, r, k, n = _bank(down, up, scale, dy)
     dy2, dyp, lddy, m = _row_operand(dy, "dy", n, dy)
@@ -551,25 +554,24 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
     if hidden.dtype != _BF16 or hidden.shape != (m, r) or not hidden.is_contiguous() or hidden.data_ptr() % 16 != 0:
         raise TypeError(f"hidden must be a contiguous bfloat16 [{m}, {r}] tensor")
     shape = (*dy.shape[:-1], k)
-    if dx is None:
-        base = torch.zeros(shape, dtype=_BF16, device=dy.device)
-    else:
-        base = dx
-    dx2, dxp, lddx, md = _row_operand(base, "dx", k, dy)
-    if md != m:
-        raise ValueError(f"dx holds {md} tokens, dy {m}")
-    if out is None:
-        res = base if dx is None else torch.empty_like(dx) if dx2 is dx and dx.shape == shape else \
-            torch.empty(shape, dtype=_BF16, device=dy.device)
-        op, ldo = res.data_ptr(), k
-    else:
-        res = out
-        _, op, ldo, mo = _row_operand(out, "out", k, dy, must_alias=True)
-        if mo != m:
-            raise ValueError(f"out holds {mo} tokens, dy {m}")
-    if out is not None and m:
-        other = ((dy2, dyp, "dy"), (x2, xp, "x"), (hidden, hidden.data_ptr(), "hidden"))
-        _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
+    res, dxp, lddx, op, ldo = None, 0, k, 0, k
+    if inputs:
+        base = torch.zeros(shape, dtype=_BF16, device=dy.device) if dx is None else dx
+        dx2, dxp, lddx, md = _row_operand(base, "dx", k, dy)
+        if md != m:
+            raise ValueError(f"dx holds {md} tokens, dy {m}")
+        if out is None:
+            res = base if dx is None else torch.empty_like(dx) if dx2 is dx and dx.shape == shape else \
+                torch.empty(shape, dtype=_BF16, device=dy.device)
+            op = res.data_ptr()
+        else:
+            res = out
+            _, op, ldo, mo = _row_operand(out, "out", k, dy, must_alias=True)
+            if mo != m:
+                raise ValueError(f"out holds {mo} tokens, dy {m}")
+            if m:
+                other = ((dy2, dyp, "dy"), (x2, xp, "x"), (hidden, hidden.data_ptr(), "hidden"))
+                _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
     ddown, dup = (torch.empty_like(down), torch.empty_like(up)) if factors else (None, None)
     with _on(dy):
         nbytes = _lib.lib().dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)

@@ -65,7 +65,8 @@ int dq_adapter_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64
  * int8 codes [M, K] of a checkpoint with its scales f32 [M, ceil(K / 128)]
  * (row stride ceil(K / 128)); K % 16 == 0 then.  Adapters without tokens get
  * zero gradients.  ddown and dup may be NULL together (input gradient only; x
- * and hidden are not read then).  Sums are float32 in a fixed order: the same
+ * and hidden are not read then), or dx and dx_out (the factors' gradients only,
+ * as for a first layer; the product with down is left out then).  Sums are float32 in a fixed order: the same
  * inputs give the same bits. */
 size_t dq_adapter_backward_workspace(int64_t M, int64_t R, int64_t K, int64_t N, int r, int A);
 int dq_adapter_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
