@@ -471,12 +471,23 @@ def _check_plan(plan: AdapterPlan, m: int, a: int, like: torch.Tensor) -> None:
         _same_device(plan.words, "plan", like)
 
 
-def _refuse_alias(out: torch.Tensor, op: int, others) -> None:
-    """out's rows are written while other tokens of `others` are still read."""
-    for t, p, name in others:
-        if p == op or (out.is_contiguous() and t.is_contiguous() and
-                       op < p + t.numel() * t.element_size() and p < op + out.numel() * out.element_size()):
-            raise ValueError(f"out must not overlap {name}")
+def _whole(t: torch.Tensor, name: str):
+    """A contiguous operand as one row of bytes."""
+    n = t.numel() * t.element_size()
+    return t.data_ptr(), n, n, 1, name
+
+
+def _refuse_alias(out, others) -> None:
+    """out's rows are written while other tokens of `others` are still read.
+    Each is (address, row stride, row width, rows, name), in bytes; rows of one
+    stride that keep to different columns do not meet."""
+    p, ld, w, m, _ = out
+    for q, ldq, wq, mq, name in others:
+        if m == 0 or mq == 0 or p + (m - 1) * ld + w <= q or q + (mq - 1) * ldq + wq <= p:
+            continue
+        if ld == ldq and w <= (q - p) % ld <= ld - wq:
+            continue
+        raise ValueError(f"out must not overlap {name}")
 
 
 def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
@@ -508,8 +519,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
         _, op, ldo, mo = _row_operand(out, "out", n_out, y, must_alias=True)
         if mo != m:
             raise ValueError(f"out holds {mo} tokens, y {m}")
-        if m:
-            _refuse_alias(out, op, ((x2, xp, "x"),) if op == yp else ((x2, xp, "x"), (y2, yp, "y unless it is y")))
+        _refuse_alias((op, 2 * ldo, 2 * n_out, m, "out"), (
+            (xp, 2 * ldx, 2 * k, m, "x"), *(() if op == yp else ((yp, 2 * ldy, 2 * n, m, "y unless it is y"),)),
+            _whole(down, "down"), _whole(up, "up"), _whole(scale, "scale"), _whole(plan.words, "plan")))
     hidden = torch.empty((m, r), dtype=_BF16, device=y.device) if return_hidden else None
     nbytes = 0 if return_hidden else plan.add_workspace * r
     ws = _scratch(nbytes, y) if nbytes else None
@@ -569,9 +581,11 @@ def adapter_backward(dy: torch.Tensor, x, hidden: torch.Tensor, down: torch.Tens
             _, op, ldo, mo = _row_operand(out, "out", k, dy, must_alias=True)
             if mo != m:
                 raise ValueError(f"out holds {mo} tokens, dy {m}")
-            if m:
-                other = ((dy2, dyp, "dy"), (x2, xp, "x"), (hidden, hidden.data_ptr(), "hidden"))
-                _refuse_alias(out, op, other if op == dxp else (*other, (dx2, dxp, "dx unless it is dx")))
+            size = x2.element_size()
+            _refuse_alias((op, 2 * ldo, 2 * k, m, "out"), (
+                (dyp, 2 * lddy, 2 * n, m, "dy"), (xp, size * ldx, size * k, m, "x"), _whole(hidden, "hidden"),
+                *(() if op == dxp else ((dxp, 2 * lddx, 2 * k, m, "dx unless it is dx"),)),
+                _whole(down, "down"), _whole(up, "up"), _whole(scale, "scale"), _whole(plan.words, "plan")))
     ddown, dup = (torch.empty_like(down), torch.empty_like(up)) if factors else (None, None)
     with _on(dy):
         nbytes = _lib.lib().dq_adapter_backward_workspace(m, plan.requests, k, n, r, a)
