@@ -18,6 +18,9 @@ inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7
 inline const __nv_bfloat16* bf(const void* p) { return static_cast<const __nv_bfloat16*>(p); }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// An output in the place of an operand has its rows.
+bool same_rows(const void* out, int64_t ld_out, const void* in, int64_t ld_in) { return out != in || ld_out == ld_in; }
+
 bool stride_ok(int64_t ld, int D) { return ld >= D && ld % 4 == 0; }
 
 int shape_ok(int64_t T, int S, int D) {
@@ -147,6 +150,11 @@ int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int6
   for (const void* p : {x, y, gate, scale, shift, post_weight, pre_weight, static_cast<const void*>(s),
                         static_cast<const void*>(h)})
     if (!aligned8(p)) return DQ_ERR_ALIGN;
+  // in place row by row, or rows of another stride are written before they are read
+  if (s == h) return DQ_ERR_ARG;
+  if (!same_rows(s, ld_s, x, ld_x) || !same_rows(s, ld_s, y, ld_y) || !same_rows(h, ld_h, x, ld_x) ||
+      !same_rows(h, ld_h, y, ld_y))
+    return DQ_ERR_SHAPE;
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
   const NormArgs a = {bf(x), bf(y), bf(gate), bf(scale), bf(shift), bf(post_weight), bf(pre_weight),
@@ -189,6 +197,13 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
     if (!aligned8(p)) return DQ_ERR_ALIGN;
   for (const float* p : {dgate, dscale, dshift, dpost_weight, dpre_weight})
     if ((reinterpret_cast<uintptr_t>(p) & 3) != 0) return DQ_ERR_ALIGN;
+  if (dx == dy) return DQ_ERR_ARG;
+  for (const void* out : {static_cast<const void*>(dx), static_cast<const void*>(dy)}) {
+    const int64_t ld = out == dx ? ld_dx : ld_dy;
+    if (!same_rows(out, ld, ds, ld_ds) || !same_rows(out, ld, dh, ld_dh) || !same_rows(out, ld, s, ld_s) ||
+        !same_rows(out, ld, y, ld_y))
+      return DQ_ERR_SHAPE;
+  }
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
   const int chunks = chunks_of(B, S, backward_slots(D, sms), 4);

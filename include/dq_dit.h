@@ -81,7 +81,7 @@ int dq_gated_residual(const void* x, int64_t ld_x, const void* gate, int64_t ld_
  * and rounds s and h once; DQ_ROUND_OPS rounds to bf16 after every tensor op
  * (norm, weight, gate, residual scale when it is not 1; norm, weight, 1 +
  * scale, product), the bits of dq_gated_residual followed by
- * dq_adaln_modulate.  s may be x or y.  D a multiple of 4 up to 8192; every
+ * dq_adaln_modulate.  s may be x or y, with that one's row stride.  D a multiple of 4 up to 8192; every
  * row start 8-byte aligned. */
 enum { DQ_NORM_NONE = 0, DQ_NORM_RMS = 1, DQ_NORM_LAYER = 2 };
 enum { DQ_ROUND_ONCE = 0, DQ_ROUND_OPS = 1 };
@@ -98,7 +98,7 @@ int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int6
  * dpre_weight f32 [D], contiguous, each may be NULL (dgate without gate is the
  * gradient of a gate of ones, and so on).  The statistics are recomputed from
  * s and y.  Sums over tokens are float32 in a fixed order.  dx may be ds, dy
- * may be y.  The workspace (dq_gated_norm_backward_workspace bytes, 16-byte
+ * may be y, with their row strides.  The workspace (dq_gated_norm_backward_workspace bytes, 16-byte
  * aligned) holds the partial sums.  B = T / S. */
 size_t dq_gated_norm_backward_workspace(int64_t T, int S, int D);
 int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_t ld_dh, const void* s,
