@@ -171,19 +171,49 @@ int launch_up(UpArgs a, int tiles, int64_t M, int64_t requests, int sms, cudaStr
                 true, dim3(1), a);
 }
 
+// Resident clusters of the small-batch kernel, once per device (it allocates no
+// tensor memory, so the runtime's count holds).
 template <int R>
-int launch_small(SmallArgs a, int64_t M, int64_t R_, int sms, cudaStream_t st) {
+int small_clusters(int* out) {
   using C = SmallCfg<R>;
-  static std::atomic<int> set[kMaxDevices];
+  static std::atomic<int> set[kMaxDevices], count[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
   const int rc = allow_smem(adapter_small_kernel<R>, C::kSmemBytes, set);
+  if (rc != DQ_OK) return rc;
+  int n = count[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kSmallCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024 * kSmallCluster);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, adapter_small_kernel<R>, &cfg) != cudaSuccess || n < 1) return DQ_ERR_LAUNCH;
+    count[dev].store(n, std::memory_order_release);
+  }
+  *out = n;
+  return DQ_OK;
+}
+
+template <int R>
+int launch_small(SmallArgs a, int64_t M, int64_t R_, cudaStream_t st) {
+  using C = SmallCfg<R>;
+  int resident = 0;
+  const int rc = small_clusters<R>(&resident);
   if (rc != DQ_OK) return rc;
   a.k_per_rank = static_cast<int>(ceil_div(ceil_div(a.K, kSmallCluster), 32) * 32);
   // clusters per tile: more than one (each repeats the down projection) only
-  // while the CTAs have more than one step of columns and the SMs have room
+  // while the CTAs have more than one step of columns and all are resident at
+  // once (rank 64, N = 12288, one token for each of 4 adapters 9.2 us, in two
+  // waves 18.7; of 8 adapters 12.5 and 21.9; N = 4096 8.0 and 12.7)
   const int64_t tiles = std::max<int64_t>(ceil_div(M, kBlockRows), std::min<int64_t>(std::min<int64_t>(a.A, R_), M));
   int clusters = 1;
-  while (clusters < 8 && a.N > clusters * kSmallCluster * C::kStepCols && 2 * clusters * kSmallCluster * tiles <= 3 * sms)
-    clusters *= 2;
+  while (clusters < 8 && a.N > clusters * kSmallCluster * C::kStepCols && 2 * clusters * tiles <= resident) clusters *= 2;
   a.cols_per_cta = static_cast<int>(ceil_div(ceil_div(a.N, clusters * kSmallCluster), 64) * 64);
   a.ctas_per_tile = clusters * kSmallCluster;
   const dim3 grid(static_cast<unsigned>(a.lay.cap / kBlockRows) * a.ctas_per_tile);
@@ -269,7 +299,7 @@ int down_up(const void* x, int64_t ldx, int64_t F_in, const void* P, const void*
     a.A = A;
     a.act = act;
     a.with_none = with_none;
-    const int e = by_rank(r, [&](auto rc) { return launch_small<decltype(rc)::value>(a, M, R, sms, st); });
+    const int e = by_rank(r, [&](auto rc) { return launch_small<decltype(rc)::value>(a, M, R, st); });
     return e != DQ_OK ? e : between();
   }
   DownArgs d = {};

@@ -682,6 +682,7 @@ struct SmallCfg {
   static constexpr int kVStride = R * 2 + 16;              // bytes of a row of the bf16 hidden tile
   static constexpr int kOffV = kOffSum + 16 * R * 4;
   static constexpr int kSmemBytes = kOffV + 16 * kVStride;
+  static constexpr int kMinCtas = 228 * 1024 / (kSmemBytes + 1024);  // per SM: 3, 2, 1, 1
 };
 
 struct SmallArgs {
@@ -697,7 +698,7 @@ struct SmallArgs {
 };
 
 template <int R>
-__global__ void __launch_bounds__(256, R <= 32 ? 3 : 1) adapter_small_kernel(const SmallArgs a) {
+__global__ void __launch_bounds__(256, SmallCfg<R>::kMinCtas) adapter_small_kernel(const SmallArgs a) {
   using C = SmallCfg<R>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);

@@ -96,3 +96,26 @@ def test_a_bias_replaced_before_the_backward_pass():
     with pytest.raises(RuntimeError, match="changed"):
         y.sum().backward()
     lin(x).sum().backward()  # without an activation the bias is not read again
+
+
+# one to eight clusters of CTAs per 16-row tile, by the tiles, the columns and
+# what a rank leaves resident
+@pytest.mark.parametrize("r", [16, 32, 64, 128])
+@pytest.mark.parametrize("tiles,n", [(1, 16392), (2, 12288), (4, 8200), (5, 16384), (8, 4096), (17, 6152)])
+def test_small_batches_of_wide_outputs(tiles, n, r):
+    from diffuser_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(tiles)
+    k, m = 264, tiles
+    x, y, dy = _rn(g, m, k), _rn(g, m, n), _rn(g, m, n)
+    down, up, scale = _rn(g, m, r, k, std=k ** -0.5), _rn(g, m, r, n, std=r ** -0.5), torch.rand(m, generator=g, device="cuda") + 0.5
+    ids = torch.arange(m, dtype=torch.int32, device="cuda")
+    plan = ops.adapter_plan(ids, torch.arange(m + 1, dtype=torch.int32, device="cuda"), m, m)
+    out, hidden = ops.adapter_add(y, x, down, up, scale, plan, return_hidden=True)
+    v = scale.double()[:, None] * torch.einsum("mk,mrk->mr", x.double(), down.double())
+    v_err = (k + 8) * U * scale.double()[:, None] * torch.einsum("mk,mrk->mr", x.double().abs(), down.double().abs())
+    assert ((hidden.double() - v).abs() <= 1.01 * (v_err + H * v.abs())).all()
+    ref = y.double() + torch.einsum("mr,mrn->mn", v, up.double())
+    size = torch.einsum("mr,mrn->mn", H * v.abs() + v_err, up.double().abs()) + (r + 4) * U * (
+        torch.einsum("mr,mrn->mn", v.abs(), up.double().abs()) + y.double().abs())
+    assert ((out.double() - ref).abs() <= 1.01 * (size + H * ref.abs())).all()
+    assert ops.device_error() == 0
