@@ -16,7 +16,6 @@ import math
 
 import torch
 import torch.nn.functional as F
-from torch.nn.attention import SDPBackend, sdpa_kernel
 from torch import nn
 
 from . import _lib, modules, ops
@@ -352,6 +351,18 @@ class _Recomputed(torch.autograd.Function):
         return (None, None, *(next(grads) if w else None for w in wanted))
 
 
+def _laid_out_as(t):
+    """A gradient hook that gives t's strides to its gradient.  The backward pass
+    of the cuDNN attention (PyTorch 2.11, cuDNN 9.22) reads its gradient's memory
+    with its output's strides: for the view [B, H, S, D] of token-major rows it
+    returned, bit for bit, the gradients of the other values that this gives."""
+    strides = t.stride()
+
+    def hook(g):
+        return g if g.stride() == strides else g.new_empty_strided(g.shape, strides).copy_(g)
+    return hook
+
+
 def _recorded(module, *tensors) -> bool:
     """Whether a call inside a model with adapters is recorded for a backward
     pass (elsewhere the fused kernels stay outside autograd)."""
@@ -615,6 +626,8 @@ class FluxAttention(nn.Module):
             q = apply_rotary_emb(q, rope)
             k = apply_rotary_emb(k, rope)
         out = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
+        if out.is_cuda and out.requires_grad:
+            out.register_hook(_laid_out_as(out))
         out = out.transpose(1, 2).flatten(2).to(x.dtype)
         if ctx is not None:
             img = out[:, txt_len:].contiguous()
@@ -680,13 +693,9 @@ class FluxAttention(nn.Module):
             q = qk_norm_rope(q_i, q_t, h, self.norm_q.weight, wq_t, rope, self.norm_q.eps)
             k = qk_norm_rope(k_i, k_t, h, self.norm_k.weight, wk_t, rope, self.norm_k.eps)
             v = qk_norm_rope(v_i, v_t, h)
+        att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
         if recorded:
-            # not by cuDNN, whose backward pass was seen to return NaN (44 tokens
-            # x 64, from finite operands, outputs and log-sums that were right)
-            with sdpa_kernel([SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION, SDPBackend.MATH]):
-                att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
-        else:
-            att = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=False)
+            att.register_hook(_laid_out_as(att))
         txt_len = 0 if ctx is None else ctx.shape[1]
         if recorded:
             rows = att.transpose(1, 2).flatten(2)
