@@ -263,6 +263,7 @@ def concat_nf4_linears(mods):
         return None
     dev = mods[0].weight_nf4.device
     fused = Ltx23Nf4Linear(sum(m.out_features for m in mods), k, bias=False).to(dev)
+    fused.differentiable = any(m.differentiable for m in mods)
     if mods[0].scales_bf16:
         fused.repack_scales_bf16()
     fused.set_nf4_weight(torch.cat([m.weight_nf4 for m in mods]),
@@ -640,6 +641,7 @@ def swap_quant_linears(model: nn.Module, is_quant_key, fmt: str = "nf4",
             q.set_fp8_weight(w8, scale.cpu())
         if has_bias:
             q.bias = mod.bias
+        q.differentiable = getattr(mod, "differentiable", False)
         if leaf.isdigit():
             parent[int(leaf)] = q
         else:

@@ -224,6 +224,8 @@ class _ColumnParallelBase(torch.nn.Module):
             self.bias.copy_(full_bias.reshape(-1)[self.n0:self.n1])
 
     def _prep(self, x):
+        if getattr(self, "differentiable", False) and torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("a column-parallel linear passes no gradients on")  # (attach_adapters marked it)
         if not x.is_cuda:
             raise RuntimeError("the column-parallel linear has no CPU path")
         if x.dtype != torch.bfloat16:
@@ -256,8 +258,6 @@ class _ColumnParallelBase(torch.nn.Module):
         return g.output_view(own, m, n)
 
     def forward(self, x):
-        if getattr(self, "differentiable", False) and torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("a column-parallel linear passes no gradients on")  # (attach_adapters marked it)
         x2, m = self._prep(x)
         y = self._forward_fused(x2, m)
         return y.reshape(*x.shape[:-1], self.out_features)

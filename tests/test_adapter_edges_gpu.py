@@ -119,3 +119,17 @@ def test_small_batches_of_wide_outputs(tiles, n, r):
         torch.einsum("mr,mrn->mn", v.abs(), up.double().abs()) + y.double().abs())
     assert ((out.double() - ref).abs() <= 1.01 * (size + H * ref.abs())).all()
     assert ops.device_error() == 0
+
+
+def test_linears_quantized_or_joined_after_the_adapters_pass_gradients_on():
+    from diffuser_b200 import modules
+    model = torch.nn.Sequential(_linear("nf4", 1), torch.nn.Linear(64, 64, bias=False).cuda().to(torch.bfloat16))
+    modules.attach_adapters(model, 1, 8, lambda key: key.startswith("0"))
+    modules.swap_quant_linears(model, lambda key: key.startswith("1"))
+    joined = modules.concat_nf4_linears([model[1], model[1]])
+    x = torch.randn(5, 128, device="cuda").to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(5, 64, device="cuda").to(torch.bfloat16)
+    one, = torch.autograd.grad(model[1](model[0](x)), x, dy)
+    two, = torch.autograd.grad(joined(model[0](x))[:, 64:], x, dy)
+    # the same products, summed next to zeros: a rounding each of two results
+    assert one.any() and ((one - two).double().norm() / one.double().norm()).item() <= 2 * H
