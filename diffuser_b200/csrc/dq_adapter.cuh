@@ -27,6 +27,7 @@
 
 #include "dq_codec.cuh"
 #include "dq_f32x2.cuh"
+#include "dq_internal.h"
 #include "dq_ptx.cuh"
 #include "dq_smallm.cuh"
 #include "dq_tile.cuh"
@@ -101,7 +102,7 @@ __device__ __forceinline__ bool check_runs(const RunList& q, unsigned int* error
   }
   bad = __syncthreads_or(bad);
   bad_id = __syncthreads_or(bad_id);
-  if ((bad || bad_id) && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(error, 1u << 10);
+  if ((bad || bad_id) && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(error, 1u << kErrIndex);
   return bad == 0;
 }
 
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(DownCfg<R>::kThreads, 2) adapter_down_kernel(c
   }
   __syncwarp();
   cluster_sync();  // the other ranks have read this one's sums
-  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << 5);
+  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << kErrTimeout);
   if (warp == C::kProducers) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
@@ -1249,7 +1250,7 @@ __global__ void __launch_bounds__(WgradCfg<R, I8>::kThreads, WgradCfg<R, I8>::kM
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << 5);
+  if (tid == 0 && *abort_flag) atomicOr(a.error, 1u << kErrTimeout);
   if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);

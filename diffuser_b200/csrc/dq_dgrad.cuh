@@ -8,6 +8,7 @@
 
 #include "dq_codec.cuh"
 #include "dq_f32x2.cuh"
+#include "dq_internal.h"
 #include "dq_tile.cuh"
 
 namespace dq {
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kDgradThreads, 1)
     const unsigned long long t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) {
     }
-    if (tid == 0) atomicOr(a.error, 1u << 5);
+    if (tid == 0) atomicOr(a.error, 1u << kErrTimeout);
   }
   __syncthreads();
   if (warp == kDgradMmaWarp) {

@@ -35,11 +35,10 @@
 
 #include "dq_codec.cuh"
 #include "dq_epilogue.cuh"
+#include "dq_internal.h"
 #include "dq_ptx.cuh"
 
 namespace dq {
-
-enum : unsigned int { kErrTimeout = 5u };
 
 // Per-device kernel error word (bit kErrTimeout: a bounded wait expired).
 // The GEMM kernels' translation unit defines it; others take its address

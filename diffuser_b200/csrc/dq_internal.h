@@ -15,8 +15,9 @@ int device_sms(int* sms);
 // The first call on a device looks it up; it is cached from then on.
 int error_word(unsigned int** word);
 
-// Bits of the error word besides kErrTimeout (dq_gemm.cuh).
-enum : unsigned int { kErrIndex = 10u };
+// Bits of the error word: a bounded wait expired; an index on the device was out
+// of range.
+enum : unsigned int { kErrTimeout = 5u, kErrIndex = 10u };
 
 // y[M, N] (row stride ldy) = x[M, K] . w[N, K]^T, all bf16, on the CTA-pair
 // GEMM without its decode.  K % 8 == 0, x / w 16-byte aligned.

@@ -8,15 +8,13 @@
 
 #include "../../include/dq_dit.h"
 #include "dq_internal.h"
+#include "dq_launch.h"
 #include "dq_norm.cuh"
 
 namespace dq {
 namespace {
 
-constexpr int kMaxDevices = 64;
-inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 inline const __nv_bfloat16* bf(const void* p) { return static_cast<const __nv_bfloat16*>(p); }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // An output in the place of an operand has its rows.
 bool same_rows(const void* out, int64_t ld_out, const void* in, int64_t ld_in) { return out != in || ld_out == ld_in; }
@@ -47,7 +45,7 @@ struct KernelInfo {
   std::atomic<int> per_sm[kMaxDevices];  // 0: not set up
 };
 template <typename K>
-int set_up(K kern, int threads, size_t most, size_t smem, KernelInfo& info, int* per_sm) {
+int set_up(K kern, int threads, size_t most, KernelInfo& info, int* per_sm) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DQ_ERR_CUDA;
   int n = info.per_sm[dev].load(std::memory_order_acquire);
@@ -67,7 +65,7 @@ int launch_forward_npt(NormArgs a, int64_t B, int sms, cudaStream_t st) {
   const size_t per_feature = kNormAhead * 4 + (OPS ? 0 : 12);
   int per_sm = 1;
   const int rc = set_up(gated_norm_kernel<NPT, OPS, FULL>, kNormThreads, per_feature * NPT * kNormThreads * 4,
-                        per_feature * a.D, info, &per_sm);
+                        info, &per_sm);
   if (rc != DQ_OK) return rc;
   a.chunks = chunks_of(B, a.S, static_cast<int64_t>(sms) * per_sm, 1);
   gated_norm_kernel<NPT, OPS, FULL><<<static_cast<unsigned>(B * a.chunks), kNormThreads, per_feature * a.D, st>>>(a);
@@ -99,7 +97,7 @@ int launch_backward_npt(const NormGradArgs& a, int64_t B, cudaStream_t st) {
   constexpr size_t kPerFeature = kNormGradAhead * 8 + 8;
   int per_sm = 1;
   const int rc = set_up(gated_norm_backward_kernel<THREADS, NPT, FULL>, THREADS, kPerFeature * THREADS * NPT * 4,
-                        kPerFeature * a.D, info, &per_sm);
+                        info, &per_sm);
   if (rc != DQ_OK) return rc;
   gated_norm_backward_kernel<THREADS, NPT, FULL>
       <<<static_cast<unsigned>(B * a.chunks), THREADS, kPerFeature * a.D, st>>>(a);
@@ -110,21 +108,6 @@ template <int THREADS, int NPT>
 int launch_backward(const NormGradArgs& a, int64_t B, cudaStream_t st) {
   return a.D == 4 * NPT * THREADS ? launch_backward_npt<THREADS, NPT, true>(a, B, st)
                                   : launch_backward_npt<THREADS, NPT, false>(a, B, st);
-}
-
-// The reduction may start while the last rows are on their way out; it waits
-// for them (griddepcontrol.wait) before it reads the sums.
-int launch_reduce(const NormReduceArgs& q, cudaStream_t st) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(q.D, 32)));
-  cfg.blockDim = dim3(32 * kReduceWarps);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gated_norm_reduce_kernel, q) == cudaSuccess ? DQ_OK : DQ_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -149,7 +132,7 @@ int dq_gated_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int6
     return DQ_ERR_SHAPE;
   for (const void* p : {x, y, gate, scale, shift, post_weight, pre_weight, static_cast<const void*>(s),
                         static_cast<const void*>(h)})
-    if (!aligned8(p)) return DQ_ERR_ALIGN;
+    if (!aligned(p, 8)) return DQ_ERR_ALIGN;
   // in place row by row, or rows of another stride are written before they are read
   if (s == h) return DQ_ERR_ARG;
   if (!same_rows(s, ld_s, x, ld_x) || !same_rows(s, ld_s, y, ld_y) || !same_rows(h, ld_h, x, ld_x) ||
@@ -194,9 +177,9 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
     return DQ_ERR_SHAPE;
   for (const void* p : {ds, dh, s, y, gate, scale, post_weight, pre_weight, static_cast<const void*>(dx),
                         static_cast<const void*>(dy)})
-    if (!aligned8(p)) return DQ_ERR_ALIGN;
+    if (!aligned(p, 8)) return DQ_ERR_ALIGN;
   for (const float* p : {dgate, dscale, dshift, dpost_weight, dpre_weight})
-    if ((reinterpret_cast<uintptr_t>(p) & 3) != 0) return DQ_ERR_ALIGN;
+    if (!aligned(p, 4)) return DQ_ERR_ALIGN;
   if (dx == dy) return DQ_ERR_ARG;
   for (const void* out : {static_cast<const void*>(dx), static_cast<const void*>(dy)}) {
     const int64_t ld = out == dx ? ld_dx : ld_dy;
@@ -207,7 +190,7 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
   int sms = 0;
   if ((rc = device_sms(&sms)) != DQ_OK) return rc;
   const int chunks = chunks_of(B, S, backward_slots(D, sms), 4);
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+  if (workspace == nullptr || !aligned(workspace, 16) ||
       workspace_bytes < static_cast<size_t>(B) * chunks * 3 * D * sizeof(float))
     return DQ_ERR_WORKSPACE;
   NormGradArgs a = {bf(ds), bf(dh), bf(s), bf(y), bf(gate), bf(scale), bf(post_weight), bf(pre_weight),
@@ -224,7 +207,9 @@ int dq_gated_norm_backward(const void* ds, int64_t ld_ds, const void* dh, int64_
   NormReduceArgs q = {a.part, a.gate, a.scale, a.post_w, a.pre_w, dgate, dscale, dshift, dpost_weight, dpre_weight,
                       ld_gate, ld_mod, static_cast<int>(B), chunks, D, residual_scale};
   if (dgate != nullptr || dscale != nullptr || dshift != nullptr || dpost_weight != nullptr || dpre_weight != nullptr)
-    return launch_reduce(q, st);
+    // it may start while the last rows are on their way out, and waits for them
+    return launch(gated_norm_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(D, 32))), 32 * kReduceWarps, 0, st, true,
+                  dim3(1), q);
   return DQ_OK;
 }
 

@@ -33,6 +33,7 @@
 
 #include "dq_f32x2.cuh"
 #include "dq_ptx.cuh"
+#include "dq_tile.cuh"
 
 namespace dq {
 
@@ -41,11 +42,6 @@ enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 // Thread-private 8-byte copy into shared memory.
 __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
@@ -132,7 +128,6 @@ struct NormFactors {
   }
 };
 
-__device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 __device__ __forceinline__ F2 bf16_round2(F2 a) { return widen(narrow(a)); }
 
 // CTA (batch element, chunk): rows chunk, chunk + chunks, ... of the element.
@@ -173,7 +168,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
         }
       }
     }
-    copies_commit();
+    cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < kNormAhead; ++i) fetch(chunk + i * a.chunks, i);
@@ -191,7 +186,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
   int par = 0, slot = 0;
   for (int row = chunk; row < a.S; row += a.chunks, par ^= 1, slot = slot + 1 == kNormAhead ? 0 : slot + 1) {
     const int64_t t = b * a.S + row;
-    copies_wait<kNormAhead - 1>();
+    cp_async_wait<kNormAhead - 1>();
     const uint32_t src = slot0 + static_cast<uint32_t>(slot) * 2u * row_bytes;
     F2 v[NPT][2];
     uint2 cx[NPT];
@@ -330,7 +325,7 @@ __global__ void __launch_bounds__(kNormThreads, NPT <= 4 ? 3 : 2) gated_norm_ker
       }
     }
   }
-  copies_wait<0>();
+  cp_async_wait<0>();
 }
 
 struct NormGradArgs {
@@ -385,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, norm_grad_ctas(THREADS, NPT))
         }
       }
     }
-    copies_commit();
+    cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < kNormGradAhead; ++i) fetch(chunk + i * a.chunks, i);
@@ -413,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, norm_grad_ctas(THREADS, NPT))
   int par = 0, slot = 0;
   for (int row = chunk; row < a.S; row += a.chunks, par ^= 1, slot = slot + 1 == kNormGradAhead ? 0 : slot + 1) {
     const int64_t t = b * a.S + row;
-    copies_wait<kNormGradAhead - 1>();
+    cp_async_wait<kNormGradAhead - 1>();
     const uint32_t src = slot0 + static_cast<uint32_t>(slot) * 4u * row_bytes;
     uint2 us[NPT], uy[NPT];
     F2 dt[NPT][2];  // dh
@@ -537,8 +532,8 @@ __global__ void __launch_bounds__(THREADS, norm_grad_ctas(THREADS, NPT))
       }
     }
   }
-  copies_wait<0>();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cp_async_wait<0>();
+  grid_launch_dependents();
   float4* part = reinterpret_cast<float4*>(a.part + static_cast<int64_t>(blockIdx.x) * 3 * a.D);
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
@@ -579,7 +574,7 @@ __global__ void __launch_bounds__(32 * kReduceWarps) gated_norm_reduce_kernel(co
   const float wq = in && a.pre_w != nullptr ? __bfloat162float(a.pre_w[col]) : 1.0f;
   const float wp = in && a.post_w != nullptr ? __bfloat162float(a.post_w[col]) : 1.0f;
   float dpre = 0.f, dpost = 0.f;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the chunks' sums
+  grid_wait();  // the chunks' sums
   auto add = [&](int b, int first, int step, float* q) {
     if (!in) return;
     for (int c0 = first; c0 < a.chunks; c0 += 8 * step) {

@@ -1,5 +1,5 @@
-// dq_tile.cuh -- instructions that the adapter, checkpoint and input-gradient
-// kernels share: asynchronous copies, matrix fragments, cluster loads, the
+// dq_tile.cuh -- instructions that the adapter, checkpoint, input-gradient and
+// norm kernels share: asynchronous copies, matrix fragments, cluster loads, the
 // single-CTA tensor-memory MMA on two shared-memory operands.
 #pragma once
 
@@ -20,14 +20,6 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
 __device__ __forceinline__ void cp_async_16_l2(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
-}
-__device__ __forceinline__ uint4 ld_global_l2(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p)
-               : "memory");
-  return v;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
