@@ -177,10 +177,13 @@ def load_quantized(model: nn.Module, art: Artifact, device=None, scales: str = "
     """Swap every quantized key of `art` into `model` as an NF4 / fp8 linear
     and copy the residents; hard errors (strict) on an artifact key that lands
     nowhere or a model parameter the artifact leaves unfilled.  scales="bf16"
-    repacks the NF4 block scales to bf16 at load time.  Returns a report
+    repacks the NF4 block scales to bf16 at load time.  A model with adapters is
+refused.  Returns a report
     {"cast": [...], "residents": [...]}."""
     if scales not in ("f32", "bf16"):
         raise ValueError("scales must be 'f32' or 'bf16'")
+    if any(isinstance(m, modules.AdapterLinear) for m in model.modules()):
+        raise RuntimeError("load the weights before attach_adapters: the linears that hold adapters would be replaced")
     cast = art.cast_keys()
     used = set()
     for key in cast:
