@@ -548,25 +548,29 @@ def attach_adapters(model: nn.Module, n_adapters: int, rank: int, is_adapted_key
     """Wrap the model's quantized linears (those whose ``<name>.weight`` key
     is_adapted_key accepts; all of them without it) in AdapterLinear.  Linears
     that flux.fuse_qkv_projections concatenated are dropped where one of their
-    parts is wrapped; linears that have a bank already keep it.  The model's
+    parts is wrapped; linears that have a bank already keep it; one in several
+    places gets one.  The model's
     modules are marked differentiable: with gradients enabled, the quantized
     linears that were not wrapped and the FLUX blocks' fused kernels then pass
     gradients on too.  Returns the wrapped names."""
     if isinstance(model, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
         raise TypeError("a linear by itself is wrapped by AdapterLinear(linear, ...)")
-    wrapped = []
+    wrapped, made = [], {}
     for mod in model.modules():
         mod.differentiable = True
-    for name, mod in list(model.named_modules()):
+    for name, mod in list(model.named_modules(remove_duplicate=False)):
         if not isinstance(mod, (Ltx23Nf4Linear, Ltx23Fp8Linear)):
             continue
         segs = name.split(".")
-        if len(segs) > 1 and isinstance(_walk(model, segs[:-1]), AdapterLinear):
+        if isinstance(_walk(model, segs), AdapterLinear) or \
+                (len(segs) > 1 and isinstance(_walk(model, segs[:-1]), AdapterLinear)):
             continue
         if segs[-1] in ("to_qkv", "add_qkv") or (is_adapted_key is not None and not is_adapted_key(name + ".weight")):
             continue
         parent = _walk(model, segs[:-1]) if len(segs) > 1 else model
-        wrap = AdapterLinear(mod, n_adapters, rank, pack_activations)
+        wrap = made.get(mod)  # (a linear in two places has one bank)
+        if wrap is None:
+            wrap = made[mod] = AdapterLinear(mod, n_adapters, rank, pack_activations)
         if segs[-1].isdigit():
             parent[int(segs[-1])] = wrap
         else:

@@ -25,3 +25,17 @@ def test_weights_are_not_loaded_over_adapters(tmp_path):
     with pytest.raises(RuntimeError, match="before attach_adapters"):
         artifact.load_quantized(model, art)
     assert model["a"] is kept and isinstance(kept, modules.AdapterLinear)
+
+
+def test_a_linear_in_two_places_is_wrapped_in_both():
+    model = _model()
+    model["again"] = model["a"]
+    model["block"] = nn.ModuleDict({"c": model["b"], "list": nn.ModuleList([model["a"]])})
+    model["twin"] = model["block"]
+    names = modules.attach_adapters(model, 2, 8)
+    banks = [m for m in model.modules() if isinstance(m, modules.AdapterLinear)]
+    assert len(banks) == 2 and names[:2] == ["a", "b"]
+    assert model["again"] is model["a"] is model["block"]["list"][0] and model["block"]["c"] is model["b"]
+    assert not any(isinstance(m, modules.Ltx23Nf4Linear) and not n.endswith("base") for n, m in model.named_modules())
+    assert modules.attach_adapters(model, 2, 8) == []
+    assert [m for m in model.modules() if isinstance(m, modules.AdapterLinear)] == banks
