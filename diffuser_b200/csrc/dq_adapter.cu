@@ -158,9 +158,9 @@ int launch_up(UpArgs a, int tiles, int64_t M, int64_t requests, int sms, cudaStr
   if (rc != DQ_OK) return rc;
   // 64-column steps per CTA: the fewest that put the whole launch into one wave
   // if eight are enough (4608 x 4096 at r = 64: six steps 22 us, four, a wave
-  // and a third, 25), else six (4613 x 16384 at r = 32, with / without GELU: six
-  // 82.5 / 69 us, four, whose CTAs' first loads weigh more, 85.7 / 73.8, sixteen,
-  // which leave the last wave emptier, 91 / 78)
+  // and a third, 25), else six (4613 x 16384 at r = 32, with / without GELU, down
+  // product included: six 77 / 67 us, four, whose CTAs' first loads weigh more,
+  // 80 / 69, sixteen, which leave the last wave emptier, 82 / 74)
   const int64_t total = ceil_div(a.N, C::kStepCols), slots = static_cast<int64_t>(sms) * C::kMinCtas;
   const int64_t most = ceil_div(M, kTileRows) + std::min<int64_t>(a.A, requests) + 1;
   int64_t steps = 1;

@@ -481,9 +481,10 @@ __device__ __forceinline__ F2 gate2(F2 x, int act) { return act == kActSwiGlu ? 
 // of a step is the ring's.
 //
 // Measured: 4613 x 16384 at r = 32 with GELU, down product included, 77 us (302
-// MB of Y and O; a copy in the same pieces takes 53), 69 without.  What is left
-// is instructions: half of the issue slots, the GELU's two special-function
-// results per element 40 us of that unit.  (Products onto zeros and Y added
+// MB of Y and O; a copy in the same pieces takes 53), 67 without.  No unit is the
+// bound: issue slots 56% busy, the special-function unit 58 (two results per
+// element), shared memory 53, DRAM 45; the stalls are fixed latencies and the
+// shared-memory pipe at 24 warps per SM.  (Products onto zeros and Y added
 // behind them in another thread layout, P scattered into place by 4-byte stores:
 // 80 and 74.  One wave of CTAs with equal shares of all column steps: 78.)
 template <int R>

@@ -15,7 +15,10 @@
 // doubled by row parity, so it takes one barrier.  (With scalar arithmetic,
 // bf16 factors from L1 and the next row prefetched in registers: 42 instructions
 // per element and 35 us forward, 68 and 98 us backward at 4608 x 4096, where
-// forward now takes 26.0, 5.8 TB/s, and backward with its reduction 51.5.)
+// forward now takes 26.5, 5.7 TB/s, and backward with its reduction 52.)  The
+// backward kernel is bound by latency: 255 registers and 96 KB leave two CTAs,
+// eight warps, per SM, whose issue slots are 33% busy and DRAM 4.4 TB/s; they
+// stall on shared-memory reads, fixed latencies, loads, the row's barriers.
 //
 // Backward.  With t = Npre(s), m = wpre (1 + scale), dt = dh m, and yh = Npost(y):
 //   dx = ds + rstd_s (dt - [mean dt] - t mean(dt t))            (mean dt: LayerNorm only)
