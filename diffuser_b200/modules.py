@@ -345,10 +345,10 @@ class AdapterSelection:
         self._recent: dict = {}                      # tokens -> plan, the KEPT used last, oldest first
         self._captured: dict = {}                    # tokens -> plan
 
-    def __getstate__(self):  # a copy builds its own plans
+    def __getstate__(self):  # a copy has ids and plans of its own
         with torch.cuda.device(self.ids.device):
             self._after(self._set, self.ids)
-        return {"ids": self.ids, "n_adapters": self.n_adapters}
+            return {"ids": self.ids.clone(), "n_adapters": self.n_adapters}
 
     def __setstate__(self, state):
         self.__dict__.update(state)

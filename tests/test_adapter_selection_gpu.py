@@ -128,3 +128,16 @@ def test_plans_of_many_lengths_are_not_all_kept():
     fresh = ops.adapter_plan(sel.ids, torch.tensor([0, 5, 10], dtype=torch.int32, device="cuda"), 10, 3)
     wide = [torch.cat([t, t])[:10] for t in operands[:2]]
     assert torch.equal(ops.adapter_add(*wide, *operands[2:], mine), ops.adapter_add(*wide, *operands[2:], fresh))
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy])
+def test_a_copy_has_ids_of_its_own(how):
+    from diffuser_b200 import modules, ops
+    sel = modules.AdapterSelection(torch.tensor([1, 0], dtype=torch.int32, device="cuda"), 3)
+    operands = _operands(2, 3)
+    twin = how(sel)
+    want = ops.adapter_add(*operands, twin.plan(6))
+    sel.update_(torch.tensor([2, 2], dtype=torch.int32, device="cuda"))
+    assert twin.ids.tolist() == [1, 0] and sel.ids.tolist() == [2, 2]
+    assert torch.equal(ops.adapter_add(*operands, how(twin).plan(6)), want)
+    assert not torch.equal(ops.adapter_add(*operands, sel.plan(6)), want)
